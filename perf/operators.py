@@ -206,7 +206,10 @@ def prepare(case, seed):
             for k in ("m", "v"):
                 scales = s[k + "s"].reshape(-1).split(blocks)
                 views[k] = [fm.Moment8(c, a) for c, a in zip(views[k + "c"], scales)]
-        s["views"] = views
+        s["grads"] = views["g"]
+        s["optimiser"] = fm.AdamW(views["p"], lr=_LR, betas=_BETAS, eps=_EPS, weight_decay=_DECAY,
+                                  moments=(views["m"], views["v"]), masters=views.get("master"),
+                                  step=s["step"])
     return {"case": case, **s}
 
 
@@ -370,12 +373,9 @@ def _own_norm(s):
 
 
 def _own_adamw(s):
-    fm, views = _framework(), s["views"]
-    s["step"] += 1
-    fm.adamw_step(views["p"], views["g"], views["m"], views["v"], step=s["step"], lr=_LR,
-                  betas=_BETAS, eps=_EPS, weight_decay=_DECAY, masters=views.get("master"))
+    s["optimiser"].step(s["grads"])
     if s["case"]["bits"] == 8:
-        fm.moment_values(views["m"] + views["v"], out=s["values"][0] + s["values"][1])
+        s["optimiser"].moment_values(out=s["values"])
     return _stepped(s)
 
 
