@@ -1,0 +1,319 @@
+// fms_adamw.hip -- one AdamW step over many tensors at once, moments in 32 or 8 bits.
+//
+//   g = grad * grad_scale
+//   m = beta1 m + (1 - beta1) g
+//   v = beta2 v + (1 - beta2) (g * g)
+//   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+// in fp32, every operation rounded by itself (the library is built without contraction), on
+// the fp32 master where a tensor has one, else on the parameter.
+//
+// 8-bit moments: 256 neighbouring elements share an fp32 scale a, the largest magnitude among
+// them (0 where that is below the least normal number).
+//   m: int8 code  c = sign(m) round(127 sqrt(|m| / a)),   value  sign(c) (c / 127)^2 a
+//   v: uint8 code c = round(255 (v / a)^(1/4)),           value  (c / 255)^4 a
+// Codes are dense near zero and even in relative terms over four decades; a v above zero keeps
+// a code of at least 1, so that sqrt(v) never becomes 0 under an m that did not.  A NaN or
+// infinity makes its block's scale NaN or infinite and with it the block's values NaN.
+//
+// Bound by memory: 28 bytes an element in fp32, 22 with 16-bit parameters and gradients, 10
+// with 8-bit moments.  A workgroup takes 2048 elements of one tensor, eight a lane, so that
+// half a wave holds a block of 8-bit moments.  The tensors' pointers travel as kernel
+// arguments, up to 56 a launch: nothing is kept between calls and nothing is uploaded.
+#include "fms_adamw.hpp"
+
+#include <float.h>
+
+#include "fms_device.hpp"
+
+namespace fms {
+namespace {
+
+constexpr int kPer = 8;                    // elements per lane
+constexpr int kChunk = 256 * kPer;         // elements per workgroup
+constexpr int kBlock = FMS_MOMENT_BLOCK;   // elements that share a scale
+static_assert(kBlock == 32 * kPer, "a half wave holds a block");
+
+// Eight neighbouring values from element k of n; vec: whole 16-byte units from the base on.
+template <class T>
+__device__ __forceinline__ void load8(float (&v)[kPer], const T* p, int64_t k, int64_t n, bool vec) {
+  if (vec && k + kPer <= n) {
+    typedef T V __attribute__((ext_vector_type(kPer)));
+    V u;
+    __builtin_memcpy(&u, __builtin_assume_aligned(p + k, sizeof(T) * kPer > 16 ? 16 : sizeof(T) * kPer),
+                     sizeof(u));
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = (float)u[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = k + e < n ? (float)p[k + e] : 0.0f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(const float (&v)[kPer], T* p, int64_t k, int64_t n, bool vec) {
+  if (vec && k + kPer <= n) {
+    typedef T V __attribute__((ext_vector_type(kPer)));
+    V u;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) u[e] = (T)v[e];
+    __builtin_memcpy(__builtin_assume_aligned(p + k, sizeof(T) * kPer > 16 ? 16 : sizeof(T) * kPer),
+                     &u, sizeof(u));
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (k + e < n) p[k + e] = (T)v[e];
+  }
+}
+__device__ __forceinline__ void load_typed(float (&v)[kPer], const void* p, int dtype, int64_t k,
+                                           int64_t n, bool vec) {
+  if (dtype == FMS_F32)
+    load8(v, static_cast<const float*>(p), k, n, vec);
+  else if (dtype == FMS_F16)
+    load8(v, static_cast<const _Float16*>(p), k, n, vec);
+  else
+    load8(v, static_cast<const __bf16*>(p), k, n, vec);
+}
+__device__ __forceinline__ void store_typed(const float (&v)[kPer], void* p, int dtype, int64_t k,
+                                            int64_t n, bool vec) {
+  if (dtype == FMS_F32)
+    store8(v, static_cast<float*>(p), k, n, vec);
+  else if (dtype == FMS_F16)
+    store8(v, static_cast<_Float16*>(p), k, n, vec);
+  else
+    store8(v, static_cast<__bf16*>(p), k, n, vec);
+}
+
+// The largest magnitude of a block, in its 32 lanes.  Magnitudes compare as their bits, NaN
+// above all: a NaN is never lost.
+__device__ __forceinline__ float block_top(const float (&v)[kPer]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    const uint32_t b = (uint32_t)__shfl_xor((int)top, o);
+    top = b > top ? b : top;
+  }
+  return __builtin_bit_cast(float, top);
+}
+
+__device__ __forceinline__ float value_m(int c, float a) {
+  const float t = (float)c * (1.0f / 127.0f);
+  const float q = t * t * a;
+  return c < 0 ? -q : q;
+}
+__device__ __forceinline__ float value_v(int c, float a) {
+  const float t = (float)c * (1.0f / 255.0f);
+  const float q = t * t;
+  return q * q * a;
+}
+// A block's scale and the reciprocal its codes are made with.
+__device__ __forceinline__ void scale_of(float top, float& a, float& inv) {
+  const bool tiny = top < FLT_MIN;
+  a = tiny ? 0.0f : top;
+  inv = tiny ? 0.0f : 1.0f / top;
+}
+__device__ __forceinline__ int code_of(float root, float steps) {  // root in 0..1, or NaN
+  const float c = __builtin_rintf(root * steps);
+  return c >= 0.0f ? (int)c : 0;
+}
+
+// Codes of eight neighbouring elements.
+struct Codes {
+  uint32_t w[2];
+  __device__ __forceinline__ int get(int e, bool sign) const {
+    const uint32_t b = w[e >> 2] >> (8 * (e & 3));
+    return sign ? (int)(int8_t)b : (int)(b & 0xffu);
+  }
+};
+__device__ __forceinline__ Codes load_codes(const uint8_t* p, int64_t k, int64_t n, bool vec) {
+  Codes c = {{0u, 0u}};
+  if (vec && k + kPer <= n) {
+    __builtin_memcpy(&c, __builtin_assume_aligned(p + k, 8), 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (k + e < n) c.w[e >> 2] |= (uint32_t)p[k + e] << (8 * (e & 3));
+  }
+  return c;
+}
+__device__ __forceinline__ void store_codes(const Codes& c, uint8_t* p, int64_t k, int64_t n, bool vec) {
+  if (vec && k + kPer <= n) {
+    __builtin_memcpy(__builtin_assume_aligned(p + k, 8), &c, 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (k + e < n) p[k + e] = (uint8_t)(c.w[e >> 2] >> (8 * (e & 3)));
+  }
+}
+
+constexpr int kTensors = 48;  // per launch: the arguments stay within 4 KiB
+struct Tensors {
+  fms_adamw_tensor t[kTensors];
+  int32_t end[kTensors];  // workgroups up to and with each tensor's
+  int32_t vec[kTensors];
+  int32_t count;
+};
+static_assert(sizeof(Tensors) + sizeof(AdamWStep) <= 4096, "kernel arguments");
+
+// The tensor a workgroup belongs to: the first whose end lies past it.
+template <class L>
+__device__ __forceinline__ int tensor_of(const L& l, int block) {
+  int lo = 0, hi = l.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (l.end[mid] > block)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
+  const int i = tensor_of(L, blockIdx.x);
+  const fms_adamw_tensor& t = L.t[i];
+  const int first = i > 0 ? L.end[i - 1] : 0;
+  const int64_t k = (int64_t)(blockIdx.x - first) * kChunk + threadIdx.x * kPer, n = t.n;
+  const bool vec = L.vec[i] != 0, codes = t.m_scale != nullptr;
+  float g[kPer], p[kPer], m[kPer], v[kPer];
+  load_typed(g, t.g, t.g_dtype, k, n, vec);
+  if (t.master)
+    load8(p, t.master, k, n, vec);
+  else
+    load_typed(p, t.p, t.p_dtype, k, n, vec);
+  if (codes) {
+    const Codes cm = load_codes(static_cast<const uint8_t*>(t.m), k, n, vec);
+    const Codes cv = load_codes(static_cast<const uint8_t*>(t.v), k, n, vec);
+    const float am = k < n ? t.m_scale[k / kBlock] : 0.0f, av = k < n ? t.v_scale[k / kBlock] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      m[e] = value_m(cm.get(e, true), am);
+      v[e] = value_v(cv.get(e, false), av);
+    }
+  } else {
+    load8(m, static_cast<const float*>(t.m), k, n, vec);
+    load8(v, static_cast<const float*>(t.v), k, n, vec);
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const float gs = g[e] * S.grad_scale;
+    m[e] = m[e] * S.beta1 + gs * S.rest1;
+    v[e] = v[e] * S.beta2 + gs * gs * S.rest2;
+    const float den = sqrtf(v[e]) * S.inv_bc2 + S.eps;
+    p[e] = p[e] * S.decay - m[e] / den * S.lr;
+  }
+  if (t.master) store8(p, t.master, k, n, vec);
+  store_typed(p, t.p, t.p_dtype, k, n, vec);
+  if (codes) {
+    // (elements past the end are zero and the whole half wave takes part)
+    float am, im, av, iv;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (k + e >= n) m[e] = v[e] = 0.0f;
+    scale_of(block_top(m), am, im);
+    scale_of(block_top(v), av, iv);
+    Codes cm = {{0u, 0u}}, cv = {{0u, 0u}};
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      int c = code_of(sqrtf(fabsf(m[e]) * im), 127.0f);
+      c = m[e] < 0.0f ? -c : c;
+      cm.w[e >> 2] |= (uint32_t)(c & 0xff) << (8 * (e & 3));
+      const float q = v[e] * iv;
+      c = code_of(sqrtf(sqrtf(q)), 255.0f);
+      c = q > 0.0f && c < 1 ? 1 : c;
+      cv.w[e >> 2] |= (uint32_t)c << (8 * (e & 3));
+    }
+    store_codes(cm, static_cast<uint8_t*>(t.m), k, n, vec);
+    store_codes(cv, static_cast<uint8_t*>(t.v), k, n, vec);
+    if ((threadIdx.x & 31) == 0 && k < n) {
+      t.m_scale[k / kBlock] = am;
+      t.v_scale[k / kBlock] = av;
+    }
+  } else {
+    store8(m, static_cast<float*>(t.m), k, n, vec);
+    store8(v, static_cast<float*>(t.v), k, n, vec);
+  }
+}
+
+constexpr int kMoments = 72;
+struct Moments {
+  fms_moment8 t[kMoments];
+  int32_t end[kMoments];
+  int32_t vec[kMoments];
+  int32_t count;
+};
+static_assert(sizeof(Moments) <= 4096, "kernel arguments");
+
+__global__ void __launch_bounds__(256) moment_values_kernel(Moments L) {
+  const int i = tensor_of(L, blockIdx.x);
+  const fms_moment8& t = L.t[i];
+  const int first = i > 0 ? L.end[i - 1] : 0;
+  const int64_t k = (int64_t)(blockIdx.x - first) * kChunk + threadIdx.x * kPer, n = t.n;
+  if (k >= n) return;
+  const bool vec = L.vec[i] != 0;
+  const Codes c = load_codes(static_cast<const uint8_t*>(t.codes), k, n, vec);
+  const float a = t.scales[k / kBlock];
+  float v[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e)
+    v[e] = t.is_signed ? value_m(c.get(e, true), a) : value_v(c.get(e, false), a);
+  store8(v, t.values, k, n, vec);
+}
+
+bool aligned(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) & 15u) return false;
+  return true;
+}
+
+// Hands `launch` lists of up to kMost tensors whose workgroups fit one grid.  A tensor's
+// workgroups beyond a grid's are no concern: 2^22 of them are 2^33 elements, and a larger
+// tensor does not fit the memory of the device with its moments.
+template <class L, class T, int kMost, class Vec, class F>
+hipError_t in_lists(int64_t count, const T* tensors, Vec&& vec, F&& launch) {
+  constexpr int64_t kGrid = (int64_t)1 << 23;
+  static thread_local L list;
+  list.count = 0;
+  int64_t blocks = 0;
+  for (int64_t i = 0; i <= count; ++i) {
+    const int64_t need = i < count ? (tensors[i].n + kChunk - 1) / kChunk : 0;
+    if (list.count > 0 && (i == count || list.count == kMost || blocks + need > kGrid)) {
+      launch(list, (unsigned)blocks);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      list.count = 0;
+      blocks = 0;
+    }
+    if (need == 0) continue;
+    blocks += need;
+    list.t[list.count] = tensors[i];
+    list.vec[list.count] = vec(tensors[i]) ? 1 : 0;
+    list.end[list.count++] = (int32_t)blocks;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t adamw_step(int64_t count, const fms_adamw_tensor* tensors, const AdamWStep& s,
+                      hipStream_t stream) {
+  return in_lists<Tensors, fms_adamw_tensor, kTensors>(
+      count, tensors,
+      [](const fms_adamw_tensor& t) { return aligned({t.p, t.g, t.m, t.v, t.master}); },
+      [&](const Tensors& l, unsigned blocks) {
+        hipLaunchKernelGGL(adamw_kernel, dim3(blocks), dim3(256), 0, stream, l, s);
+      });
+}
+
+hipError_t moment_values(int64_t count, const fms_moment8* moments, hipStream_t stream) {
+  return in_lists<Moments, fms_moment8, kMoments>(
+      count, moments, [](const fms_moment8& t) { return aligned({t.codes, t.values}); },
+      [&](const Moments& l, unsigned blocks) {
+        hipLaunchKernelGGL(moment_values_kernel, dim3(blocks), dim3(256), 0, stream, l);
+      });
+}
+
+}  // namespace fms

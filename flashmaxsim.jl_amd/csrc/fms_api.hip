@@ -13,11 +13,14 @@
 #include <mutex>
 
 #include "../../include/flashmaxsim_hip.h"
+#include "fms_adamw.hpp"
 #include "fms_backward.hpp"
+#include "fms_ffn.hpp"
 #include "fms_group.hpp"
 #include "fms_inbatch.hpp"
 #include "fms_inbatch_split.hpp"
 #include "fms_misc.hpp"
+#include "fms_norm.hpp"
 #include "fms_topk.hpp"
 #include "fms_scan_decl.hpp"
 #include "fms_runs.hpp"
@@ -996,6 +999,171 @@ fms_status fms_varlen_pullback(int32_t dtype, void* dQ, void* dD, const void* Qt
                                  nq_tokens, nd_tokens, max_q, dim);
   a.zero_dq = true;  // query tokens outside every pair's range get no gather
   return from_hip(launch_pullback(lay, a, as_stream(stream)));
+}
+
+// ---- token block ---------------------------------------------------------------
+
+namespace {
+
+fms_status ffn_check(const FfnArgs& a) {
+  if (elem_bytes(a.dtype) == 0) return FMS_EUNSUPPORTED;
+  if (a.act < FMS_ACT_SILU || a.act > FMS_ACT_GELU_TANH) return FMS_EINVAL;
+  if (a.tokens < 0 || a.dim < 0 || a.hidden < 0) return FMS_EINVAL;
+  if (!ffn_supported(a)) return FMS_EUNSUPPORTED;
+  const bool weights = a.hidden > 0 && a.dim > 0;
+  if ((a.tokens > 0 && a.dim > 0 && !a.x) || (weights && (!a.wg || !a.wu))) return FMS_EINVAL;
+  return FMS_OK;
+}
+
+FfnArgs ffn_args(int32_t dtype, const void* x, const void* wg, const void* wu, int32_t act,
+                 int64_t tokens, int64_t dim, int64_t hidden) {
+  FfnArgs a;
+  a.dtype = dtype;
+  a.act = act;
+  a.tokens = tokens;
+  a.dim = dim;
+  a.hidden = hidden;
+  a.x = x;
+  a.wg = wg;
+  a.wu = wu;
+  return a;
+}
+
+}  // namespace
+
+fms_status fms_gated_ffn(int32_t dtype, void* h, const void* x, const void* wg, const void* wu,
+                         int32_t act, int64_t tokens, int64_t dim, int64_t hidden, void* stream) {
+  const FfnArgs a = ffn_args(dtype, x, wg, wu, act, tokens, dim, hidden);
+  const fms_status s = ffn_check(a);
+  if (s != FMS_OK) return s;
+  if (tokens == 0 || hidden == 0) return FMS_OK;
+  if (!h) return FMS_EINVAL;
+  return from_hip(ffn_forward(a, h, as_stream(stream)));
+}
+
+fms_status fms_gated_ffn_pullback(int32_t dtype, void* dx, void* dwg, void* dwu, const void* dh,
+                                  const void* x, const void* wg, const void* wu, int32_t act,
+                                  int64_t tokens, int64_t dim, int64_t hidden, void* stream) {
+  const FfnArgs a = ffn_args(dtype, x, wg, wu, act, tokens, dim, hidden);
+  const fms_status s = ffn_check(a);
+  if (s != FMS_OK) return s;
+  if ((dwg == nullptr) != (dwu == nullptr)) return FMS_EINVAL;
+  if (dim == 0 || (!dx && !dwg)) return FMS_OK;
+  if (tokens > 0 && hidden > 0 && !dh) return FMS_EINVAL;
+  return from_hip(ffn_pullback(a, tokens > 0 ? dx : nullptr, hidden > 0 ? dwg : nullptr, dwu, dh,
+                               as_stream(stream)));
+}
+
+namespace {
+
+// Reports FMS_OK with *work = false where there is nothing to do.
+fms_status norm_check(const NormArgs& a, bool* work) {
+  *work = false;
+  if (elem_bytes(a.dtype) == 0) return FMS_EUNSUPPORTED;
+  if (a.kind != FMS_NORM_RMS && a.kind != FMS_NORM_LAYER) return FMS_EINVAL;
+  if (a.rows < 0 || a.dim < 0) return FMS_EINVAL;
+  // (an empty array's pointer may be NULL)
+  if (a.rows > 0 && a.dim > 0 && !a.f && (a.gate || a.wpost)) return FMS_EINVAL;
+  if (a.gate && (a.gate_rows < 1 || a.rows % a.gate_rows != 0)) return FMS_EINVAL;
+  if (a.dim > kNormMaxDim || a.rows > kMaxTokens) return FMS_EUNSUPPORTED;
+  *work = a.rows > 0 && a.dim > 0;
+  return *work && !a.x ? FMS_EINVAL : FMS_OK;
+}
+
+NormArgs norm_args(int32_t dtype, const void* x, const void* f, const void* gate, const void* wpost,
+                   const void* wpre, int32_t kind, float scale, float eps, int64_t rows,
+                   int64_t dim, int64_t gate_rows) {
+  NormArgs a;
+  a.dtype = dtype;
+  a.kind = kind;
+  a.scale = scale;
+  a.eps = eps;
+  a.rows = rows;
+  a.dim = dim;
+  a.gate_rows = gate_rows;
+  a.x = x;
+  a.f = f;
+  a.gate = gate;
+  a.wpost = wpost;
+  a.wpre = wpre;
+  return a;
+}
+
+}  // namespace
+
+fms_status fms_block_norm(int32_t dtype, void* r, void* n, const void* x, const void* f,
+                          const void* gate, const void* wpost, const void* wpre, int32_t kind,
+                          float scale, float eps, int64_t rows, int64_t dim, int64_t gate_rows,
+                          void* stream) {
+  const NormArgs a =
+      norm_args(dtype, x, f, gate, wpost, wpre, kind, scale, eps, rows, dim, gate_rows);
+  bool work;
+  const fms_status s = norm_check(a, &work);
+  if (s != FMS_OK || !work) return s;
+  if ((f && !r) || (wpre && !n)) return FMS_EINVAL;
+  if (!f && !wpre) return FMS_OK;
+  return from_hip(norm_forward(a, r, n, as_stream(stream)));
+}
+
+fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgate, void* dwpost,
+                                   void* dwpre, const void* dr, const void* dn, const void* x,
+                                   const void* f, const void* gate, const void* wpost,
+                                   const void* wpre, int32_t kind, float scale, float eps,
+                                   int64_t rows, int64_t dim, int64_t gate_rows, void* stream) {
+  const NormArgs a =
+      norm_args(dtype, x, f, gate, wpost, wpre, kind, scale, eps, rows, dim, gate_rows);
+  bool work;
+  const fms_status s = norm_check(a, &work);
+  if (s != FMS_OK) return s;
+  if (dn && !wpre) return FMS_EINVAL;
+  if (dim == 0) return FMS_OK;
+  if ((wpost && !dwpost) || (wpre && !dwpre)) return FMS_EINVAL;
+  if (work && (!dx || (f && !df) || (gate && !dgate))) return FMS_EINVAL;
+  NormGrads g;
+  g.dr = dr;
+  g.dn = dn;
+  g.dx = dx;
+  g.df = df;
+  g.dgate = dgate;
+  g.dwpost = wpost ? dwpost : nullptr;
+  g.dwpre = wpre ? dwpre : nullptr;
+  return from_hip(norm_pullback(a, g, as_stream(stream)));
+}
+
+fms_status fms_adamw_step(int64_t count, const fms_adamw_tensor* tensors, int64_t step, double lr,
+                          double beta1, double beta2, double eps, double weight_decay,
+                          double grad_scale, void* stream) {
+  if (count < 0 || (count > 0 && !tensors) || step < 1) return FMS_EINVAL;
+  // (negated: a NaN is refused too)
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return FMS_EINVAL;
+  for (int64_t i = 0; i < count; ++i) {
+    const fms_adamw_tensor& t = tensors[i];
+    if (elem_bytes(t.p_dtype) == 0 || elem_bytes(t.g_dtype) == 0) return FMS_EUNSUPPORTED;
+    if (t.n < 0 || (t.m_scale == nullptr) != (t.v_scale == nullptr)) return FMS_EINVAL;
+    if (t.n > 0 && (!t.p || !t.g || !t.m || !t.v)) return FMS_EINVAL;
+    if (t.n > ((int64_t)1 << 33)) return FMS_EUNSUPPORTED;
+  }
+  AdamWStep s;
+  s.beta1 = (float)beta1;
+  s.rest1 = (float)(1.0 - beta1);
+  s.beta2 = (float)beta2;
+  s.rest2 = (float)(1.0 - beta2);
+  s.eps = (float)eps;
+  s.decay = (float)(1.0 - lr * weight_decay);
+  s.lr = (float)(lr / (1.0 - pow(beta1, (double)step)));
+  s.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+  s.grad_scale = (float)grad_scale;
+  return from_hip(adamw_step(count, tensors, s, as_stream(stream)));
+}
+
+fms_status fms_moment_values(int64_t count, const fms_moment8* moments, void* stream) {
+  if (count < 0 || (count > 0 && !moments)) return FMS_EINVAL;
+  for (int64_t i = 0; i < count; ++i) {
+    const fms_moment8& t = moments[i];
+    if (t.n < 0 || (t.n > 0 && (!t.codes || !t.scales || !t.values))) return FMS_EINVAL;
+    if (t.n > ((int64_t)1 << 33)) return FMS_EUNSUPPORTED;
+  }
+  return from_hip(moment_values(count, moments, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -423,11 +423,11 @@ void workspace_lender(WorkspaceLender lender) { t_lender = lender; }
 
 uint64_t workspace_alloc_count() { return g_workspace_allocs.load(std::memory_order_relaxed); }
 
-hipError_t workspace_alloc(void** ptr, size_t bytes, hipStream_t stream) {
+hipError_t workspace_alloc(void** ptr, size_t bytes, hipStream_t stream, bool captured) {
   g_workspace_allocs.fetch_add(1, std::memory_order_relaxed);
   if (t_lender != nullptr && t_nlent < kMaxLent) {
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusActive;
-    if (hipStreamIsCapturing(stream, &cap) != hipSuccess) {
+    hipStreamCaptureStatus cap = captured ? hipStreamCaptureStatusNone : hipStreamCaptureStatusActive;
+    if (!captured && hipStreamIsCapturing(stream, &cap) != hipSuccess) {
       (void)hipGetLastError();
       cap = hipStreamCaptureStatusActive;
     }

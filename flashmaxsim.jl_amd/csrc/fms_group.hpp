@@ -48,9 +48,11 @@ hipError_t stream_device(hipStream_t stream, int* dev);
 // Stream-ordered workspace from a library-owned memory pool of the stream's
 // device (created on first use, kept for the life of the process so repeated
 // calls do not return memory to the driver between synchronisations).
-hipError_t workspace_alloc(void** ptr, size_t bytes, hipStream_t stream);
+// `captured`: the call may ask the lender under graph capture too, and the memory is the
+// graph's from then on.
+hipError_t workspace_alloc(void** ptr, size_t bytes, hipStream_t stream, bool captured = false);
 // This host thread's lender (null: none), asked first for every workspace outside graph
-// capture; workspace_free of what it gave does nothing.
+// capture (and under it where the call says so); workspace_free of what it gave does nothing.
 typedef void* (*WorkspaceLender)(int64_t bytes, void* stream);
 void workspace_lender(WorkspaceLender lender);
 // Number of workspace_alloc calls so far in this process (a test probe).

@@ -14,6 +14,8 @@ torch tensor of shape ``(c, b, a)`` (row-major) -- the same bytes.  So
 from .api import AtomicUnified, InBatch, InvGrid, MaxSim, dot_accum, maxsim, score_eltype
 from .backward import (candidates_pullback, inbatch_pullback, packed_pullback, pair_pullback,
                        paired_pullback, varlen_pullback)
+from .block import (block_norm, block_norm_forward, block_norm_pullback, gated_ffn,
+                    gated_ffn_forward, gated_ffn_pullback)
 from .boundary import (inbatch_device_scan, launch_candidates_scan, launch_int8_candidates_scan,
                        launch_int8_pair_scan, launch_int8_paired_scan, launch_packed_scan,
                        launch_pair_scan, launch_paired_scan, launch_varlen_scan,
@@ -22,6 +24,7 @@ from .errors import ArgumentError, DimensionMismatch, HIPError, UnsupportedError
 from .forward import (candidates_forward, inbatch_forward, int8_candidates_forward,
                       int8_pair_forward, int8_paired_forward, packed_forward,
                       packed_multi_forward, paired_forward, pair_forward, topk, varlen_forward)
+from .optim import AdamW, Moment8, moment_values
 from .packed import PackedSeq, nseq, pack_docs, pack_pairs
 from .quant import (Int8Index, dequant_int8, load_int8_index, quantize_int8_symmetric,
                     save_int8_index)
@@ -36,6 +39,8 @@ __all__ = [
     "int8_candidates_forward", "topk",
     "pair_pullback", "paired_pullback", "inbatch_pullback", "candidates_pullback",
     "packed_pullback", "varlen_pullback", "rrule", "MaxSimFunction",
+    "gated_ffn", "gated_ffn_forward", "gated_ffn_pullback",
+    "block_norm", "block_norm_forward", "block_norm_pullback", "AdamW", "Moment8", "moment_values",
     "launch_pair_scan", "launch_paired_scan", "launch_candidates_scan", "inbatch_device_scan",
     "launch_packed_scan", "launch_varlen_scan", "launch_int8_pair_scan",
     "launch_int8_paired_scan", "launch_int8_candidates_scan", "tensor_cores_active",

@@ -26,7 +26,20 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f = ctypes.c_float
+_d = ctypes.c_double
 LENDER = ctypes.CFUNCTYPE(_p, _i64, _p)  # fms_workspace_lender: (bytes, stream) -> memory
+
+
+class AdamWEntry(ctypes.Structure):
+    """fms_adamw_tensor"""
+    _fields_ = [("p", _p), ("g", _p), ("m", _p), ("v", _p), ("master", _p), ("m_scale", _p),
+                ("v_scale", _p), ("n", _i64), ("p_dtype", _i32), ("g_dtype", _i32)]
+
+
+class Moment8Entry(ctypes.Structure):
+    """fms_moment8"""
+    _fields_ = [("codes", _p), ("scales", _p), ("values", _p), ("n", _i64), ("is_signed", _i64)]
+
 
 # name -> argtypes (restype fms_status = int32 unless listed in _RESTYPES)
 SIGNATURES = {
@@ -74,6 +87,13 @@ SIGNATURES = {
     "fms_packed_pullback": [_i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p],
     "fms_varlen_pullback": [_i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                             _p],
+    "fms_gated_ffn": [_i32, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _p],
+    "fms_gated_ffn_pullback": [_i32, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _p],
+    "fms_block_norm": [_i32, _p, _p, _p, _p, _p, _p, _p, _i32, _f, _f, _i64, _i64, _i64, _p],
+    "fms_block_norm_pullback": [_i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _f, _f,
+                                _i64, _i64, _i64, _p],
+    "fms_adamw_step": [_i64, _p, _i64, _d, _d, _d, _d, _d, _d, _p],
+    "fms_moment_values": [_i64, _p, _p],
 }
 _RESTYPES = {
     "fms_status_string": ctypes.c_char_p,

@@ -25,6 +25,9 @@ package (Julia ``(dim, T, B)`` == torch ``(B, T, dim)``).
 | candidates_apply_pullback | candidates_apply_pullback! (backward_layouts.jl:187-202)|
 | packed_apply_pullback     | packed_apply_pullback!   (packed.jl:384-417)         |
 | varlen_apply_pullback     | varlen_apply_pullback!   (packed.jl:449-485)         |
+| launch_gated_ffn, gated_ffn_apply_pullback     | (no reference method; block.py) |
+| launch_block_norm, block_norm_apply_pullback   | (no reference method; block.py) |
+| adamw_step, moment_values                      | (no reference method; optim.py) |
 
 The pullbacks overwrite their gradient outputs in full (the reference
 accumulates into zeros_like buffers); all of them run the InvGrid form
@@ -115,7 +118,8 @@ def _norm(normalize) -> int:
 # memory instead: the library asks for what the call needs (_lend), the pieces come
 # from the caching allocator on the call's stream and go back to it, to be reused
 # in stream order, when the call returns.  Whatever _lend declines, and every
-# allocation under graph capture, comes from the library's pool.
+# allocation under graph capture, comes from the library's pool.  (The token block's
+# calls are lent memory under capture too: torch's allocator takes it from the graph's own.)
 
 class _Call:
     """The call a thread is in: its device and the pieces lent to it."""
@@ -644,3 +648,105 @@ def varlen_apply_pullback(dQ, dD, Qp, Dp, cu_q, cu_d, args, Delta, inv_n):
         ptr(_tape(args)), ptr(Delta), ptr(inv_n), dim, max_q, N, Qp.shape[0], Dp.shape[0],
         stream_handle(dev))
     _lib.check(st, "varlen_apply_pullback")
+
+
+# ---- token block (no reference method) --------------------------------------------------
+
+def _rows(x):
+    dim = x.shape[-1]
+    return (x.numel() // dim if dim else x.shape[:-1].numel()), dim
+
+
+def _same(t, shape, proto, what):
+    """A feature array of an exact shape and the call's eltype."""
+    if t.dtype != proto.dtype:
+        raise ArgumentError(f"{what} must have the feature eltype {proto.dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise DimensionMismatch(f"{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def launch_gated_ffn(h, x, wg, wu, act):
+    """h <- act(x wg^T) * (x wu^T); act is the library's code."""
+    dev = require_device(h, x, wg, wu)
+    rows, dim = _rows(x)
+    hidden = wg.shape[0]
+    for w, what in ((wg, "wg"), (wu, "wu")):
+        _same(w, (hidden, dim), x, what)
+    _same(h, x.shape[:-1] + (hidden,), x, "h")
+    st = _call_with_workspace(_lib.lib().fms_gated_ffn, dev, dtype_code(x), ptr(h), ptr(x), ptr(wg),
+                              ptr(wu), act, rows, dim, hidden, stream_handle(dev))
+    _lib.check(st, "launch_gated_ffn")
+
+
+def gated_ffn_apply_pullback(dx, dwg, dwu, dh, x, wg, wu, act):
+    """dx, dwg, dwu <- pullback of dh; dx, or dwg and dwu, may be None."""
+    dev = require_device(dx, dwg, dwu, dh, x, wg, wu)
+    rows, dim = _rows(x)
+    hidden = wg.shape[0]
+    for w, what in ((wg, "wg"), (wu, "wu"), (dwg, "dwg"), (dwu, "dwu")):
+        if w is not None:
+            _same(w, (hidden, dim), x, what)
+    if dx is not None:
+        _same(dx, x.shape, x, "dx")
+    _same(dh, x.shape[:-1] + (hidden,), x, "dh")
+    st = _call_with_workspace(_lib.lib().fms_gated_ffn_pullback, dev, dtype_code(x), ptr(dx),
+                              ptr(dwg), ptr(dwu), ptr(dh), ptr(x), ptr(wg), ptr(wu), act, rows, dim,
+                              hidden, stream_handle(dev))
+    _lib.check(st, "gated_ffn_apply_pullback")
+
+
+def _norm_arrays(x, gate_rows, gate, *groups):
+    """Checks block_norm's arrays: groups of (shape, arrays with their names)."""
+    rows, dim = _rows(x)
+    if gate_rows < 1 or (gate is not None and rows % gate_rows != 0):
+        raise DimensionMismatch(f"{rows} rows in gates of {gate_rows}")
+    for shape, arrays in groups:
+        for t, what in arrays:
+            if t is not None:
+                _same(t, shape, x, what)
+    if gate is not None and rows > 0 and gate.numel() != rows // gate_rows * dim:
+        raise DimensionMismatch(f"gate: {gate.numel()} elements for {rows // gate_rows} gates")
+    return rows, dim
+
+
+def launch_block_norm(r, n, x, f, gate, wpost, wpre, kind, scale, eps, gate_rows):
+    """r, n <- x + scale gate norm(f) wpost, norm(r) wpre; kind is the library's code."""
+    dev = require_device(r, n, x, f, gate, wpost, wpre)
+    rows, dim = _norm_arrays(x, gate_rows, gate, (x.shape, ((r, "r"), (n, "n"), (f, "f"))),
+                             (x.shape[-1:], ((wpost, "post_weight"), (wpre, "pre_weight"))))
+    if gate is not None:
+        _same(gate, gate.shape, x, "gate")
+    st = _lib.lib().fms_block_norm(dtype_code(x), ptr(r), ptr(n), ptr(x), ptr(f), ptr(gate),
+                                   ptr(wpost), ptr(wpre), kind, scale, eps, rows, dim, gate_rows,
+                                   stream_handle(dev))
+    _lib.check(st, "launch_block_norm")
+
+
+def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre, kind,
+                              scale, eps, gate_rows):
+    dev = require_device(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre)
+    rows, dim = _norm_arrays(
+        x, gate_rows, gate,
+        (x.shape, ((dx, "dx"), (df, "df"), (dr, "dr"), (dn, "dn"), (f, "f"))),
+        (x.shape[-1:], ((wpost, "post_weight"), (wpre, "pre_weight"), (dwpost, "dpost_weight"),
+                        (dwpre, "dpre_weight"))))
+    if gate is not None:
+        _same(gate, gate.shape, x, "gate")
+        _same(dgate, gate.shape, x, "dgate")
+    st = _call_with_workspace(
+        _lib.lib().fms_block_norm_pullback, dev, dtype_code(x), ptr(dx), ptr(df), ptr(dgate),
+        ptr(dwpost), ptr(dwpre), ptr(dr), ptr(dn), ptr(x), ptr(f), ptr(gate), ptr(wpost), ptr(wpre),
+        kind, scale, eps, rows, dim, gate_rows, stream_handle(dev))
+    _lib.check(st, "block_norm_apply_pullback")
+
+
+def adamw_step(table, step, lr, betas, eps, weight_decay, grad_scale, dev):
+    """One step over a table of the library's entries, whose arrays the caller has checked."""
+    st = _lib.lib().fms_adamw_step(len(table), table, step, lr, betas[0], betas[1], eps, weight_decay,
+                                   grad_scale, stream_handle(dev))
+    _lib.check(st, "adamw_step")
+
+
+def moment_values(table, dev):
+    """Values of a table of 8-bit moments, whose arrays the caller has checked."""
+    _lib.check(_lib.lib().fms_moment_values(len(table), table, stream_handle(dev)), "moment_values")

@@ -1,0 +1,181 @@
+"""AdamW over many tensors at once, with its moments in 32 or in 8 bits.
+
+The step that uses MaxSim's gradients (extension; the reference leaves the optimiser to its
+caller).  All tensors of a step go through one kernel, up to 48 a launch, in place:
+
+    m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+    p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+in fp32.  With fp32 masters beside 16-bit parameters the step works on the masters and the
+parameters become their roundings.
+
+8-bit moments (``Moment8``) hold a code for each element and an fp32 scale for every 256
+neighbouring elements, the largest magnitude among them: m as int8 codes with the value
+sign(c) (c/127)^2 scale, v as uint8 codes with the value (c/255)^4 scale.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib, boundary
+from .errors import ArgumentError, DimensionMismatch
+
+MOMENT_BLOCK = 256
+
+
+class Moment8:
+    """A moment in 8 bits: ``codes`` (int8 for m, uint8 for v) in the parameter's shape and
+    ``scales``, one float32 for each 256 of its elements in memory order."""
+
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype not in (torch.int8, torch.uint8):
+            raise ArgumentError(f"moment codes are int8 or uint8, got {codes.dtype}")
+        if scales.dtype != torch.float32:
+            raise ArgumentError(f"moment scales are float32, got {scales.dtype}")
+        if scales.numel() != -(-codes.numel() // MOMENT_BLOCK):
+            raise DimensionMismatch(f"{scales.numel()} moment scales for {codes.numel()} codes")
+        self.codes, self.scales = codes, scales
+
+    @classmethod
+    def zeros(cls, p: torch.Tensor, signed: bool) -> "Moment8":
+        """The moment of a first step: m (signed) or v of the parameter p."""
+        return cls(torch.zeros(p.shape, dtype=torch.int8 if signed else torch.uint8, device=p.device),
+                   torch.zeros(-(-p.numel() // MOMENT_BLOCK), dtype=torch.float32, device=p.device))
+
+    def __repr__(self):
+        return f"Moment8(codes={tuple(self.codes.shape)} {self.codes.dtype})"
+
+
+def moment_values(moments, out=None):
+    """The float32 values of Moment8s, many at once; ``out``: tensors to write them to."""
+    moments = list(moments)
+    if out is None:
+        out = [torch.empty(m.codes.shape, dtype=torch.float32, device=m.codes.device)
+               for m in moments]
+    out = list(out)
+    if len(out) != len(moments):
+        raise DimensionMismatch(f"{len(out)} outputs for {len(moments)} moments")
+    if not moments:
+        return out
+    dev = boundary.require_device(*(t for m in moments for t in (m.codes, m.scales)), *out)
+    table = (_lib.Moment8Entry * len(moments))()
+    for e, m, o in zip(table, moments, out):
+        if o.dtype != torch.float32:
+            raise ArgumentError(f"moment values are float32, got {o.dtype}")
+        if o.numel() != m.codes.numel():
+            raise DimensionMismatch(f"{o.numel()} values for {m.codes.numel()} codes")
+        e.codes, e.scales, e.values = m.codes.data_ptr(), m.scales.data_ptr(), o.data_ptr()
+        e.n, e.is_signed = o.numel(), int(m.codes.dtype == torch.int8)
+    boundary.moment_values(table, dev)
+    return out
+
+
+class AdamW:
+    """AdamW over a list of parameters.
+
+    bits: 32 (float32 moments) or 8 (``Moment8``); masters: True to keep float32 copies of
+    16-bit parameters, or a list of them (None where a parameter has none); moments: a pair
+    of lists (m, v) to go on from, with ``step`` the steps already taken."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32,
+                 masters=None, moments=None, step=0):
+        self.params = list(params)
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
+        self.steps = int(step)
+        if bits not in (8, 32):
+            raise ArgumentError(f"moments are held in 32 or in 8 bits, got {bits!r}")
+        b1, b2 = self.betas
+        if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and self.steps >= 0):
+            raise ArgumentError(f"AdamW: betas {self.betas}, eps {eps}, step {step}")
+        self._device = boundary.require_device(*self.params)
+        codes = [boundary.dtype_code(p) for p in self.params]
+        if moments is None:
+            if bits == 8:
+                moments = ([Moment8.zeros(p, True) for p in self.params],
+                           [Moment8.zeros(p, False) for p in self.params])
+            else:
+                moments = tuple([torch.zeros_like(p, dtype=torch.float32) for p in self.params]
+                                for _ in range(2))
+        self.m, self.v = tuple(moments[0]), tuple(moments[1])
+        if masters is True:
+            masters = [None if p.dtype == torch.float32 else p.detach().float() for p in self.params]
+        self.masters = (None,) * len(self.params) if not masters else tuple(masters)
+        if not len(self.params) == len(self.m) == len(self.v) == len(self.masters):
+            raise DimensionMismatch("AdamW: as many moments and masters as parameters")
+        self._shapes = [(p.numel(), p.dtype) for p in self.params]
+        # the table of the library; a step fills in where parameters and gradients lie
+        self._held = self.m, self.v, self.masters  # what its other addresses belong to
+        self._table = (_lib.AdamWEntry * len(self.params))()
+        for e, p, c, m, v, w in zip(self._table, self.params, codes, self.m, self.v, self.masters):
+            e.n, e.p_dtype = p.numel(), c
+            self._place(e, p, m, v, w)
+
+    def _place(self, e, p, m, v, master):
+        if isinstance(m, Moment8) != isinstance(v, Moment8):
+            raise ArgumentError("AdamW: both moments of a parameter in 32 or both in 8 bits")
+        if isinstance(m, Moment8):
+            boundary.require_device(p, m.codes, m.scales, v.codes, v.scales)
+            if m.codes.dtype != torch.int8 or v.codes.dtype != torch.uint8:
+                raise ArgumentError("AdamW: m has int8 codes and v uint8 codes")
+            e.m_scale, e.v_scale = m.scales.data_ptr(), v.scales.data_ptr()
+            m, v = m.codes, v.codes
+        else:
+            boundary.require_device(p, m, v)
+            if m.dtype != torch.float32 or v.dtype != torch.float32:
+                raise ArgumentError("AdamW: moments are float32 or Moment8")
+        if not m.numel() == v.numel() == p.numel():
+            raise DimensionMismatch("AdamW: the moments have their parameter's size")
+        e.m, e.v = m.data_ptr(), v.data_ptr()
+        if master is not None:
+            boundary.require_device(p, master)
+            if master.dtype != torch.float32:
+                raise ArgumentError("AdamW: masters are float32")
+            if master.numel() != p.numel():
+                raise DimensionMismatch("AdamW: a master has its parameter's size")
+            e.master = master.data_ptr()
+
+    def step(self, grads=None, lr=None, grad_scale=1.0):
+        """One step, in place.  grads: one per parameter, None to leave it as it is (default: the
+        parameters' .grad); lr: instead of the optimiser's; grad_scale: multiplies the
+        gradients (loss scaling, clipping)."""
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise DimensionMismatch(f"{len(grads)} gradients for {len(self.params)} parameters")
+        table, params = self._table, self.params
+        if [(p.numel(), p.dtype) for p in params] != self._shapes:
+            raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
+        if any(g is None for g in grads):
+            keep = [i for i, g in enumerate(grads) if g is not None]
+            params, grads = [params[i] for i in keep], [grads[i] for i in keep]
+            table = (_lib.AdamWEntry * len(keep))(*(table[i] for i in keep))
+        if not grads:
+            return
+        if boundary.require_device(*params, *grads) != self._device:
+            raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+        for e, p, g in zip(table, params, grads):
+            if g.numel() != e.n:
+                raise DimensionMismatch("AdamW: a gradient has its parameter's size")
+            e.p, e.g, e.g_dtype = p.data_ptr(), g.data_ptr(), boundary.dtype_code(g)
+        boundary.adamw_step(table, self.steps + 1, self.lr if lr is None else lr, self.betas,
+                            self.eps, self.weight_decay, grad_scale, self._device)
+        self.steps += 1
+        torch.autograd.graph.increment_version(params)
+
+    def moment_values(self, out=None):
+        """(m, v) as float32 lists; out: such a pair to write the values of 8-bit moments to."""
+        both = self.m + self.v
+        to = [None] * len(both) if out is None else list(out[0]) + list(out[1])
+        at = [i for i, m in enumerate(both) if isinstance(m, Moment8)]
+        got = moment_values([both[i] for i in at], None if out is None else [to[i] for i in at])
+        values = list(both)
+        for i, t in zip(at, got):
+            values[i] = t
+        return values[:len(self.m)], values[len(self.m):]
+
+    def __repr__(self):
+        bits = "8" if self.m and isinstance(self.m[0], Moment8) else "32"
+        return f"AdamW({len(self.params)} tensors, {bits}-bit moments, step {self.steps})"

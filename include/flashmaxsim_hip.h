@@ -72,6 +72,15 @@ typedef int32_t fms_status;
 #define FMS_F16 1
 #define FMS_BF16 2
 
+/* Activations of fms_gated_ffn. */
+#define FMS_ACT_SILU 0      /* g / (1 + exp(-g)) */
+#define FMS_ACT_GELU 1      /* g (1 + erf(g / sqrt 2)) / 2 */
+#define FMS_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2 */
+
+/* Norms of fms_block_norm. */
+#define FMS_NORM_RMS 0   /* a / sqrt(mean(a^2) + eps) */
+#define FMS_NORM_LAYER 1 /* (a - mean(a)) / sqrt(mean((a - mean(a))^2) + eps) */
+
 /* Human-readable text for a status code (static storage). */
 const char* fms_status_string(fms_status s);
 
@@ -432,6 +441,95 @@ fms_status fms_varlen_pullback(int32_t dtype, void* dQ, void* dD, const void* Qt
                                int64_t nd_tokens, void* stream);
 
 /*
+ * ---- Token block (extension; no reference counterpart) -----------------------------
+ * Operators around the scans: the block that makes token embeddings out of an encoder's
+ * token states, and the optimiser step on its weights.  The conventions above hold
+ * (outputs first, asynchronous, features of `dtype`, fp32 sums).  Matrices are given with
+ * the last index contiguous: x (tokens, dim) is Julia's (dim, tokens).
+ */
+
+/*
+ * Gated feed-forward block, both projections, activation and product in one kernel:
+ *   h[t, j] = act(sum_k x[t, k] wg[j, k]) * sum_k x[t, k] wu[j, k]
+ * x (tokens, dim), wg and wu (hidden, dim), h (tokens, hidden).  Any sizes and
+ * alignments; rows that are no whole 16-byte units are copied into workspace first.
+ */
+fms_status fms_gated_ffn(int32_t dtype, void* h, const void* x, const void* wg, const void* wu,
+                         int32_t act, int64_t tokens, int64_t dim, int64_t hidden, void* stream);
+
+/*
+ * Its pullback for the cotangent dh (tokens, hidden): dx (tokens, dim), dwg and dwu
+ * (hidden, dim), each overwritten in full.  dx, or dwg and dwu together, may be NULL when
+ * not wanted.  The projections are computed again (nothing is kept from the forward); dg
+ * and du are rounded once to `dtype` between the products.  Deterministic.
+ */
+fms_status fms_gated_ffn_pullback(int32_t dtype, void* dx, void* dwg, void* dwu, const void* dh,
+                                  const void* x, const void* wg, const void* wu, int32_t act,
+                                  int64_t tokens, int64_t dim, int64_t hidden, void* stream);
+
+/*
+ * Norms before and after a block, fused with its gate and residual:
+ *   z = norm(f) * wpost   (f itself without wpost)
+ *   r = x + scale * gate * z
+ *   n = norm(r) * wpre
+ * x, f, r and n are (rows, dim), the weights (dim,), gate (rows / gate_rows, dim): each
+ * vector of it serves gate_rows neighbouring rows.  f, gate, wpost and wpre may be NULL:
+ * without f, r is x and not written (gate and wpost are then NULL too); without gate it is
+ * 1; without wpre there is no n.  dim is at most 16384.
+ */
+fms_status fms_block_norm(int32_t dtype, void* r, void* n, const void* x, const void* f,
+                          const void* gate, const void* wpost, const void* wpre, int32_t kind,
+                          float scale, float eps, int64_t rows, int64_t dim, int64_t gate_rows,
+                          void* stream);
+
+/*
+ * Its pullback for the cotangents dr and dn (either may be NULL: zero; dn only with
+ * wpre).  dx and, where the input they belong to was given, df, dgate, dwpost and dwpre are
+ * overwritten in full.  Deterministic.
+ */
+fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgate, void* dwpost,
+                                   void* dwpre, const void* dr, const void* dn, const void* x,
+                                   const void* f, const void* gate, const void* wpost,
+                                   const void* wpre, int32_t kind, float scale, float eps,
+                                   int64_t rows, int64_t dim, int64_t gate_rows, void* stream);
+
+/*
+ * One AdamW step over many tensors at once, in place.  In fp32, t = step counted from 1:
+ *   g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * With a master, p is computed from and to it, and the parameter is its rounding.  m and v
+ * are n floats each, or, with m_scale and v_scale (both), n codes each (int8 / uint8) and a
+ * float for every FMS_MOMENT_BLOCK elements:
+ *   m = sign(c) (c / 127)^2 scale,  v = (c / 255)^4 scale
+ * The table is read before the call returns.
+ */
+#define FMS_MOMENT_BLOCK 256
+typedef struct fms_adamw_tensor {
+  void* p;       /* n values of p_dtype */
+  const void* g; /* n values of g_dtype */
+  void* m;
+  void* v;
+  float* master;  /* n floats or NULL */
+  float* m_scale; /* ceil(n / FMS_MOMENT_BLOCK) floats or NULL */
+  float* v_scale;
+  int64_t n;
+  int32_t p_dtype, g_dtype;
+} fms_adamw_tensor;
+fms_status fms_adamw_step(int64_t count, const fms_adamw_tensor* tensors, int64_t step, double lr,
+                          double beta1, double beta2, double eps, double weight_decay,
+                          double grad_scale, void* stream);
+
+/* The values of 8-bit moments, many at once: is_signed 1 for m's codes, 0 for v's. */
+typedef struct fms_moment8 {
+  const void* codes;
+  const float* scales;
+  float* values; /* n floats */
+  int64_t n;
+  int64_t is_signed;
+} fms_moment8;
+fms_status fms_moment_values(int64_t count, const fms_moment8* moments, void* stream);
+
+/*
  * Test-only: MFMA accumulator layout probe (no reference counterpart).  Runs
  * one 32x32 MFMA of the given feature type (FMS_F32 / FMS_F16 / FMS_BF16, or
  * 3 = int8) twice -- A[i][0] = i+1, B[0][j] = 1, then A[i][0] = 1,
@@ -460,7 +558,9 @@ fms_status fms_debug_cross_lane(float* out, void* stream);
  * `stream` before the call returns, and none of it is used by a later call: the
  * owner may reuse it in stream order from then on.  The lender belongs to the
  * calling host thread (NULL: none, the default), may be asked several times by a
- * call, and is not asked while the stream is being captured.
+ * call, and is not asked while the stream is being captured -- except by the token
+ * block's calls, which take no memory from the pool then: what it lends to a captured
+ * call belongs to the graph as long as that is replayed (NULL fails the call).
  */
 typedef void* (*fms_workspace_lender)(int64_t bytes, void* stream);
 void fms_set_workspace_lender(fms_workspace_lender lender);
