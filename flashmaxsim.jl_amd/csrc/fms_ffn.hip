@@ -198,7 +198,7 @@ __device__ __forceinline__ void gate_epilogue(const typename P::Acc (&acc)[2][P:
 
 // Forward (kPull false): h.  Pullback: dg and du, their rows filled up with zeros to out_cols.
 template <class P, bool kPull>
-__global__ void __launch_bounds__(P::kThreads, P::kThreads / 256) ffn_gate_kernel(GateArgs A) {
+__global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
   typedef typename P::Op Op;
   typedef typename OutOf<Op>::T T;
   constexpr int kCols = P::kBN / 2;
@@ -241,7 +241,7 @@ struct ProductArgs {
 };
 
 template <class P>
-__global__ void __launch_bounds__(P::kThreads, P::kThreads / 256) ffn_product_kernel(ProductArgs A) {
+__global__ void __launch_bounds__(P::kThreads, 2) ffn_product_kernel(ProductArgs A) {
   typedef typename P::Op Op;
   typedef typename OutOf<Op>::T T;
   typedef LdsTile<Op, P::kBM, P::kBN, P::kThreads> Tile;

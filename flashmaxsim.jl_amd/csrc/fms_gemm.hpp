@@ -1,23 +1,28 @@
 // fms_gemm.hpp -- device building blocks of the products behind the gated
 // feed-forward block (fms_ffn.hip): out[m][n] = sum_k M(m, k) * N(n, k).
 //
-// A workgroup owns a kBM x kBN tile of the output and walks k in steps of
-// 128 bytes per row.  Each step's slices of both operands go HBM/L2 -> LDS
-// directly (buffer loads with an LDS destination, no registers), into the
-// half of a double buffer that the step before left free; the MFMAs of a step
-// run while the next step's slices are in flight.
+// A workgroup owns a kBM x kBN tile of the output and walks k in steps of 128
+// bytes per row.  Each step's slices of both operands go HBM/L2 -> LDS directly
+// (buffer loads with an LDS destination, no registers) into one of two buffers
+// while the step before is multiplied.  Two schedules:
+//   four waves: small tiles, two workgroups to a CU; one's MFMAs run while the
+//     other waits at its barrier or is in its epilogue.
+//   eight waves, two to a SIMD: the first four and the last four take turns.  While
+//     one half multiplies two of a step's four k groups, the other reads the
+//     fragments of its next two, and a barrier swaps them: the matrix cores see one
+//     wave after the other without a gap, and no wave waits for LDS in between.
 //
 // An operand's matrix lies in memory either with k contiguous (a row per m or
 // n: "rows") or with m / n contiguous (a row per k: "columns").  Both land in
 // LDS as they lie, in 16-byte units:
-//   rows:    kSpan rows of 128 bytes; the unit u of row r is at r*8 + (u ^ (r & 7)).
+//   rows:    kSpan rows of 128 bytes; the unit u of row r is at r*8 + (u ^ ((r >> 1) & 7)).
 //   columns: 128 / kEsz rows (k) of kSpan elements; unit u of row r is at
 //            r*kUpr + (u ^ (4 * (r & 3))).
-// The exclusive-or spreads the rows that one read touches over the banks.  An
-// LDS load's destination is linear in the lane, so it is the lane's global
-// address that is permuted.  16-bit columns are read with the transposing LDS
-// read (four k of one column per lane from a 4 x 16 block that sixteen lanes
-// hold), 32-bit columns need none.
+// The exclusive-or spreads the rows that sixteen lanes read together over all
+// 64 banks.  An LDS load's destination is linear in the lane, so it is the
+// lane's global address that is permuted.  16-bit columns are read with the
+// transposing LDS read (four k of one column per lane from a 4 x 16 block that
+// sixteen lanes hold), 32-bit columns need none.
 //
 // Every load is bounds-checked by its buffer resource: rows past the matrix'
 // end read as zero, and units past a row's end are sent out of bounds.
@@ -31,6 +36,7 @@ typedef __attribute__((address_space(3))) void* lds_void_ptr;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStepBytes = 128;            // k bytes of a row per step
+constexpr int kGroups = 4;                 // fragments of k per step
 constexpr int kOutOfBounds = (int)0x80000000u;  // an offset past every resource
 
 // A matrix as a product's operand: `rows` rows of `rowbytes` used bytes (a
@@ -58,58 +64,83 @@ struct Stage {
   static constexpr int kUnits = kBytes / 16;
   static constexpr int kLoads = kUnits / kThreads;         // per thread and step
   static constexpr int kStepK = kStepBytes / Op::kEsz;     // k values per step
-  static constexpr int kUpr = kRows ? 8 : kSpan * Op::kEsz / 16;  // units per LDS row
+  static constexpr int kUpr = kRows ? kStepBytes / 16 : kSpan * Op::kEsz / 16;  // units per LDS row
   static_assert(kUnits % (kThreads * kParts) == 0, "whole loads per part");
   static_assert(kRows || kParts == 1, "two parts only of rows");
   static_assert(kRows || kUpr >= 16, "the swizzle spans 16 units");
 
-  int voff[kLoads];   // this lane's offsets into the resource
-  int unit[kLoads];   // rows: the byte of the row's step its unit starts at
-
-  __device__ __forceinline__ void init(int tid, int64_t pitch) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int u = i * kThreads + tid;
-      const int row = u / kUpr, phys = u % kUpr;
-      const int log = kRows ? phys ^ (row & 7) : phys ^ (4 * (row & 3));
-      unit[i] = log * 16;
-      const int part_row = kRows ? row % (kSpan / kParts) : row;
-      voff[i] = (int)((int64_t)part_row * pitch) + log * 16;
-    }
+  // What unit indices of LDS row r are exclusive-or'ed with.
+  __device__ static __forceinline__ int mix(int r) {
+    return kRows ? (r >> 1) & 7 : 4 * (r & 3);
   }
 
-  // Requests step `step` of the tile at m/n = first into `lds`.
-  __device__ __forceinline__ void load(const Matrix (&mat)[kParts], int64_t first, int step,
-                                       char* lds, int wave) const {
+  int voff[kLoads];  // this lane's offsets into the resource
+  // the next step's slice: where it starts and what is left of the matrix from there
+  const char* base[kParts];
+  int64_t left[kParts];
+  int64_t stride;  // bytes from a step's start to the next one's
+  int rest;        // rows: bytes of a row from the next step on
+
+  __device__ __forceinline__ void init(int tid, const Matrix (&mat)[kParts], int64_t first, int step) {
+    stride = kRows ? kStepBytes : (int64_t)kStepK * mat[0].pitch;
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
       const Matrix& m = mat[p];
-      int64_t at;
-      int tail = kStepBytes;  // rows: used bytes of this step
-      if constexpr (kRows) {
-        at = first * m.pitch + (int64_t)step * kStepBytes;
-        const int64_t left = m.rowbytes - (int64_t)step * kStepBytes;
-        tail = left < kStepBytes ? (int)left : kStepBytes;
-      } else {
-        at = (int64_t)step * kStepK * m.pitch + first * Op::kEsz;
-      }
-      const rsrc_t r = matrix_from(m, at);
+      const int64_t at = step * stride + first * (kRows ? m.pitch : (int64_t)Op::kEsz);
+      base[p] = reinterpret_cast<const char*>(rfl64(reinterpret_cast<uint64_t>(m.base + at)));
+      left[p] = (int64_t)rfl64((uint64_t)((m.rows - 1) * m.pitch + m.rowbytes - at));
+    }
+    const int64_t r = mat[0].rowbytes - step * stride;
+    rest = !kRows || r > 0x7fffffff ? 0x7fffffff : (int)r;
 #pragma unroll
-      for (int i = p * kLoads / kParts; i < (p + 1) * kLoads / kParts; ++i) {
-        const int off = (kRows && unit[i] >= tail) ? kOutOfBounds : voff[i];
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (lds_void_ptr)(lds + (i * kThreads + wave * 64) * 16), 16, off, 0, 0, 0);
-      }
+    for (int i = 0; i < kLoads; ++i) {
+      const int u = i * kThreads + tid;
+      const int row = u / kUpr, log = (u % kUpr) ^ mix(row);
+      voff[i] = (int)((kRows ? row % (kSpan / kParts) : row) * mat[0].pitch) + log * 16;
     }
   }
 
-  // The 16-byte fragment of 32 rows / columns from `at` on, k group ks (0..3) of the
+  // Sends the units past a row's end out of bounds, before a request of its last, shorter step.
+  __device__ __forceinline__ void trim(int tid) {
+    if constexpr (kRows) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int u = i * kThreads + tid;
+        if (((u % kUpr) ^ mix(u / kUpr)) * 16 >= rest) voff[i] = kOutOfBounds;
+      }
+    }
+  }
+  __device__ __forceinline__ bool last() const { return kRows && rest < kStepBytes; }
+
+  // Requests load i of the next step's slice into `lds`.
+  __device__ __forceinline__ void load(int i, const rsrc_t (&from)[kParts], char* lds, int wave) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        from[i / (kLoads / kParts)], (lds_void_ptr)(lds + (i * kThreads + wave * 64) * 16), 16, voff[i],
+        0, 0, 0);
+  }
+  __device__ __forceinline__ void resources(rsrc_t (&r)[kParts]) const {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      const int64_t n = left[p] < 0 ? 0 : (left[p] > 0x7fffffff ? 0x7fffffff : left[p]);
+      r[p] = make_rsrc(base[p], (uint32_t)n);
+    }
+  }
+  __device__ __forceinline__ void advance() {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      base[p] += stride;
+      left[p] -= stride;
+    }
+    rest -= kRows ? kStepBytes : 0;
+  }
+
+  // The 16-byte fragment of 32 rows / columns from `at` on, k group ks of the
   // step: 16-bit, eight k from 16 ks + 8 h; 32-bit, four k from 8 ks + 4 h (h = lane / 32).
   __device__ static __forceinline__ u32x4 frag(const char* lds, int at, int ks, int lane) {
     const int h = lane >> 5;
     if constexpr (kRows) {
       const int row = at + (lane & 31);
-      return *reinterpret_cast<const u32x4*>(lds + row * 128 + (((2 * ks + h) ^ (row & 7)) * 16));
+      return *reinterpret_cast<const u32x4*>(lds + row * kStepBytes + (((2 * ks + h) ^ mix(row)) * 16));
     } else if constexpr (Op::kEsz == 2) {
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
       const int i = lane & 15;
@@ -157,8 +188,9 @@ struct Product {
   static constexpr int kBM = kWM * kMF * 32, kBN = kWN * 64;
   typedef Stage<Op, kMRows_, kBM, kThreads, 1> StageM;
   typedef Stage<Op, kNRows_, kBN, kThreads, kParts> StageN;
-  static constexpr int kHalf = StageM::kBytes + StageN::kBytes;  // one of the two buffers
-  static constexpr int kLds = 2 * kHalf;
+  static constexpr int kBuffer = StageM::kBytes + StageN::kBytes;
+  static constexpr int kLds = 2 * kBuffer;
+  static constexpr bool kTurns = kWM * kWN == 8;
   static constexpr int kStepK = StageM::kStepK;
   typedef typename Op::Acc Acc;
 
@@ -177,39 +209,117 @@ struct Product {
     const int wm = wave / kWN, wn = wave % kWN;
     StageM sm;
     StageN sn;
-    sm.init(tid, M[0].pitch);
-    sn.init(tid, N[0].pitch);
-    if (s0 < s1) {
-      sm.load(M, m0, s0, lds, wave);
-      sn.load(N, n0, s0, lds + StageM::kBytes, wave);
-    }
-    for (int s = s0; s < s1; ++s) {
-      char* cur = lds + ((s - s0) & 1) * kHalf;
-      char* nxt = lds + (((s - s0) & 1) ^ 1) * kHalf;
-      // this step's slices have landed, and every wave is done with the other buffer
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (s + 1 < s1) {
-        sm.load(M, m0, s + 1, nxt, wave);
-        sn.load(N, n0, s + 1, nxt + StageM::kBytes, wave);
+    sm.init(tid, M, m0, s0);
+    sn.init(tid, N, n0, s0);
+    // Load i of both operands' next slices into the buffer of step s, from the resources made
+    // before its first.  (A request past the last step reads zeros or values that no one uses.)
+    rsrc_t rm[1], rn[kParts];
+    const auto aim = [&] {
+      if (sm.last()) sm.trim(tid);
+      if (sn.last()) sn.trim(tid);
+      sm.resources(rm);
+      sn.resources(rn);
+    };
+    const auto load = [&](int i, int s) {
+      char* const to = lds + ((s - s0) & 1) * kBuffer;
+      if (i < StageM::kLoads)
+        sm.load(i, rm, to, wave);
+      else
+        sn.load(i - StageM::kLoads, rn, to + StageM::kBytes, wave);
+    };
+    constexpr int kLoads = StageM::kLoads + StageN::kLoads;
+    const auto request = [&](int s) {
+      aim();
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load(i, s);
+      sm.advance();
+      sn.advance();
+    };
+    // Fragments of k group g of the step in `cur`, and their products.
+    u32x4 fn[2][kNF], fm[2][kMF];
+    const auto read = [&](const char* cur, int g, int i) {
+#pragma unroll
+      for (int f = 0; f < kNF; ++f) fn[i][f] = StageN::frag(cur + StageM::kBytes, col(wn, f), g, lane);
+#pragma unroll
+      for (int f = 0; f < kMF; ++f) fm[i][f] = StageM::frag(cur, (wm * kMF + f) * 32, g, lane);
+    };
+    const auto multiply = [&](int i, int b) {
+#pragma unroll
+      for (int a = 0; a < kNF; ++a) acc[a][b] = mma_frag<Op>(fn[i][a], fm[i][b], acc[a][b]);
+    };
+    const auto multiply_all = [&](int i) {
+#pragma unroll
+      for (int b = 0; b < kMF; ++b) multiply(i, b);
+    };
+    if (s0 >= s1) return;
+    request(s0);
+    if constexpr (!kTurns) {
+      for (int s = s0; s < s1; ++s) {
+        // this step's slices have landed; every wave has its last fragments of the step before
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        turn();
+        const char* const cur = lds + ((s - s0) & 1) * kBuffer;
+        read(cur, 0, 0);
+        if (s + 1 < s1) request(s + 1);
+        if (s > s0) multiply_all(1);
+        read(cur, 1, 1);
+        multiply_all(0);
+        read(cur, 2, 0);
+        multiply_all(1);
+        read(cur, 3, 1);
+        multiply_all(0);
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      turn();
+      multiply_all(1);
+    } else {
+      // Turn p: the first half of the waves reads at even p and multiplies at odd p, the
+      // second half one turn later.  Step s0 + j is read in turns 4j .. 4j + 3, and its buffer
+      // is free from turn 4j + 4 on.  A wave requests in the one multiplying turn of each step
+      // that comes right after a buffer became free, a load after every two MFMAs: the first
+      // half step s + 1 in turn 4j + 1, the second half step s + 2 in turn 4j + 4.  Each wave
+      // waits for its requests before the barrier that ends turn 4j + 3.
+      const bool second = wave >= 4;
+      if (second) request(s0 + 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      turn();
+      if (second) turn();
+      for (int s = s0; s < s1; ++s) {
+        const char* const cur = lds + ((s - s0) & 1) * kBuffer;
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        u32x4 fn[kNF], fm[kMF];
+        for (int half = 0; half < 2; ++half) {
+          read(cur, 2 * half, 0);
+          read(cur, 2 * half + 1, 1);
+          if (half == 0) aim();
+          if (half == 1 && second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          turn();
+          const bool now = (half == 1) == second;
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int i = 0; i < kNF; ++i)
-          fn[i] = StageN::frag(cur + StageM::kBytes, col(wn, i), ks, lane);
-#pragma unroll
-        for (int i = 0; i < kMF; ++i) fm[i] = StageM::frag(cur, (wm * kMF + i) * 32, ks, lane);
-#pragma unroll
-        for (int j = 0; j < kMF; ++j)
-#pragma unroll
-          for (int i = 0; i < kNF; ++i) acc[i][j] = mma_frag<Op>(fn[i], fm[j], acc[i][j]);
+          for (int i = 0; i < 2 * kMF; ++i) {
+            multiply(i / kMF, i % kMF);
+            if (now && i < kLoads) load(i, s + 1 + half);
+          }
+          static_assert(kLoads <= 2 * kMF, "a load for every two MFMAs");
+          __builtin_amdgcn_s_setprio(0);
+          if (half == 1 && !second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          turn();
+        }
+        sm.advance();
+        sn.advance();
       }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (!second) turn();
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+
+  // The barrier between turns: nothing moves across it.
+  __device__ static __forceinline__ void turn() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
   }
 };
