@@ -228,41 +228,44 @@ __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
                 n0, A.out_vec);
 }
 
-// out[z] = sum over segments of M_s N_s, or one of its `splits` parts over k in fp32.
+// A product of the pullback.  Unit u of its tiles * splits * outputs: out[z] or, with splits,
+// a part of it over k, in fp32.
 struct ProductArgs {
   Matrix m[2], n[2];
-  int32_t segments;  // 2: out[0] = m0 n0 + m1 n1; 1: out[z] = m_z n_z (z = blockIdx.z)
-  int32_t tm, tn, steps, splits;
+  int32_t segments;  // 2: out[0] = m0 n0 + m1 n1; 1: out[z] = m_z n_z
+  int32_t outputs;
+  int32_t tm, tn, steps, splits;  // steps of all segments
   int64_t rows, cols;
   void* out[2];
   int32_t vec;
-  float* parts;  // splits > 1: (splits, gridDim.z, rows, part_pitch)
+  float* parts;  // splits > 1: (splits, outputs, rows, part_pitch)
   int64_t part_pitch;
 };
 
-template <class P>
-__global__ void __launch_bounds__(P::kThreads, 2) ffn_product_kernel(ProductArgs A) {
+template <class P, int kLds>
+__device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, char (&lds)[kLds]) {
   typedef typename P::Op Op;
   typedef typename OutOf<Op>::T T;
   typedef LdsTile<Op, P::kBM, P::kBN, P::kThreads> Tile;
-  static_assert(Tile::kBytes <= P::kLds, "the output tile reuses the LDS");
-  __shared__ __attribute__((aligned(16))) char lds[P::kLds];
+  static_assert(Tile::kBytes <= kLds && P::kLds <= kLds, "the output tile reuses the LDS");
+  const int tiles = A.tm * A.tn, z = unit / (tiles * A.splits), split = unit / tiles % A.splits;
   int im, in;
-  tile_of(blockIdx.x, A.tm, A.tn, im, in);
+  tile_of(unit % tiles, A.tm, A.tn, im, in);
   const int64_t m0 = (int64_t)im * P::kBM, n0 = (int64_t)in * P::kBN;
-  const int z = blockIdx.z, split = blockIdx.y;
   typename P::Acc acc[2][P::kMF] = {};
+  // the split's steps, counted over the segments
+  const int s0 = (int)((int64_t)A.steps * split / A.splits);
+  const int s1 = (int)((int64_t)A.steps * (split + 1) / A.splits);
+  const int each = A.steps / A.segments;
   for (int s = 0; s < A.segments; ++s) {
     const Matrix M[1] = {A.m[z + s]}, N[1] = {A.n[z + s]};
-    const int s0 = (int)((int64_t)A.steps * split / A.splits);
-    const int s1 = (int)((int64_t)A.steps * (split + 1) / A.splits);
-    P::run(acc, M, N, m0, n0, s0, s1, lds);
+    const int from = s0 - s * each, to = s1 - s * each;
+    P::run(acc, M, N, m0, n0, from > 0 ? from : 0, to < each ? to : each, lds);
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::kWN, wn = wave % P::kWN, h = lane >> 5;
-  float* part = A.splits > 1
-                    ? A.parts + ((int64_t)split * gridDim.z + z) * A.rows * A.part_pitch
-                    : nullptr;
+  float* const part = A.splits > 1 ? A.parts + ((int64_t)split * A.outputs + z) * A.rows * A.part_pitch
+                                   : nullptr;
 #pragma unroll
   for (int mf = 0; mf < P::kMF; ++mf) {
     const int row = (wm * P::kMF + mf) * 32 + (lane & 31);
@@ -285,6 +288,20 @@ __global__ void __launch_bounds__(P::kThreads, 2) ffn_product_kernel(ProductArgs
   if (part != nullptr) return;
   __syncthreads();
   Tile::store(lds, static_cast<T*>(A.out[z]), A.rows, A.cols, A.cols, m0, n0, A.vec);
+}
+
+// Both products in one launch: the first `weights` workgroups take units of dwg and dwu, the
+// others units of dx.
+template <class PW, class PX>
+__global__ void __launch_bounds__(PW::kThreads, 2) ffn_products_kernel(ProductArgs W, ProductArgs X,
+                                                                       int weights) {
+  typedef LdsTile<typename PW::Op, PW::kBM, PW::kBN, PW::kThreads> Tile;
+  static_assert(PW::kBM == PX::kBM && PW::kBN == PX::kBN && PW::kLds == PX::kLds, "one shape");
+  __shared__ __attribute__((aligned(16))) char lds[Tile::kBytes > PW::kLds ? Tile::kBytes : PW::kLds];
+  if ((int)blockIdx.x < weights)
+    product_unit<PW>(W, blockIdx.x, lds);
+  else
+    product_unit<PX>(X, blockIdx.x - weights, lds);
 }
 
 // out[z][r][c] = sum over splits of parts[s][z][r][c], in the order of s.
@@ -422,47 +439,114 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
   return launch_gate<typename S::Small, kPull>(g, st);
 }
 
-template <class P>
-hipError_t launch_product(ProductArgs p, int nz, int splits, hipStream_t st) {
-  p.tm = (int32_t)cdiv(p.rows, P::kBM);
-  p.tn = (int32_t)cdiv(p.cols, P::kBN);
-  p.splits = splits;
-  hipLaunchKernelGGL((ffn_product_kernel<P>), dim3((unsigned)(p.tm * p.tn), (unsigned)splits, (unsigned)nz),
-                     dim3(P::kThreads), 0, st, p);
-  return hipGetLastError();
+// ---- how the pullback's products are cut --------------------------------------------------
+// dwg and dwu have few tiles of many steps (a step is 64 tokens), dx has many tiles of few.
+// One launch takes both, the longer units first, so that the shorter ones fill what the
+// longer leave idle; a product whose units would outlast the others is cut along k into parts
+// that a second kernel adds.  The choice is the least estimate over tile shapes and numbers of
+// parts, with the times measured on this card: of 23040 x 1024 x 4096 in bf16 the two
+// products take 620 us in one launch and 890 one after the other.
+struct Cut {
+  bool big;
+  int w, x;  // splits of the weights' products and of dx
+};
+// When `slots` workgroups at a time are through with nw units of uw us and then nx of ux.
+double makespan(int64_t nw, double uw, int64_t nx, double ux, int64_t slots) {
+  if (nw + nx > 16 * slots) return ((double)nw * uw + (double)nx * ux) / (double)slots;
+  struct Group {
+    int64_t slots;
+    double free;
+  } g[2] = {{slots - nw % slots, (double)(nw / slots) * uw}, {nw % slots, (double)(nw / slots + 1) * uw}};
+  double end = g[1].slots > 0 ? g[1].free : g[0].free;
+  while (nx > 0) {
+    Group& first = g[1].slots > 0 && g[1].free < g[0].free ? g[1] : g[0];
+    nx -= first.slots;  // (the last round's idle slots do not matter)
+    first.free += ux;
+    end = first.free > end ? first.free : end;
+  }
+  return end;
+}
+struct Costs {  // us: of a step, of a unit besides, of a MiB of parts written and read again
+  double step, unit, part;
+  int slots;
+};
+
+int64_t units_of(const ProductArgs& p, int64_t span) {
+  return cdiv(p.rows, span) * cdiv(p.cols, span) * p.outputs;
 }
 
-template <class Op, bool kMRows, bool kNRows>
-hipError_t run_product(ProductArgs p, int nz, hipStream_t st) {
-  if (p.rows == 0 || p.cols == 0) return hipSuccess;
-  typedef Shapes<Op, kMRows, kNRows, 1> S;
-  const bool big = Op::kEsz == 2 && big_tiles(p.rows * nz, p.cols);
-  // k is cut where the tiles alone leave CUs idle, into parts of at least 8 steps
-  const int64_t tiles = cdiv(p.rows, big ? 256 : 128) * cdiv(p.cols, big ? 256 : 128) * nz;
-  int64_t splits = tiles < 256 ? 512 / tiles : 1;
-  splits = splits < p.steps / 8 ? splits : p.steps / 8;
-  if (splits < 1) splits = 1;
+Cut choose_cut(const ProductArgs* w, const ProductArgs* x, bool wide) {
+  Cut best = {false, 1, 1};
+  double least = 1e300;
+  for (int big = 0; big < (wide ? 2 : 1); ++big) {
+    const Costs c = wide ? (big ? Costs{1.55, 4.0, 0.4, 256} : Costs{1.0, 3.0, 0.4, 512})
+                         : Costs{4.0, 3.0, 0.4, 512};
+    const int64_t span = big ? 256 : 128;
+    for (int sw = 1; sw <= (w ? 64 : 1); sw *= 2)
+      for (int sx = 1; sx <= (x ? 16 : 1); sx *= 2) {
+        double unit[2] = {0.0, 0.0}, joins = 0.0;
+        int64_t units[2] = {0, 0};
+        const auto add = [&](int i, const ProductArgs* p, int splits) {
+          if (p == nullptr) return;
+          unit[i] = c.unit + c.step * (double)cdiv(p->steps, splits);
+          units[i] = units_of(*p, span) * splits;
+          if (splits > 1)
+            joins += 4.0 + c.part * splits * (double)(p->outputs * p->rows * p->cols) * 4 / (1 << 20);
+        };
+        add(0, w, sw);
+        add(1, x, sx);
+        const double t = makespan(units[0], unit[0], units[1], unit[1], c.slots) + joins;
+        if (t < least) {
+          least = t;
+          best = Cut{big != 0, sw, sx};
+        }
+      }
+  }
+  return best;
+}
+
+template <class Op, class PW, class PX>
+hipError_t launch_products(ProductArgs w, ProductArgs x, const Cut& cut, hipStream_t st) {
+  const auto shape = [](ProductArgs& p, int64_t bm, int64_t bn, int splits) {
+    p.tm = (int32_t)cdiv(p.rows, bm);
+    p.tn = (int32_t)cdiv(p.cols, bn);
+    p.splits = splits < p.steps ? splits : (p.steps > 0 ? p.steps : 1);
+    p.part_pitch = round_up(p.cols, 4);
+    return p.splits > 1 ? round_up((int64_t)p.splits * p.outputs * p.rows * p.part_pitch * 4, 256) : 0;
+  };
+  const int64_t wb = shape(w, PW::kBM, PW::kBN, cut.w), xb = shape(x, PX::kBM, PX::kBN, cut.x);
   Workspace ws(st);
-  p.part_pitch = round_up(p.cols, 4);
-  if (splits > 1) {
-    const hipError_t e = ws.take(splits * nz * p.rows * p.part_pitch * 4);
-    if (e != hipSuccess) return e;
-    p.parts = reinterpret_cast<float*>(ws.p);
+  hipError_t e = ws.take(wb + xb);
+  if (e != hipSuccess) return e;
+  w.parts = reinterpret_cast<float*>(ws.p);
+  x.parts = reinterpret_cast<float*>(ws.p + wb);
+  const int64_t nw = (int64_t)w.tm * w.tn * w.splits * w.outputs;
+  const int64_t nx = (int64_t)x.tm * x.tn * x.splits * x.outputs;
+  if (nw + nx == 0) return hipSuccess;
+  hipLaunchKernelGGL((ffn_products_kernel<PW, PX>), dim3((unsigned)(nw + nx)), dim3(PW::kThreads), 0, st,
+                     w, x, (int)nw);
+  e = hipGetLastError();
+  for (const ProductArgs* p : {&w, &x}) {
+    if (e != hipSuccess || p->splits == 1 || p->rows * p->cols == 0) continue;
+    hipLaunchKernelGGL((ffn_join_kernel<Op>), dim3(grid_for(p->outputs * p->rows * p->part_pitch / 4)),
+                       dim3(256), 0, st, p->out[0], p->out[1], p->parts, p->splits, p->outputs, p->rows,
+                       p->cols, p->part_pitch);
+    e = hipGetLastError();
   }
-  hipError_t e;
-  if constexpr (Op::kEsz == 2) {
-    if (big)
-      e = launch_product<typename S::Big>(p, nz, (int)splits, st);
-    else
-      e = launch_product<typename S::Small>(p, nz, (int)splits, st);
-  } else {
-    e = launch_product<typename S::Small>(p, nz, (int)splits, st);
-  }
-  if (e != hipSuccess || splits == 1) return e;
-  hipLaunchKernelGGL((ffn_join_kernel<Op>), dim3(grid_for(nz * p.rows * p.part_pitch / 4)), dim3(256),
-                     0, st, p.out[0], p.out[1], p.parts, (int)splits, nz, p.rows, p.cols,
-                     p.part_pitch);
-  return hipGetLastError();
+  return e;
+}
+
+// w: dwg and dwu (or null), x: dx (or null).
+template <class Op>
+hipError_t run_products(const ProductArgs* w, const ProductArgs* x, hipStream_t st) {
+  typedef Shapes<Op, false, false, 1> W;
+  typedef Shapes<Op, true, false, 1> X;
+  const Cut cut = choose_cut(w, x, Op::kEsz == 2);
+  const ProductArgs none = {};
+  if constexpr (Op::kEsz == 2)
+    if (cut.big)
+      return launch_products<Op, typename W::Big, typename X::Big>(w ? *w : none, x ? *x : none, cut, st);
+  return launch_products<Op, typename W::Small, typename X::Small>(w ? *w : none, x ? *x : none, cut, st);
 }
 
 GateArgs gate_args(const FfnArgs& a, const Matrix (&m)[3]) {
@@ -516,36 +600,30 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
   e = run_gate<Op, true>(g, st);
   if (e != hipSuccess) return e;
   const Matrix d[2] = {{dg, a.tokens, pitch, pitch}, {dg + each, a.tokens, pitch, pitch}};
-  if (dwg != nullptr) {
-    ProductArgs p = {};
-    p.m[0] = d[0];
-    p.m[1] = d[1];
-    p.n[0] = p.n[1] = m[0];
-    p.segments = 1;
-    p.steps = (int32_t)cdiv(a.tokens * Op::kEsz, kStepBytes);
-    p.rows = a.hidden;
-    p.cols = a.dim;
-    p.out[0] = dwg;
-    p.out[1] = dwu;
-    p.vec = whole_units(dwg, a.dim * Op::kEsz) && whole_units(dwu, a.dim * Op::kEsz);
-    e = run_product<Op, false, false>(p, 2, st);
-    if (e != hipSuccess) return e;
-  }
-  if (dx != nullptr) {
-    ProductArgs p = {};
-    p.m[0] = d[0];
-    p.m[1] = d[1];
-    p.n[0] = m[1];
-    p.n[1] = m[2];
-    p.segments = 2;
-    p.steps = (int32_t)cdiv(pitch, kStepBytes);
-    p.rows = a.tokens;
-    p.cols = a.dim;
-    p.out[0] = dx;
-    p.vec = whole_units(dx, a.dim * Op::kEsz);
-    e = run_product<Op, true, false>(p, 1, st);
-  }
-  return e;
+  ProductArgs w = {}, x = {};
+  w.m[0] = d[0];
+  w.m[1] = d[1];
+  w.n[0] = w.n[1] = m[0];
+  w.segments = 1;
+  w.outputs = 2;
+  w.steps = (int32_t)cdiv(a.tokens * Op::kEsz, kStepBytes);
+  w.rows = a.hidden;
+  w.cols = a.dim;
+  w.out[0] = dwg;
+  w.out[1] = dwu;
+  w.vec = whole_units(dwg, a.dim * Op::kEsz) && whole_units(dwu, a.dim * Op::kEsz);
+  x.m[0] = d[0];
+  x.m[1] = d[1];
+  x.n[0] = m[1];
+  x.n[1] = m[2];
+  x.segments = 2;
+  x.outputs = 1;
+  x.steps = 2 * (int32_t)cdiv(pitch, kStepBytes);
+  x.rows = a.tokens;
+  x.cols = a.dim;
+  x.out[0] = dx;
+  x.vec = whole_units(dx, a.dim * Op::kEsz);
+  return run_products<Op>(dwg ? &w : nullptr, dx ? &x : nullptr, st);
 }
 
 }  // namespace

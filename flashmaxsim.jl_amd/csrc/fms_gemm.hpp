@@ -303,13 +303,13 @@ struct Product {
           }
           static_assert(kLoads <= 2 * kMF, "a load for every two MFMAs");
           __builtin_amdgcn_s_setprio(0);
-          if (half == 1 && !second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          // (at the end the second half waits too: none is in flight when the LDS is free)
+          if (half == 1 && (!second || s + 1 == s1)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
           turn();
         }
         sm.advance();
         sn.advance();
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (!second) turn();
     }
   }
