@@ -68,71 +68,124 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
   da = d > 0.0f ? s + g * d * dy : s;  // (past the last step of s, y' may be infinite)
 }
 
-// Four neighbouring values as one LDS word.
+// A lane holds, of one row, columns 8 q + 4 h + 0..3 of 32 in quad q (h = lane / 32).  Its
+// part of the quads 2p and 2p + 1 goes to and from memory without LDS: in 16 bits the halves
+// trade a quad, so that each has eight neighbouring columns (from 16 p + 8 h on), 16 bytes; in
+// 32 bits a quad is 16 bytes already.
 template <class Op>
-struct Quad {
+struct Quads {
   typedef typename OutOf<Op>::T T;
-  typedef T V __attribute__((ext_vector_type(4)));
-  __device__ static __forceinline__ V pack(float a, float b, float c, float d) {
-    return V{(T)a, (T)b, (T)c, (T)d};
-  }
-};
+  static constexpr bool kTrade = Op::kEsz == 2;
+  static constexpr int kPer = 16 / Op::kEsz;  // neighbouring columns
+  typedef T V __attribute__((ext_vector_type(kPer)));
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// A kBM x kCols tile of feature values in LDS, rows of 16-byte units permuted over the
-// banks by their row, and its way from and to memory.
-template <class Op, int kBM, int kCols, int kThreads>
-struct LdsTile {
-  typedef typename OutOf<Op>::T T;
-  typedef typename Quad<Op>::V V;
-  static constexpr int kPer = 16 / Op::kEsz;      // values per unit
-  static constexpr int kUpr = kCols / kPer;       // units per row
-  static constexpr int kBytes = kBM * kCols * Op::kEsz;
-  static constexpr int kMix = (kUpr < 16 ? kUpr : 16) - 1;
-
-  __device__ static __forceinline__ V* quad(char* lds, int row, int col) {
-    const int unit = (col / kPer) ^ (row & kMix);
-    return reinterpret_cast<V*>(lds + (row * kUpr + unit) * 16 + (col % kPer) * Op::kEsz);
+  // First column of this lane's 16 bytes i of the pair p.
+  __device__ static __forceinline__ int col(int p, int i, int h) {
+    return kTrade ? 16 * p + 8 * h : 16 * p + 8 * i + 4 * h;
   }
-  // rows [m0, m0 + kBM) x columns [n0, n0 + kCols) of a (rows, cols) matrix, `pitch`
-  // values a row; `vec`: base and pitch are whole 16-byte units.
-  __device__ static __forceinline__ void store(const char* lds, T* out, int64_t rows, int64_t cols,
-                                               int64_t pitch, int64_t m0, int64_t n0, bool vec) {
-#pragma unroll 4
-    for (int u = threadIdx.x; u < kBM * kUpr; u += kThreads) {
-      const int row = u / kUpr, log = (u % kUpr) ^ (row & kMix);
-      const int64_t m = m0 + row, n = n0 + log * kPer;
-      if (m >= rows || n >= cols) continue;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + u * 16);
-      T* p = out + m * pitch + n;
-      if (vec && n + kPer <= cols) {
-        *reinterpret_cast<u32x4*>(p) = v;
-      } else {
-        const T* e = reinterpret_cast<const T*>(lds + u * 16);
-        for (int k = 0; k < kPer && n + k < cols; ++k) p[k] = e[k];
+  static constexpr int kWords = kTrade ? 1 : 2;  // 16 bytes per pair and lane
+
+  // 16 bytes at byte `at` of a resource, of which `left` columns are inside the row; kVec:
+  // all or none are, and the address is a multiple of 16.
+  template <bool kVec>
+  __device__ static __forceinline__ void put(V v, rsrc_t to, int at, int left) {
+    if constexpr (kVec) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to,
+                                             left > 0 ? at : kOutOfBounds, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int a = e < left ? at + e * Op::kEsz : kOutOfBounds;
+        if constexpr (kTrade)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)v[e]), to, a, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (T)v[e]), to, a, 0, 0);
       }
     }
   }
-  __device__ static __forceinline__ void load(char* lds, const T* in, int64_t rows, int64_t cols,
-                                              int64_t pitch, int64_t m0, int64_t n0, bool vec) {
-#pragma unroll 4
-    for (int u = threadIdx.x; u < kBM * kUpr; u += kThreads) {
-      const int row = u / kUpr, log = (u % kUpr) ^ (row & kMix);
-      const int64_t m = m0 + row, n = n0 + log * kPer;
-      u32x4 v{0u, 0u, 0u, 0u};
-      if (m < rows && n < cols) {
-        const T* p = in + m * pitch + n;
-        if (vec && n + kPer <= cols) {
-          v = *reinterpret_cast<const u32x4*>(p);
-        } else {
-          T e[kPer];
-          for (int k = 0; k < kPer; ++k) e[k] = n + k < cols ? p[k] : (T)0.0f;
-          __builtin_memcpy(&v, e, 16);
-        }
+  template <bool kVec>
+  __device__ static __forceinline__ V get(rsrc_t from, int at, int left) {
+    if constexpr (kVec) {
+      return __builtin_bit_cast(V, buf_load16(from, left > 0 ? at : kOutOfBounds));
+    } else {
+      V v;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int a = e < left ? at + e * Op::kEsz : kOutOfBounds;
+        if constexpr (kTrade)
+          v[e] = __builtin_bit_cast(T, (uint16_t)buf_load2(from, a));
+        else
+          v[e] = __builtin_bit_cast(T, buf_load4(from, a));
       }
-      *reinterpret_cast<u32x4*>(lds + u * 16) = v;
+      return v;
+    }
+  }
+  // Stores the pair a, b at byte `at` of the row's first column (of `cols` from there).
+  template <bool kVec>
+  __device__ static __forceinline__ void store(const float (&a)[4], const float (&b)[4], rsrc_t to,
+                                               int at, int p, int h, int cols) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    const V4 qa = {(T)a[0], (T)a[1], (T)a[2], (T)a[3]}, qb = {(T)b[0], (T)b[1], (T)b[2], (T)b[3]};
+    const int c0 = col(p, 0, h);
+    if constexpr (kTrade) {
+      const u32x2 wa = __builtin_bit_cast(u32x2, qa), wb = __builtin_bit_cast(u32x2, qb);
+      const auto r0 = __builtin_amdgcn_permlane32_swap(wa[0], wb[0], false, false);
+      const auto r1 = __builtin_amdgcn_permlane32_swap(wa[1], wb[1], false, false);
+      const u32x4 w = {(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
+      put<kVec>(__builtin_bit_cast(V, w), to, at + c0 * Op::kEsz, cols - c0);
+    } else {
+      const int c1 = col(p, 1, h);
+      put<kVec>(qa, to, at + c0 * Op::kEsz, cols - c0);
+      put<kVec>(qb, to, at + c1 * Op::kEsz, cols - c1);
+    }
+  }
+  // Reads such a pair.
+  template <bool kVec>
+  __device__ static __forceinline__ void fetch(V (&w)[kWords], rsrc_t from, int at, int p, int h,
+                                               int cols) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      w[i] = get<kVec>(from, at + col(p, i, h) * Op::kEsz, cols - col(p, i, h));
+  }
+  __device__ static __forceinline__ void split(const V (&w)[kWords], float (&a)[4], float (&b)[4]) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    V4 qa, qb;
+    if constexpr (kTrade) {
+      const u32x4 x = __builtin_bit_cast(u32x4, w[0]);
+      const auto r0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+      const auto r1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+      qa = __builtin_bit_cast(V4, u32x2{(uint32_t)r0[0], (uint32_t)r1[0]});
+      qb = __builtin_bit_cast(V4, u32x2{(uint32_t)r0[1], (uint32_t)r1[1]});
+    } else {
+      qa = w[0];
+      qb = w[1];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = (float)qa[e];
+      b[e] = (float)qb[e];
     }
   }
 };
+
+// A tile of a row-major matrix as a resource: rows past its end are out of bounds.
+template <class T>
+__device__ __forceinline__ rsrc_t tile_at(const void* p, int64_t rows, int64_t pitch, int64_t m0,
+                                          int64_t n0) {
+  const int64_t at = m0 * pitch + n0, left = (rows * pitch - at) * (int64_t)sizeof(T);
+  return make_rsrc_u(static_cast<const T*>(p) + at,
+                     (uint32_t)(left < 0 ? 0 : (left > 0x7fffffff ? 0x7fffffff : left)));
+}
+// x, as if it were not known before: what an epilogue derives from it is computed there, not
+// held in registers all through the products.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ int columns_left(int64_t cols, int64_t n0) {
+  return cols - n0 > 0x7fffffff ? 0x7fffffff : (int)(cols - n0);
+}
 
 // Workgroup -> tile.  Workgroup ids go round robin over the 8 XCDs, each with an L2 of
 // its own: every XCD takes a contiguous run of tiles, and a run walks kGroupM row tiles
@@ -157,75 +210,107 @@ struct GateArgs {
   void *out0, *out1;
   const void* in;
   int64_t out_cols, out_pitch, in_pitch;  // values
-  int32_t out_vec, in_vec;
+  int32_t vec;  // whole 16-byte units of outputs and input
 };
 
-// The accumulators' tile -> LDS: h, or dg over the dh that lies there and du behind it.
-template <class P, bool kPull, int kAct>
-__device__ __forceinline__ void gate_epilogue(const typename P::Acc (&acc)[2][P::kMF], char* lds) {
-  typedef typename P::Op Op;
-  typedef LdsTile<Op, P::kBM, P::kBN / 2, P::kThreads> Tile;
+// A tile's sums -> h, or dg and du.
+template <class P, bool kPull, int kAct, bool kVec>
+__device__ __forceinline__ void gate_store(const GateArgs& A, const typename P::Acc (&acc)[2][P::kMF],
+                                           int64_t m0, int64_t n0) {
+  typedef Quads<typename P::Op> Q;
+  typedef typename Q::T T;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::kWN, wn = wave % P::kWN, h = lane >> 5;
+  const rsrc_t to0 = tile_at<T>(A.out0, A.tokens, A.out_pitch, m0, n0);
+  const rsrc_t to1 = tile_at<T>(A.out1, kPull ? A.tokens : 0, A.out_pitch, m0, n0);
+  const rsrc_t from = tile_at<T>(A.in, kPull ? A.tokens : 0, A.in_pitch, m0, n0);
+  const int row0 = here(wm * P::kMF * 32 + (lane & 31));
+  const int out = (row0 * (int)A.out_pitch + wn * 32) * (int)sizeof(T);
+  const int in = (row0 * (int)A.in_pitch + wn * 32) * (int)sizeof(T);
+  const int out_left = columns_left(A.out_cols, n0) - wn * 32, in_left = columns_left(A.hidden, n0) - wn * 32;
+  // the cotangent's part of a row fragment, read one ahead
+  typename Q::V dh[2][2][Q::kWords];
+  const auto fetch = [&](int mf) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      Q::template fetch<kVec>(dh[mf & 1][p], from, in + mf * 32 * (int)A.in_pitch * (int)sizeof(T), p, h,
+                              in_left);
+  };
+  if constexpr (kPull) fetch(0);
 #pragma unroll
   for (int mf = 0; mf < P::kMF; ++mf) {
-    const int row = (wm * P::kMF + mf) * 32 + (lane & 31);
+    if constexpr (kPull)
+      if (mf + 1 < P::kMF) fetch(mf + 1);
+    const int at = out + mf * 32 * (int)A.out_pitch * (int)sizeof(T);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int col = wn * 32 + 8 * q + 4 * h;
-      auto* at = Tile::quad(lds, row, col);
-      float a[4], da[4];
+    for (int p = 0; p < 2; ++p) {
+      float y[2][4], z[2][4];
+      if constexpr (kPull) Q::split(dh[mf & 1][p], y[0], y[1]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) activate<kAct>(acc[0][mf][4 * q + e], a[e], da[e]);
-      if constexpr (kPull) {
-        const auto d = *at;
-        float dg[4], du[4];
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          dg[e] = (float)d[e] * acc[1][mf][4 * q + e] * da[e];
-          du[e] = (float)d[e] * a[e];
+          const float g = acc[0][mf][4 * (2 * p + i) + e], u = acc[1][mf][4 * (2 * p + i) + e];
+          float a, da;
+          activate<kAct>(g, a, da);
+          if constexpr (kPull) {
+            z[i][e] = y[i][e] * a;
+            y[i][e] = y[i][e] * u * da;
+          } else {
+            y[i][e] = a * u;
+          }
         }
-        *at = Quad<Op>::pack(dg[0], dg[1], dg[2], dg[3]);
-        *Tile::quad(lds + Tile::kBytes, row, col) = Quad<Op>::pack(du[0], du[1], du[2], du[3]);
-      } else {
-        const auto& u = acc[1][mf];
-        *at = Quad<Op>::pack(a[0] * u[4 * q], a[1] * u[4 * q + 1], a[2] * u[4 * q + 2],
-                             a[3] * u[4 * q + 3]);
-      }
+      Q::template store<kVec>(y[0], y[1], to0, at, p, h, out_left);
+      if constexpr (kPull) Q::template store<kVec>(z[0], z[1], to1, at, p, h, out_left);
+      __builtin_amdgcn_sched_barrier(0);  // (few values at a time)
     }
   }
 }
 
+template <class P, bool kPull, bool kVec>
+__device__ __forceinline__ void by_act(const GateArgs& A, const typename P::Acc (&acc)[2][P::kMF],
+                                       int64_t m0, int64_t n0) {
+  if (A.act == FMS_ACT_SILU)
+    gate_store<P, kPull, FMS_ACT_SILU, kVec>(A, acc, m0, n0);
+  else if (A.act == FMS_ACT_GELU)
+    gate_store<P, kPull, FMS_ACT_GELU, kVec>(A, acc, m0, n0);
+  else
+    gate_store<P, kPull, FMS_ACT_GELU_TANH, kVec>(A, acc, m0, n0);
+}
+
 // Forward (kPull false): h.  Pullback: dg and du, their rows filled up with zeros to out_cols.
+// Workgroup b takes tiles b, b + gridDim.x, ...
 template <class P, bool kPull>
 __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
-  typedef typename P::Op Op;
-  typedef typename OutOf<Op>::T T;
   constexpr int kCols = P::kBN / 2;
-  typedef LdsTile<Op, P::kBM, kCols, P::kThreads> Tile;
-  static_assert((kPull ? 2 : 1) * Tile::kBytes <= P::kLds, "the output tile reuses the LDS");
   __shared__ __attribute__((aligned(16))) char lds[P::kLds];
-  int im, in;
-  tile_of(blockIdx.x, A.tm, A.tn, im, in);
-  const int64_t m0 = (int64_t)im * P::kBM, n0 = (int64_t)in * kCols;
-  typename P::Acc acc[2][P::kMF] = {};
-  const Matrix M[1] = {A.x}, N[2] = {A.wg, A.wu};
-  P::run(acc, M, N, m0, n0, 0, A.steps, lds);
-  if constexpr (kPull) {
-    Tile::load(lds, static_cast<const T*>(A.in), A.tokens, A.hidden, A.in_pitch, m0, n0, A.in_vec);
-    __syncthreads();
-  }
-  if (A.act == FMS_ACT_SILU)
-    gate_epilogue<P, kPull, FMS_ACT_SILU>(acc, lds);
-  else if (A.act == FMS_ACT_GELU)
-    gate_epilogue<P, kPull, FMS_ACT_GELU>(acc, lds);
-  else
-    gate_epilogue<P, kPull, FMS_ACT_GELU_TANH>(acc, lds);
-  __syncthreads();
-  Tile::store(lds, static_cast<T*>(A.out0), A.tokens, A.out_cols, A.out_pitch, m0, n0, A.out_vec);
-  if constexpr (kPull)
-    Tile::store(lds + Tile::kBytes, static_cast<T*>(A.out1), A.tokens, A.out_cols, A.out_pitch, m0,
-                n0, A.out_vec);
+  const int tiles = A.tm * A.tn, mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const auto place = [&](int j, int64_t& m0, int64_t& n0) {
+    int im, in;
+    tile_of(blockIdx.x + j * gridDim.x, A.tm, A.tn, im, in);
+    m0 = (int64_t)im * P::kBM;
+    n0 = (int64_t)in * kCols;
+  };
+  const auto leg = [&](int j) {
+    typename P::Legs l;
+    l.m[0] = A.x;
+    l.n[0] = A.wg;
+    l.n[1] = A.wu;
+    place(j, l.m0, l.n0);
+    l.first = 0;
+    l.steps = A.steps;
+    l.ends = true;
+    return l;
+  };
+  const auto after = [&](int j, const typename P::Acc(&acc)[2][P::kMF]) {
+    int64_t m0, n0;
+    place(j, m0, n0);
+    if (!A.vec)
+      by_act<P, kPull, false>(A, acc, m0, n0);
+    else
+      by_act<P, kPull, true>(A, acc, m0, n0);
+  };
+  P::run(mine, leg, after, lds);
 }
 
 // A product of the pullback.  Unit u of its tiles * splits * outputs: out[z] or, with splits,
@@ -242,52 +327,72 @@ struct ProductArgs {
   int64_t part_pitch;
 };
 
-template <class P, int kLds>
-__device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, char (&lds)[kLds]) {
-  typedef typename P::Op Op;
-  typedef typename OutOf<Op>::T T;
-  typedef LdsTile<Op, P::kBM, P::kBN, P::kThreads> Tile;
-  static_assert(Tile::kBytes <= kLds && P::kLds <= kLds, "the output tile reuses the LDS");
+// A tile's sums -> rows of `cols` values, `pitch` apart.
+template <class P, class Q, bool kVec>
+__device__ __forceinline__ void product_store(const typename P::Acc (&acc)[2][P::kMF], void* out,
+                                              int64_t rows, int64_t cols, int64_t pitch, int64_t m0,
+                                              int64_t n0) {
+  typedef typename Q::T T;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const rsrc_t to = tile_at<T>(out, rows, pitch, m0, n0);
+  const int row0 = here(wave / P::kWN * P::kMF * 32 + (lane & 31));
+#pragma unroll
+  for (int mf = 0; mf < P::kMF; ++mf)
+#pragma unroll
+    for (int nf = 0; nf < 2; ++nf) {
+      const int n = P::col(wave % P::kWN, nf);
+      const int at = ((row0 + mf * 32) * (int)pitch + n) * (int)sizeof(T);
+      const auto& c = acc[nf][mf];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const float a[4] = {c[8 * p], c[8 * p + 1], c[8 * p + 2], c[8 * p + 3]};
+        const float b[4] = {c[8 * p + 4], c[8 * p + 5], c[8 * p + 6], c[8 * p + 7]};
+        Q::template store<kVec>(a, b, to, at, p, h, columns_left(cols, n0) - n);
+      }
+    }
+}
+
+template <class P>
+__device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, char* lds) {
   const int tiles = A.tm * A.tn, z = unit / (tiles * A.splits), split = unit / tiles % A.splits;
   int im, in;
   tile_of(unit % tiles, A.tm, A.tn, im, in);
   const int64_t m0 = (int64_t)im * P::kBM, n0 = (int64_t)in * P::kBN;
-  typename P::Acc acc[2][P::kMF] = {};
-  // the split's steps, counted over the segments
+  // the split's steps, counted over the segments: a leg in each that it reaches into
   const int s0 = (int)((int64_t)A.steps * split / A.splits);
   const int s1 = (int)((int64_t)A.steps * (split + 1) / A.splits);
   const int each = A.steps / A.segments;
-  for (int s = 0; s < A.segments; ++s) {
-    const Matrix M[1] = {A.m[z + s]}, N[1] = {A.n[z + s]};
-    const int from = s0 - s * each, to = s1 - s * each;
-    P::run(acc, M, N, m0, n0, from > 0 ? from : 0, to < each ? to : each, lds);
+  const int lo = each > 0 ? s0 / each : 0, hi = each > 0 ? (s1 - 1) / each : 0;
+  const auto leg = [&](int j) {
+    const int s = lo + j, from = s0 - s * each, to = s1 - s * each;
+    typename P::Legs l;
+    l.m[0] = z + s == 0 ? A.m[0] : A.m[1];
+    l.n[0] = z + s == 0 ? A.n[0] : A.n[1];
+    l.m0 = m0;
+    l.n0 = n0;
+    l.first = from > 0 ? from : 0;
+    l.steps = (to < each ? to : each) - l.first;
+    l.ends = s == hi;
+    return l;
+  };
+  const auto after = [&](int, const typename P::Acc(&acc)[2][P::kMF]) {
+    if (A.splits > 1)
+      product_store<P, Quads<OpF32>, true>(
+          acc, A.parts + ((int64_t)split * A.outputs + z) * A.rows * A.part_pitch, A.rows, A.part_pitch,
+          A.part_pitch, m0, n0);
+    else if (A.vec)
+      product_store<P, Quads<typename P::Op>, true>(acc, z == 0 ? A.out[0] : A.out[1], A.rows, A.cols,
+                                                    A.cols, m0, n0);
+    else
+      product_store<P, Quads<typename P::Op>, false>(acc, z == 0 ? A.out[0] : A.out[1], A.rows, A.cols,
+                                                     A.cols, m0, n0);
+  };
+  if (s0 < s1) {
+    P::run(hi - lo + 1, leg, after, lds);
+  } else {  // a sum of nothing
+    const typename P::Acc zero[2][P::kMF] = {};
+    after(0, zero);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave / P::kWN, wn = wave % P::kWN, h = lane >> 5;
-  float* const part = A.splits > 1 ? A.parts + ((int64_t)split * A.outputs + z) * A.rows * A.part_pitch
-                                   : nullptr;
-#pragma unroll
-  for (int mf = 0; mf < P::kMF; ++mf) {
-    const int row = (wm * P::kMF + mf) * 32 + (lane & 31);
-#pragma unroll
-    for (int nf = 0; nf < 2; ++nf)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = P::col(wn, nf) + 8 * q + 4 * h;
-        const auto& c = acc[nf][mf];
-        if (part != nullptr) {
-          if (m0 + row < A.rows && n0 + col < A.part_pitch)
-            *reinterpret_cast<f32x4*>(part + (m0 + row) * A.part_pitch + n0 + col) =
-                f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
-        } else {
-          *Tile::quad(lds, row, col) =
-              Quad<Op>::pack(c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]);
-        }
-      }
-  }
-  if (part != nullptr) return;
-  __syncthreads();
-  Tile::store(lds, static_cast<T*>(A.out[z]), A.rows, A.cols, A.cols, m0, n0, A.vec);
 }
 
 // Both products in one launch: the first `weights` workgroups take units of dwg and dwu, the
@@ -295,9 +400,8 @@ __device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, cha
 template <class PW, class PX>
 __global__ void __launch_bounds__(PW::kThreads, 2) ffn_products_kernel(ProductArgs W, ProductArgs X,
                                                                        int weights) {
-  typedef LdsTile<typename PW::Op, PW::kBM, PW::kBN, PW::kThreads> Tile;
-  static_assert(PW::kBM == PX::kBM && PW::kBN == PX::kBN && PW::kLds == PX::kLds, "one shape");
-  __shared__ __attribute__((aligned(16))) char lds[Tile::kBytes > PW::kLds ? Tile::kBytes : PW::kLds];
+  static_assert(PW::kThreads == PX::kThreads && PW::kLds == PX::kLds, "one shape");
+  __shared__ __attribute__((aligned(16))) char lds[PW::kLds];
   if ((int)blockIdx.x < weights)
     product_unit<PW>(W, blockIdx.x, lds);
   else
@@ -421,8 +525,9 @@ hipError_t launch_gate(GateArgs g, hipStream_t st) {
   g.tm = (int32_t)cdiv(g.tokens, P::kBM);
   g.tn = (int32_t)cdiv(g.out_cols, P::kBN / 2);
   g.steps = (int32_t)cdiv(g.x.rowbytes, kStepBytes);
-  hipLaunchKernelGGL((ffn_gate_kernel<P, kPull>), dim3((unsigned)(g.tm * g.tn)), dim3(P::kThreads),
-                     0, st, g);
+  const int tiles = g.tm * g.tn, most = P::kThreads == 512 ? 256 : 512;  // a round of workgroups
+  hipLaunchKernelGGL((ffn_gate_kernel<P, kPull>), dim3((unsigned)(tiles < most ? tiles : most)),
+                     dim3(P::kThreads), 0, st, g);
   return hipGetLastError();
 }
 
@@ -433,6 +538,16 @@ bool big_tiles(int64_t rows, int64_t cols) { return cdiv(rows, 256) * cdiv(cols,
 template <class Op, bool kPull>
 hipError_t run_gate(const GateArgs& g, hipStream_t st) {
   if (g.tokens == 0 || g.out_cols == 0) return hipSuccess;
+  if (g.x.rowbytes == 0) {  // sums of nothing: h, dg and du are zero
+    const int64_t n = g.tokens * g.out_pitch;
+    for (void* out : {g.out0, g.out1})
+      if (out != nullptr)
+        hipLaunchKernelGGL(ffn_pad_kernel<typename Quads<Op>::T>, dim3(grid_for(n)), dim3(256), 0, st,
+                           static_cast<typename Quads<Op>::T*>(out),
+                           static_cast<const typename Quads<Op>::T*>(nullptr), g.tokens, (int64_t)0,
+                           g.out_pitch);
+    return hipGetLastError();
+  }
   typedef Shapes<Op, true, true, 2> S;
   if constexpr (Op::kEsz == 2)
     if (big_tiles(g.tokens, 2 * g.out_cols)) return launch_gate<typename S::Big, kPull>(g, st);
@@ -572,7 +687,7 @@ hipError_t forward(const FfnArgs& a, void* h, hipStream_t st) {
   GateArgs g = gate_args(a, m);
   g.out0 = h;
   g.out_cols = g.out_pitch = a.hidden;
-  g.out_vec = whole_units(h, a.hidden * Op::kEsz);
+  g.vec = whole_units(h, a.hidden * Op::kEsz);
   return run_gate<Op, false>(g, st);
 }
 
@@ -592,11 +707,10 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
   GateArgs g = gate_args(a, m);
   g.in = dh;
   g.in_pitch = a.hidden;
-  g.in_vec = whole_units(dh, a.hidden * Op::kEsz);
+  g.vec = whole_units(dh, a.hidden * Op::kEsz);
   g.out0 = dg;
   g.out1 = dg + each;
   g.out_cols = g.out_pitch = pitch / Op::kEsz;
-  g.out_vec = 1;
   e = run_gate<Op, true>(g, st);
   if (e != hipSuccess) return e;
   const Matrix d[2] = {{dg, a.tokens, pitch, pitch}, {dg + each, a.tokens, pitch, pitch}};

@@ -179,6 +179,16 @@ __device__ __forceinline__ typename Op::Acc mma_frag(u32x4 a, u32x4 b, typename 
   }
 }
 
+// A stretch of k of one tile: steps [first, first + steps) of the products of M's and N's
+// rows / columns from m0 and n0 on (n0 counts within a part).  The last leg of a tile ends it.
+template <int kParts>
+struct Leg {
+  Matrix m[1], n[kParts];
+  int64_t m0, n0;
+  int first, steps;
+  bool ends;
+};
+
 // The tile's shape: kWM x kWN waves, each 32 kMF rows by 64 columns.
 template <class Op_, bool kMRows_, bool kNRows_, int kParts_, int kWM_, int kWN_, int kMF_>
 struct Product {
@@ -193,6 +203,7 @@ struct Product {
   static constexpr bool kTurns = kWM * kWN == 8;
   static constexpr int kStepK = StageM::kStepK;
   typedef typename Op::Acc Acc;
+  typedef Leg<kParts> Legs;
 
   // Column of the tile that fragment nf of wave column wn starts at.  With two parts, a
   // wave holds 32 columns of each, so that gate and up of one hidden unit share a lane.
@@ -200,19 +211,31 @@ struct Product {
     return kParts == 2 ? nf * (kBN / 2) + wn * 32 : wn * 64 + nf * 32;
   }
 
-  // acc[nf][mf] += over steps [s0, s1) of the tile at (m0, n0); n0 counts within a part.
-  // All threads of the workgroup call it; it ends with the LDS free for other use.
-  __device__ static __forceinline__ void run(Acc (&acc)[kNF][kMF], const Matrix (&M)[1],
-                                             const Matrix (&N)[kParts], int64_t m0, int64_t n0,
-                                             int s0, int s1, char* lds) {
+  // Walks the workgroup's legs 0 .. legs - 1 (all of at least one step), which leg(j) gives,
+  // as one run of steps: a tile's first slices are on their way before the tile before is
+  // through.  after(j, acc) takes a tile's sums when its last leg j is done, without touching
+  // the LDS.  All threads of the workgroup call it.
+  template <class LegOf, class After>
+  __device__ static __forceinline__ void run(int legs, LegOf&& leg, After&& after, char* lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / kWN, wn = wave % kWN;
+    // where the requests are: leg `ahead` with `left` of its steps to come
     StageM sm;
     StageN sn;
-    sm.init(tid, M, m0, s0);
-    sn.init(tid, N, n0, s0);
-    // Load i of both operands' next slices into the buffer of step s, from the resources made
-    // before its first.  (A request past the last step reads zeros or values that no one uses.)
+    int ahead = 0, left = 0;
+    const auto enter = [&] {
+      const Legs l = leg(ahead);
+      sm.init(tid, l.m, l.m0, l.first);
+      sn.init(tid, l.n, l.n0, l.first);
+      left = l.steps;
+    };
+    // (past the last leg it asks for more of that one, which no one uses)
+    const auto advance = [&] {
+      sm.advance();
+      sn.advance();
+      if (--left == 0 && ++ahead < legs) enter();
+    };
+    // Load i of both operands' next slices into a buffer, from the resources made before.
     rsrc_t rm[1], rn[kParts];
     const auto aim = [&] {
       if (sm.last()) sm.trim(tid);
@@ -220,22 +243,21 @@ struct Product {
       sm.resources(rm);
       sn.resources(rn);
     };
-    const auto load = [&](int i, int s) {
-      char* const to = lds + ((s - s0) & 1) * kBuffer;
+    const auto load = [&](int i, char* to) {
       if (i < StageM::kLoads)
         sm.load(i, rm, to, wave);
       else
         sn.load(i - StageM::kLoads, rn, to + StageM::kBytes, wave);
     };
     constexpr int kLoads = StageM::kLoads + StageN::kLoads;
-    const auto request = [&](int s) {
+    const auto request = [&](char* to) {
       aim();
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) load(i, s);
-      sm.advance();
-      sn.advance();
+      for (int i = 0; i < kLoads; ++i) load(i, to);
+      advance();
     };
     // Fragments of k group g of the step in `cur`, and their products.
+    Acc acc[kNF][kMF];
     u32x4 fn[2][kNF], fm[2][kMF];
     const auto read = [&](const char* cur, int g, int i) {
 #pragma unroll
@@ -251,66 +273,92 @@ struct Product {
 #pragma unroll
       for (int b = 0; b < kMF; ++b) multiply(i, b);
     };
-    if (s0 >= s1) return;
-    request(s0);
+    const auto clear = [&] {
+#pragma unroll
+      for (int a = 0; a < kNF; ++a)
+#pragma unroll
+        for (int b = 0; b < kMF; ++b) acc[a][b] = Acc{};
+    };
+    enter();
+    clear();
+    char *cur = lds, *other = lds + kBuffer;
+    const auto swap = [&] {
+      char* const x = cur;
+      cur = other;
+      other = x;
+    };
+    request(cur);
     if constexpr (!kTurns) {
-      for (int s = s0; s < s1; ++s) {
-        // this step's slices have landed; every wave has its last fragments of the step before
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        turn();
-        const char* const cur = lds + ((s - s0) & 1) * kBuffer;
-        read(cur, 0, 0);
-        if (s + 1 < s1) request(s + 1);
-        if (s > s0) multiply_all(1);
-        read(cur, 1, 1);
-        multiply_all(0);
-        read(cur, 2, 0);
+      for (int j = 0; j < legs; ++j) {
+        const Legs l = leg(j);
+        for (int s = 0; s < l.steps; ++s) {
+          // this step's slices have landed; every wave has its last fragments of the step before
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          turn();
+          read(cur, 0, 0);
+          if (ahead < legs) request(other);
+          if (s > 0) multiply_all(1);
+          read(cur, 1, 1);
+          multiply_all(0);
+          read(cur, 2, 0);
+          multiply_all(1);
+          read(cur, 3, 1);
+          multiply_all(0);
+          swap();
+        }
         multiply_all(1);
-        read(cur, 3, 1);
-        multiply_all(0);
+        if (l.ends) {
+          after(j, acc);
+          clear();
+        }
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      turn();
-      multiply_all(1);
     } else {
       // Turn p: the first half of the waves reads at even p and multiplies at odd p, the
-      // second half one turn later.  Step s0 + j is read in turns 4j .. 4j + 3, and its buffer
-      // is free from turn 4j + 4 on.  A wave requests in the one multiplying turn of each step
+      // second half one turn later.  Step i is read in turns 4i .. 4i + 3, and its buffer is
+      // free from turn 4i + 4 on.  A wave requests in the one multiplying turn of each step
       // that comes right after a buffer became free, a load after every two MFMAs: the first
-      // half step s + 1 in turn 4j + 1, the second half step s + 2 in turn 4j + 4.  Each wave
-      // waits for its requests before the barrier that ends turn 4j + 3.
+      // half step i + 1 in turn 4i + 1, the second half step i + 2 in turn 4i + 4.  Each wave
+      // waits for its requests before the barrier that ends turn 4i + 3.
       const bool second = wave >= 4;
-      if (second) request(s0 + 1);
+      if (second) request(other);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       turn();
       if (second) turn();
-      for (int s = s0; s < s1; ++s) {
-        const char* const cur = lds + ((s - s0) & 1) * kBuffer;
+      for (int j = 0; j < legs; ++j) {
+        const Legs l = leg(j);
+        for (int s = 0; s < l.steps; ++s) {
+          const bool end = j + 1 == legs && s + 1 == l.steps;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          read(cur, 2 * half, 0);
-          read(cur, 2 * half + 1, 1);
-          if (half == 0) aim();
-          if (half == 1 && second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          turn();
-          const bool now = (half == 1) == second;
-          __builtin_amdgcn_s_setprio(1);
+          for (int half = 0; half < 2; ++half) {
+            read(cur, 2 * half, 0);
+            read(cur, 2 * half + 1, 1);
+            if (half == 0) aim();
+            if (half == 1 && second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            turn();
+            const bool now = (half == 1) == second;
+            char* const to = half == 0 ? other : cur;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-          for (int i = 0; i < 2 * kMF; ++i) {
-            multiply(i / kMF, i % kMF);
-            if (now && i < kLoads) load(i, s + 1 + half);
+            for (int i = 0; i < 2 * kMF; ++i) {
+              multiply(i / kMF, i % kMF);
+              if (now && i < kLoads) load(i, to);
+            }
+            static_assert(kLoads <= 2 * kMF, "a load for every two MFMAs");
+            __builtin_amdgcn_s_setprio(0);
+            // (at the very end the second half waits too: none is in flight when it is done)
+            if (half == 1 && (!second || end)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            turn();
           }
-          static_assert(kLoads <= 2 * kMF, "a load for every two MFMAs");
-          __builtin_amdgcn_s_setprio(0);
-          // (at the end the second half waits too: none is in flight when the LDS is free)
-          if (half == 1 && (!second || s + 1 == s1)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          turn();
+          advance();
+          swap();
         }
-        sm.advance();
-        sn.advance();
+        if (j + 1 == legs && !second) turn();
+        if (l.ends) {
+          after(j, acc);
+          clear();
+        }
       }
-      if (!second) turn();
     }
   }
 
