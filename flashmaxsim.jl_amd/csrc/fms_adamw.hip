@@ -18,7 +18,7 @@
 // Bound by memory: 28 bytes an element in fp32, 22 with 16-bit parameters and gradients, 10
 // with 8-bit moments.  A workgroup takes 2048 elements of one tensor, eight a lane, so that
 // half a wave holds a block of 8-bit moments.  The tensors' pointers travel as kernel
-// arguments, up to 56 a launch: nothing is kept between calls and nothing is uploaded.
+// arguments, up to 52 a launch: nothing is kept between calls and nothing is uploaded.
 #include "fms_adamw.hpp"
 
 #include <float.h>
@@ -115,9 +115,19 @@ __device__ __forceinline__ void scale_of(float top, float& a, float& inv) {
   a = tiny ? 0.0f : top;
   inv = tiny ? 0.0f : 1.0f / top;
 }
-__device__ __forceinline__ int code_of(float root, float steps) {  // root in 0..1, or NaN
-  const float c = __builtin_rintf(root * steps);
+// round(sqrt(q) * 127) and round(q^(1/4) * 255) for q in 0..1 (NaN: 0), as IEEE square roots
+// give them.  The hardware's root is within a unit or two of that: only a product within
+// 2e-4 of a tie, one in 2500, needs the exact one (without this the step of 64 million
+// elements was bound by the roots' instructions, 205 us; now PLACEHOLDER).
+__device__ __forceinline__ int code_m(float q) {
+  float t = __builtin_amdgcn_sqrtf(q) * 127.0f, c = __builtin_rintf(t);
+  if (__builtin_expect(fabsf(t - c) > 0.4998f, 0)) c = __builtin_rintf(sqrtf(q) * 127.0f);
   return c >= 0.0f ? (int)c : 0;
+}
+__device__ __forceinline__ int code_v(float q) {
+  float t = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(q)) * 255.0f, c = __builtin_rintf(t);
+  if (__builtin_expect(fabsf(t - c) > 0.4998f, 0)) c = __builtin_rintf(sqrtf(sqrtf(q)) * 255.0f);
+  return q > 0.0f && c < 1.0f ? 1 : (c >= 0.0f ? (int)c : 0);
 }
 
 // Codes of eight neighbouring elements.
@@ -149,14 +159,18 @@ __device__ __forceinline__ void store_codes(const Codes& c, uint8_t* p, int64_t 
   }
 }
 
-constexpr int kTensors = 48;  // per launch: the arguments stay within 4 KiB
+constexpr int kTensors = 52;  // per launch: the arguments stay within 4 KiB
 struct Tensors {
   fms_adamw_tensor t[kTensors];
   int32_t end[kTensors];  // workgroups up to and with each tensor's
-  int32_t vec[kTensors];
   int32_t count;
 };
 static_assert(sizeof(Tensors) + sizeof(AdamWStep) <= 4096, "kernel arguments");
+
+template <class... P>
+__device__ __forceinline__ bool aligned(P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
+}
 
 // The tensor a workgroup belongs to: the first whose end lies past it.
 template <class L>
@@ -177,7 +191,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
   const fms_adamw_tensor& t = L.t[i];
   const int first = i > 0 ? L.end[i - 1] : 0;
   const int64_t k = (int64_t)(blockIdx.x - first) * kChunk + threadIdx.x * kPer, n = t.n;
-  const bool vec = L.vec[i] != 0, codes = t.m_scale != nullptr;
+  const bool vec = aligned(t.p, t.g, t.m, t.v, t.master), codes = t.m_scale != nullptr;
   float g[kPer], p[kPer], m[kPer], v[kPer];
   load_typed(g, t.g, t.g_dtype, k, n, vec);
   if (t.master)
@@ -218,12 +232,10 @@ __global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
     Codes cm = {{0u, 0u}}, cv = {{0u, 0u}};
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      int c = code_of(sqrtf(fabsf(m[e]) * im), 127.0f);
+      int c = code_m(fabsf(m[e]) * im);
       c = m[e] < 0.0f ? -c : c;
       cm.w[e >> 2] |= (uint32_t)(c & 0xff) << (8 * (e & 3));
-      const float q = v[e] * iv;
-      c = code_of(sqrtf(sqrtf(q)), 255.0f);
-      c = q > 0.0f && c < 1 ? 1 : c;
+      c = code_v(v[e] * iv);
       cv.w[e >> 2] |= (uint32_t)c << (8 * (e & 3));
     }
     store_codes(cm, static_cast<uint8_t*>(t.m), k, n, vec);
@@ -238,11 +250,10 @@ __global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
   }
 }
 
-constexpr int kMoments = 72;
+constexpr int kMoments = 92;
 struct Moments {
   fms_moment8 t[kMoments];
   int32_t end[kMoments];
-  int32_t vec[kMoments];
   int32_t count;
 };
 static_assert(sizeof(Moments) <= 4096, "kernel arguments");
@@ -253,7 +264,7 @@ __global__ void __launch_bounds__(256) moment_values_kernel(Moments L) {
   const int first = i > 0 ? L.end[i - 1] : 0;
   const int64_t k = (int64_t)(blockIdx.x - first) * kChunk + threadIdx.x * kPer, n = t.n;
   if (k >= n) return;
-  const bool vec = L.vec[i] != 0;
+  const bool vec = aligned(t.codes, t.values);
   const Codes c = load_codes(static_cast<const uint8_t*>(t.codes), k, n, vec);
   const float a = t.scales[k / kBlock];
   float v[kPer];
@@ -263,17 +274,11 @@ __global__ void __launch_bounds__(256) moment_values_kernel(Moments L) {
   store8(v, t.values, k, n, vec);
 }
 
-bool aligned(std::initializer_list<const void*> ptrs) {
-  for (const void* p : ptrs)
-    if (reinterpret_cast<uintptr_t>(p) & 15u) return false;
-  return true;
-}
-
 // Hands `launch` lists of up to kMost tensors whose workgroups fit one grid.  A tensor's
 // workgroups beyond a grid's are no concern: 2^22 of them are 2^33 elements, and a larger
 // tensor does not fit the memory of the device with its moments.
-template <class L, class T, int kMost, class Vec, class F>
-hipError_t in_lists(int64_t count, const T* tensors, Vec&& vec, F&& launch) {
+template <class L, class T, int kMost, class F>
+hipError_t in_lists(int64_t count, const T* tensors, F&& launch) {
   constexpr int64_t kGrid = (int64_t)1 << 23;
   static thread_local L list;
   list.count = 0;
@@ -290,7 +295,6 @@ hipError_t in_lists(int64_t count, const T* tensors, Vec&& vec, F&& launch) {
     if (need == 0) continue;
     blocks += need;
     list.t[list.count] = tensors[i];
-    list.vec[list.count] = vec(tensors[i]) ? 1 : 0;
     list.end[list.count++] = (int32_t)blocks;
   }
   return hipSuccess;
@@ -301,17 +305,14 @@ hipError_t in_lists(int64_t count, const T* tensors, Vec&& vec, F&& launch) {
 hipError_t adamw_step(int64_t count, const fms_adamw_tensor* tensors, const AdamWStep& s,
                       hipStream_t stream) {
   return in_lists<Tensors, fms_adamw_tensor, kTensors>(
-      count, tensors,
-      [](const fms_adamw_tensor& t) { return aligned({t.p, t.g, t.m, t.v, t.master}); },
-      [&](const Tensors& l, unsigned blocks) {
+      count, tensors, [&](const Tensors& l, unsigned blocks) {
         hipLaunchKernelGGL(adamw_kernel, dim3(blocks), dim3(256), 0, stream, l, s);
       });
 }
 
 hipError_t moment_values(int64_t count, const fms_moment8* moments, hipStream_t stream) {
   return in_lists<Moments, fms_moment8, kMoments>(
-      count, moments, [](const fms_moment8& t) { return aligned({t.codes, t.values}); },
-      [&](const Moments& l, unsigned blocks) {
+      count, moments, [&](const Moments& l, unsigned blocks) {
         hipLaunchKernelGGL(moment_values_kernel, dim3(blocks), dim3(256), 0, stream, l);
       });
 }

@@ -86,43 +86,16 @@ struct Quads {
   }
   static constexpr int kWords = kTrade ? 1 : 2;  // 16 bytes per pair and lane
 
-  // 16 bytes at byte `at` of a resource, of which `left` columns are inside the row; kVec:
-  // all or none are, and the address is a multiple of 16.
-  template <bool kVec>
+  // 16 bytes at byte `at` of a resource, with `left` columns of the row from there (none or
+  // all of them are inside).
   __device__ static __forceinline__ void put(V v, rsrc_t to, int at, int left) {
-    if constexpr (kVec) {
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to,
-                                             left > 0 ? at : kOutOfBounds, 0, 0);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int a = e < left ? at + e * Op::kEsz : kOutOfBounds;
-        if constexpr (kTrade)
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)v[e]), to, a, 0, 0);
-        else
-          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (T)v[e]), to, a, 0, 0);
-      }
-    }
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to,
+                                           left > 0 ? at : kOutOfBounds, 0, 0);
   }
-  template <bool kVec>
   __device__ static __forceinline__ V get(rsrc_t from, int at, int left) {
-    if constexpr (kVec) {
-      return __builtin_bit_cast(V, buf_load16(from, left > 0 ? at : kOutOfBounds));
-    } else {
-      V v;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int a = e < left ? at + e * Op::kEsz : kOutOfBounds;
-        if constexpr (kTrade)
-          v[e] = __builtin_bit_cast(T, (uint16_t)buf_load2(from, a));
-        else
-          v[e] = __builtin_bit_cast(T, buf_load4(from, a));
-      }
-      return v;
-    }
+    return __builtin_bit_cast(V, buf_load16(from, left > 0 ? at : kOutOfBounds));
   }
   // Stores the pair a, b at byte `at` of the row's first column (of `cols` from there).
-  template <bool kVec>
   __device__ static __forceinline__ void store(const float (&a)[4], const float (&b)[4], rsrc_t to,
                                                int at, int p, int h, int cols) {
     typedef T V4 __attribute__((ext_vector_type(4)));
@@ -133,20 +106,19 @@ struct Quads {
       const auto r0 = __builtin_amdgcn_permlane32_swap(wa[0], wb[0], false, false);
       const auto r1 = __builtin_amdgcn_permlane32_swap(wa[1], wb[1], false, false);
       const u32x4 w = {(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
-      put<kVec>(__builtin_bit_cast(V, w), to, at + c0 * Op::kEsz, cols - c0);
+      put(__builtin_bit_cast(V, w), to, at + c0 * Op::kEsz, cols - c0);
     } else {
       const int c1 = col(p, 1, h);
-      put<kVec>(qa, to, at + c0 * Op::kEsz, cols - c0);
-      put<kVec>(qb, to, at + c1 * Op::kEsz, cols - c1);
+      put(qa, to, at + c0 * Op::kEsz, cols - c0);
+      put(qb, to, at + c1 * Op::kEsz, cols - c1);
     }
   }
   // Reads such a pair.
-  template <bool kVec>
   __device__ static __forceinline__ void fetch(V (&w)[kWords], rsrc_t from, int at, int p, int h,
                                                int cols) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i)
-      w[i] = get<kVec>(from, at + col(p, i, h) * Op::kEsz, cols - col(p, i, h));
+      w[i] = get(from, at + col(p, i, h) * Op::kEsz, cols - col(p, i, h));
   }
   __device__ static __forceinline__ void split(const V (&w)[kWords], float (&a)[4], float (&b)[4]) {
     typedef T V4 __attribute__((ext_vector_type(4)));
@@ -166,6 +138,61 @@ struct Quads {
       a[e] = (float)qa[e];
       b[e] = (float)qb[e];
     }
+  }
+
+  // Rows that are no whole 16-byte units: 32 x 32 values pass through `box`, the wave's own
+  // LDS, and go to or come from memory element by element, two rows at a time.
+  static constexpr int kBox = 32 * 32 * Op::kEsz;
+  __device__ static __forceinline__ void box_in(char* box, int lane, int q, const float (&a)[4]) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<V4*>(box + ((lane & 31) * 32 + 8 * q + 4 * (lane >> 5)) * Op::kEsz) =
+        V4{(T)a[0], (T)a[1], (T)a[2], (T)a[3]};
+  }
+  __device__ static __forceinline__ void box_out(const char* box, int lane, int q, float (&a)[4]) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    const V4 v = *reinterpret_cast<const V4*>(box + ((lane & 31) * 32 + 8 * q + 4 * (lane >> 5)) * Op::kEsz);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = (float)v[e];
+  }
+  // `at`: byte of the box's first value, `pitch` bytes a row, `cols` columns left there.
+  __device__ static __forceinline__ void box_store(const char* box, int lane, rsrc_t to, int at, int pitch,
+                                                   int cols) {
+    box_wait();
+    const int c = lane & 31;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int r = 2 * i + (lane >> 5), to_at = c < cols ? at + r * pitch + c * Op::kEsz : kOutOfBounds;
+      const T v = reinterpret_cast<const T*>(box)[r * 32 + c];
+      if constexpr (kTrade)
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), to, to_at, 0, 0);
+      else
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), to, to_at, 0, 0);
+    }
+    box_wait();
+  }
+  __device__ static __forceinline__ void box_load(char* box, int lane, rsrc_t from, int at, int pitch,
+                                                  int cols) {
+    const int c = lane & 31;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 16; i0 += 8) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int off = c < cols ? at + (2 * (i0 + i) + (lane >> 5)) * pitch + c * Op::kEsz : kOutOfBounds;
+        if constexpr (kTrade)
+          v[i] = __builtin_bit_cast(T, (uint16_t)buf_load2(from, off));
+        else
+          v[i] = __builtin_bit_cast(T, buf_load4(from, off));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(box)[(2 * (i0 + i) + (lane >> 5)) * 32 + c] = v[i];
+    }
+    box_wait();
+  }
+  // A wave's LDS accesses are done, for all its lanes.
+  __device__ static __forceinline__ void box_wait() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
   }
 };
 
@@ -213,69 +240,92 @@ struct GateArgs {
   int32_t vec;  // whole 16-byte units of outputs and input
 };
 
-// A tile's sums -> h, or dg and du.
+// LDS behind the products' buffers, a box for each wave.
+template <class P>
+constexpr int kBoxes = P::kThreads / 64 * Quads<typename P::Op>::kBox;
+
+// A tile's sums -> h, or dg and du.  kVec: rows of whole 16-byte units; else through `box`.
 template <class P, bool kPull, int kAct, bool kVec>
 __device__ __forceinline__ void gate_store(const GateArgs& A, const typename P::Acc (&acc)[2][P::kMF],
-                                           int64_t m0, int64_t n0) {
+                                           int64_t m0, int64_t n0, char* box) {
   typedef Quads<typename P::Op> Q;
   typedef typename Q::T T;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kSize = (int)sizeof(T);
+  const int lane = here(threadIdx.x & 63), wave = threadIdx.x >> 6;
   const int wm = wave / P::kWN, wn = wave % P::kWN, h = lane >> 5;
   const rsrc_t to0 = tile_at<T>(A.out0, A.tokens, A.out_pitch, m0, n0);
   const rsrc_t to1 = tile_at<T>(A.out1, kPull ? A.tokens : 0, A.out_pitch, m0, n0);
   const rsrc_t from = tile_at<T>(A.in, kPull ? A.tokens : 0, A.in_pitch, m0, n0);
-  const int row0 = here(wm * P::kMF * 32 + (lane & 31));
-  const int out = (row0 * (int)A.out_pitch + wn * 32) * (int)sizeof(T);
-  const int in = (row0 * (int)A.in_pitch + wn * 32) * (int)sizeof(T);
+  // of the wave's first row
+  const int out_pitch = (int)A.out_pitch * kSize, in_pitch = (int)A.in_pitch * kSize;
+  const int out = wm * P::kMF * 32 * out_pitch + wn * 32 * kSize;
+  const int in = wm * P::kMF * 32 * in_pitch + wn * 32 * kSize;
   const int out_left = columns_left(A.out_cols, n0) - wn * 32, in_left = columns_left(A.hidden, n0) - wn * 32;
   // the cotangent's part of a row fragment, read one ahead
   typename Q::V dh[2][2][Q::kWords];
   const auto fetch = [&](int mf) {
 #pragma unroll
     for (int p = 0; p < 2; ++p)
-      Q::template fetch<kVec>(dh[mf & 1][p], from, in + mf * 32 * (int)A.in_pitch * (int)sizeof(T), p, h,
-                              in_left);
+      Q::fetch(dh[mf & 1][p], from, in + (mf * 32 + (lane & 31)) * in_pitch, p, h, in_left);
   };
-  if constexpr (kPull) fetch(0);
+  if constexpr (kPull && kVec) fetch(0);
 #pragma unroll
   for (int mf = 0; mf < P::kMF; ++mf) {
-    if constexpr (kPull)
+    if constexpr (kPull && kVec)
       if (mf + 1 < P::kMF) fetch(mf + 1);
-    const int at = out + mf * 32 * (int)A.out_pitch * (int)sizeof(T);
+    const int at = out + (mf * 32 + (lane & 31)) * out_pitch;
+    float y[4][4], z[4][4];
+    if constexpr (kPull && !kVec) {
+      Q::box_load(box, lane, from, in + mf * 32 * in_pitch, in_pitch, in_left);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) Q::box_out(box, lane, q, y[q]);
+      Q::box_wait();
+    }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      float y[2][4], z[2][4];
-      if constexpr (kPull) Q::split(dh[mf & 1][p], y[0], y[1]);
+      if constexpr (kPull && kVec) Q::split(dh[mf & 1][p], y[2 * p], y[2 * p + 1]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int q = 2 * p; q < 2 * p + 2; ++q)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float g = acc[0][mf][4 * (2 * p + i) + e], u = acc[1][mf][4 * (2 * p + i) + e];
+          const float g = acc[0][mf][4 * q + e], u = acc[1][mf][4 * q + e];
           float a, da;
           activate<kAct>(g, a, da);
           if constexpr (kPull) {
-            z[i][e] = y[i][e] * a;
-            y[i][e] = y[i][e] * u * da;
+            z[q][e] = y[q][e] * a;
+            y[q][e] = y[q][e] * u * da;
           } else {
-            y[i][e] = a * u;
+            y[q][e] = a * u;
           }
         }
-      Q::template store<kVec>(y[0], y[1], to0, at, p, h, out_left);
-      if constexpr (kPull) Q::template store<kVec>(z[0], z[1], to1, at, p, h, out_left);
-      __builtin_amdgcn_sched_barrier(0);  // (few values at a time)
+      if constexpr (kVec) {
+        Q::store(y[2 * p], y[2 * p + 1], to0, at, p, h, out_left);
+        if constexpr (kPull) Q::store(z[2 * p], z[2 * p + 1], to1, at, p, h, out_left);
+        __builtin_amdgcn_sched_barrier(0);  // (few values at a time)
+      }
+    }
+    if constexpr (!kVec) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) Q::box_in(box, lane, q, y[q]);
+      Q::box_store(box, lane, to0, out + mf * 32 * out_pitch, out_pitch, out_left);
+      if constexpr (kPull) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) Q::box_in(box, lane, q, z[q]);
+        Q::box_store(box, lane, to1, out + mf * 32 * out_pitch, out_pitch, out_left);
+      }
     }
   }
 }
 
 template <class P, bool kPull, bool kVec>
 __device__ __forceinline__ void by_act(const GateArgs& A, const typename P::Acc (&acc)[2][P::kMF],
-                                       int64_t m0, int64_t n0) {
+                                       int64_t m0, int64_t n0, char* box) {
   if (A.act == FMS_ACT_SILU)
-    gate_store<P, kPull, FMS_ACT_SILU, kVec>(A, acc, m0, n0);
+    gate_store<P, kPull, FMS_ACT_SILU, kVec>(A, acc, m0, n0, box);
   else if (A.act == FMS_ACT_GELU)
-    gate_store<P, kPull, FMS_ACT_GELU, kVec>(A, acc, m0, n0);
+    gate_store<P, kPull, FMS_ACT_GELU, kVec>(A, acc, m0, n0, box);
   else
-    gate_store<P, kPull, FMS_ACT_GELU_TANH, kVec>(A, acc, m0, n0);
+    gate_store<P, kPull, FMS_ACT_GELU_TANH, kVec>(A, acc, m0, n0, box);
 }
 
 // Forward (kPull false): h.  Pullback: dg and du, their rows filled up with zeros to out_cols.
@@ -283,7 +333,8 @@ __device__ __forceinline__ void by_act(const GateArgs& A, const typename P::Acc 
 template <class P, bool kPull>
 __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
   constexpr int kCols = P::kBN / 2;
-  __shared__ __attribute__((aligned(16))) char lds[P::kLds];
+  __shared__ __attribute__((aligned(16))) char lds[P::kLds + kBoxes<P>];
+  char* const box = lds + P::kLds + (threadIdx.x >> 6) * Quads<typename P::Op>::kBox;
   const int tiles = A.tm * A.tn, mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   const auto place = [&](int j, int64_t& m0, int64_t& n0) {
     int im, in;
@@ -306,11 +357,113 @@ __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
     int64_t m0, n0;
     place(j, m0, n0);
     if (!A.vec)
-      by_act<P, kPull, false>(A, acc, m0, n0);
+      by_act<P, kPull, false>(A, acc, m0, n0, box);
     else
-      by_act<P, kPull, true>(A, acc, m0, n0);
+      by_act<P, kPull, true>(A, acc, m0, n0, box);
   };
   P::run(mine, leg, after, lds);
+}
+
+// ---- few tokens ----------------------------------------------------------------------------
+// Bound by the weights' bytes, and for one query by latency: no LDS staging and no barrier on
+// the way.  A workgroup takes 16 hidden units (their 16 rows of wg and of wu) and 16 kNT
+// tokens; its eight waves share k, 128 bytes of every row at a time, each loading its operands
+// straight into the 16 x 16 MFMAs' registers with everything of a round in flight, and join
+// their sums through LDS.
+template <class Op>
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 acc) {
+  if constexpr (std::is_same_v<Op, OpF16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  } else if constexpr (std::is_same_v<Op, OpBF16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  } else {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+    return acc;
+  }
+}
+
+constexpr int kFewWaves = 8;
+constexpr int kFewHidden = 16;
+
+template <class Op, int kNT>
+__global__ void __launch_bounds__(64 * kFewWaves) ffn_few_kernel(GateArgs A) {
+  typedef typename OutOf<Op>::T T;
+  // lane: row (hidden unit, token) lane % 16 of a fragment, bytes 16 (lane / 16) of 64
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * kFewHidden, m0 = (int64_t)blockIdx.y * 16 * kNT;
+  const int pitch = (int)A.x.pitch, bytes = (int)A.x.rowbytes, in = 16 * (lane >> 4);
+  const rsrc_t rg = matrix_from(A.wg, n0 * A.wg.pitch), ru = matrix_from(A.wu, n0 * A.wu.pitch);
+  const rsrc_t rx = matrix_from(A.x, m0 * A.x.pitch);
+  const int row = (lane & 15) * pitch + in;
+  f32x4 acc[2][kNT] = {};
+  struct Round {
+    u32x4 g[2], u[2], x[2][kNT];
+  };
+  const auto load = [&](Round& r, int at) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int off = at + 64 * i + in < bytes ? row + at + 64 * i : kOutOfBounds;
+      r.g[i] = buf_load16(rg, off);
+      r.u[i] = buf_load16(ru, off);
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+        r.x[i][t] = buf_load16(rx, off == kOutOfBounds ? off : off + t * 16 * pitch);
+    }
+  };
+  const auto multiply = [&](const Round& r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+        acc[0][t] = mma16<Op>(r.g[i], r.x[i][t], acc[0][t]);
+        acc[1][t] = mma16<Op>(r.u[i], r.x[i][t], acc[1][t]);
+      }
+  };
+  constexpr int kRound = kFewWaves * 128;  // bytes of k between a wave's rounds
+  Round a, b;
+  int at = wave * 128;
+  load(a, at);
+  load(b, at + kRound);
+  for (; at < bytes; at += 2 * kRound) {  // (rounds past the end read zeros)
+    multiply(a);
+    load(a, at + 2 * kRound);
+    multiply(b);
+    load(b, at + 3 * kRound);
+  }
+  // sums of the waves: lane holds hidden units 4 (lane / 16) + e of token lane % 16
+  __shared__ __attribute__((aligned(16))) f32x4 sums[kFewWaves][2][kNT][64];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) sums[wave][p][t][lane] = acc[p][t];
+  __syncthreads();
+  for (int o = tid; o < 64 * kNT; o += 64 * kFewWaves) {
+    const int t = o >> 6, l = o & 63;
+    f32x4 g = {}, u = {};
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      g += sums[w][0][t][l];
+      u += sums[w][1][t][l];
+    }
+    const int64_t m = m0 + t * 16 + (l & 15), n = n0 + 4 * (l >> 4);
+    if (m >= A.tokens) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float y, dy;
+      if (A.act == FMS_ACT_SILU)
+        activate<FMS_ACT_SILU>(g[e], y, dy);
+      else if (A.act == FMS_ACT_GELU)
+        activate<FMS_ACT_GELU>(g[e], y, dy);
+      else
+        activate<FMS_ACT_GELU_TANH>(g[e], y, dy);
+      if (n + e < A.hidden) static_cast<T*>(A.out0)[m * A.out_pitch + n + e] = (T)(y * u[e]);
+    }
+  }
 }
 
 // A product of the pullback.  Unit u of its tiles * splits * outputs: out[z] or, with splits,
@@ -327,33 +480,48 @@ struct ProductArgs {
   int64_t part_pitch;
 };
 
-// A tile's sums -> rows of `cols` values, `pitch` apart.
+// A tile's sums -> rows of `cols` values, `pitch` apart.  kVec: rows of whole 16-byte units.
 template <class P, class Q, bool kVec>
 __device__ __forceinline__ void product_store(const typename P::Acc (&acc)[2][P::kMF], void* out,
-                                              int64_t rows, int64_t cols, int64_t pitch, int64_t m0,
-                                              int64_t n0) {
+                                              int64_t rows, int64_t cols, int64_t pitch_, int64_t m0,
+                                              int64_t n0, char* box) {
   typedef typename Q::T T;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const rsrc_t to = tile_at<T>(out, rows, pitch, m0, n0);
-  const int row0 = here(wave / P::kWN * P::kMF * 32 + (lane & 31));
+  const int lane = here(threadIdx.x & 63), wave = threadIdx.x >> 6, h = lane >> 5;
+  const rsrc_t to = tile_at<T>(out, rows, pitch_, m0, n0);
+  const int pitch = (int)pitch_ * (int)sizeof(T), left = columns_left(cols, n0);
 #pragma unroll
   for (int mf = 0; mf < P::kMF; ++mf)
 #pragma unroll
     for (int nf = 0; nf < 2; ++nf) {
       const int n = P::col(wave % P::kWN, nf);
-      const int at = ((row0 + mf * 32) * (int)pitch + n) * (int)sizeof(T);
+      const int at = (wave / P::kWN * P::kMF + mf) * 32 * pitch + n * (int)sizeof(T);
       const auto& c = acc[nf][mf];
+      const auto quad = [&](int q, float (&a)[4]) {
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const float a[4] = {c[8 * p], c[8 * p + 1], c[8 * p + 2], c[8 * p + 3]};
-        const float b[4] = {c[8 * p + 4], c[8 * p + 5], c[8 * p + 6], c[8 * p + 7]};
-        Q::template store<kVec>(a, b, to, at, p, h, columns_left(cols, n0) - n);
+        for (int e = 0; e < 4; ++e) a[e] = c[4 * q + e];
+      };
+      float a[4], b[4];
+      if constexpr (kVec) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          quad(2 * p, a);
+          quad(2 * p + 1, b);
+          Q::store(a, b, to, at + (lane & 31) * pitch, p, h, left - n);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          quad(q, a);
+          Q::box_in(box, lane, q, a);
+        }
+        Q::box_store(box, lane, to, at, pitch, left - n);
       }
     }
 }
 
 template <class P>
 __device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, char* lds) {
+  char* const box = lds + P::kLds + (threadIdx.x >> 6) * Quads<typename P::Op>::kBox;
   const int tiles = A.tm * A.tn, z = unit / (tiles * A.splits), split = unit / tiles % A.splits;
   int im, in;
   tile_of(unit % tiles, A.tm, A.tn, im, in);
@@ -379,13 +547,13 @@ __device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, cha
     if (A.splits > 1)
       product_store<P, Quads<OpF32>, true>(
           acc, A.parts + ((int64_t)split * A.outputs + z) * A.rows * A.part_pitch, A.rows, A.part_pitch,
-          A.part_pitch, m0, n0);
+          A.part_pitch, m0, n0, box);
     else if (A.vec)
       product_store<P, Quads<typename P::Op>, true>(acc, z == 0 ? A.out[0] : A.out[1], A.rows, A.cols,
-                                                    A.cols, m0, n0);
+                                                    A.cols, m0, n0, box);
     else
       product_store<P, Quads<typename P::Op>, false>(acc, z == 0 ? A.out[0] : A.out[1], A.rows, A.cols,
-                                                     A.cols, m0, n0);
+                                                     A.cols, m0, n0, box);
   };
   if (s0 < s1) {
     P::run(hi - lo + 1, leg, after, lds);
@@ -401,7 +569,7 @@ template <class PW, class PX>
 __global__ void __launch_bounds__(PW::kThreads, 2) ffn_products_kernel(ProductArgs W, ProductArgs X,
                                                                        int weights) {
   static_assert(PW::kThreads == PX::kThreads && PW::kLds == PX::kLds, "one shape");
-  __shared__ __attribute__((aligned(16))) char lds[PW::kLds];
+  __shared__ __attribute__((aligned(16))) char lds[PW::kLds + kBoxes<PW>];
   if ((int)blockIdx.x < weights)
     product_unit<PW>(W, blockIdx.x, lds);
   else
@@ -430,14 +598,22 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(void* out0, void* out1, c
   }
 }
 
-// Rows of `cols` values copied to rows of `pitch`, the rest zero.
+// Up to three matrices' rows of `cols` values copied to rows of `pitch`, the rest zero.
+struct PadArgs {
+  void* out[3];
+  const void* in[3];
+  int64_t rows[3];
+  int64_t cols, pitch;
+};
 template <class T>
-__global__ void __launch_bounds__(256) ffn_pad_kernel(T* out, const T* in, int64_t rows,
-                                                      int64_t cols, int64_t pitch) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pitch;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / pitch, c = i % pitch;
-    out[i] = c < cols ? in[r * cols + c] : (T)0;
+__global__ void __launch_bounds__(256) ffn_pad_kernel(PadArgs A) {
+  const int y = blockIdx.y;
+  T* const out = static_cast<T*>(y == 0 ? A.out[0] : y == 1 ? A.out[1] : A.out[2]);
+  const T* const in = static_cast<const T*>(y == 0 ? A.in[0] : y == 1 ? A.in[1] : A.in[2]);
+  const int64_t n = (y == 0 ? A.rows[0] : y == 1 ? A.rows[1] : A.rows[2]) * A.pitch;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / A.pitch, c = i % A.pitch;
+    out[i] = c < A.cols ? in[r * A.cols + c] : (T)0;
   }
 }
 
@@ -481,36 +657,27 @@ Inputs inputs_of(const FfnArgs& a) {
   in.bytes = in.copy ? round_up((a.tokens + 2 * a.hidden) * in.pitch, 256) : 0;
   return in;
 }
+hipError_t launch_pad(int esz, const PadArgs& p, hipStream_t st) {
+  int64_t most = p.rows[0] > p.rows[1] ? p.rows[0] : p.rows[1];
+  most = (most > p.rows[2] ? most : p.rows[2]) * p.pitch;
+  const dim3 grid(grid_for(most), 3);
+  if (esz == 4)
+    hipLaunchKernelGGL(ffn_pad_kernel<uint32_t>, grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL(ffn_pad_kernel<uint16_t>, grid, dim3(256), 0, st, p);
+  return hipGetLastError();
+}
 hipError_t place_inputs(const FfnArgs& a, const Inputs& in, char* ws, Matrix (&m)[3],
                         hipStream_t st) {
-  const void* src[3] = {a.x, a.wg, a.wu};
-  const int64_t rows[3] = {a.tokens, a.hidden, a.hidden};
   const int esz = esz_of(a.dtype);
+  PadArgs p = {{nullptr, nullptr, nullptr}, {a.x, a.wg, a.wu}, {a.tokens, a.hidden, a.hidden},
+               a.dim, in.pitch / esz};
   for (int i = 0; i < 3; ++i) {
-    const void* base = src[i];
-    if (in.copy) {
-      const int64_t n = rows[i] * in.pitch / esz;
-      if (n > 0) {
-        if (esz == 4)
-          hipLaunchKernelGGL(ffn_pad_kernel<uint32_t>, dim3(grid_for(n)), dim3(256), 0, st,
-                             reinterpret_cast<uint32_t*>(ws), static_cast<const uint32_t*>(src[i]),
-                             rows[i], a.dim, in.pitch / esz);
-        else
-          hipLaunchKernelGGL(ffn_pad_kernel<uint16_t>, dim3(grid_for(n)), dim3(256), 0, st,
-                             reinterpret_cast<uint16_t*>(ws), static_cast<const uint16_t*>(src[i]),
-                             rows[i], a.dim, in.pitch / esz);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-      }
-      base = ws;
-      ws += rows[i] * in.pitch;
-    }
-    m[i].base = static_cast<const char*>(base);
-    m[i].rows = rows[i];
-    m[i].pitch = in.pitch;
-    m[i].rowbytes = in.pitch;
+    p.out[i] = ws;
+    m[i] = Matrix{in.copy ? ws : static_cast<const char*>(p.in[i]), p.rows[i], in.pitch, in.pitch};
+    ws += in.copy ? p.rows[i] * in.pitch : 0;
   }
-  return hipSuccess;
+  return in.copy && in.bytes > 0 ? launch_pad(esz, p, st) : hipSuccess;
 }
 
 // The tile shapes by element size: wave grid and 32-row fragments per wave.
@@ -535,19 +702,35 @@ hipError_t launch_gate(GateArgs g, hipStream_t st) {
 // fills more CUs.
 bool big_tiles(int64_t rows, int64_t cols) { return cdiv(rows, 256) * cdiv(cols, 256) >= 192; }
 
+template <class Op, int kNT>
+hipError_t launch_few(const GateArgs& g, hipStream_t st) {
+  hipLaunchKernelGGL((ffn_few_kernel<Op, kNT>),
+                     dim3((unsigned)cdiv(g.hidden, kFewHidden), (unsigned)cdiv(g.tokens, 16 * kNT)),
+                     dim3(64 * kFewWaves), 0, st, g);
+  return hipGetLastError();
+}
+
+// A round of few-token workgroups, each with 64 tokens, against the tiles' kernel, which below
+// 512 tiles takes the latency of its steps whatever the tokens (us, 768 x 2048 / 1024 x 4096):
+//   16 bits: 1 token 4.9 / 5.2 (tiles 9.8 / 11.9), 64 tokens 8.5 / 9.6 (10.0 / 12.2),
+//     128 tokens 8.6 / 17 (10.0 / 12.3): up to 256 workgroups.
+//   32 bits: 1 token 6.4 / 7.7 (53 / 70), 256 tokens 30 / 66 (54 / 71): up to 768 workgroups.
+bool few_tokens(const GateArgs& g, int esz) {
+  return cdiv(g.hidden, kFewHidden) * cdiv(g.tokens, 64) <= (esz == 2 ? 256 : 768);
+}
+
 template <class Op, bool kPull>
 hipError_t run_gate(const GateArgs& g, hipStream_t st) {
   if (g.tokens == 0 || g.out_cols == 0) return hipSuccess;
   if (g.x.rowbytes == 0) {  // sums of nothing: h, dg and du are zero
-    const int64_t n = g.tokens * g.out_pitch;
-    for (void* out : {g.out0, g.out1})
-      if (out != nullptr)
-        hipLaunchKernelGGL(ffn_pad_kernel<typename Quads<Op>::T>, dim3(grid_for(n)), dim3(256), 0, st,
-                           static_cast<typename Quads<Op>::T*>(out),
-                           static_cast<const typename Quads<Op>::T*>(nullptr), g.tokens, (int64_t)0,
-                           g.out_pitch);
-    return hipGetLastError();
+    return launch_pad(Op::kEsz, PadArgs{{g.out0, g.out1, nullptr}, {}, {g.tokens, g.out1 ? g.tokens : 0, 0},
+                                        0, g.out_pitch}, st);
   }
+  if constexpr (!kPull)
+    if (few_tokens(g, Op::kEsz)) {
+      if (g.tokens <= 16) return launch_few<Op, 1>(g, st);
+      return g.tokens <= 32 ? launch_few<Op, 2>(g, st) : launch_few<Op, 4>(g, st);
+    }
   typedef Shapes<Op, true, true, 2> S;
   if constexpr (Op::kEsz == 2)
     if (big_tiles(g.tokens, 2 * g.out_cols)) return launch_gate<typename S::Big, kPull>(g, st);

@@ -37,11 +37,28 @@ struct Row {
   static constexpr int kWaves = kWaves_;                    // waves that share a row
   static constexpr int kThreads = kWaves == 16 ? 1024 : 256;
   static constexpr int kRows = kThreads / 64 / kWaves;      // rows in flight
-  typedef T V __attribute__((ext_vector_type(kUnit)));
+  typedef T V __attribute__((ext_vector_type(kUnit)));  // (one element: a vector of one)
   // Rows of at most 64 elements, one a lane, are computed in double: a short row's gradient
   // is a difference of nearly equal terms (of two elements, all of it), and one value a
   // lane costs nothing beside the load.
   typedef std::conditional_t<kPer == 1, double, float> F;
+
+  // A share as it lies in memory: what is read before it is needed, and weights.
+  struct Packed {
+    V v[kUnits];
+    __device__ __forceinline__ F operator[](int j) const { return (F)(float)v[j / kUnit][j % kUnit]; }
+  };
+  __device__ static __forceinline__ void load(Packed& p, const T* row, int dim) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      p.v[i] = V{};
+      if (at(i) < dim) p.v[i] = *reinterpret_cast<const V*>(row + at(i));
+    }
+  }
+  __device__ static __forceinline__ void unpack(F (&v)[kPer], const Packed& p) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = p[j];
+  }
 
   // The first element of this thread's unit i.
   __device__ static __forceinline__ int at(int i) {
@@ -86,8 +103,19 @@ struct Row {
 // The sum over a row's threads of one value each, the same in all of them.
 template <class R>
 __device__ __forceinline__ typename R::F row_sum(typename R::F v, float* lds) {
+  if constexpr (R::kPer == 1) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  } else {  // rotations within 16 lanes, then the four sixteens (no trip through LDS)
+    v = dpp_add<0x121>(v);
+    v = dpp_add<0x122>(v);
+    v = dpp_add<0x124>(v);
+    v = dpp_add<0x128>(v);
+    const auto of = [&](int lane) {
+      return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    };
+    v = (of(0) + of(16)) + (of(32) + of(48));
+  }
   if constexpr (R::kWaves > 1) {
     const int wave = threadIdx.x >> 6;
     __syncthreads();
@@ -151,7 +179,7 @@ __global__ void __launch_bounds__(R::kThreads) norm_forward_kernel(NormArgs A, t
   const int dim = (int)A.dim;
   const F inv_dim = (F)1 / (F)dim;
   const int sub = R::kWaves == 1 ? threadIdx.x >> 6 : 0;
-  F wpost[R::kPer], wpre[R::kPer], gate[R::kPer];
+  typename R::Packed wpost, wpre, gate;
   if (A.wpost) R::load(wpost, static_cast<const T*>(A.wpost), dim);
   if (A.wpre) R::load(wpre, static_cast<const T*>(A.wpre), dim);
   int64_t group = -1;
@@ -221,6 +249,24 @@ __device__ __forceinline__ void join_columns(const typename R::F (&v)[R::kPer], 
   }
 }
 
+// What the pullback reads of a row; what was not given is zero.
+template <class R>
+struct Inputs {
+  typename R::Packed dr, dn, x, f;
+  __device__ __forceinline__ void load(const NormArgs& A, const NormGrads& G, int64_t row) {
+    typedef typename R::T T;
+    const int64_t at = row * A.dim;
+    const auto one = [&](typename R::Packed& p, const void* from, bool given) {
+      p = typename R::Packed{};
+      if (given) R::load(p, static_cast<const T*>(from) + at, (int)A.dim);
+    };
+    one(dr, G.dr, G.dr != nullptr);
+    one(dn, G.dn, G.dn != nullptr);
+    one(x, A.x, G.dn != nullptr);
+    one(f, A.f, A.f != nullptr);
+  }
+};
+
 // Partial sums of a workgroup: parts[block][0] dwpost, [1] dwpre, [2] dgate (only where a
 // group has several parts), each dim floats.
 template <class R>
@@ -232,7 +278,7 @@ __global__ void __launch_bounds__(R::kThreads) norm_pullback_kernel(NormArgs A, 
   const int dim = (int)A.dim;
   const F inv_dim = (F)1 / (F)dim;
   const int sub = R::kWaves == 1 ? threadIdx.x >> 6 : 0;
-  F wpost[R::kPer], wpre[R::kPer], gate[R::kPer];
+  typename R::Packed wpost, wpre, gate;
   F spost[R::kPer] = {}, spre[R::kPer] = {};
   if (A.wpost) R::load(wpost, static_cast<const T*>(A.wpost), dim);
   if (A.wpre) R::load(wpre, static_cast<const T*>(A.wpre), dim);
@@ -246,21 +292,14 @@ __global__ void __launch_bounds__(R::kThreads) norm_pullback_kernel(NormArgs A, 
     if (A.gate && !own_gate) R::load(gate, static_cast<const T*>(A.gate) + g * A.dim, dim);
     for (int64_t row = first + sub; row < last; row += R::kRows) {
       const int64_t at = row * A.dim;
-      F d[R::kPer];
-      if (G.dr)
-        R::load(d, static_cast<const T*>(G.dr) + at, dim);
-      else
-#pragma unroll
-        for (int j = 0; j < R::kPer; ++j) d[j] = 0;
-      F r[R::kPer], fhat[R::kPer], dn[R::kPer], finv = 0;
+      Inputs<R> in;
+      in.load(A, G, row);
+      F d[R::kPer], r[R::kPer], fhat[R::kPer], dn[R::kPer], finv = 0;
+      R::unpack(d, in.dr);
+      R::unpack(r, in.x);
+      R::unpack(fhat, in.f);
+      R::unpack(dn, in.dn);
       if (own_gate) R::load(gate, static_cast<const T*>(A.gate) + at, dim);
-      if (A.f) {
-        R::load(fhat, static_cast<const T*>(A.f) + at, dim);
-      }
-      if (G.dn) {
-        R::load(r, static_cast<const T*>(A.x) + at, dim);
-        R::load(dn, static_cast<const T*>(G.dn) + at, dim);
-      }
       if (A.f && A.wpost) finv = standardise<R>(fhat, A.kind, dim, inv_dim, A.eps, lds);
       if (G.dn) {
         if (A.f)

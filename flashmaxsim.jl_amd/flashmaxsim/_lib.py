@@ -29,18 +29,6 @@ _f = ctypes.c_float
 _d = ctypes.c_double
 LENDER = ctypes.CFUNCTYPE(_p, _i64, _p)  # fms_workspace_lender: (bytes, stream) -> memory
 
-
-class AdamWEntry(ctypes.Structure):
-    """fms_adamw_tensor"""
-    _fields_ = [("p", _p), ("g", _p), ("m", _p), ("v", _p), ("master", _p), ("m_scale", _p),
-                ("v_scale", _p), ("n", _i64), ("p_dtype", _i32), ("g_dtype", _i32)]
-
-
-class Moment8Entry(ctypes.Structure):
-    """fms_moment8"""
-    _fields_ = [("codes", _p), ("scales", _p), ("values", _p), ("n", _i64), ("is_signed", _i64)]
-
-
 # name -> argtypes (restype fms_status = int32 unless listed in _RESTYPES)
 SIGNATURES = {
     "fms_status_string": [_i32],

@@ -35,30 +35,26 @@ def _cotangent(d, shape, proto, what):
     """A cotangent as a dense array of the feature eltype (None: zero)."""
     if d is None:
         return None
-    if not isinstance(d, torch.Tensor) or tuple(d.shape) != tuple(shape):
+    if not isinstance(d, torch.Tensor) or d.shape != shape:
         raise DimensionMismatch(f"{what} must have the shape {tuple(shape)}")
-    return d.to(device=proto.device, dtype=proto.dtype).contiguous()
+    if d.dtype != proto.dtype or d.device != proto.device:
+        d = d.to(device=proto.device, dtype=proto.dtype)
+    return d.contiguous()
 
 
 # ---- gated feed-forward --------------------------------------------------------------------
 
-def _ffn_check(x, wg, wu):
-    boundary.require_device(x, wg, wu)
+def _hidden(x, wg, wu):
+    """The weights' hidden units (the boundary checks shapes, eltypes and devices)."""
     if x.dim() < 1 or wg.dim() != 2 or wu.dim() != 2:
         raise DimensionMismatch("gated_ffn takes x (..., dim) and weights (hidden, dim)")
-    if wg.shape != wu.shape:
-        raise DimensionMismatch(f"wg {tuple(wg.shape)} and wu {tuple(wu.shape)} differ")
-    if wg.shape[1] != x.shape[-1]:
-        raise DimensionMismatch(f"feature dim: weights have {wg.shape[1]}, x has {x.shape[-1]}")
-    if wg.dtype != x.dtype or wu.dtype != x.dtype:
-        raise ArgumentError(f"the weights must have x's eltype {x.dtype}")
+    return wg.shape[0]
 
 
 def gated_ffn_forward(x, wg, wu, act="silu"):
     """h (..., hidden) = act(x wgᵀ) * (x wuᵀ) for x (..., dim), wg and wu (hidden, dim)."""
     code = _code(act, ACTIVATIONS, "act")
-    _ffn_check(x, wg, wu)
-    h = x.new_empty(x.shape[:-1] + (wg.shape[0],))
+    h = x.new_empty((*x.shape[:-1], _hidden(x, wg, wu)))
     boundary.launch_gated_ffn(h, x, wg, wu, code)
     return h
 
@@ -66,8 +62,7 @@ def gated_ffn_forward(x, wg, wu, act="silu"):
 def gated_ffn_pullback(dh, x, wg, wu, act="silu", need_dx=True, need_dw=True):
     """(dx, dwg, dwu) for the cotangent dh (..., hidden); None where not needed."""
     code = _code(act, ACTIVATIONS, "act")
-    _ffn_check(x, wg, wu)
-    dh = _cotangent(dh, x.shape[:-1] + (wg.shape[0],), x, "dh")
+    dh = _cotangent(dh, (*x.shape[:-1], _hidden(x, wg, wu)), x, "dh")
     if dh is None:
         raise DimensionMismatch("dh: missing")
     dx = torch.empty_like(x) if need_dx else None
@@ -100,32 +95,21 @@ def gated_ffn(x, wg, wu, act="silu"):
 # ---- norms around a block ------------------------------------------------------------------
 
 def _norm_check(x, f, gate, post_weight, pre_weight):
-    boundary.require_device(x, f, gate, post_weight, pre_weight)
+    """How many neighbouring rows share a gate vector (the boundary checks shapes, eltypes and
+    devices)."""
     if x.dim() < 1:
         raise DimensionMismatch("block_norm takes x (..., dim)")
-    for t, what in ((f, "f"), (gate, "gate"), (post_weight, "post_weight"),
-                    (pre_weight, "pre_weight")):
-        if t is not None and t.dtype != x.dtype:
-            raise ArgumentError(f"{what} must have x's eltype {x.dtype}, got {t.dtype}")
-    dim = x.shape[-1]
-    for t, what in ((post_weight, "post_weight"), (pre_weight, "pre_weight")):
-        if t is not None and tuple(t.shape) != (dim,):
-            raise DimensionMismatch(f"{what} must have the shape ({dim},), got {tuple(t.shape)}")
     if f is None:
         if gate is not None or post_weight is not None:
             raise ArgumentError("gate and post_weight need the branch f")
         if pre_weight is None:
             raise ArgumentError("block_norm has nothing to compute without f and pre_weight")
-    elif f.shape != x.shape:
-        raise DimensionMismatch(f"f {tuple(f.shape)} and x {tuple(x.shape)} differ")
     return _gate_rows(x, gate)
 
 
 def _gate_rows(x, gate):
-    """How many neighbouring rows share a gate vector."""
-    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
     if gate is None:
-        return max(rows, 1)
+        return max(x.shape[:-1].numel(), 1)
     lead = gate.dim() - 1
     if lead < 0 or lead > x.dim() - 1 or gate.shape != x.shape[:lead] + x.shape[-1:]:
         raise DimensionMismatch(

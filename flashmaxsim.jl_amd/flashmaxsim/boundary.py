@@ -90,6 +90,20 @@ def require_device(*ts):
     return dev
 
 
+def require_device_many(*lists):
+    """require_device for lists of many tensors."""
+    devices, dense = set(), True
+    for ts in lists:
+        try:
+            devices.update(map(torch.Tensor.get_device, ts))
+            dense = dense and all(map(torch.Tensor.is_contiguous, ts))
+        except TypeError:  # not a tensor
+            dense = False
+    if not dense or len(devices) != 1 or min(devices) < 0:
+        return require_device(*(t for ts in lists for t in ts))  # (says which check fails)
+    return next(t for ts in lists for t in ts).device
+
+
 def _mask(m):
     if m is None:
         return None
@@ -657,22 +671,26 @@ def _rows(x):
     return (x.numel() // dim if dim else x.shape[:-1].numel()), dim
 
 
+def _given(*ts):
+    return [t for t in ts if t is not None]
+
+
 def _same(t, shape, proto, what):
     """A feature array of an exact shape and the call's eltype."""
     if t.dtype != proto.dtype:
         raise ArgumentError(f"{what} must have the feature eltype {proto.dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise DimensionMismatch(f"{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def launch_gated_ffn(h, x, wg, wu, act):
     """h <- act(x wg^T) * (x wu^T); act is the library's code."""
-    dev = require_device(h, x, wg, wu)
+    dev = require_device_many([h, x, wg, wu])
     rows, dim = _rows(x)
     hidden = wg.shape[0]
     for w, what in ((wg, "wg"), (wu, "wu")):
         _same(w, (hidden, dim), x, what)
-    _same(h, x.shape[:-1] + (hidden,), x, "h")
+    _same(h, (*x.shape[:-1], hidden), x, "h")
     st = _call_with_workspace(_lib.lib().fms_gated_ffn, dev, dtype_code(x), ptr(h), ptr(x), ptr(wg),
                               ptr(wu), act, rows, dim, hidden, stream_handle(dev))
     _lib.check(st, "launch_gated_ffn")
@@ -680,7 +698,7 @@ def launch_gated_ffn(h, x, wg, wu, act):
 
 def gated_ffn_apply_pullback(dx, dwg, dwu, dh, x, wg, wu, act):
     """dx, dwg, dwu <- pullback of dh; dx, or dwg and dwu, may be None."""
-    dev = require_device(dx, dwg, dwu, dh, x, wg, wu)
+    dev = require_device_many(_given(dx, dwg, dwu, dh, x, wg, wu))
     rows, dim = _rows(x)
     hidden = wg.shape[0]
     for w, what in ((wg, "wg"), (wu, "wu"), (dwg, "dwg"), (dwu, "dwu")):
@@ -688,7 +706,7 @@ def gated_ffn_apply_pullback(dx, dwg, dwu, dh, x, wg, wu, act):
             _same(w, (hidden, dim), x, what)
     if dx is not None:
         _same(dx, x.shape, x, "dx")
-    _same(dh, x.shape[:-1] + (hidden,), x, "dh")
+    _same(dh, (*x.shape[:-1], hidden), x, "dh")
     st = _call_with_workspace(_lib.lib().fms_gated_ffn_pullback, dev, dtype_code(x), ptr(dx),
                               ptr(dwg), ptr(dwu), ptr(dh), ptr(x), ptr(wg), ptr(wu), act, rows, dim,
                               hidden, stream_handle(dev))
@@ -711,7 +729,7 @@ def _norm_arrays(x, gate_rows, gate, *groups):
 
 def launch_block_norm(r, n, x, f, gate, wpost, wpre, kind, scale, eps, gate_rows):
     """r, n <- x + scale gate norm(f) wpost, norm(r) wpre; kind is the library's code."""
-    dev = require_device(r, n, x, f, gate, wpost, wpre)
+    dev = require_device_many(_given(r, n, x, f, gate, wpost, wpre))
     rows, dim = _norm_arrays(x, gate_rows, gate, (x.shape, ((r, "r"), (n, "n"), (f, "f"))),
                              (x.shape[-1:], ((wpost, "post_weight"), (wpre, "pre_weight"))))
     if gate is not None:
@@ -724,7 +742,8 @@ def launch_block_norm(r, n, x, f, gate, wpost, wpre, kind, scale, eps, gate_rows
 
 def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre, kind,
                               scale, eps, gate_rows):
-    dev = require_device(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre)
+    dev = require_device_many(
+        _given(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre))
     rows, dim = _norm_arrays(
         x, gate_rows, gate,
         (x.shape, ((dx, "dx"), (df, "df"), (dr, "dr"), (dn, "dn"), (f, "f"))),
@@ -741,12 +760,13 @@ def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, 
 
 
 def adamw_step(table, step, lr, betas, eps, weight_decay, grad_scale, dev):
-    """One step over a table of the library's entries, whose arrays the caller has checked."""
-    st = _lib.lib().fms_adamw_step(len(table), table, step, lr, betas[0], betas[1], eps, weight_decay,
+    """One step over a (numpy) table of the library's entries, whose arrays the caller has checked."""
+    st = _lib.lib().fms_adamw_step(len(table), table.ctypes.data, step, lr, betas[0], betas[1], eps, weight_decay,
                                    grad_scale, stream_handle(dev))
     _lib.check(st, "adamw_step")
 
 
 def moment_values(table, dev):
     """Values of a table of 8-bit moments, whose arrays the caller has checked."""
-    _lib.check(_lib.lib().fms_moment_values(len(table), table, stream_handle(dev)), "moment_values")
+    _lib.check(_lib.lib().fms_moment_values(len(table), table.ctypes.data, stream_handle(dev)),
+               "moment_values")

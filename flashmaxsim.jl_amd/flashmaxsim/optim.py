@@ -1,7 +1,7 @@
 """AdamW over many tensors at once, with its moments in 32 or in 8 bits.
 
 The step that uses MaxSim's gradients (extension; the reference leaves the optimiser to its
-caller).  All tensors of a step go through one kernel, up to 48 a launch, in place:
+caller).  All tensors of a step go through one kernel, up to 52 a launch, in place:
 
     m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
@@ -15,14 +15,19 @@ sign(c) (c/127)^2 scale, v as uint8 codes with the value (c/255)^4 scale.
 """
 from __future__ import annotations
 
-import ctypes
-
+import numpy as np
 import torch
 
-from . import _lib, boundary
+from . import boundary
 from .errors import ArgumentError, DimensionMismatch
 
 MOMENT_BLOCK = 256
+# Entries of the library's tables (fms_adamw_tensor, fms_moment8).
+_ADAMW_ENTRY = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("master", "u8"),
+                         ("m_scale", "u8"), ("v_scale", "u8"), ("n", "i8"), ("p_dtype", "i4"),
+                         ("g_dtype", "i4")])
+_MOMENT_ENTRY = np.dtype([("codes", "u8"), ("scales", "u8"), ("values", "u8"), ("n", "i8"),
+                          ("is_signed", "i8")])
 
 
 class Moment8:
@@ -61,15 +66,18 @@ def moment_values(moments, out=None):
         raise DimensionMismatch(f"{len(out)} outputs for {len(moments)} moments")
     if not moments:
         return out
-    dev = boundary.require_device(*(t for m in moments for t in (m.codes, m.scales)), *out)
-    table = (_lib.Moment8Entry * len(moments))()
-    for e, m, o in zip(table, moments, out):
-        if o.dtype != torch.float32:
-            raise ArgumentError(f"moment values are float32, got {o.dtype}")
-        if o.numel() != m.codes.numel():
-            raise DimensionMismatch(f"{o.numel()} values for {m.codes.numel()} codes")
-        e.codes, e.scales, e.values = m.codes.data_ptr(), m.scales.data_ptr(), o.data_ptr()
-        e.n, e.is_signed = o.numel(), int(m.codes.dtype == torch.int8)
+    codes, scales = [m.codes for m in moments], [m.scales for m in moments]
+    dev = boundary.require_device_many(codes, scales, out)
+    numels = [c.numel() for c in codes]
+    if any(o.dtype != torch.float32 for o in out):
+        raise ArgumentError("moment values are float32")
+    if [o.numel() for o in out] != numels:
+        raise DimensionMismatch("as many values as codes")
+    table = np.empty(len(moments), _MOMENT_ENTRY)
+    for name, ts in (("codes", codes), ("scales", scales), ("values", out)):
+        table[name] = [t.data_ptr() for t in ts]
+    table["n"] = numels
+    table["is_signed"] = [c.dtype == torch.int8 for c in codes]
     boundary.moment_values(table, dev)
     return out
 
@@ -106,12 +114,12 @@ class AdamW:
         self.masters = (None,) * len(self.params) if not masters else tuple(masters)
         if not len(self.params) == len(self.m) == len(self.v) == len(self.masters):
             raise DimensionMismatch("AdamW: as many moments and masters as parameters")
-        self._shapes = [(p.numel(), p.dtype) for p in self.params]
         # the table of the library; a step fills in where parameters and gradients lie
-        self._held = self.m, self.v, self.masters  # what its other addresses belong to
-        self._table = (_lib.AdamWEntry * len(self.params))()
-        for e, p, c, m, v, w in zip(self._table, self.params, codes, self.m, self.v, self.masters):
-            e.n, e.p_dtype = p.numel(), c
+        self._numels, self._dtypes = [p.numel() for p in self.params], [p.dtype for p in self.params]
+        self._held = []  # what its other addresses belong to
+        self._table = np.zeros(len(self.params), _ADAMW_ENTRY)
+        self._table["n"], self._table["p_dtype"] = self._numels, codes
+        for e, p, m, v, w in zip(self._table, self.params, self.m, self.v, self.masters):
             self._place(e, p, m, v, w)
 
     def _place(self, e, p, m, v, master):
@@ -121,7 +129,8 @@ class AdamW:
             boundary.require_device(p, m.codes, m.scales, v.codes, v.scales)
             if m.codes.dtype != torch.int8 or v.codes.dtype != torch.uint8:
                 raise ArgumentError("AdamW: m has int8 codes and v uint8 codes")
-            e.m_scale, e.v_scale = m.scales.data_ptr(), v.scales.data_ptr()
+            e["m_scale"], e["v_scale"] = m.scales.data_ptr(), v.scales.data_ptr()
+            self._held += [m.scales, v.scales]
             m, v = m.codes, v.codes
         else:
             boundary.require_device(p, m, v)
@@ -129,14 +138,15 @@ class AdamW:
                 raise ArgumentError("AdamW: moments are float32 or Moment8")
         if not m.numel() == v.numel() == p.numel():
             raise DimensionMismatch("AdamW: the moments have their parameter's size")
-        e.m, e.v = m.data_ptr(), v.data_ptr()
+        e["m"], e["v"] = m.data_ptr(), v.data_ptr()
+        self._held += [m, v, master]
         if master is not None:
             boundary.require_device(p, master)
             if master.dtype != torch.float32:
                 raise ArgumentError("AdamW: masters are float32")
             if master.numel() != p.numel():
                 raise DimensionMismatch("AdamW: a master has its parameter's size")
-            e.master = master.data_ptr()
+            e["master"] = master.data_ptr()
 
     def step(self, grads=None, lr=None, grad_scale=1.0):
         """One step, in place.  grads: one per parameter, None to leave it as it is (default: the
@@ -145,21 +155,22 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise DimensionMismatch(f"{len(grads)} gradients for {len(self.params)} parameters")
-        table, params = self._table, self.params
-        if [(p.numel(), p.dtype) for p in params] != self._shapes:
+        params, numels, table = self.params, self._numels, self._table
+        if [p.numel() for p in params] != numels or [p.dtype for p in params] != self._dtypes:
             raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
-        if any(g is None for g in grads):
+        if [g for g in grads if g is None]:
             keep = [i for i, g in enumerate(grads) if g is not None]
             params, grads = [params[i] for i in keep], [grads[i] for i in keep]
-            table = (_lib.AdamWEntry * len(keep))(*(table[i] for i in keep))
+            numels, table = [numels[i] for i in keep], table[keep]
         if not grads:
             return
-        if boundary.require_device(*params, *grads) != self._device:
+        if boundary.require_device_many(params, grads) != self._device:
             raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
-        for e, p, g in zip(table, params, grads):
-            if g.numel() != e.n:
-                raise DimensionMismatch("AdamW: a gradient has its parameter's size")
-            e.p, e.g, e.g_dtype = p.data_ptr(), g.data_ptr(), boundary.dtype_code(g)
+        if [g.numel() for g in grads] != numels:
+            raise DimensionMismatch("AdamW: a gradient has its parameter's size")
+        table["p"] = [p.data_ptr() for p in params]
+        table["g"] = [g.data_ptr() for g in grads]
+        table["g_dtype"] = [boundary.dtype_code(g) for g in grads]
         boundary.adamw_step(table, self.steps + 1, self.lr if lr is None else lr, self.betas,
                             self.eps, self.weight_decay, grad_scale, self._device)
         self.steps += 1
