@@ -685,6 +685,7 @@ template <class Op, bool kMRows, bool kNRows, int kParts>
 struct Shapes {
   typedef Product<Op, kMRows, kNRows, kParts, 2, 4, 4> Big;    // 256 x 256, 8 waves
   typedef Product<Op, kMRows, kNRows, kParts, 2, 2, 2> Small;  // 128 x 128, 4 waves
+  typedef Product<Op, kMRows, kNRows, kParts, 2, 2, 1> Tiny;   // 64 x 128, 4 waves
 };
 
 template <class P, bool kPull>
@@ -698,9 +699,14 @@ hipError_t launch_gate(GateArgs g, hipStream_t st) {
   return hipGetLastError();
 }
 
-// 256 x 256 tiles run one workgroup to a CU; below one round of them the smaller tile
-// fills more CUs.
-bool big_tiles(int64_t rows, int64_t cols) { return cdiv(rows, 256) * cdiv(cols, 256) >= 192; }
+// 256 x 256 tiles run one workgroup to a CU; below one round of them 128 x 128 fills more
+// CUs, and where those leave every CU at most one, 64 x 128 does (2048 tokens of 768 x 2048 in
+// bf16: 16 us with 128 rows a tile, 21 with 64; 512 tokens: 11 and 9; in fp32 98 and 106, 54 and 32).
+enum class Shape { kTiny, kSmall, kBig };
+Shape gate_shape(int64_t rows, int64_t cols, int esz) {
+  if (esz == 2 && cdiv(rows, 256) * cdiv(cols, 256) >= 192) return Shape::kBig;
+  return cdiv(rows, 128) * cdiv(cols, 128) > 256 ? Shape::kSmall : Shape::kTiny;
+}
 
 template <class Op, int kNT>
 hipError_t launch_few(const GateArgs& g, hipStream_t st) {
@@ -710,13 +716,13 @@ hipError_t launch_few(const GateArgs& g, hipStream_t st) {
   return hipGetLastError();
 }
 
-// A round of few-token workgroups, each with 64 tokens, against the tiles' kernel, which below
-// 512 tiles takes the latency of its steps whatever the tokens (us, 768 x 2048 / 1024 x 4096):
-//   16 bits: 1 token 4.9 / 5.2 (tiles 9.8 / 11.9), 64 tokens 8.5 / 9.6 (10.0 / 12.2),
-//     128 tokens 8.6 / 17 (10.0 / 12.3): up to 256 workgroups.
-//   32 bits: 1 token 6.4 / 7.7 (53 / 70), 256 tokens 30 / 66 (54 / 71): up to 768 workgroups.
+// Few tokens: against the 64-row tiles, whose time does not fall with the tokens (us at
+// 768 x 2048 / 1024 x 4096):
+//   16 bits: 1 token 4.9 / 5.2, 32 tokens 6.4 / 7.2, 64 tokens 8.9 / 9.8 (tiles 8.0 / 9.6);
+//   32 bits: 1 token 6.4 / 7.7, 128 tokens 17 / 35 (tiles 31 / 42), 256 tokens 32 / 67 (32 / 42).
 bool few_tokens(const GateArgs& g, int esz) {
-  return cdiv(g.hidden, kFewHidden) * cdiv(g.tokens, 64) <= (esz == 2 ? 256 : 768);
+  if (esz == 2) return g.tokens <= 32;
+  return g.tokens <= 256 && cdiv(g.hidden, kFewHidden) * cdiv(g.tokens, 64) <= 512;
 }
 
 template <class Op, bool kPull>
@@ -732,9 +738,11 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
       return g.tokens <= 32 ? launch_few<Op, 2>(g, st) : launch_few<Op, 4>(g, st);
     }
   typedef Shapes<Op, true, true, 2> S;
+  const Shape shape = gate_shape(g.tokens, 2 * g.out_cols, Op::kEsz);
   if constexpr (Op::kEsz == 2)
-    if (big_tiles(g.tokens, 2 * g.out_cols)) return launch_gate<typename S::Big, kPull>(g, st);
-  return launch_gate<typename S::Small, kPull>(g, st);
+    if (shape == Shape::kBig) return launch_gate<typename S::Big, kPull>(g, st);
+  return shape == Shape::kSmall ? launch_gate<typename S::Small, kPull>(g, st)
+                                : launch_gate<typename S::Tiny, kPull>(g, st);
 }
 
 // ---- how the pullback's products are cut --------------------------------------------------
@@ -745,9 +753,10 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
 // parts, with the times measured on this card: of 23040 x 1024 x 4096 in bf16 the two
 // products take 620 us in one launch and 890 one after the other.
 struct Cut {
-  bool big;
+  Shape shape;
   int w, x;  // splits of the weights' products and of dx
 };
+
 // When `slots` workgroups at a time are through with nw units of uw us and then nx of ux.
 double makespan(int64_t nw, double uw, int64_t nx, double ux, int64_t slots) {
   if (nw + nx > 16 * slots) return ((double)nw * uw + (double)nx * ux) / (double)slots;
@@ -764,39 +773,40 @@ double makespan(int64_t nw, double uw, int64_t nx, double ux, int64_t slots) {
   }
   return end;
 }
-struct Costs {  // us: of a step, of a unit besides, of a MiB of parts written and read again
-  double step, unit, part;
-  int slots;
+// us of a step of a tile's unit that has a CU to itself, and of one of two on a CU.
+struct Costs {
+  int64_t rows, cols;  // of the tile
+  double alone, shared;
 };
+constexpr Costs kCosts16[3] = {{64, 128, 0.45, 0.70}, {128, 128, 0.58, 1.00}, {256, 256, 1.55, 0.0}};
+constexpr Costs kCosts32[2] = {{64, 128, 1.15, 2.20}, {128, 128, 2.10, 4.00}};
 
-int64_t units_of(const ProductArgs& p, int64_t span) {
-  return cdiv(p.rows, span) * cdiv(p.cols, span) * p.outputs;
-}
-
-Cut choose_cut(const ProductArgs* w, const ProductArgs* x, bool wide) {
-  Cut best = {false, 1, 1};
+Cut choose_cut(const ProductArgs* w, const ProductArgs* x, int esz) {
+  Cut best = {Shape::kSmall, 1, 1};
   double least = 1e300;
-  for (int big = 0; big < (wide ? 2 : 1); ++big) {
-    const Costs c = wide ? (big ? Costs{1.55, 4.0, 0.4, 256} : Costs{1.0, 3.0, 0.4, 512})
-                         : Costs{4.0, 3.0, 0.4, 512};
-    const int64_t span = big ? 256 : 128;
+  for (int shape = 0; shape < (esz == 2 ? 3 : 2); ++shape) {
+    const Costs& c = esz == 2 ? kCosts16[shape] : kCosts32[shape];
+    const auto tiles = [&](const ProductArgs* p) {
+      return p ? cdiv(p->rows, c.rows) * cdiv(p->cols, c.cols) * p->outputs : 0;
+    };
+    const int64_t tw = tiles(w), tx = tiles(x);
     for (int sw = 1; sw <= (w ? 64 : 1); sw *= 2)
       for (int sx = 1; sx <= (x ? 16 : 1); sx *= 2) {
-        double unit[2] = {0.0, 0.0}, joins = 0.0;
-        int64_t units[2] = {0, 0};
-        const auto add = [&](int i, const ProductArgs* p, int splits) {
-          if (p == nullptr) return;
-          unit[i] = c.unit + c.step * (double)cdiv(p->steps, splits);
-          units[i] = units_of(*p, span) * splits;
+        const bool alone = shape == (int)Shape::kBig || tw * sw + tx * sx <= 256;
+        // (besides its steps a unit takes about 3 us to begin and to end, and a second kernel 3
+        // us and the parts' way to memory and back)
+        double joins = 0.0;
+        const auto unit = [&](const ProductArgs* p, int splits) {
+          if (p == nullptr) return 0.0;
           if (splits > 1)
-            joins += 4.0 + c.part * splits * (double)(p->outputs * p->rows * p->cols) * 4 / (1 << 20);
+            joins += 3.0 + 0.4 * splits * (double)(p->outputs * p->rows * p->cols) * 4 / (1 << 20);
+          return 3.0 + (alone ? c.alone : c.shared) * (double)cdiv(p->steps, splits);
         };
-        add(0, w, sw);
-        add(1, x, sx);
-        const double t = makespan(units[0], unit[0], units[1], unit[1], c.slots) + joins;
+        const double uw = unit(w, sw), ux = unit(x, sx);
+        const double t = makespan(tw * sw, uw, tx * sx, ux, alone ? 256 : 512) + joins;
         if (t < least) {
           least = t;
-          best = Cut{big != 0, sw, sx};
+          best = Cut{(Shape)shape, sw, sx};
         }
       }
   }
@@ -839,12 +849,15 @@ template <class Op>
 hipError_t run_products(const ProductArgs* w, const ProductArgs* x, hipStream_t st) {
   typedef Shapes<Op, false, false, 1> W;
   typedef Shapes<Op, true, false, 1> X;
-  const Cut cut = choose_cut(w, x, Op::kEsz == 2);
+  const Cut cut = choose_cut(w, x, Op::kEsz);
   const ProductArgs none = {};
+  const ProductArgs &pw = w ? *w : none, &px = x ? *x : none;
   if constexpr (Op::kEsz == 2)
-    if (cut.big)
-      return launch_products<Op, typename W::Big, typename X::Big>(w ? *w : none, x ? *x : none, cut, st);
-  return launch_products<Op, typename W::Small, typename X::Small>(w ? *w : none, x ? *x : none, cut, st);
+    if (cut.shape == Shape::kBig)
+      return launch_products<Op, typename W::Big, typename X::Big>(pw, px, cut, st);
+  if (cut.shape == Shape::kSmall)
+    return launch_products<Op, typename W::Small, typename X::Small>(pw, px, cut, st);
+  return launch_products<Op, typename W::Tiny, typename X::Tiny>(pw, px, cut, st);
 }
 
 GateArgs gate_args(const FfnArgs& a, const Matrix (&m)[3]) {

@@ -17,7 +17,7 @@
 // LDS as they lie, in 16-byte units:
 //   rows:    kSpan rows of 128 bytes; the unit u of row r is at r*8 + (u ^ ((r >> 1) & 7)).
 //   columns: 128 / kEsz rows (k) of kSpan elements; unit u of row r is at
-//            r*kUpr + (u ^ (4 * (r & 3))).
+//            r*kUpr + (u ^ (4 * (r & 3))), or u ^ (4 * ((r >> 1) & 1)) in rows of 8 units.
 // The exclusive-or spreads the rows that sixteen lanes read together over all
 // 64 banks.  An LDS load's destination is linear in the lane, so it is the
 // lane's global address that is permuted.  16-bit columns are read with the
@@ -67,11 +67,11 @@ struct Stage {
   static constexpr int kUpr = kRows ? kStepBytes / 16 : kSpan * Op::kEsz / 16;  // units per LDS row
   static_assert(kUnits % (kThreads * kParts) == 0, "whole loads per part");
   static_assert(kRows || kParts == 1, "two parts only of rows");
-  static_assert(kRows || kUpr >= 16, "the swizzle spans 16 units");
+  static_assert(kRows || kUpr == 8 || kUpr >= 16, "the swizzle's span");
 
   // What unit indices of LDS row r are exclusive-or'ed with.
   __device__ static __forceinline__ int mix(int r) {
-    return kRows ? (r >> 1) & 7 : 4 * (r & 3);
+    return kRows ? (r >> 1) & 7 : kUpr == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
   }
 
   int voff[kLoads];  // this lane's offsets into the resource
@@ -146,7 +146,7 @@ struct Stage {
       const int i = lane & 15;
       const int r3 = (i >> 2) & 3;  // row & 3: the other parts of the row are multiples of 4
       const int unit = (at >> 3) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-      const char* p = lds + (16 * ks + 8 * h + r3) * (kUpr * 16) + ((unit ^ (4 * r3)) * 16) + (i & 1) * 8;
+      const char* p = lds + (16 * ks + 8 * h + r3) * (kUpr * 16) + ((unit ^ mix(r3)) * 16) + (i & 1) * 8;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * kUpr * 16));
       typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -159,7 +159,7 @@ struct Stage {
       for (int e = 0; e < 4; ++e) {
         const int row = 8 * ks + 4 * h + e;
         f[e] = *reinterpret_cast<const uint32_t*>(lds + row * (kUpr * 16) +
-                                                  (((col >> 2) ^ (4 * e)) * 16) + (col & 3) * 4);
+                                                  (((col >> 2) ^ mix(e)) * 16) + (col & 3) * 4);
       }
       return f;
     }
