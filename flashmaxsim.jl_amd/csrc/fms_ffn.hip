@@ -472,6 +472,7 @@ struct ProductArgs {
   Matrix m[2], n[2];
   int32_t segments;  // 2: out[0] = m0 n0 + m1 n1; 1: out[z] = m_z n_z
   int32_t outputs;
+  int64_t bytes;                  // of a segment's k
   int32_t tm, tn, steps, splits;  // steps of all segments
   int64_t rows, cols;
   void* out[2];
@@ -683,7 +684,11 @@ hipError_t place_inputs(const FfnArgs& a, const Inputs& in, char* ws, Matrix (&m
 // The tile shapes by element size: wave grid and 32-row fragments per wave.
 template <class Op, bool kMRows, bool kNRows, int kParts>
 struct Shapes {
-  typedef Product<Op, kMRows, kNRows, kParts, 2, 4, 4> Big;    // 256 x 256, 8 waves
+  // 256 x 256, 8 waves.  The pullback's products read dg and du from HBM and keep three
+  // shorter steps in flight (23040 x 1024 x 4096: 1490 us a training step, 1512 with one of 128
+  // bytes); the projections' operands come from the caches (290 us for 46080 x 768 x 2048, 315
+  // with shorter steps).
+  typedef Product<Op, kMRows, kNRows, kParts, 2, 4, 4, kParts == 2 ? 128 : 64> Big;
   typedef Product<Op, kMRows, kNRows, kParts, 2, 2, 2> Small;  // 128 x 128, 4 waves
   typedef Product<Op, kMRows, kNRows, kParts, 2, 2, 1> Tiny;   // 64 x 128, 4 waves
 };
@@ -692,7 +697,7 @@ template <class P, bool kPull>
 hipError_t launch_gate(GateArgs g, hipStream_t st) {
   g.tm = (int32_t)cdiv(g.tokens, P::kBM);
   g.tn = (int32_t)cdiv(g.out_cols, P::kBN / 2);
-  g.steps = (int32_t)cdiv(g.x.rowbytes, kStepBytes);
+  g.steps = (int32_t)cdiv(g.x.rowbytes, P::kStepBytes);
   const int tiles = g.tm * g.tn, most = P::kThreads == 512 ? 256 : 512;  // a round of workgroups
   hipLaunchKernelGGL((ffn_gate_kernel<P, kPull>), dim3((unsigned)(tiles < most ? tiles : most)),
                      dim3(P::kThreads), 0, st, g);
@@ -773,7 +778,7 @@ double makespan(int64_t nw, double uw, int64_t nx, double ux, int64_t slots) {
   }
   return end;
 }
-// us of a step of a tile's unit that has a CU to itself, and of one of two on a CU.
+// us of a step (128 bytes of k) of a tile's unit that has a CU to itself, and of one of two on a CU.
 struct Costs {
   int64_t rows, cols;  // of the tile
   double alone, shared;
@@ -800,7 +805,7 @@ Cut choose_cut(const ProductArgs* w, const ProductArgs* x, int esz) {
           if (p == nullptr) return 0.0;
           if (splits > 1)
             joins += 3.0 + 0.4 * splits * (double)(p->outputs * p->rows * p->cols) * 4 / (1 << 20);
-          return 3.0 + (alone ? c.alone : c.shared) * (double)cdiv(p->steps, splits);
+          return 3.0 + (alone ? c.alone : c.shared) * (double)cdiv(p->segments * cdiv(p->bytes, 128), splits);
         };
         const double uw = unit(w, sw), ux = unit(x, sx);
         const double t = makespan(tw * sw, uw, tx * sx, ux, alone ? 256 : 512) + joins;
@@ -818,6 +823,7 @@ hipError_t launch_products(ProductArgs w, ProductArgs x, const Cut& cut, hipStre
   const auto shape = [](ProductArgs& p, int64_t bm, int64_t bn, int splits) {
     p.tm = (int32_t)cdiv(p.rows, bm);
     p.tn = (int32_t)cdiv(p.cols, bn);
+    p.steps = p.segments * (int32_t)cdiv(p.bytes, PW::kStepBytes);
     p.splits = splits < p.steps ? splits : (p.steps > 0 ? p.steps : 1);
     p.part_pitch = round_up(p.cols, 4);
     return p.splits > 1 ? round_up((int64_t)p.splits * p.outputs * p.rows * p.part_pitch * 4, 256) : 0;
@@ -916,7 +922,7 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
   w.n[0] = w.n[1] = m[0];
   w.segments = 1;
   w.outputs = 2;
-  w.steps = (int32_t)cdiv(a.tokens * Op::kEsz, kStepBytes);
+  w.bytes = a.tokens * Op::kEsz;
   w.rows = a.hidden;
   w.cols = a.dim;
   w.out[0] = dwg;
@@ -928,7 +934,7 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
   x.n[1] = m[2];
   x.segments = 2;
   x.outputs = 1;
-  x.steps = 2 * (int32_t)cdiv(pitch, kStepBytes);
+  x.bytes = pitch;
   x.rows = a.tokens;
   x.cols = a.dim;
   x.out[0] = dx;

@@ -1,22 +1,25 @@
 // fms_gemm.hpp -- device building blocks of the products behind the gated
 // feed-forward block (fms_ffn.hip): out[m][n] = sum_k M(m, k) * N(n, k).
 //
-// A workgroup owns a kBM x kBN tile of the output and walks k in steps of 128
-// bytes per row.  Each step's slices of both operands go HBM/L2 -> LDS directly
-// (buffer loads with an LDS destination, no registers) into one of two buffers
-// while the step before is multiplied.  Two schedules:
+// A workgroup owns a kBM x kBN tile of the output at a time and walks k in steps of
+// kStepBytes per row.  A step's slices of both operands go HBM/L2 -> LDS directly
+// (buffer loads with an LDS destination, no registers) into one of 256 / kStepBytes
+// buffers while the steps before are multiplied.  Two schedules:
 //   four waves: small tiles, two workgroups to a CU; one's MFMAs run while the
 //     other waits at its barrier or is in its epilogue.
 //   eight waves, two to a SIMD: the first four and the last four take turns.  While
-//     one half multiplies two of a step's four k groups, the other reads the
-//     fragments of its next two, and a barrier swaps them: the matrix cores see one
-//     wave after the other without a gap, and no wave waits for LDS in between.
+//     one half multiplies two k groups, the other reads the fragments of its next
+//     two, and a barrier swaps them: the matrix cores see one wave after the
+//     other without a gap, and no wave waits for LDS in between.
+// Tiles of 256 x 256 multiply 8192-long random bf16 rows at 1.38 PFLOP/s (the card's
+// power bounds it: zeros run at 1.95), 128 x 128 at 1.1.
 //
 // An operand's matrix lies in memory either with k contiguous (a row per m or
 // n: "rows") or with m / n contiguous (a row per k: "columns").  Both land in
 // LDS as they lie, in 16-byte units:
-//   rows:    kSpan rows of 128 bytes; the unit u of row r is at r*8 + (u ^ ((r >> 1) & 7)).
-//   columns: 128 / kEsz rows (k) of kSpan elements; unit u of row r is at
+//   rows:    kSpan rows of kStepBytes; the unit u of row r is at r*8 + (u ^ ((r >> 1) & 7))
+//            (128 bytes) or r*4 + (u ^ ((r >> 2) & 3)) (64).
+//   columns: kStepBytes / kEsz rows (k) of kSpan elements; unit u of row r is at
 //            r*kUpr + (u ^ (4 * (r & 3))), or u ^ (4 * ((r >> 1) & 1)) in rows of 8 units.
 // The exclusive-or spreads the rows that sixteen lanes read together over all
 // 64 banks.  An LDS load's destination is linear in the lane, so it is the
@@ -35,8 +38,6 @@ namespace fms {
 typedef __attribute__((address_space(3))) void* lds_void_ptr;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kStepBytes = 128;            // k bytes of a row per step
-constexpr int kGroups = 4;                 // fragments of k per step
 constexpr int kOutOfBounds = (int)0x80000000u;  // an offset past every resource
 
 // A matrix as a product's operand: `rows` rows of `rowbytes` used bytes (a
@@ -58,7 +59,7 @@ __device__ __forceinline__ rsrc_t matrix_from(const Matrix& m, int64_t at) {
 // One operand's staging and fragment reads.  kRows: k contiguous.  kParts: the
 // span is made of 1 or 2 equal parts, each from a matrix of its own (gate and up
 // projections side by side).
-template <class Op, bool kRows, int kSpan, int kThreads, int kParts>
+template <class Op, bool kRows, int kSpan, int kThreads, int kParts, int kStepBytes>
 struct Stage {
   static constexpr int kBytes = kSpan * kStepBytes;
   static constexpr int kUnits = kBytes / 16;
@@ -71,7 +72,8 @@ struct Stage {
 
   // What unit indices of LDS row r are exclusive-or'ed with.
   __device__ static __forceinline__ int mix(int r) {
-    return kRows ? (r >> 1) & 7 : kUpr == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
+    if (kRows) return kUpr == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+    return kUpr == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
   }
 
   int voff[kLoads];  // this lane's offsets into the resource
@@ -189,17 +191,21 @@ struct Leg {
   bool ends;
 };
 
-// The tile's shape: kWM x kWN waves, each 32 kMF rows by 64 columns.
-template <class Op_, bool kMRows_, bool kNRows_, int kParts_, int kWM_, int kWN_, int kMF_>
+// The tile's shape: kWM x kWN waves, each 32 kMF rows by 64 columns; kStepBytes of k a step.
+template <class Op_, bool kMRows_, bool kNRows_, int kParts_, int kWM_, int kWN_, int kMF_,
+          int kStepBytes_ = 128>
 struct Product {
   typedef Op_ Op;
   static constexpr int kParts = kParts_, kWM = kWM_, kWN = kWN_, kMF = kMF_, kNF = 2;
   static constexpr int kThreads = 64 * kWM * kWN;
+  static constexpr int kStepBytes = kStepBytes_;
+  static constexpr int kGroups = kStepBytes / 32;  // fragments of k per step
+  static constexpr int kBuffers = 256 / kStepBytes;
   static constexpr int kBM = kWM * kMF * 32, kBN = kWN * 64;
-  typedef Stage<Op, kMRows_, kBM, kThreads, 1> StageM;
-  typedef Stage<Op, kNRows_, kBN, kThreads, kParts> StageN;
+  typedef Stage<Op, kMRows_, kBM, kThreads, 1, kStepBytes> StageM;
+  typedef Stage<Op, kNRows_, kBN, kThreads, kParts, kStepBytes> StageN;
   static constexpr int kBuffer = StageM::kBytes + StageN::kBytes;
-  static constexpr int kLds = 2 * kBuffer;
+  static constexpr int kLds = kBuffers * kBuffer;
   static constexpr bool kTurns = kWM * kWN == 8;
   static constexpr int kStepK = StageM::kStepK;
   typedef typename Op::Acc Acc;
@@ -281,22 +287,25 @@ struct Product {
     };
     enter();
     clear();
-    char *cur = lds, *other = lds + kBuffer;
-    const auto swap = [&] {
-      char* const x = cur;
-      cur = other;
-      other = x;
+    // the buffers in turn: step i is in buffer i % kBuffers
+    int at = 0;
+    const auto buffer = [&](int i) {  // of the i-th step from the current one
+      i += at;
+      return lds + (i >= kBuffers ? i - kBuffers : i) * kBuffer;
     };
-    request(cur);
+    const auto next = [&] { at = at + 1 == kBuffers ? 0 : at + 1; };
+    request(buffer(0));
     if constexpr (!kTurns) {
+      static_assert(kBuffers == 2 && kGroups == 4, "two buffers, four groups");
       for (int j = 0; j < legs; ++j) {
         const Legs l = leg(j);
         for (int s = 0; s < l.steps; ++s) {
           // this step's slices have landed; every wave has its last fragments of the step before
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
           turn();
+          const char* const cur = buffer(0);
           read(cur, 0, 0);
-          if (ahead < legs) request(other);
+          if (ahead < legs) request(buffer(1));
           if (s > 0) multiply_all(1);
           read(cur, 1, 1);
           multiply_all(0);
@@ -304,7 +313,7 @@ struct Product {
           multiply_all(1);
           read(cur, 3, 1);
           multiply_all(0);
-          swap();
+          next();
         }
         multiply_all(1);
         if (l.ends) {
@@ -313,31 +322,38 @@ struct Product {
         }
       }
     } else {
-      // Turn p: the first half of the waves reads at even p and multiplies at odd p, the
-      // second half one turn later.  Step i is read in turns 4i .. 4i + 3, and its buffer is
-      // free from turn 4i + 4 on.  A wave requests in the one multiplying turn of each step
-      // that comes right after a buffer became free, a load after every two MFMAs: the first
-      // half step i + 1 in turn 4i + 1, the second half step i + 2 in turn 4i + 4.  Each wave
-      // waits for its requests before the barrier that ends turn 4i + 3.
+      // Two k groups are read in one turn and multiplied in the next: the first half of the
+      // waves reads at even turns, the second half at odd ones.  With H = kGroups / 2, step i is
+      // read in turns 2H i .. 2H i + 2H - 1, and its buffer is free from turn 2H (i + 1) on.  A
+      // wave requests in the one multiplying turn of each step that comes right after a buffer
+      // became free, a load after every two MFMAs: the first half step i + kBuffers - 1 in turn
+      // 2H i + 1, the second half step i + kBuffers in turn 2H (i + 1).  Each wave waits for its
+      // requests of step i + 1, leaving the later ones in flight, before the barrier that ends
+      // turn 2H i + 2H - 1.
+      constexpr int kHalves = kGroups / 2, kInFlight = (kBuffers - 2) * kLoads;
       const bool second = wave >= 4;
-      if (second) request(other);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const auto landed = [] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight) : "memory"); };
+#pragma unroll
+      for (int i = 1; i < kBuffers - 1; ++i) request(buffer(i));
+      if (second) request(buffer(kBuffers - 1));
+      landed();
       turn();
       if (second) turn();
       for (int j = 0; j < legs; ++j) {
         const Legs l = leg(j);
         for (int s = 0; s < l.steps; ++s) {
           const bool end = j + 1 == legs && s + 1 == l.steps;
+          const char* const cur = buffer(0);
+          char* const to = buffer(second ? 0 : kBuffers - 1);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < kHalves; ++half) {
             read(cur, 2 * half, 0);
             read(cur, 2 * half + 1, 1);
             if (half == 0) aim();
-            if (half == 1 && second) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (half == kHalves - 1 && second) landed();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             turn();
-            const bool now = (half == 1) == second;
-            char* const to = half == 0 ? other : cur;
+            const bool now = kHalves == 1 || (half == 1) == second;
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < 2 * kMF; ++i) {
@@ -346,12 +362,13 @@ struct Product {
             }
             static_assert(kLoads <= 2 * kMF, "a load for every two MFMAs");
             __builtin_amdgcn_s_setprio(0);
-            // (at the very end the second half waits too: none is in flight when it is done)
-            if (half == 1 && (!second || end)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (half == kHalves - 1 && !second) landed();
+            // (at the very end no load is left in flight)
+            if (half == kHalves - 1 && end) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             turn();
           }
           advance();
-          swap();
+          next();
         }
         if (j + 1 == legs && !second) turn();
         if (l.ends) {
