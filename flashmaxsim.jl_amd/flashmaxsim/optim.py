@@ -26,6 +26,7 @@ MOMENT_BLOCK = 256
 _ADAMW_ENTRY = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("master", "u8"),
                          ("m_scale", "u8"), ("v_scale", "u8"), ("n", "i8"), ("p_dtype", "i4"),
                          ("g_dtype", "i4")])
+_numel, _address, _dtype = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.dtype.__get__
 _MOMENT_ENTRY = np.dtype([("codes", "u8"), ("scales", "u8"), ("values", "u8"), ("n", "i8"),
                           ("is_signed", "i8")])
 
@@ -156,7 +157,7 @@ class AdamW:
         if len(grads) != len(self.params):
             raise DimensionMismatch(f"{len(grads)} gradients for {len(self.params)} parameters")
         params, numels, table = self.params, self._numels, self._table
-        if [p.numel() for p in params] != numels or [p.dtype for p in params] != self._dtypes:
+        if list(map(_numel, params)) != numels or list(map(_dtype, params)) != self._dtypes:
             raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
         if [g for g in grads if g is None]:
             keep = [i for i, g in enumerate(grads) if g is not None]
@@ -166,11 +167,13 @@ class AdamW:
             return
         if boundary.require_device_many(params, grads) != self._device:
             raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
-        if [g.numel() for g in grads] != numels:
+        if list(map(_numel, grads)) != numels:
             raise DimensionMismatch("AdamW: a gradient has its parameter's size")
-        table["p"] = [p.data_ptr() for p in params]
-        table["g"] = [g.data_ptr() for g in grads]
-        table["g_dtype"] = [boundary.dtype_code(g) for g in grads]
+        table["p"] = list(map(_address, params))
+        table["g"] = list(map(_address, grads))
+        one_type = len(set(map(_dtype, grads))) == 1
+        table["g_dtype"] = (boundary.dtype_code(grads[0]) if one_type
+                            else [boundary.dtype_code(g) for g in grads])
         boundary.adamw_step(table, self.steps + 1, self.lr if lr is None else lr, self.betas,
                             self.eps, self.weight_decay, grad_scale, self._device)
         self.steps += 1
