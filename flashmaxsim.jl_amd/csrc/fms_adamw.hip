@@ -101,8 +101,7 @@ __device__ __forceinline__ float block_top(const float (&v)[kPer]) {
 
 __device__ __forceinline__ float value_m(int c, float a) {
   const float t = (float)c * (1.0f / 127.0f);
-  const float q = t * t * a;
-  return c < 0 ? -q : q;
+  return t * fabsf(t) * a;
 }
 __device__ __forceinline__ float value_v(int c, float a) {
   const float t = (float)c * (1.0f / 255.0f);
@@ -115,19 +114,21 @@ __device__ __forceinline__ void scale_of(float top, float& a, float& inv) {
   a = tiny ? 0.0f : top;
   inv = tiny ? 0.0f : 1.0f / top;
 }
-// round(sqrt(q) * 127) and round(q^(1/4) * 255) for q in 0..1 (NaN: 0), as IEEE square roots
-// give them.  The hardware's root is within a unit or two of that: only a product within
-// 2e-4 of a tie, one in 2500, needs the exact one (without this the step of 64 million
-// elements was bound by the roots' instructions, 205 us; now PLACEHOLDER).
-__device__ __forceinline__ int code_m(float q) {
-  float t = __builtin_amdgcn_sqrtf(q) * 127.0f, c = __builtin_rintf(t);
-  if (__builtin_expect(fabsf(t - c) > 0.4998f, 0)) c = __builtin_rintf(sqrtf(q) * 127.0f);
-  return c >= 0.0f ? (int)c : 0;
+// round(sqrt(q) * 127) and round(q^(1/4) * 255) for q in 0..1, as IEEE square roots give them,
+// the second at least 1 for a q above 0.  The hardware's root is within a unit or two of that:
+// only a product within 1e-4 of a tie needs the exact one.  (The step of 64 million 8-bit
+// elements is bound by its instructions: 205 us with exact roots, 143.)
+__device__ __forceinline__ float code_m(float q) {
+  const float t = __builtin_amdgcn_sqrtf(q) * 127.0f;
+  float c = __builtin_rintf(t);
+  if (__builtin_expect(fabsf(t - c) > 0.4999f, 0)) c = __builtin_rintf(sqrtf(q) * 127.0f);
+  return c;
 }
-__device__ __forceinline__ int code_v(float q) {
-  float t = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(q)) * 255.0f, c = __builtin_rintf(t);
-  if (__builtin_expect(fabsf(t - c) > 0.4998f, 0)) c = __builtin_rintf(sqrtf(sqrtf(q)) * 255.0f);
-  return q > 0.0f && c < 1.0f ? 1 : (c >= 0.0f ? (int)c : 0);
+__device__ __forceinline__ float code_v(float q) {
+  const float t = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(q)) * 255.0f;
+  float c = __builtin_rintf(t);
+  if (__builtin_expect(fabsf(t - c) > 0.4999f, 0)) c = __builtin_rintf(sqrtf(sqrtf(q)) * 255.0f);
+  return fmaxf(c, __builtin_ceilf(q));
 }
 
 // Codes of eight neighbouring elements.
@@ -232,12 +233,13 @@ __global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
     Codes cm = {{0u, 0u}}, cv = {{0u, 0u}};
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      int c = code_m(fabsf(m[e]) * im);
-      c = m[e] < 0.0f ? -c : c;
-      cm.w[e >> 2] |= (uint32_t)(c & 0xff) << (8 * (e & 3));
-      c = code_v(v[e] * iv);
-      cv.w[e >> 2] |= (uint32_t)c << (8 * (e & 3));
+      // (c + 128 as a byte, its top bit turned: c in two's complement)
+      const float c = copysignf(code_m(fabsf(m[e]) * im), m[e]) + 128.0f;
+      cm.w[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(c, e & 3, cm.w[e >> 2]);
+      cv.w[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(code_v(v[e] * iv), e & 3, cv.w[e >> 2]);
     }
+    cm.w[0] ^= 0x80808080u;
+    cm.w[1] ^= 0x80808080u;
     store_codes(cm, static_cast<uint8_t*>(t.m), k, n, vec);
     store_codes(cv, static_cast<uint8_t*>(t.v), k, n, vec);
     if ((threadIdx.x & 31) == 0 && k < n) {
