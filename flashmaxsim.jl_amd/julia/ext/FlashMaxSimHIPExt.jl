@@ -31,10 +31,11 @@
 #   candidates_apply_pullback!  src/backward_layouts.jl:187-202
 #   packed_apply_pullback!      src/packed.jl:384-390
 #   varlen_apply_pullback!      src/packed.jl:449-455
-# Three functions have no reference method and are called through the
+# These functions have no reference method and are called through the
 # extension module: packed_multi_scan (nq queries against one PackedSeq in
-# one pass), topk (the k best scores of every query column) and
-# load_int8_index (an Int8Index read from its at-rest file).
+# one pass), topk (the k best scores of every query column),
+# load_int8_index (an Int8Index read from its at-rest file), and the operators
+# of a token block: gated_ffn, gated_ffn_pullback, block_norm, block_norm_pullback.
 #
 # Score buffers.  Every scan entry point writes Float32 partials and scores.
 # The reference allocates them as dot_accum(T) / score_eltype(T)
@@ -672,6 +673,130 @@ function topk(scores::ROCMatrix{Float32}, k::Integer)
                 dptr(scores), nrows, ncols, k, dptr(vals), dptr(idx), stream_ptr()),
           "topk")
     vals, idx
+end
+
+# ---- token block -------------------------------------------------------------------
+# The block that makes token embeddings out of an encoder's token states, in Julia's
+# column-major shapes: states (dim, T...), weights (dim, hidden) and (dim,).
+
+const ACTIVATIONS = Dict(:silu => Int32(0), :gelu => Int32(1), :gelu_tanh => Int32(2))
+const NORMS = Dict(:rms => Int32(0), :layer => Int32(1))
+named(d, k, what) = get(() -> throw(ArgumentError("$what: $k")), d, k)
+same_size(a, b, what) = size(a) == size(b) || throw(DimensionMismatch(what))
+tokens_of(x) = prod(size(x)[2:end]; init = 1)
+
+function ffn_sizes(x, wg, wu)
+    same_size(wg, wu, "wg and wu")
+    size(wg, 1) == size(x, 1) || throw(DimensionMismatch("feature dim"))
+    size(x, 1), tokens_of(x), size(wg, 2)
+end
+
+"""
+    gated_ffn(x, wg, wu; act = :silu) -> h (hidden, T...)
+
+`act.(wg' x) .* (wu' x)`, both projections, activation and product in one kernel.
+"""
+function gated_ffn(x::ROCArray{T}, wg::ROCMatrix{T}, wu::ROCMatrix{T};
+                   act::Symbol = :silu) where {T<:AnyFeature}
+    require_gfx950("gated feed-forward")
+    dim, tokens, hidden = ffn_sizes(x, wg, wu)
+    h = similar(x, hidden, size(x)[2:end]...)
+    check(ccall((:fms_gated_ffn, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int64, Int64, Int64,
+                 Ptr{Cvoid}),
+                dtype_code(T), dptr(h), dptr(x), dptr(wg), dptr(wu),
+                named(ACTIVATIONS, act, "activation"), tokens, dim, hidden, stream_ptr()),
+          "gated feed-forward")
+    h
+end
+
+"""
+    gated_ffn_pullback(dh, x, wg, wu; act = :silu) -> (dx, dwg, dwu)
+"""
+function gated_ffn_pullback(dh::ROCArray{T}, x::ROCArray{T}, wg::ROCMatrix{T}, wu::ROCMatrix{T};
+                            act::Symbol = :silu) where {T<:AnyFeature}
+    require_gfx950("gated feed-forward pullback")
+    dim, tokens, hidden = ffn_sizes(x, wg, wu)
+    size(dh) == (hidden, size(x)[2:end]...) || throw(DimensionMismatch("dh"))
+    dx, dwg, dwu = similar(x), similar(wg), similar(wu)
+    check(ccall((:fms_gated_ffn_pullback, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Int32, Int64, Int64, Int64, Ptr{Cvoid}),
+                dtype_code(T), dptr(dx), dptr(dwg), dptr(dwu), dptr(dh), dptr(x), dptr(wg), dptr(wu),
+                named(ACTIVATIONS, act, "activation"), tokens, dim, hidden, stream_ptr()),
+          "gated feed-forward pullback")
+    dx, dwg, dwu
+end
+
+const MaybeArray{T} = Union{ROCArray{T}, Nothing}
+const MaybeVector{T} = Union{ROCVector{T}, Nothing}
+
+# Tokens per gate vector: gate is (dim,) or dim and x's trailing dimensions.
+function norm_sizes(x, f, gate, wpost, wpre)
+    dim = size(x, 1)
+    f === nothing || same_size(f, x, "f")
+    for w in (wpost, wpre)
+        w === nothing || length(w) == dim || throw(DimensionMismatch("norm weights"))
+    end
+    f === nothing && !(gate === nothing && wpost === nothing) &&
+        throw(ArgumentError("gate and wpost need the branch f"))
+    rows = tokens_of(x)
+    gate === nothing && return dim, rows, max(rows, 1)
+    tail = size(x)[(ndims(x) - ndims(gate) + 2):end]
+    ndims(gate) <= ndims(x) && size(gate) == (dim, tail...) || throw(DimensionMismatch("gate"))
+    dim, rows, max(rows ÷ max(prod(tail; init = 1), 1), 1)
+end
+
+"""
+    block_norm(x, f = nothing; gate, wpost, wpre, scale = 1, kind = :rms, eps = 1f-6) -> (r, n)
+
+`r = x .+ scale .* gate .* norm(f) .* wpost` and `n = norm(r) .* wpre` in one kernel; a part
+that is not given is left out (without `f`, r is x; without `wpre`, n is nothing).
+"""
+function block_norm(x::ROCArray{T}, f::MaybeArray{T} = nothing; gate::MaybeArray{T} = nothing,
+                    wpost::MaybeVector{T} = nothing, wpre::MaybeVector{T} = nothing, scale = 1,
+                    kind::Symbol = :rms, eps = 1.0f-6) where {T<:AnyFeature}
+    require_gfx950("block norm")
+    dim, rows, gate_rows = norm_sizes(x, f, gate, wpost, wpre)
+    r = f === nothing ? nothing : similar(x)
+    n = wpre === nothing ? nothing : similar(x)
+    check(ccall((:fms_block_norm, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Int32, Float32, Float32, Int64, Int64, Int64, Ptr{Cvoid}),
+                dtype_code(T), dptr(r), dptr(n), dptr(x), dptr(f), dptr(gate), dptr(wpost), dptr(wpre),
+                named(NORMS, kind, "norm"), Float32(scale), Float32(eps), rows, dim, gate_rows,
+                stream_ptr()),
+          "block norm")
+    (r === nothing ? x : r), n
+end
+
+"""
+    block_norm_pullback(dr, dn, x, f = nothing; gate, wpost, wpre, scale, kind, eps)
+        -> (dx, df, dgate, dwpost, dwpre)
+
+`dr` and `dn` are the cotangents of r and n, either `nothing` for zero.
+"""
+function block_norm_pullback(dr::MaybeArray{T}, dn::MaybeArray{T}, x::ROCArray{T},
+                             f::MaybeArray{T} = nothing; gate::MaybeArray{T} = nothing,
+                             wpost::MaybeVector{T} = nothing, wpre::MaybeVector{T} = nothing, scale = 1,
+                             kind::Symbol = :rms, eps = 1.0f-6) where {T<:AnyFeature}
+    require_gfx950("block norm pullback")
+    dim, rows, gate_rows = norm_sizes(x, f, gate, wpost, wpre)
+    for d in (dr, dn)
+        d === nothing || same_size(d, x, "cotangent")
+    end
+    like(a) = a === nothing ? nothing : similar(a)
+    dx, df, dgate, dwpost, dwpre = similar(x), like(f), like(gate), like(wpost), like(wpre)
+    check(ccall((:fms_block_norm_pullback, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Float32,
+                 Float32, Int64, Int64, Int64, Ptr{Cvoid}),
+                dtype_code(T), dptr(dx), dptr(df), dptr(dgate), dptr(dwpost), dptr(dwpre), dptr(dr),
+                dptr(dn), dptr(x), dptr(f), dptr(gate), dptr(wpost), dptr(wpre),
+                named(NORMS, kind, "norm"), Float32(scale), Float32(eps), rows, dim, gate_rows,
+                stream_ptr()),
+          "block norm pullback")
+    dx, df, dgate, dwpost, dwpre
 end
 
 # ---- Int8Index at rest -------------------------------------------------------------
