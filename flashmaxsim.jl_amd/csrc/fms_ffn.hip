@@ -740,7 +740,9 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
   if constexpr (!kPull)
     if (few_tokens(g, Op::kEsz)) {
       if (g.tokens <= 16) return launch_few<Op, 1>(g, st);
-      return g.tokens <= 32 ? launch_few<Op, 2>(g, st) : launch_few<Op, 4>(g, st);
+      if constexpr (Op::kEsz == 4)
+        if (g.tokens > 32) return launch_few<Op, 4>(g, st);
+      return launch_few<Op, 2>(g, st);
     }
   typedef Shapes<Op, true, true, 2> S;
   const Shape shape = gate_shape(g.tokens, 2 * g.out_cols, Op::kEsz);

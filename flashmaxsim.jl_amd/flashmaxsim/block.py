@@ -16,6 +16,7 @@ Sums run in fp32 and each output is rounded once.  Arrays must be dense and on t
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import boundary
 from .errors import ArgumentError, DimensionMismatch
@@ -79,6 +80,7 @@ class _GatedFFN(torch.autograd.Function):
         return gated_ffn_forward(x, wg, wu, act)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh):
         need = ctx.needs_input_grad
         x, wg, wu = ctx.saved_tensors
@@ -158,6 +160,7 @@ class _BlockNorm(torch.autograd.Function):
         return (None if f is None else r), n
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dr, dn):
         x, f, gate, post_weight, pre_weight = ctx.saved_tensors
         grads = block_norm_pullback(dr, dn, x, f, gate=gate, post_weight=post_weight,

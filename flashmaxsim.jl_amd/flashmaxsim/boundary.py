@@ -92,16 +92,14 @@ def require_device(*ts):
 
 def require_device_many(*lists):
     """require_device for lists of many tensors."""
-    devices, dense = set(), True
-    for ts in lists:
-        try:
-            devices.update(map(torch.Tensor.get_device, ts))
-            dense = dense and all(map(torch.Tensor.is_contiguous, ts))
-        except TypeError:  # not a tensor
-            dense = False
-    if not dense or len(devices) != 1 or min(devices) < 0:
-        return require_device(*(t for ts in lists for t in ts))  # (says which check fails)
-    return next(t for ts in lists for t in ts).device
+    ts = lists[0] if len(lists) == 1 else [t for ts in lists for t in ts]
+    try:
+        devices = set(map(torch.Tensor.get_device, ts))
+        if len(devices) == 1 and -1 not in devices and all(map(torch.Tensor.is_contiguous, ts)):
+            return ts[0].device
+    except TypeError:  # not a tensor
+        pass
+    return require_device(*ts)  # (says which check fails)
 
 
 def _mask(m):
@@ -666,97 +664,87 @@ def varlen_apply_pullback(dQ, dD, Qp, Dp, cu_q, cu_d, args, Delta, inv_n):
 
 # ---- token block (no reference method) --------------------------------------------------
 
-def _rows(x):
-    dim = x.shape[-1]
-    return (x.numel() // dim if dim else x.shape[:-1].numel()), dim
-
-
-def _given(*ts):
-    return [t for t in ts if t is not None]
-
-
-def _same(t, shape, proto, what):
-    """A feature array of an exact shape and the call's eltype."""
-    if t.dtype != proto.dtype:
-        raise ArgumentError(f"{what} must have the feature eltype {proto.dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise DimensionMismatch(f"{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+def _check_block(x, *groups):
+    """Device, density, eltype and shapes of a call's arrays: groups of (shape, names, arrays), an
+    array None where it is not given.  The device."""
+    given = [x]
+    dtype = x.dtype
+    for shape, names, arrays in groups:
+        for i, t in enumerate(arrays):
+            if t is None:
+                continue
+            given.append(t)
+            if t.dtype != dtype or t.shape != shape:
+                require_device_many(given)
+                what = names.split()[i]
+                if t.dtype != dtype:
+                    raise ArgumentError(f"{what} must have the feature eltype {dtype}, got {t.dtype}")
+                raise DimensionMismatch(
+                    f"{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+    return require_device_many(given)
 
 
 def launch_gated_ffn(h, x, wg, wu, act):
     """h <- act(x wg^T) * (x wu^T); act is the library's code."""
-    dev = require_device_many([h, x, wg, wu])
-    rows, dim = _rows(x)
-    hidden = wg.shape[0]
-    for w, what in ((wg, "wg"), (wu, "wu")):
-        _same(w, (hidden, dim), x, what)
-    _same(h, (*x.shape[:-1], hidden), x, "h")
-    st = _call_with_workspace(_lib.lib().fms_gated_ffn, dev, dtype_code(x), ptr(h), ptr(x), ptr(wg),
-                              ptr(wu), act, rows, dim, hidden, stream_handle(dev))
-    _lib.check(st, "launch_gated_ffn")
+    shape, hidden = x.shape, wg.shape[0]
+    dim, lead = shape[-1], shape[:-1]
+    dev = _check_block(x, ((hidden, dim), "wg wu", (wg, wu)), ((*lead, hidden), "h", (h,)))
+    st = _call_with_workspace(_lib.lib().fms_gated_ffn, dev, dtype_code(x), h.data_ptr(),
+                              x.data_ptr(), wg.data_ptr(), wu.data_ptr(), act, lead.numel(), dim,
+                              hidden, stream_handle(dev))
+    if st:
+        _lib.check(st, "launch_gated_ffn")
 
 
 def gated_ffn_apply_pullback(dx, dwg, dwu, dh, x, wg, wu, act):
     """dx, dwg, dwu <- pullback of dh; dx, or dwg and dwu, may be None."""
-    dev = require_device_many(_given(dx, dwg, dwu, dh, x, wg, wu))
-    rows, dim = _rows(x)
-    hidden = wg.shape[0]
-    for w, what in ((wg, "wg"), (wu, "wu"), (dwg, "dwg"), (dwu, "dwu")):
-        if w is not None:
-            _same(w, (hidden, dim), x, what)
-    if dx is not None:
-        _same(dx, x.shape, x, "dx")
-    _same(dh, (*x.shape[:-1], hidden), x, "dh")
+    shape, hidden = x.shape, wg.shape[0]
+    dim, lead = shape[-1], shape[:-1]
+    dev = _check_block(x, ((hidden, dim), "wg wu dwg dwu", (wg, wu, dwg, dwu)), (shape, "dx", (dx,)),
+                       ((*lead, hidden), "dh", (dh,)))
     st = _call_with_workspace(_lib.lib().fms_gated_ffn_pullback, dev, dtype_code(x), ptr(dx),
-                              ptr(dwg), ptr(dwu), ptr(dh), ptr(x), ptr(wg), ptr(wu), act, rows, dim,
-                              hidden, stream_handle(dev))
-    _lib.check(st, "gated_ffn_apply_pullback")
+                              ptr(dwg), ptr(dwu), dh.data_ptr(), x.data_ptr(), wg.data_ptr(),
+                              wu.data_ptr(), act, lead.numel(), dim, hidden, stream_handle(dev))
+    if st:
+        _lib.check(st, "gated_ffn_apply_pullback")
 
 
-def _norm_arrays(x, gate_rows, gate, *groups):
-    """Checks block_norm's arrays: groups of (shape, arrays with their names)."""
-    rows, dim = _rows(x)
-    if gate_rows < 1 or (gate is not None and rows % gate_rows != 0):
-        raise DimensionMismatch(f"{rows} rows in gates of {gate_rows}")
-    for shape, arrays in groups:
-        for t, what in arrays:
-            if t is not None:
-                _same(t, shape, x, what)
-    if gate is not None and rows > 0 and gate.numel() != rows // gate_rows * dim:
-        raise DimensionMismatch(f"gate: {gate.numel()} elements for {rows // gate_rows} gates")
-    return rows, dim
+def _check_gate(gate, rows, dim, gate_rows):
+    if gate is not None and (gate_rows < 1 or rows % gate_rows != 0
+                             or (rows > 0 and gate.numel() != rows // gate_rows * dim)):
+        raise DimensionMismatch(f"gate: {gate.numel()} elements, one vector for {gate_rows} of {rows} rows")
 
 
 def launch_block_norm(r, n, x, f, gate, wpost, wpre, kind, scale, eps, gate_rows):
     """r, n <- x + scale gate norm(f) wpost, norm(r) wpre; kind is the library's code."""
-    dev = require_device_many(_given(r, n, x, f, gate, wpost, wpre))
-    rows, dim = _norm_arrays(x, gate_rows, gate, (x.shape, ((r, "r"), (n, "n"), (f, "f"))),
-                             (x.shape[-1:], ((wpost, "post_weight"), (wpre, "pre_weight"))))
-    if gate is not None:
-        _same(gate, gate.shape, x, "gate")
-    st = _lib.lib().fms_block_norm(dtype_code(x), ptr(r), ptr(n), ptr(x), ptr(f), ptr(gate),
+    shape = x.shape
+    dim, rows = shape[-1], shape[:-1].numel()
+    dev = _check_block(x, (shape, "f r n", (f, r, n)),
+                       (shape[-1:], "post_weight pre_weight", (wpost, wpre)),
+                       (None if gate is None else gate.shape, "gate", (gate,)))
+    _check_gate(gate, rows, dim, gate_rows)
+    st = _lib.lib().fms_block_norm(dtype_code(x), ptr(r), ptr(n), x.data_ptr(), ptr(f), ptr(gate),
                                    ptr(wpost), ptr(wpre), kind, scale, eps, rows, dim, gate_rows,
                                    stream_handle(dev))
-    _lib.check(st, "launch_block_norm")
+    if st:
+        _lib.check(st, "launch_block_norm")
 
 
 def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre, kind,
                               scale, eps, gate_rows):
-    dev = require_device_many(
-        _given(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, wpost, wpre))
-    rows, dim = _norm_arrays(
-        x, gate_rows, gate,
-        (x.shape, ((dx, "dx"), (df, "df"), (dr, "dr"), (dn, "dn"), (f, "f"))),
-        (x.shape[-1:], ((wpost, "post_weight"), (wpre, "pre_weight"), (dwpost, "dpost_weight"),
-                        (dwpre, "dpre_weight"))))
-    if gate is not None:
-        _same(gate, gate.shape, x, "gate")
-        _same(dgate, gate.shape, x, "dgate")
+    shape = x.shape
+    dim, rows = shape[-1], shape[:-1].numel()
+    dev = _check_block(x, (shape, "f dx df dr dn", (f, dx, df, dr, dn)),
+                       (shape[-1:], "post_weight pre_weight dpost_weight dpre_weight",
+                        (wpost, wpre, dwpost, dwpre)),
+                       (None if gate is None else gate.shape, "gate dgate", (gate, dgate)))
+    _check_gate(gate, rows, dim, gate_rows)
     st = _call_with_workspace(
-        _lib.lib().fms_block_norm_pullback, dev, dtype_code(x), ptr(dx), ptr(df), ptr(dgate),
-        ptr(dwpost), ptr(dwpre), ptr(dr), ptr(dn), ptr(x), ptr(f), ptr(gate), ptr(wpost), ptr(wpre),
+        _lib.lib().fms_block_norm_pullback, dev, dtype_code(x), dx.data_ptr(), ptr(df), ptr(dgate),
+        ptr(dwpost), ptr(dwpre), ptr(dr), ptr(dn), x.data_ptr(), ptr(f), ptr(gate), ptr(wpost), ptr(wpre),
         kind, scale, eps, rows, dim, gate_rows, stream_handle(dev))
-    _lib.check(st, "block_norm_apply_pullback")
+    if st:
+        _lib.check(st, "block_norm_apply_pullback")
 
 
 def adamw_step(table, step, lr, betas, eps, weight_decay, grad_scale, dev):

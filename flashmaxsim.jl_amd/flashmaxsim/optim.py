@@ -88,7 +88,10 @@ class AdamW:
 
     bits: 32 (float32 moments) or 8 (``Moment8``); masters: True to keep float32 copies of
     16-bit parameters, or a list of them (None where a parameter has none); moments: a pair
-    of lists (m, v) to go on from, with ``step`` the steps already taken."""
+    of lists (m, v) to go on from, with ``step`` the steps already taken.
+
+    A step's number, rate and addresses are arguments of its kernels: captured in a graph it
+    would repeat the same step."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32,
                  masters=None, moments=None, step=0):
@@ -101,6 +104,8 @@ class AdamW:
         if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and self.steps >= 0):
             raise ArgumentError(f"AdamW: betas {self.betas}, eps {eps}, step {step}")
         self._device = boundary.require_device(*self.params)
+        if len(set(map(id, self.params))) != len(self.params):
+            raise ArgumentError("AdamW: a parameter is given twice")
         codes = [boundary.dtype_code(p) for p in self.params]
         if moments is None:
             if bits == 8:

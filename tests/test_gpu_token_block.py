@@ -57,3 +57,19 @@ def test_a_query_is_encoded_as_in_its_batch(example, device):
     with torch.no_grad():
         whole, alone = block(q), block(q[3:4])
     assert (whole[3:4].float() - alone.float()).abs().max() <= 4e-3
+
+
+def test_second_derivatives_are_refused(device):
+    """The pullbacks are not differentiable themselves, and say so."""
+    x = torch.randn(4, 32, device=device, requires_grad=True)
+    w = torch.randn(8, 32, device=device)
+    for y in (fm.gated_ffn(x, w, w), fm.block_norm(x, pre_weight=w[0])[1]):
+        (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+def test_a_parameter_given_twice_is_refused(device):
+    p = torch.zeros(8, device=device)
+    with pytest.raises(fm.ArgumentError):
+        fm.AdamW([p, p])
