@@ -577,25 +577,38 @@ __global__ void __launch_bounds__(PW::kThreads, 2) ffn_products_kernel(ProductAr
     product_unit<PX>(X, blockIdx.x - weights, lds);
 }
 
-// out[z][r][c] = sum over splits of parts[s][z][r][c], in the order of s.
+// out[z][r][c] = sum over splits of parts[s][z][r][c], in the order of s, of up to two products.
+struct JoinArgs {
+  void* out[2];
+  const float* parts;
+  int32_t splits, outputs;  // splits 0: nothing to join
+  int64_t rows, cols, pitch;
+};
 template <class Op>
-__global__ void __launch_bounds__(256) ffn_join_kernel(void* out0, void* out1, const float* parts,
-                                                       int splits, int nz, int64_t rows,
-                                                       int64_t cols, int64_t pitch) {
+__device__ __forceinline__ void join(const JoinArgs& A, int64_t i) {
   typedef typename OutOf<Op>::T T;
-  const int64_t quads = pitch / 4, each = rows * quads;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nz * each;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t z = i / each, r = i % each / quads, c = i % each % quads * 4;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; ++s) {
-      const f32x4 v =
-          *reinterpret_cast<const f32x4*>(parts + (((int64_t)s * nz + z) * rows + r) * pitch + c);
+  const int64_t quads = A.pitch / 4, each = A.rows * quads;
+  const int64_t z = i / each, r = i % each / quads, c = i % each % quads * 4;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = 0; s < A.splits; ++s) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(
+        A.parts + (((int64_t)s * A.outputs + z) * A.rows + r) * A.pitch + c);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += v[e];
-    }
-    T* p = static_cast<T*>(z ? out1 : out0) + r * cols + c;
-    for (int e = 0; e < 4 && c + e < cols; ++e) p[e] = (T)sum[e];
+    for (int e = 0; e < 4; ++e) sum[e] += v[e];
+  }
+  T* const p = static_cast<T*>(z ? A.out[1] : A.out[0]) + r * A.cols + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < A.cols) p[e] = (T)sum[e];
+}
+template <class Op>
+__global__ void __launch_bounds__(256) ffn_join_kernel(JoinArgs W, JoinArgs X, int64_t nw, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    if (i < nw)
+      join<Op>(W, i);
+    else
+      join<Op>(X, i - nw);
   }
 }
 
@@ -842,14 +855,18 @@ hipError_t launch_products(ProductArgs w, ProductArgs x, const Cut& cut, hipStre
   hipLaunchKernelGGL((ffn_products_kernel<PW, PX>), dim3((unsigned)(nw + nx)), dim3(PW::kThreads), 0, st,
                      w, x, (int)nw);
   e = hipGetLastError();
-  for (const ProductArgs* p : {&w, &x}) {
-    if (e != hipSuccess || p->splits == 1 || p->rows * p->cols == 0) continue;
-    hipLaunchKernelGGL((ffn_join_kernel<Op>), dim3(grid_for(p->outputs * p->rows * p->part_pitch / 4)),
-                       dim3(256), 0, st, p->out[0], p->out[1], p->parts, p->splits, p->outputs, p->rows,
-                       p->cols, p->part_pitch);
-    e = hipGetLastError();
-  }
-  return e;
+  const auto joined = [](const ProductArgs& p) {
+    return JoinArgs{{p.out[0], p.out[1]}, p.parts, p.splits > 1 ? p.splits : 0, p.outputs, p.rows, p.cols,
+                    p.part_pitch};
+  };
+  const auto quads = [](const ProductArgs& p) {
+    return p.splits > 1 ? p.outputs * p.rows * p.part_pitch / 4 : 0;
+  };
+  const int64_t jw = quads(w), jx = quads(x);
+  if (e != hipSuccess || jw + jx == 0) return e;
+  hipLaunchKernelGGL((ffn_join_kernel<Op>), dim3(grid_for(jw + jx)), dim3(256), 0, st, joined(w), joined(x),
+                     jw, jw + jx);
+  return hipGetLastError();
 }
 
 // w: dwg and dwu (or null), x: dx (or null).
