@@ -127,6 +127,19 @@ class AdamW:
         self._table["n"], self._table["p_dtype"] = self._numels, codes
         for e, p, m, v, w in zip(self._table, self.params, self.m, self.v, self.masters):
             self._place(e, p, m, v, w)
+        self._place_params()
+
+    def _place_params(self):
+        """Checks the parameters and notes where they lie.  Their memory is held until they are
+        seen elsewhere, so it is theirs as long as they are seen there."""
+        if ([p.numel() for p in self.params] != self._numels
+                or [p.dtype for p in self.params] != self._dtypes):
+            raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
+        if self.params and boundary.require_device(*self.params) != self._device:
+            raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+        self._memory = [p.detach() for p in self.params]
+        self._addresses = list(map(_address, self._memory))
+        self._table["p"] = self._addresses
 
     def _place(self, e, p, m, v, master):
         if isinstance(m, Moment8) != isinstance(v, Moment8):
@@ -162,19 +175,19 @@ class AdamW:
         if len(grads) != len(self.params):
             raise DimensionMismatch(f"{len(grads)} gradients for {len(self.params)} parameters")
         params, numels, table = self.params, self._numels, self._table
-        if list(map(_numel, params)) != numels or list(map(_dtype, params)) != self._dtypes:
-            raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
+        if (list(map(_address, params)) != self._addresses or list(map(_numel, params)) != numels
+                or not all(map(torch.Tensor.is_contiguous, params))):
+            self._place_params()
         if [g for g in grads if g is None]:
             keep = [i for i, g in enumerate(grads) if g is not None]
             params, grads = [params[i] for i in keep], [grads[i] for i in keep]
             numels, table = [numels[i] for i in keep], table[keep]
         if not grads:
             return
-        if boundary.require_device_many(params, grads) != self._device:
+        if boundary.require_device_many(grads) != self._device:
             raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
         if list(map(_numel, grads)) != numels:
             raise DimensionMismatch("AdamW: a gradient has its parameter's size")
-        table["p"] = list(map(_address, params))
         table["g"] = list(map(_address, grads))
         one_type = len(set(map(_dtype, grads))) == 1
         table["g_dtype"] = (boundary.dtype_code(grads[0]) if one_type

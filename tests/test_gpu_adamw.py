@@ -261,3 +261,21 @@ def test_refusals(device):
     with pytest.raises(fm.DimensionMismatch):
         fm.moment_values([fm.Moment8.zeros(torch.zeros(8, device=device), True)], [])
     assert opt.steps == 0
+
+
+def test_parameters_may_move(device):
+    """A parameter given new memory is stepped there; one turned into a strided view is refused."""
+    params, grads = tensors(device, torch.float32, sizes=[300, 64])
+    other = [p.clone() for p in params]
+    opt, ref = fm.AdamW(params, **HYPER), fm.AdamW(other, **HYPER)
+    opt.step(grads)
+    old = params[0].data
+    params[0].data = params[0].data.clone()
+    kept = old.clone()
+    opt.step(grads)
+    ref.step(grads)
+    ref.step(grads)
+    assert all(torch.equal(a, b) for a, b in zip(params, other)) and torch.equal(old, kept)
+    params[1].data = params[1].data.view(8, 8).t()
+    with pytest.raises(fm.ArgumentError):
+        opt.step(grads)
