@@ -17,8 +17,11 @@
 //
 // Bound by memory: 28 bytes an element in fp32, 22 with 16-bit parameters and gradients, 10
 // with 8-bit moments.  A workgroup takes 2048 elements of one tensor, eight a lane, so that
-// half a wave holds a block of 8-bit moments.  The tensors' pointers travel as kernel
-// arguments, up to 52 a launch: nothing is kept between calls and nothing is uploaded.
+// half a wave holds a block of 8-bit moments.  What stays (parameters, moments, sizes, and which
+// tensor a workgroup belongs to) is read from the caller's plan in device memory; the gradients'
+// addresses travel as kernel arguments, 480 to a launch.  (With whole tables as arguments, 52 to a
+// launch, 148 tensors of 8 million elements took three launches and 68 us,
+// now one and 62; 64 million 8-bit elements in 12 tensors take 262 us with their values, 254 then.)
 #include "fms_adamw.hpp"
 
 #include <float.h>
@@ -33,34 +36,41 @@ constexpr int kChunk = 256 * kPer;         // elements per workgroup
 constexpr int kBlock = FMS_MOMENT_BLOCK;   // elements that share a scale
 static_assert(kBlock == 32 * kPer, "a half wave holds a block");
 
+// The tensors' pointers come out of memory, where the compiler cannot tell that they are to
+// device memory (a flat access instead of a global one: 277 us against 273 for 64 million 8-bit
+// elements).
+template <class T>
+using Global = __attribute__((address_space(1))) T;
+template <class T>
+__device__ __forceinline__ Global<T>* global(T* p) {
+  return (Global<T>*)p;
+}
+
 // Eight neighbouring values from element k of n; vec: whole 16-byte units from the base on.
 template <class T>
 __device__ __forceinline__ void load8(float (&v)[kPer], const T* p, int64_t k, int64_t n, bool vec) {
+  typedef T V __attribute__((ext_vector_type(kPer), aligned(16)));
   if (vec && k + kPer <= n) {
-    typedef T V __attribute__((ext_vector_type(kPer)));
-    V u;
-    __builtin_memcpy(&u, __builtin_assume_aligned(p + k, sizeof(T) * kPer > 16 ? 16 : sizeof(T) * kPer),
-                     sizeof(u));
+    const V u = *(const Global<V>*)(global(p) + k);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) v[e] = (float)u[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = k + e < n ? (float)p[k + e] : 0.0f;
+    for (int e = 0; e < kPer; ++e) v[e] = k + e < n ? (float)global(p)[k + e] : 0.0f;
   }
 }
 template <class T>
 __device__ __forceinline__ void store8(const float (&v)[kPer], T* p, int64_t k, int64_t n, bool vec) {
+  typedef T V __attribute__((ext_vector_type(kPer), aligned(16)));
   if (vec && k + kPer <= n) {
-    typedef T V __attribute__((ext_vector_type(kPer)));
     V u;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) u[e] = (T)v[e];
-    __builtin_memcpy(__builtin_assume_aligned(p + k, sizeof(T) * kPer > 16 ? 16 : sizeof(T) * kPer),
-                     &u, sizeof(u));
+    *(Global<V>*)(global(p) + k) = u;
   } else {
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
-      if (k + e < n) p[k + e] = (T)v[e];
+      if (k + e < n) global(p)[k + e] = (T)v[e];
   }
 }
 __device__ __forceinline__ void load_typed(float (&v)[kPer], const void* p, int dtype, int64_t k,
@@ -117,7 +127,7 @@ __device__ __forceinline__ void scale_of(float top, float& a, float& inv) {
 // round(sqrt(q) * 127) and round(q^(1/4) * 255) for q in 0..1, as IEEE square roots give them,
 // the second at least 1 for a q above 0.  The hardware's root is within a unit or two of that:
 // only a product within 1e-4 of a tie needs the exact one.  (The step of 64 million 8-bit
-// elements is bound by its instructions: 205 us with exact roots, 143.)
+// elements is bound by its instructions: 205 us with exact roots, 149.)
 __device__ __forceinline__ float code_m(float q) {
   const float t = __builtin_amdgcn_sqrtf(q) * 127.0f;
   float c = __builtin_rintf(t);
@@ -139,70 +149,59 @@ struct Codes {
     return sign ? (int)(int8_t)b : (int)(b & 0xffu);
   }
 };
+typedef uint32_t CodeWords __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ Codes load_codes(const uint8_t* p, int64_t k, int64_t n, bool vec) {
   Codes c = {{0u, 0u}};
   if (vec && k + kPer <= n) {
-    __builtin_memcpy(&c, __builtin_assume_aligned(p + k, 8), 8);
+    const CodeWords w = *(const Global<CodeWords>*)(global(p) + k);
+    c.w[0] = w[0];
+    c.w[1] = w[1];
   } else {
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
-      if (k + e < n) c.w[e >> 2] |= (uint32_t)p[k + e] << (8 * (e & 3));
+      if (k + e < n) c.w[e >> 2] |= (uint32_t)global(p)[k + e] << (8 * (e & 3));
   }
   return c;
 }
 __device__ __forceinline__ void store_codes(const Codes& c, uint8_t* p, int64_t k, int64_t n, bool vec) {
   if (vec && k + kPer <= n) {
-    __builtin_memcpy(__builtin_assume_aligned(p + k, 8), &c, 8);
+    *(Global<CodeWords>*)(global(p) + k) = CodeWords{c.w[0], c.w[1]};
   } else {
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
-      if (k + e < n) p[k + e] = (uint8_t)(c.w[e >> 2] >> (8 * (e & 3)));
+      if (k + e < n) global(p)[k + e] = (uint8_t)(c.w[e >> 2] >> (8 * (e & 3)));
   }
 }
-
-constexpr int kTensors = 52;  // per launch: the arguments stay within 4 KiB
-struct Tensors {
-  fms_adamw_tensor t[kTensors];
-  int32_t end[kTensors];  // workgroups up to and with each tensor's
-  int32_t count;
-};
-static_assert(sizeof(Tensors) + sizeof(AdamWStep) <= 4096, "kernel arguments");
 
 template <class... P>
 __device__ __forceinline__ bool aligned(P... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
 }
 
-// The tensor a workgroup belongs to: the first whose end lies past it.
-template <class L>
-__device__ __forceinline__ int tensor_of(const L& l, int block) {
-  int lo = 0, hi = l.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (l.end[mid] > block)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return lo;
-}
+constexpr int kTensors = 480;  // per launch: the arguments stay within 4 KiB
+constexpr int kTypeShift = 56;  // a gradient's address and, above it, its element type
+struct Grads {
+  uint64_t g[kTensors];  // 0: none
+  int32_t first;         // tensor of the launch
+};
+static_assert(sizeof(Grads) + sizeof(AdamWStep) + 32 <= 4096, "kernel arguments");
 
-__global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
-  const int i = tensor_of(L, blockIdx.x);
-  const fms_adamw_tensor& t = L.t[i];
-  const int first = i > 0 ? L.end[i - 1] : 0;
-  const int64_t k = (int64_t)(blockIdx.x - first) * kChunk + threadIdx.x * kPer, n = t.n;
-  const bool vec = aligned(t.p, t.g, t.m, t.v, t.master), codes = t.m_scale != nullptr;
+// Eight elements a lane from k on; whole half waves take part past the tensor's end.
+__device__ __forceinline__ void adamw_elements(const fms_adamw_tensor& t, const void* grad, int g_dtype,
+                                           const AdamWStep& S, int64_t k, bool vec) {
+  const int64_t n = t.n;
+  const bool codes = t.m_scale != nullptr;
   float g[kPer], p[kPer], m[kPer], v[kPer];
-  load_typed(g, t.g, t.g_dtype, k, n, vec);
+  load_typed(g, grad, g_dtype, k, n, vec);
   if (t.master)
     load8(p, t.master, k, n, vec);
   else
-    load_typed(p, t.p, t.p_dtype, k, n, vec);
+    load_typed(p, t.p, (int)t.p_dtype, k, n, vec);
   if (codes) {
     const Codes cm = load_codes(static_cast<const uint8_t*>(t.m), k, n, vec);
     const Codes cv = load_codes(static_cast<const uint8_t*>(t.v), k, n, vec);
-    const float am = k < n ? t.m_scale[k / kBlock] : 0.0f, av = k < n ? t.v_scale[k / kBlock] : 0.0f;
+    const float am = k < n ? global(t.m_scale)[k / kBlock] : 0.0f;
+    const float av = k < n ? global(t.v_scale)[k / kBlock] : 0.0f;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       m[e] = value_m(cm.get(e, true), am);
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
     p[e] = p[e] * S.decay - m[e] / den * S.lr;
   }
   if (t.master) store8(p, t.master, k, n, vec);
-  store_typed(p, t.p, t.p_dtype, k, n, vec);
+  store_typed(p, t.p, (int)t.p_dtype, k, n, vec);
   if (codes) {
     // (elements past the end are zero and the whole half wave takes part)
     float am, im, av, iv;
@@ -243,13 +242,38 @@ __global__ void __launch_bounds__(256) adamw_kernel(Tensors L, AdamWStep S) {
     store_codes(cm, static_cast<uint8_t*>(t.m), k, n, vec);
     store_codes(cv, static_cast<uint8_t*>(t.v), k, n, vec);
     if ((threadIdx.x & 31) == 0 && k < n) {
-      t.m_scale[k / kBlock] = am;
-      t.v_scale[k / kBlock] = av;
+      global(t.m_scale)[k / kBlock] = am;
+      global(t.v_scale)[k / kBlock] = av;
     }
   } else {
     store8(m, static_cast<float*>(t.m), k, n, vec);
     store8(v, static_cast<float*>(t.v), k, n, vec);
   }
+}
+
+// A wave-uniform entry in scalar registers.
+__device__ __forceinline__ AdamWEntry uniform(const AdamWEntry& e) {
+  uint64_t w[sizeof(AdamWEntry) / 8];
+  __builtin_memcpy(w, &e, sizeof(e));
+#pragma unroll
+  for (uint64_t& x : w) x = rfl64(x);
+  AdamWEntry u;
+  __builtin_memcpy(&u, w, sizeof(u));
+  return u;
+}
+
+__global__ void __launch_bounds__(256) adamw_kernel(const AdamWEntry* entries, const int32_t* tensor_of,
+                                                    int64_t first_block, Grads G, AdamWStep S) {
+  const int64_t block = first_block + blockIdx.x;
+  const int at = __builtin_amdgcn_readfirstlane(tensor_of[block]), i = at - G.first;
+  const uint64_t g = G.g[i];
+  if (g == 0) return;  // (the whole workgroup)
+  const void* const grad = reinterpret_cast<const void*>(g & (((uint64_t)1 << kTypeShift) - 1));
+  // (copied to scalar registers: what the stores below may alias would be read again after them)
+  const AdamWEntry entry = uniform(entries[at]);
+  const fms_adamw_tensor& t = entry.t;
+  adamw_elements(t, grad, (int)(g >> kTypeShift), S, (block - entry.first) * kChunk + threadIdx.x * kPer,
+                 aligned(t.p, grad, t.m, t.v, t.master));
 }
 
 constexpr int kMoments = 92;
@@ -261,7 +285,15 @@ struct Moments {
 static_assert(sizeof(Moments) <= 4096, "kernel arguments");
 
 __global__ void __launch_bounds__(256) moment_values_kernel(Moments L) {
-  const int i = tensor_of(L, blockIdx.x);
+  // the first whose workgroups end past this one
+  int i = 0;
+  for (int hi = L.count - 1; i < hi;) {
+    const int mid = (i + hi) >> 1;
+    if (L.end[mid] > (int)blockIdx.x)
+      hi = mid;
+    else
+      i = mid + 1;
+  }
   const fms_moment8& t = L.t[i];
   const int first = i > 0 ? L.end[i - 1] : 0;
   const int64_t k = (int64_t)(blockIdx.x - first) * kChunk + threadIdx.x * kPer, n = t.n;
@@ -276,19 +308,49 @@ __global__ void __launch_bounds__(256) moment_values_kernel(Moments L) {
   store8(v, t.values, k, n, vec);
 }
 
-// Hands `launch` lists of up to kMost tensors whose workgroups fit one grid.  A tensor's
-// workgroups beyond a grid's are no concern: 2^22 of them are 2^33 elements, and a larger
-// tensor does not fit the memory of the device with its moments.
-template <class L, class T, int kMost, class F>
-hipError_t in_lists(int64_t count, const T* tensors, F&& launch) {
+}  // namespace
+
+int64_t adamw_blocks(const fms_adamw_tensor& t) { return (t.n + kChunk - 1) / kChunk; }
+
+hipError_t adamw_step(const AdamWPlan* plan, const void* device_plan, const void* const* grads,
+                      const int32_t* g_dtypes, const AdamWStep& s, hipStream_t stream) {
+  const AdamWEntry* const entries = reinterpret_cast<const AdamWEntry*>(plan + 1);
+  const AdamWEntry* const on_device =
+      reinterpret_cast<const AdamWEntry*>(static_cast<const AdamWPlan*>(device_plan) + 1);
+  const int32_t* const tensor_of = reinterpret_cast<const int32_t*>(on_device + plan->count);
   constexpr int64_t kGrid = (int64_t)1 << 23;
-  static thread_local L list;
+  for (int64_t i = 0; i < plan->count;) {
+    // as many tensors as the arguments and the grid take (a tensor alone fits: fms_adamw_plan)
+    Grads g;
+    g.first = (int32_t)i;
+    const int64_t first = entries[i].first;
+    int64_t last = first;
+    int n = 0;
+    for (; i < plan->count && n < kTensors; ++i, ++n) {
+      const int64_t end = entries[i].first + adamw_blocks(entries[i].t);
+      if (n > 0 && end - first > kGrid) break;
+      last = end;
+      g.g[n] = reinterpret_cast<uint64_t>(grads[i]);
+      if (g.g[n] != 0) g.g[n] |= (uint64_t)g_dtypes[i] << kTypeShift;
+    }
+    if (last == first) continue;
+    hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)(last - first)), dim3(256), 0, stream, on_device,
+                       tensor_of, first, g, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t moment_values(int64_t count, const fms_moment8* moments, hipStream_t stream) {
+  // lists of as many as the arguments and the grid take
+  Moments list;
   list.count = 0;
   int64_t blocks = 0;
   for (int64_t i = 0; i <= count; ++i) {
-    const int64_t need = i < count ? (tensors[i].n + kChunk - 1) / kChunk : 0;
-    if (list.count > 0 && (i == count || list.count == kMost || blocks + need > kGrid)) {
-      launch(list, (unsigned)blocks);
+    const int64_t need = i < count ? (moments[i].n + kChunk - 1) / kChunk : 0;
+    if (list.count > 0 && (i == count || list.count == kMoments || blocks + need > ((int64_t)1 << 23))) {
+      hipLaunchKernelGGL(moment_values_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, list);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       list.count = 0;
@@ -296,27 +358,10 @@ hipError_t in_lists(int64_t count, const T* tensors, F&& launch) {
     }
     if (need == 0) continue;
     blocks += need;
-    list.t[list.count] = tensors[i];
+    list.t[list.count] = moments[i];
     list.end[list.count++] = (int32_t)blocks;
   }
   return hipSuccess;
-}
-
-}  // namespace
-
-hipError_t adamw_step(int64_t count, const fms_adamw_tensor* tensors, const AdamWStep& s,
-                      hipStream_t stream) {
-  return in_lists<Tensors, fms_adamw_tensor, kTensors>(
-      count, tensors, [&](const Tensors& l, unsigned blocks) {
-        hipLaunchKernelGGL(adamw_kernel, dim3(blocks), dim3(256), 0, stream, l, s);
-      });
-}
-
-hipError_t moment_values(int64_t count, const fms_moment8* moments, hipStream_t stream) {
-  return in_lists<Moments, fms_moment8, kMoments>(
-      count, moments, [&](const Moments& l, unsigned blocks) {
-        hipLaunchKernelGGL(moment_values_kernel, dim3(blocks), dim3(256), 0, stream, l);
-      });
 }
 
 }  // namespace fms

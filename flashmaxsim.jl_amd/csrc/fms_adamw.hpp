@@ -18,8 +18,18 @@ struct AdamWStep {
   float grad_scale;
 };
 
-hipError_t adamw_step(int64_t count, const fms_adamw_tensor* tensors, const AdamWStep& s,
-                      hipStream_t stream);
+// A plan: this header, `count` entries, and for each workgroup of a step over all tensors the
+// tensor it belongs to.  The same bytes on the host and on the device.
+struct AdamWPlan {
+  int64_t count, blocks;
+};
+struct AdamWEntry {
+  fms_adamw_tensor t;
+  int64_t first;  // workgroup of its first element
+};
+int64_t adamw_blocks(const fms_adamw_tensor& t);
+hipError_t adamw_step(const AdamWPlan* plan, const void* device_plan, const void* const* grads,
+                      const int32_t* g_dtypes, const AdamWStep& s, hipStream_t stream);
 hipError_t moment_values(int64_t count, const fms_moment8* moments, hipStream_t stream);
 
 }  // namespace fms

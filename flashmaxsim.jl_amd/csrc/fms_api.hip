@@ -1130,19 +1130,63 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
   return from_hip(norm_pullback(a, g, as_stream(stream)));
 }
 
-fms_status fms_adamw_step(int64_t count, const fms_adamw_tensor* tensors, int64_t step, double lr,
-                          double beta1, double beta2, double eps, double weight_decay,
-                          double grad_scale, void* stream) {
-  if (count < 0 || (count > 0 && !tensors) || step < 1) return FMS_EINVAL;
-  // (negated: a NaN is refused too)
-  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return FMS_EINVAL;
+// The workgroups of a step over all tensors; -1 and *status where a tensor is not valid.
+static int64_t adamw_check(int64_t count, const fms_adamw_tensor* tensors, fms_status* status) {
+  *status = FMS_EINVAL;
+  if (count < 0 || count > INT32_MAX || (count > 0 && !tensors)) return -1;
+  int64_t blocks = 0;
   for (int64_t i = 0; i < count; ++i) {
     const fms_adamw_tensor& t = tensors[i];
-    if (elem_bytes(t.p_dtype) == 0 || elem_bytes(t.g_dtype) == 0) return FMS_EUNSUPPORTED;
-    if (t.n < 0 || (t.m_scale == nullptr) != (t.v_scale == nullptr)) return FMS_EINVAL;
-    if (t.n > 0 && (!t.p || !t.g || !t.m || !t.v)) return FMS_EINVAL;
-    if (t.n > ((int64_t)1 << 33)) return FMS_EUNSUPPORTED;
+    if (t.n < 0 || (t.m_scale == nullptr) != (t.v_scale == nullptr)) return -1;
+    if (t.n > 0 && (!t.p || !t.m || !t.v)) return -1;
+    if (t.p_dtype < 0 || t.p_dtype > FMS_BF16 || t.n > ((int64_t)1 << 33)) {
+      *status = FMS_EUNSUPPORTED;
+      return -1;
+    }
+    blocks += adamw_blocks(t);
   }
+  *status = FMS_OK;
+  return blocks;
+}
+
+int64_t fms_adamw_plan_bytes(int64_t count, const fms_adamw_tensor* tensors) {
+  fms_status s;
+  const int64_t blocks = adamw_check(count, tensors, &s);
+  return blocks < 0 ? -1
+                    : (int64_t)sizeof(AdamWPlan) + count * (int64_t)sizeof(AdamWEntry) + blocks * 4;
+}
+
+fms_status fms_adamw_plan(int64_t count, const fms_adamw_tensor* tensors, void* plan) {
+  fms_status s;
+  const int64_t blocks = adamw_check(count, tensors, &s);
+  if (s != FMS_OK) return s;
+  if (!plan) return FMS_EINVAL;
+  AdamWPlan* const head = static_cast<AdamWPlan*>(plan);
+  head->count = count;
+  head->blocks = blocks;
+  AdamWEntry* const entries = reinterpret_cast<AdamWEntry*>(head + 1);
+  int32_t* const tensor_of = reinterpret_cast<int32_t*>(entries + count);
+  int64_t at = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    entries[i].t = tensors[i];
+    entries[i].first = at;
+    for (const int64_t end = at + adamw_blocks(tensors[i]); at < end; ++at) tensor_of[at] = (int32_t)i;
+  }
+  return FMS_OK;
+}
+
+fms_status fms_adamw_step(const void* plan, const void* device_plan, const void* const* grads,
+                          const int32_t* g_dtypes, int64_t step, double lr, double beta1,
+                          double beta2, double eps, double weight_decay, double grad_scale,
+                          void* stream) {
+  if (!plan || step < 1) return FMS_EINVAL;
+  // (negated: a NaN is refused too)
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return FMS_EINVAL;
+  const AdamWPlan* const p = static_cast<const AdamWPlan*>(plan);
+  if (p->blocks == 0) return FMS_OK;
+  if (!device_plan || !grads || !g_dtypes) return FMS_EINVAL;
+  for (int64_t i = 0; i < p->count; ++i)
+    if (grads[i] && elem_bytes(g_dtypes[i]) == 0) return FMS_EUNSUPPORTED;
   AdamWStep s;
   s.beta1 = (float)beta1;
   s.rest1 = (float)(1.0 - beta1);
@@ -1153,7 +1197,7 @@ fms_status fms_adamw_step(int64_t count, const fms_adamw_tensor* tensors, int64_
   s.lr = (float)(lr / (1.0 - pow(beta1, (double)step)));
   s.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
   s.grad_scale = (float)grad_scale;
-  return from_hip(adamw_step(count, tensors, s, as_stream(stream)));
+  return from_hip(adamw_step(p, device_plan, grads, g_dtypes, s, as_stream(stream)));
 }
 
 fms_status fms_moment_values(int64_t count, const fms_moment8* moments, void* stream) {

@@ -80,7 +80,9 @@ SIGNATURES = {
     "fms_block_norm": [_i32, _p, _p, _p, _p, _p, _p, _p, _i32, _f, _f, _i64, _i64, _i64, _p],
     "fms_block_norm_pullback": [_i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _f, _f,
                                 _i64, _i64, _i64, _p],
-    "fms_adamw_step": [_i64, _p, _i64, _d, _d, _d, _d, _d, _d, _p],
+    "fms_adamw_plan_bytes": [_i64, _p],
+    "fms_adamw_plan": [_i64, _p, _p],
+    "fms_adamw_step": [_p, _p, _p, _p, _i64, _d, _d, _d, _d, _d, _d, _p],
     "fms_moment_values": [_i64, _p, _p],
 }
 _RESTYPES = {
@@ -88,6 +90,7 @@ _RESTYPES = {
     "fms_arch_supported": ctypes.c_int,
     "fms_version": ctypes.c_char_p,
     "fms_debug_workspace_allocs": ctypes.c_uint64,
+    "fms_adamw_plan_bytes": _i64,
     "fms_set_workspace_lender": None,
 }
 

@@ -38,6 +38,7 @@ from __future__ import annotations
 
 import threading
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -747,10 +748,20 @@ def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, 
         _lib.check(st, "block_norm_apply_pullback")
 
 
-def adamw_step(table, step, lr, betas, eps, weight_decay, grad_scale, dev):
-    """One step over a (numpy) table of the library's entries, whose arrays the caller has checked."""
-    st = _lib.lib().fms_adamw_step(len(table), table.ctypes.data, step, lr, betas[0], betas[1], eps, weight_decay,
-                                   grad_scale, stream_handle(dev))
+def adamw_plan(table):
+    """The library's plan for a (numpy) table of fms_adamw_tensor entries, as host bytes."""
+    n = _lib.lib().fms_adamw_plan_bytes(len(table), table.ctypes.data)
+    plan = np.zeros(max(n, 16), np.uint8)
+    _lib.check(_lib.lib().fms_adamw_plan(len(table), table.ctypes.data, plan.ctypes.data), "adamw_plan")
+    return plan
+
+
+def adamw_step(plan, device_plan, grads, g_dtypes, step, lr, betas, eps, weight_decay, grad_scale, dev):
+    """One step over a plan and its copy on the device; grads and g_dtypes are numpy arrays of
+    the gradients' addresses (0: none) and element types, which the caller has checked."""
+    st = _lib.lib().fms_adamw_step(plan.ctypes.data, device_plan.data_ptr(), grads.ctypes.data,
+                                   g_dtypes.ctypes.data, step, lr, betas[0], betas[1], eps,
+                                   weight_decay, grad_scale, stream_handle(dev))
     _lib.check(st, "adamw_step")
 
 

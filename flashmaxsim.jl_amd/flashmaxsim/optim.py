@@ -1,7 +1,7 @@
 """AdamW over many tensors at once, with its moments in 32 or in 8 bits.
 
 The step that uses MaxSim's gradients (extension; the reference leaves the optimiser to its
-caller).  All tensors of a step go through one kernel, up to 52 a launch, in place:
+caller).  All tensors of a step go through one kernel, up to 480 a launch, in place:
 
     m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
@@ -23,9 +23,8 @@ from .errors import ArgumentError, DimensionMismatch
 
 MOMENT_BLOCK = 256
 # Entries of the library's tables (fms_adamw_tensor, fms_moment8).
-_ADAMW_ENTRY = np.dtype([("p", "u8"), ("g", "u8"), ("m", "u8"), ("v", "u8"), ("master", "u8"),
-                         ("m_scale", "u8"), ("v_scale", "u8"), ("n", "i8"), ("p_dtype", "i4"),
-                         ("g_dtype", "i4")])
+_ADAMW_ENTRY = np.dtype([(k, "u8") for k in ("p", "m", "v", "master", "m_scale", "v_scale")]
+                        + [("n", "i8"), ("p_dtype", "i8")])
 _numel, _address, _dtype = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.dtype.__get__
 _MOMENT_ENTRY = np.dtype([("codes", "u8"), ("scales", "u8"), ("values", "u8"), ("n", "i8"),
                           ("is_signed", "i8")])
@@ -120,9 +119,9 @@ class AdamW:
         self.masters = (None,) * len(self.params) if not masters else tuple(masters)
         if not len(self.params) == len(self.m) == len(self.v) == len(self.masters):
             raise DimensionMismatch("AdamW: as many moments and masters as parameters")
-        # the table of the library; a step fills in where parameters and gradients lie
+        # the table of the library, and what its addresses belong to
         self._numels, self._dtypes = [p.numel() for p in self.params], [p.dtype for p in self.params]
-        self._held = []  # what its other addresses belong to
+        self._held = []
         self._table = np.zeros(len(self.params), _ADAMW_ENTRY)
         self._table["n"], self._table["p_dtype"] = self._numels, codes
         for e, p, m, v, w in zip(self._table, self.params, self.m, self.v, self.masters):
@@ -140,6 +139,11 @@ class AdamW:
         self._memory = [p.detach() for p in self.params]
         self._addresses = list(map(_address, self._memory))
         self._table["p"] = self._addresses
+        self._plan = boundary.adamw_plan(self._table)
+        if self.params:
+            if hasattr(self, "_device_plan"):
+                torch.cuda.synchronize(self._device)  # (steps on any stream may still read the old one)
+            self._device_plan = torch.from_numpy(self._plan).to(self._device)
 
     def _place(self, e, p, m, v, master):
         if isinstance(m, Moment8) != isinstance(v, Moment8):
@@ -174,26 +178,30 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise DimensionMismatch(f"{len(grads)} gradients for {len(self.params)} parameters")
-        params, numels, table = self.params, self._numels, self._table
+        params, numels = self.params, self._numels
         if (list(map(_address, params)) != self._addresses or list(map(_numel, params)) != numels
                 or not all(map(torch.Tensor.is_contiguous, params))):
             self._place_params()
+        addresses = np.zeros(len(params), np.uint64)
+        keep = slice(None)
         if [g for g in grads if g is None]:
             keep = [i for i, g in enumerate(grads) if g is not None]
             params, grads = [params[i] for i in keep], [grads[i] for i in keep]
-            numels, table = [numels[i] for i in keep], table[keep]
+            numels = [numels[i] for i in keep]
         if not grads:
             return
         if boundary.require_device_many(grads) != self._device:
             raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
         if list(map(_numel, grads)) != numels:
             raise DimensionMismatch("AdamW: a gradient has its parameter's size")
-        table["g"] = list(map(_address, grads))
+        addresses[keep] = list(map(_address, grads))
+        dtypes = np.zeros(len(addresses), np.int32)
         one_type = len(set(map(_dtype, grads))) == 1
-        table["g_dtype"] = (boundary.dtype_code(grads[0]) if one_type
-                            else [boundary.dtype_code(g) for g in grads])
-        boundary.adamw_step(table, self.steps + 1, self.lr if lr is None else lr, self.betas,
-                            self.eps, self.weight_decay, grad_scale, self._device)
+        dtypes[keep] = (boundary.dtype_code(grads[0]) if one_type
+                        else [boundary.dtype_code(g) for g in grads])
+        boundary.adamw_step(self._plan, self._device_plan, addresses, dtypes, self.steps + 1,
+                            self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay,
+                            grad_scale, self._device)
         self.steps += 1
         torch.autograd.graph.increment_version(params)
 

@@ -501,23 +501,30 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
  * are n floats each, or, with m_scale and v_scale (both), n codes each (int8 / uint8) and a
  * float for every FMS_MOMENT_BLOCK elements:
  *   m = sign(c) (c / 127)^2 scale,  v = (c / 255)^4 scale
- * The table is read before the call returns.
+ *
+ * The tensors are laid out once, in a plan: fms_adamw_plan writes fms_adamw_plan_bytes
+ * bytes of host memory, of which the caller keeps a copy in device memory (16-byte aligned).
+ * A step reads both and the gradients' addresses and element types, host arrays that are read
+ * before the call returns; a NULL gradient leaves its tensor as it is.  One launch takes up
+ * to 480 tensors.
  */
 #define FMS_MOMENT_BLOCK 256
 typedef struct fms_adamw_tensor {
-  void* p;       /* n values of p_dtype */
-  const void* g; /* n values of g_dtype */
+  void* p; /* n values of p_dtype */
   void* m;
   void* v;
   float* master;  /* n floats or NULL */
   float* m_scale; /* ceil(n / FMS_MOMENT_BLOCK) floats or NULL */
   float* v_scale;
   int64_t n;
-  int32_t p_dtype, g_dtype;
+  int64_t p_dtype;
 } fms_adamw_tensor;
-fms_status fms_adamw_step(int64_t count, const fms_adamw_tensor* tensors, int64_t step, double lr,
-                          double beta1, double beta2, double eps, double weight_decay,
-                          double grad_scale, void* stream);
+int64_t fms_adamw_plan_bytes(int64_t count, const fms_adamw_tensor* tensors); /* -1: invalid */
+fms_status fms_adamw_plan(int64_t count, const fms_adamw_tensor* tensors, void* plan);
+fms_status fms_adamw_step(const void* plan, const void* device_plan, const void* const* grads,
+                          const int32_t* g_dtypes, int64_t step, double lr, double beta1,
+                          double beta2, double eps, double weight_decay, double grad_scale,
+                          void* stream);
 
 /* The values of 8-bit moments, many at once: is_signed 1 for m's codes, 0 for v's. */
 typedef struct fms_moment8 {

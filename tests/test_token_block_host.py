@@ -1,7 +1,5 @@
 """CPU checks of the token-block operators: status codes of the C entries and refusals of the
 Python layer, all before any HIP call."""
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -11,6 +9,14 @@ from flashmaxsim import _lib, optim
 
 OK, EINVAL, EUNSUP = _lib.FMS_OK, _lib.FMS_EINVAL, _lib.FMS_EUNSUPPORTED
 NAN = float("nan")
+
+
+def adamw(L, plan=0, step=1, beta1=0.9, beta2=0.999, eps=1e-8):
+    """fms_adamw_step over an empty plan."""
+    empty = np.zeros(16, np.uint8)
+    assert L.fms_adamw_plan_bytes(0, None) == 16 and L.fms_adamw_plan(0, None, empty.ctypes.data) == OK
+    return L.fms_adamw_step(empty.ctypes.data if plan == 0 else plan, None, None, None, step, 1e-3, beta1,
+                            beta2, eps, 0.0, 1.0, None)
 
 
 @pytest.mark.parametrize("call,expect", [
@@ -50,14 +56,16 @@ NAN = float("nan")
                                          1.0, 1e-6, 4, 8, 4, None), EINVAL),  # no df
     (lambda L: L.fms_block_norm_pullback(0, 1, 1, None, None, None, 1, None, 1, 1, 1, None, None, 0,
                                          1.0, 1e-6, 4, 8, 4, None), EINVAL),  # no dgate
-    # AdamW: table, step, hyperparameters
-    (lambda L: L.fms_adamw_step(-1, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None), EINVAL),
-    (lambda L: L.fms_adamw_step(1, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None), EINVAL),
-    (lambda L: L.fms_adamw_step(0, None, 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None), EINVAL),
-    (lambda L: L.fms_adamw_step(0, None, 1, 1e-3, 1.0, 0.999, 1e-8, 0.0, 1.0, None), EINVAL),
-    (lambda L: L.fms_adamw_step(0, None, 1, 1e-3, 0.9, NAN, 1e-8, 0.0, 1.0, None), EINVAL),
-    (lambda L: L.fms_adamw_step(0, None, 1, 1e-3, 0.9, 0.999, -1.0, 0.0, 1.0, None), EINVAL),
-    (lambda L: L.fms_adamw_step(0, None, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None), OK),
+    # AdamW: plan, step, hyperparameters
+    (lambda L: L.fms_adamw_plan(-1, None, 1), EINVAL),
+    (lambda L: L.fms_adamw_plan(1, None, 1), EINVAL),
+    (lambda L: L.fms_adamw_plan(0, None, None), EINVAL),
+    (lambda L: adamw(L, plan=None), EINVAL),
+    (lambda L: adamw(L, step=0), EINVAL),
+    (lambda L: adamw(L, beta1=1.0), EINVAL),
+    (lambda L: adamw(L, beta2=NAN), EINVAL),
+    (lambda L: adamw(L, eps=-1.0), EINVAL),
+    (lambda L: adamw(L), OK),  # a plan of nothing
     (lambda L: L.fms_moment_values(-1, None, None), EINVAL),
     (lambda L: L.fms_moment_values(2, None, None), EINVAL),
     (lambda L: L.fms_moment_values(0, None, None), OK),
@@ -66,28 +74,47 @@ def test_status_codes(call, expect):
     assert call(_lib.lib()) == expect
 
 
-def test_adamw_table_entries_are_checked():
+def test_adamw_plans():
+    """Entries are checked, and a plan holds them with the tensor of each 2048 elements."""
+    L = _lib.lib()
+
     def status(**entry):
         t = np.zeros(1, optim._ADAMW_ENTRY)
-        for k, v in (dict(p=1, g=1, m=1, v=1, n=8) | entry).items():
+        for k, v in (dict(p=1, m=1, v=1, n=8) | entry).items():
             t[k] = v
-        return _lib.lib().fms_adamw_step(1, t.ctypes.data, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None)
+        plan = np.zeros(4096, np.uint8)
+        s = L.fms_adamw_plan(1, t.ctypes.data, plan.ctypes.data)
+        assert (L.fms_adamw_plan_bytes(1, t.ctypes.data) < 0) == (s != OK)
+        return s
 
-    assert status(p_dtype=9) == EUNSUP and status(g_dtype=-1) == EUNSUP
-    assert status(n=-1) == EINVAL and status(g=0) == EINVAL and status(v=0) == EINVAL
+    assert status(p_dtype=9) == EUNSUP and status(p_dtype=-1) == EUNSUP
+    assert status(n=-1) == EINVAL and status(p=0) == EINVAL and status(v=0) == EINVAL
     assert status(m_scale=1) == EINVAL  # one scale without the other
     assert status(n=(1 << 33) + 1) == EUNSUP
-    assert status(n=0, p=0, g=0, m=0, v=0) == OK
+    assert status(n=0, p=0, m=0, v=0) == OK
+
+    t = np.zeros(4, optim._ADAMW_ENTRY)
+    t["p"] = t["m"] = t["v"] = 16
+    t["n"] = [1, 0, 2049, 4096]
+    n = L.fms_adamw_plan_bytes(4, t.ctypes.data)
+    assert n == 16 + 4 * 72 + 5 * 4
+    plan = np.zeros(n + 4, np.uint8)
+    assert L.fms_adamw_plan(4, t.ctypes.data, plan.ctypes.data) == OK
+    assert plan[:16].view(np.int64).tolist() == [4, 5] and not plan[n:].any()
+    assert plan[16 + 4 * 72:n].view(np.int32).tolist() == [0, 2, 2, 3, 3]
+    entries = plan[16:16 + 4 * 72].view(np.int64).reshape(4, 9)
+    assert entries[:, 8].tolist() == [0, 1, 1, 3] and entries[:, 6].tolist() == [1, 0, 2049, 4096]
+    # a step refuses gradients of unknown types and missing arrays before it launches
+    grads, dtypes = np.full(4, 16, np.uint64), np.array([0, 1, 7, 2], np.int32)
+    args = (1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None)
+    assert L.fms_adamw_step(plan.ctypes.data, 16, grads.ctypes.data, dtypes.ctypes.data, *args) == EUNSUP
+    assert L.fms_adamw_step(plan.ctypes.data, None, grads.ctypes.data, dtypes.ctypes.data, *args) == EINVAL
+    assert L.fms_adamw_step(plan.ctypes.data, 16, None, dtypes.ctypes.data, *args) == EINVAL
 
 
 def test_table_layout_is_the_headers():
-    """fms_adamw_tensor: seven pointers, n, two dtypes; fms_moment8: three pointers, n, a flag."""
-    class Entry(ctypes.Structure):
-        _fields_ = [(k, ctypes.c_void_p) for k in ("p", "g", "m", "v", "master", "m_scale", "v_scale")] + [
-            ("n", ctypes.c_int64), ("p_dtype", ctypes.c_int32), ("g_dtype", ctypes.c_int32)]
-
-    assert optim._ADAMW_ENTRY.itemsize == ctypes.sizeof(Entry) == 72
-    assert all(optim._ADAMW_ENTRY.fields[k][1] == getattr(Entry, k).offset for k, _ in Entry._fields_)
+    """fms_adamw_tensor: six pointers, n, a dtype; fms_moment8: three pointers, n, a flag."""
+    assert optim._ADAMW_ENTRY.itemsize == 64 and optim._ADAMW_ENTRY.fields["n"][1] == 48
     assert optim._MOMENT_ENTRY.itemsize == 40
 
 
