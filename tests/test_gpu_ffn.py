@@ -48,10 +48,10 @@ def inputs(device, t, k, f, dtype, seed=0, offset=0):
     return make(t, k, scale=1.0), make(f, k, scale=s), make(f, k, scale=s), make(t, f, scale=0.1)
 
 
-def reference(x, wg, wu, dh, act, dtype):
+def reference(x, wg, wu, dh, act, dtype, where="cpu"):
     """{name: (value, bound)} in 64 bits."""
     u_out, least = HALF_ULP[dtype], LEAST[dtype]
-    x, wg, wu, dh = (a.cpu().double() for a in (x, wg, wu, dh))
+    x, wg, wu, dh = (a.to(where).double() for a in (x, wg, wu, dh))
     k, f, t = x.shape[1], wg.shape[0], x.shape[0]
     g, u = x @ wg.T, x @ wu.T
     eg = 2 * F32 * (k + 2) * (x.abs() @ wg.abs().T)
@@ -78,7 +78,7 @@ def reference(x, wg, wu, dh, act, dtype):
 
 def check(got, want, what):
     value, bound = want
-    off = (got.cpu().double() - value).abs()
+    off = (got.to(value.device).double() - value).abs()
     bad = ~(off <= bound)
     assert not bad.any(), (what, int(bad.sum()), bad.numel(), float((off / bound).max()))
 
@@ -103,6 +103,18 @@ def test_many_tiles(device, shape, dtype):
     want = reference(x, wg, wu, dh, "silu", dtype)
     check(fm.gated_ffn_forward(x, wg, wu), want["h"], "h")
     for name, got in zip(("dx", "dwg", "dwu"), fm.gated_ffn_pullback(dh, x, wg, wu)):
+        check(got, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(6200, 264, 1037), (6200, 201, 1032), (9001, 513, 2055),
+                                   (20011, 1000, 2000)], ids=str)
+def test_large_and_odd(device, shape, dtype):
+    """The large tiles with rows and widths that end inside them, whole 16-byte units or not."""
+    x, wg, wu, dh = inputs(device, *shape, dtype)
+    want = reference(x, wg, wu, dh, "gelu_tanh", dtype, device)
+    check(fm.gated_ffn_forward(x, wg, wu, "gelu_tanh"), want["h"], "h")
+    for name, got in zip(("dx", "dwg", "dwu"), fm.gated_ffn_pullback(dh, x, wg, wu, "gelu_tanh")):
         check(got, want[name], name)
 
 
