@@ -434,10 +434,13 @@ hipError_t norm_pullback(const NormArgs& a, const NormGrads& g, hipStream_t stre
     Spans s;
     s.group_rows = a.gate && a.gate_rows > 1 ? a.gate_rows : a.rows;
     s.ngroups = a.rows / s.group_rows;
-    // about two workgroups of four waves to a CU, at least four rows a wave
+    // about two workgroups of four waves to a CU; with fewer rows one or two rows a wave, so that
+    // they are read at once (999 rows of 531 in fp32: 16 us, 24 with four a wave and 21 with one,
+    // whose many partial sums take longer to join; 32 rows of 768: 9 with one, 11 with two)
     const int64_t target = 512 * 256 / R::kThreads;
     int64_t span = cdiv(a.rows, target);
-    if (span < 4 * R::kRows) span = 4 * R::kRows;
+    const int64_t least = a.rows <= 64 * R::kRows ? R::kRows : 2 * R::kRows;
+    if (span < least) span = least;
     s.parts = s.group_rows > span ? cdiv(s.group_rows, span) : 1;
     s.groups = s.parts == 1 ? span / s.group_rows : 1;
     s.blocks = s.parts == 1 ? cdiv(s.ngroups, s.groups) : s.ngroups * s.parts;
