@@ -771,7 +771,7 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
 // longer leave idle; a product whose units would outlast the others is cut along k into parts
 // that a second kernel adds.  The choice is the least estimate over tile shapes and numbers of
 // parts, with the times measured on this card: of 23040 x 1024 x 4096 in bf16 the two
-// products take 620 us in one launch and 890 one after the other.
+// products take 750 us in one launch and 850 one after the other.
 struct Cut {
   Shape shape;
   int w, x;  // splits of the weights' products and of dx
