@@ -13,7 +13,7 @@
 //   v: uint8 code c = round(255 (v / a)^(1/4)),           value  (c / 255)^4 a
 // Codes are dense near zero and even in relative terms over four decades; a v above zero keeps
 // a code of at least 1, so that sqrt(v) never becomes 0 under an m that did not.  A NaN or
-// infinity makes its block's scale NaN or infinite and with it the block's values NaN.
+// infinity makes its block's scale NaN and with it the block's values.
 //
 // Bound by memory: 28 bytes an element in fp32, 22 with 16-bit parameters and gradients, 10
 // with 8-bit moments.  A workgroup takes 2048 elements of one tensor, eight a lane, so that
@@ -118,10 +118,11 @@ __device__ __forceinline__ float value_v(int c, float a) {
   const float q = t * t;
   return q * q * a;
 }
-// A block's scale and the reciprocal its codes are made with.
+// A block's scale and the reciprocal its codes are made with.  An infinity is NaN here: no
+// code stands for it beside finite values.
 __device__ __forceinline__ void scale_of(float top, float& a, float& inv) {
   const bool tiny = top < FLT_MIN;
-  a = tiny ? 0.0f : top;
+  a = tiny ? 0.0f : top + (top - top);
   inv = tiny ? 0.0f : 1.0f / top;
 }
 // round(sqrt(q) * 127) and round(q^(1/4) * 255) for q in 0..1, as IEEE square roots give them,

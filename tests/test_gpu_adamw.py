@@ -170,6 +170,19 @@ def test_zero_and_non_finite_gradients(device, bits):
         assert torch.isnan(p[0][block]).all() if bits == 8 else torch.isfinite(p[0][keep]).all()
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_non_finite_moments_have_no_values(device, bad):
+    """8-bit moments with a NaN or infinity among them are NaN throughout their block."""
+    g = torch.sin(torch.arange(600, device=device) + 1.0)
+    g[300] = bad
+    opt = fm.AdamW([torch.ones(600, device=device)], bits=8, **HYPER)
+    opt.step([g])
+    block = torch.arange(600, device=device) // 256 == 1
+    for (values,), moment in zip(opt.moment_values(), (opt.m[0], opt.v[0])):
+        assert torch.isnan(values[block]).all() and torch.isfinite(values[~block]).all()
+        assert torch.isnan(moment.scales).tolist() == [False, True, False]
+
+
 def test_step_arguments(device):
     params, grads = tensors(device, torch.float32, sizes=[300, 20])
     before = [p.clone() for p in params]
