@@ -136,14 +136,29 @@ class AdamW:
             raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
         if self.params and boundary.require_device(*self.params) != self._device:
             raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
-        self._memory = [p.detach() for p in self.params]
-        self._addresses = list(map(_address, self._memory))
-        self._table["p"] = self._addresses
-        self._plan = boundary.adamw_plan(self._table)
+        memory = [p.detach() for p in self.params]
+        addresses = list(map(_address, memory))
+        self._table["p"] = addresses
+        self._check_apart()
+        plan = boundary.adamw_plan(self._table)
         if self.params:
-            if hasattr(self, "_device_plan"):
-                torch.cuda.synchronize(self._device)  # (steps on any stream may still read the old one)
-            self._device_plan = torch.from_numpy(self._plan).to(self._device)
+            self._device_plan = torch.from_numpy(plan).to(self._device)
+            self._plan_stream = boundary.stream_handle(self._device)
+        self._memory, self._addresses, self._plan = memory, addresses, plan  # (all checked)
+
+    def _check_apart(self):
+        """A step writes every array from workgroups in no order: none may share memory."""
+        t, scales = self._table, -(-self._table["n"] // MOMENT_BLOCK) * 4
+        moment = np.where(t["m_scale"] != 0, 1, 4) * t["n"]
+        sizes = np.concatenate([t["n"] * [p.element_size() for p in self.params], moment, moment,
+                                t["n"] * 4, scales, scales])
+        starts = np.concatenate([t[k] for k in ("p", "m", "v", "master", "m_scale", "v_scale")])
+        given = (starts != 0) & (sizes > 0)
+        starts, sizes = starts[given].astype(np.int64), sizes[given].astype(np.int64)
+        order = np.argsort(starts)
+        starts, ends = starts[order], (starts + sizes)[order]
+        if (starts[1:] < ends[:-1]).any():
+            raise ArgumentError("AdamW: parameters, moments and masters must not share memory")
 
     def _place(self, e, p, m, v, master):
         if isinstance(m, Moment8) != isinstance(v, Moment8):
@@ -199,6 +214,9 @@ class AdamW:
         one_type = len(set(map(_dtype, grads))) == 1
         dtypes[keep] = (boundary.dtype_code(grads[0]) if one_type
                         else [boundary.dtype_code(g) for g in grads])
+        if boundary.stream_handle(self._device) != self._plan_stream:
+            # (its memory goes back to the stream it came from, past steps on this one)
+            self._device_plan.record_stream(torch.cuda.current_stream(self._device))
         boundary.adamw_step(self._plan, self._device_plan, addresses, dtypes, self.steps + 1,
                             self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay,
                             grad_scale, self._device)

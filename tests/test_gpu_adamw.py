@@ -239,6 +239,30 @@ def test_other_stream_and_graph(device):
     assert all(torch.equal(a, b) for a, b in zip(params, other))
 
 
+def test_stepped_on_another_stream_and_dropped(device):
+    """The memory of an optimiser that is dropped after a step on a stream of its own is not
+    given out again before that step."""
+    params, grads = tensors(device, torch.float32, sizes=[70001] * 4)
+    other = [p.clone() for p in params]
+    fm.AdamW(params, **HYPER).step(grads)
+    moments = [[torch.zeros_like(p) for p in other] for _ in range(2)]
+    opt = fm.AdamW(other, moments=moments, **HYPER)
+    nbytes = opt._device_plan.numel()
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    busy = torch.ones(4096, 4096, device=device)
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy = busy @ busy * 2.0 ** -12
+        opt.step(grads)
+    at = opt._device_plan.data_ptr()
+    del opt
+    later = [torch.empty(nbytes, dtype=torch.uint8, device=device) for _ in range(8)]
+    assert all(t.data_ptr() != at for t in later)
+    torch.cuda.current_stream(device).wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(params, other))
+
+
 def test_refusals(device):
     p = [torch.zeros(8, device=device)]
     with pytest.raises(fm.ArgumentError):
@@ -274,6 +298,33 @@ def test_refusals(device):
     with pytest.raises(fm.DimensionMismatch):
         fm.moment_values([fm.Moment8.zeros(torch.zeros(8, device=device), True)], [])
     assert opt.steps == 0
+
+
+def test_arrays_lie_apart(device):
+    """No array of a step may share memory with another; neighbours in one buffer may be stepped."""
+    whole = torch.zeros(600, device=device)
+    m, v = torch.zeros(300, device=device), torch.zeros(300, device=device)
+    opt = fm.AdamW([whole[:300], whole[300:]], **HYPER)
+    opt.step([torch.ones(300, device=device)] * 2)
+    assert (whole == whole[0]).all() and whole[0] < 0
+    for params, given in (([whole, whole[300:]], {}), ([whole[:301], whole[300:]], {}),
+                          ([whole[:300], whole[:300].view(3, 100)], {}),
+                          ([whole[:300]], dict(moments=([m], [m]))),
+                          ([whole[:300]], dict(moments=([m], [v]), masters=[whole[:300]])),
+                          ([whole[:300]], dict(moments=([m], [whole[200:500]])))):
+        with pytest.raises(fm.ArgumentError, match="share memory"):
+            fm.AdamW(params, **given)
+    p = [torch.zeros(300, device=device), torch.zeros(300, device=device)]
+    opt = fm.AdamW(p, **HYPER)
+    p[0].data = p[1].data
+    for _ in range(2):  # (refused once more, not stepped where it was)
+        with pytest.raises(fm.ArgumentError, match="share memory"):
+            opt.step([m, v])
+    p[0].data = m
+    opt.step([v, v])
+    assert opt.steps == 1
+    opt = fm.AdamW([torch.zeros(0, device=device), torch.zeros(0, device=device)], bits=8)
+    opt.step([torch.zeros(0, device=device)] * 2)
 
 
 def test_parameters_may_move(device):
