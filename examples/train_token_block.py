@@ -88,7 +88,7 @@ def train(steps, bits=8, dtype=torch.bfloat16, device="cuda:0", batch=64, query_
         losses.append(loss.detach())
         if log and (step % 10 == 0 or step + 1 == steps):
             hit = (scores.argmax(1) == target).float().mean()
-            log(f"step {step:4d}  loss {float(loss):.4f}  own document first {float(hit):.3f}")
+            log(f"step {step:4d}  loss {float(loss.detach()):.4f}  own document first {float(hit):.3f}")
     return torch.stack(losses), block
 
 
