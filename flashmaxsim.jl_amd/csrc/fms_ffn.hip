@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
 
 // ---- few tokens ----------------------------------------------------------------------------
 // Bound by the weights' bytes, and for one query by latency: no LDS staging and no barrier on
-// the way.  A workgroup takes 16 hidden units (their 16 rows of wg and of wu) and 16 kNT
+// the way.  A workgroup takes kHidden units (their rows of wg and of wu) and 16 kNT
 // tokens; its eight waves share k, 128 bytes of every row at a time, each loading its operands
 // straight into the 16 x 16 MFMAs' registers with everything of a round in flight, and join
 // their sums through LDS.
@@ -388,28 +388,37 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 acc) {
 }
 
 constexpr int kFewWaves = 8;
-constexpr int kFewHidden = 16;
 
-template <class Op, int kNT>
+template <class Op, int kNT, int kHidden>
 __global__ void __launch_bounds__(64 * kFewWaves) ffn_few_kernel(GateArgs A) {
   typedef typename OutOf<Op>::T T;
   // lane: row (hidden unit, token) lane % 16 of a fragment, bytes 16 (lane / 16) of 64
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * kFewHidden, m0 = (int64_t)blockIdx.y * 16 * kNT;
+  const int64_t n0 = (int64_t)blockIdx.x * kHidden, m0 = (int64_t)blockIdx.y * 16 * kNT;
   const int pitch = (int)A.x.pitch, bytes = (int)A.x.rowbytes, in = 16 * (lane >> 4);
-  const rsrc_t rg = matrix_from(A.wg, n0 * A.wg.pitch), ru = matrix_from(A.wu, n0 * A.wu.pitch);
   const rsrc_t rx = matrix_from(A.x, m0 * A.x.pitch);
   const int row = (lane & 15) * pitch + in;
-  f32x4 acc[2][kNT] = {};
+  // 16 hidden units: a fragment of each projection; 8: one, its rows 0..7 of wg and 8..15 of wu
+  constexpr int kFrags = kHidden / 8;
+  const int64_t unit = n0 + (lane & (kHidden - 1));
+  const int wbytes = unit < A.hidden ? bytes - in : 0;  // of this lane's row, from its first on
+  const char* w[kFrags];
+#pragma unroll
+  for (int f = 0; f < kFrags; ++f)
+    w[f] = ((kFrags == 2 ? f == 1 : (lane & 8) != 0) ? A.wu.base : A.wg.base) + unit * A.wg.pitch + in;
+  f32x4 acc[kFrags][kNT] = {};
   struct Round {
-    u32x4 g[2], u[2], x[2][kNT];
+    u32x4 w[2][kFrags], x[2][kNT];
   };
   const auto load = [&](Round& r, int at) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int off = at + 64 * i + in < bytes ? row + at + 64 * i : kOutOfBounds;
-      r.g[i] = buf_load16(rg, off);
-      r.u[i] = buf_load16(ru, off);
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f) {
+        r.w[i][f] = u32x4{0u, 0u, 0u, 0u};
+        if (at + 64 * i < wbytes) r.w[i][f] = *reinterpret_cast<const u32x4*>(w[f] + at + 64 * i);
+      }
 #pragma unroll
       for (int t = 0; t < kNT; ++t)
         r.x[i][t] = buf_load16(rx, off == kOutOfBounds ? off : off + t * 16 * pitch);
@@ -419,10 +428,9 @@ __global__ void __launch_bounds__(64 * kFewWaves) ffn_few_kernel(GateArgs A) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-        acc[0][t] = mma16<Op>(r.g[i], r.x[i][t], acc[0][t]);
-        acc[1][t] = mma16<Op>(r.u[i], r.x[i][t], acc[1][t]);
-      }
+      for (int t = 0; t < kNT; ++t)
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f) acc[f][t] = mma16<Op>(r.w[i][f], r.x[i][t], acc[f][t]);
   };
   constexpr int kRound = kFewWaves * 128;  // bytes of k between a wave's rounds
   Round a, b;
@@ -435,20 +443,21 @@ __global__ void __launch_bounds__(64 * kFewWaves) ffn_few_kernel(GateArgs A) {
     multiply(b);
     load(b, at + 3 * kRound);
   }
-  // sums of the waves: lane holds hidden units 4 (lane / 16) + e of token lane % 16
-  __shared__ __attribute__((aligned(16))) f32x4 sums[kFewWaves][2][kNT][64];
+  // sums of the waves: lane holds rows 4 (lane / 16) + e of token lane % 16, gate and then up
+  __shared__ __attribute__((aligned(16))) f32x4 sums[kFewWaves][kFrags][kNT][64];
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int f = 0; f < kFrags; ++f)
 #pragma unroll
-    for (int t = 0; t < kNT; ++t) sums[wave][p][t][lane] = acc[p][t];
+    for (int t = 0; t < kNT; ++t) sums[wave][f][t][lane] = acc[f][t];
   __syncthreads();
-  for (int o = tid; o < 64 * kNT; o += 64 * kFewWaves) {
-    const int t = o >> 6, l = o & 63;
+  constexpr int kLanes = 4 * kHidden;  // that hold gates
+  for (int o = tid; o < kLanes * kNT; o += 64 * kFewWaves) {
+    const int t = o / kLanes, l = o % kLanes;
     f32x4 g = {}, u = {};
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
+    for (int w = 0; w < kFewWaves; ++w) {  // (in order)
       g += sums[w][0][t][l];
-      u += sums[w][1][t][l];
+      u += kFrags == 2 ? sums[w][kFrags - 1][t][l] : sums[w][0][t][l + 32];
     }
     const int64_t m = m0 + t * 16 + (l & 15), n = n0 + 4 * (l >> 4);
     if (m >= A.tokens) continue;
@@ -726,21 +735,29 @@ Shape gate_shape(int64_t rows, int64_t cols, int esz) {
   return cdiv(rows, 128) * cdiv(cols, 128) > 256 ? Shape::kSmall : Shape::kTiny;
 }
 
+// Eight hidden units a workgroup where sixteen would leave half the CUs without one (us at dim
+// 1024, one and 32 tokens: hidden 2048, 128 workgroups of sixteen, bf16 3.8 and 5.6 against 4.6
+// and 6.3, fp32 5.1 and 8.3 against 7.6 and 11.5; hidden 2560 bf16 5.0 and 8.6 against 4.6 and 6.4).
 template <class Op, int kNT>
 hipError_t launch_few(const GateArgs& g, hipStream_t st) {
-  hipLaunchKernelGGL((ffn_few_kernel<Op, kNT>),
-                     dim3((unsigned)cdiv(g.hidden, kFewHidden), (unsigned)cdiv(g.tokens, 16 * kNT)),
-                     dim3(64 * kFewWaves), 0, st, g);
-  return hipGetLastError();
+  const int64_t ny = cdiv(g.tokens, 16 * kNT);
+  const auto launch = [&](auto kernel, int hidden) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(g.hidden, hidden), (unsigned)ny), dim3(64 * kFewWaves), 0, st,
+                       g);
+    return hipGetLastError();
+  };
+  if (cdiv(g.hidden, 16) * ny <= 128) return launch(ffn_few_kernel<Op, kNT, 8>, 8);
+  return launch(ffn_few_kernel<Op, kNT, 16>, 16);
 }
 
 // Few tokens: against the 64-row tiles, whose time does not fall with the tokens (us at
 // 768 x 2048 / 1024 x 4096):
-//   16 bits: 1 token 4.9 / 5.2, 32 tokens 6.4 / 7.2, 64 tokens 8.9 / 9.8 (tiles 8.0 / 9.6);
-//   32 bits: 1 token 6.4 / 7.7, 128 tokens 17 / 35 (tiles 31 / 42), 256 tokens 32 / 67 (32 / 42).
+//   16 bits: 1 token 3.7 / 4.7, 32 tokens 5.1 / 6.5, 64 tokens 6.9 / 8.9 (tiles 7.8 / 9.6;
+//   at dim 512 6.0 / 6.7 and 6.1 / 6.2, at dim 256 4.6 / 4.9 and 4.5 / 4.5);
+//   32 bits: 1 token 4.9 / 7.7, 128 tokens 16 / 34 (tiles 31 / 42), 256 tokens 31 / 67 (32 / 42).
 bool few_tokens(const GateArgs& g, int esz) {
-  if (esz == 2) return g.tokens <= 32;
-  return g.tokens <= 256 && cdiv(g.hidden, kFewHidden) * cdiv(g.tokens, 64) <= 512;
+  if (esz == 2) return g.tokens <= (g.x.rowbytes > 1024 ? 64 : 32);
+  return g.tokens <= 256 && cdiv(g.hidden, 16) * cdiv(g.tokens, 64) <= 512;
 }
 
 template <class Op, bool kPull>
@@ -753,8 +770,7 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
   if constexpr (!kPull)
     if (few_tokens(g, Op::kEsz)) {
       if (g.tokens <= 16) return launch_few<Op, 1>(g, st);
-      if constexpr (Op::kEsz == 4)
-        if (g.tokens > 32) return launch_few<Op, 4>(g, st);
+      if (g.tokens > 32) return launch_few<Op, 4>(g, st);
       return launch_few<Op, 2>(g, st);
     }
   typedef Shapes<Op, true, true, 2> S;

@@ -119,6 +119,17 @@ def test_large_and_odd(device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("tokens, dim", [(1, 520), (16, 16), (17, 1029), (33, 520), (48, 1024), (64, 513),
+                                         (65, 520), (200, 72)])
+@pytest.mark.parametrize("hidden", [3, 2048, 2049])
+def test_few_tokens(device, tokens, dim, hidden, dtype):
+    """Few tokens, on both sides of where their kernel changes its share of hidden units."""
+    x, wg, wu, dh = inputs(device, tokens, dim, hidden, dtype)
+    want = reference(x, wg, wu, dh, "silu", dtype, device)
+    check(fm.gated_ffn_forward(x, wg, wu), want["h"], "h")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("offset", [1, 2, 3])
 def test_bases_off_16_bytes(device, dtype, offset):
     x, wg, wu, dh = inputs(device, 70, 64, 72, dtype, offset=offset)
