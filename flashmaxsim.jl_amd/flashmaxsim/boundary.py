@@ -668,21 +668,30 @@ def varlen_apply_pullback(dQ, dD, Qp, Dp, cu_q, cu_d, args, Delta, inv_n):
 def _check_block(x, *groups):
     """Device, density, eltype and shapes of a call's arrays: groups of (shape, names, arrays), an
     array None where it is not given.  The device."""
-    given = [x]
-    dtype = x.dtype
+    dtype, at = x.dtype, x.get_device()
+    good = at >= 0 and x.is_contiguous()
+    for shape, _, arrays in groups:
+        for t in arrays:
+            if t is not None:
+                good = (good and t.dtype is dtype and t.shape == shape and t.get_device() == at
+                        and t.is_contiguous())
+    if not good:
+        _refuse_block(x, groups)
+    return x.device
+
+
+def _refuse_block(x, groups):
+    """Says what _check_block found."""
+    require_device(x, *(t for _, _, arrays in groups for t in arrays))
     for shape, names, arrays in groups:
-        for i, t in enumerate(arrays):
+        for what, t in zip(names.split(), arrays):
             if t is None:
                 continue
-            given.append(t)
-            if t.dtype != dtype or t.shape != shape:
-                require_device_many(given)
-                what = names.split()[i]
-                if t.dtype != dtype:
-                    raise ArgumentError(f"{what} must have the feature eltype {dtype}, got {t.dtype}")
+            if t.dtype != x.dtype:
+                raise ArgumentError(f"{what} must have the feature eltype {x.dtype}, got {t.dtype}")
+            if t.shape != shape:
                 raise DimensionMismatch(
                     f"{what} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
-    return require_device_many(given)
 
 
 def launch_gated_ffn(h, x, wg, wu, act):
