@@ -7,10 +7,19 @@
 //
 // Products run on the matrix cores (fms_gemm.hpp) and accumulate in fp32.  g and
 // u never leave the registers: forward writes h alone and keeps nothing, and the
-// pullback computes them again in the kernel that makes dg and du, which are
-// rounded once to the feature type for the three products after it.  (Keeping g
-// and u from the forward in 16 bits would round them once more, and in fp32
-// would move 16 bytes a hidden unit, against 4 dim operations to compute them.)
+// pullback computes them again in the kernel that makes dg and du for the three
+// products after it.  (Keeping g and u from the forward in 16 bits would round them,
+// and in fp32 would move 16 bytes a hidden unit, against 4 dim operations to compute them.)
+//
+// The matrix cores take dg and du in the feature type, and one rounding to 16 bits there
+// costs as much as the outputs' own: 1.41 times the error of the result, and in fp16 their
+// range, since each is a product of three values.  So in 16 bits they are held as two values
+// each, the rounding and what it left (two planes), and the products sum both: 16 significant
+// bits in bf16, 22 in fp16, for twice the products' work (a pullback of 23040 x 1024 x 4096 in
+// bf16: 2040 us, about 1130 with one plane; 2100 in fp16).  In fp16 they are multiplied with a
+// power of two, from a bound of the largest of them (ffn_bound_kernel, 50 us there), and the
+// products' results with its reciprocal: the bound comes to 2^14 .. 2^15, so nothing overflows
+// and what falls off the second plane is less than 2^-39 of the bound.
 //
 // act(g) = g s with s = sigmoid(y(g)) for silu (y = g) and gelu_tanh
 // (y = 2 sqrt(2/pi) (g + 0.044715 g^3), since (1 + tanh z) / 2 = sigmoid(2z));
@@ -111,6 +120,21 @@ struct Quads {
       const int c1 = col(p, 1, h);
       put(qa, to, at + c0 * Op::kEsz, cols - c0);
       put(qb, to, at + c1 * Op::kEsz, cols - c1);
+    }
+  }
+  // To be called before a is rounded in two places: a as it is in a register.  (The compiler
+  // fuses a product with its conversion to fp16, which rounds once where product and conversion
+  // round twice: near a tie the two places would have had different roundings.)
+  __device__ static __forceinline__ void settle(float (&a)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(a[e]));
+  }
+  // What a's rounding to the type leaves, in a; nothing where that is not finite.
+  __device__ static __forceinline__ void rest(float (&a)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float r = a[e] - (float)(T)a[e];
+      a[e] = fabsf(r) < INFINITY ? r : 0.0f;
     }
   }
   // Reads such a pair.
@@ -233,12 +257,119 @@ struct GateArgs {
   Matrix x, wg, wu;
   int32_t act, tm, tn, steps;
   int64_t tokens, hidden;
-  // forward: out0 = h; pullback: in = dh, out0 = dg, out1 = du
+  // forward: out0 = h; pullback: in = dh, out0 = dg, out1 = du, each kPlanes planes
   void *out0, *out1;
   const void* in;
   int64_t out_cols, out_pitch, in_pitch;  // values
-  int32_t vec;  // whole 16-byte units of outputs and input
+  int64_t plane;  // bytes from a plane of dg or du to its second one
+  int32_t vec;    // whole 16-byte units of outputs and input
+  // fp16 pullback: the parts of the bound, and where the reciprocal of its power of two goes
+  int32_t nbounds;
+  const float2* bounds;
+  float* unscale;
 };
+
+// How many values hold one of dg or du, and whether they are scaled.
+template <class Op>
+constexpr int kPlanes = Op::kEsz == 2 ? 2 : 1;
+template <class Op>
+constexpr bool kScaled = std::is_same_v<Op, OpF16>;
+
+// |act(g)| <= |g| and |act'(g)| < 1.13, so with Cauchy and Schwarz no dg or du is larger than
+//   1.13 max over tokens (max |dh| of its row, |x|_2) * max over hidden units (|wg|_2, |wu|_2).
+// A workgroup's part of the two maxima, over rows that are finite (others' products are not
+// finite whatever they are scaled by).  One read of the inputs, a wave a row.
+constexpr int kMostBounds = 256, kBoundWaves = 16;
+struct BoundArgs {
+  Matrix x, wg, wu;  // fp16, whole 16-byte units, zero beyond dim
+  const _Float16* dh;
+  int64_t tokens, hidden;
+  int32_t vec;  // whole 16-byte units of dh
+  float2* bounds;
+};
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// A lane's part of |row|_2^2.
+__device__ __forceinline__ float squares(const Matrix& m, int64_t row, int lane) {
+  const char* const p = m.base + row * m.pitch;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int64_t at = lane * 16; at < m.rowbytes; at += 64 * 16) {
+    const f16x8 v = *reinterpret_cast<const f16x8*>(p + at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (float)v[e] * (float)v[e];
+  }
+  return s;
+}
+// The length that the lanes' parts make, 0 where it is not finite.
+__device__ __forceinline__ float length(float part) {
+  const float s = wave_sum(part);
+  return s < INFINITY ? sqrtf(s) : 0.0f;
+}
+__global__ void __launch_bounds__(64 * kBoundWaves) ffn_bound_kernel(BoundArgs A) {
+  __shared__ float2 lds[kBoundWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float token = 0.0f, unit = 0.0f;
+  for (int64_t i = (int64_t)blockIdx.x * kBoundWaves + wave; i < A.tokens + 2 * A.hidden;
+       i += (int64_t)gridDim.x * kBoundWaves) {
+    if (i >= A.tokens) {
+      const int64_t j = i - A.tokens;
+      unit = fmaxf(unit, length(j < A.hidden ? squares(A.wg, j, lane) : squares(A.wu, j - A.hidden, lane)));
+      continue;
+    }
+    const float part = squares(A.x, i, lane);
+    const _Float16* const row = A.dh + i * A.hidden;
+    float top = 0.0f;
+    const auto see = [&](_Float16 h) {
+      const float v = fabsf((float)h);
+      top = v < INFINITY && v > top ? v : top;
+    };
+    if (A.vec) {
+#pragma unroll 4
+      for (int64_t k = lane * 8; k < A.hidden; k += 64 * 8) {
+        const f16x8 v = *reinterpret_cast<const f16x8*>(row + k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) see(v[e]);
+      }
+    } else {
+#pragma unroll 4
+      for (int64_t k = lane; k < A.hidden; k += 64) see(row[k]);
+    }
+    token = fmaxf(token, wave_max(top) * length(part));
+  }
+  if (lane == 0) lds[wave] = make_float2(token, unit);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kBoundWaves; ++w) {
+      token = fmaxf(token, lds[w].x);
+      unit = fmaxf(unit, lds[w].y);
+    }
+    A.bounds[blockIdx.x] = make_float2(token, unit);
+  }
+}
+// The power of two that takes the bound (without its 1.13) to 2^14 .. 2^15, as an exponent; a
+// wave's lanes all take part.
+__device__ __forceinline__ int scale_exponent(const GateArgs& A) {
+  float token = 0.0f, unit = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kMostBounds; j += 64) {
+    const int i = j + (threadIdx.x & 63);
+    if (i >= A.nbounds) break;
+    token = fmaxf(token, A.bounds[i].x);
+    unit = fmaxf(unit, A.bounds[i].y);
+  }
+  const float bound = wave_max(token) * wave_max(unit);  // (2^-72 .. 2^70, or 0)
+  const int e = bound > 0.0f ? 14 - ilogbf(bound) : 0;
+  return __builtin_amdgcn_readfirstlane(e);
+}
 
 // LDS behind the products' buffers, a box for each wave.
 template <class P>
@@ -247,14 +378,17 @@ constexpr int kBoxes = P::kThreads / 64 * Quads<typename P::Op>::kBox;
 // A tile's sums -> h, or dg and du.  kVec: rows of whole 16-byte units; else through `box`.
 template <class P, bool kPull, int kAct, bool kVec>
 __device__ __forceinline__ void gate_store(const GateArgs& A, const typename P::Acc (&acc)[2][P::kMF],
-                                           int64_t m0, int64_t n0, char* box) {
+                                           int64_t m0, int64_t n0, char* box, float scale) {
   typedef Quads<typename P::Op> Q;
   typedef typename Q::T T;
   constexpr int kSize = (int)sizeof(T);
+  constexpr bool kTwo = kPull && kPlanes<typename P::Op> == 2;
   const int lane = here(threadIdx.x & 63), wave = threadIdx.x >> 6;
   const int wm = wave / P::kWN, wn = wave % P::kWN, h = lane >> 5;
   const rsrc_t to0 = tile_at<T>(A.out0, A.tokens, A.out_pitch, m0, n0);
   const rsrc_t to1 = tile_at<T>(A.out1, kPull ? A.tokens : 0, A.out_pitch, m0, n0);
+  const rsrc_t rest0 = tile_at<T>(static_cast<char*>(A.out0) + A.plane, kTwo ? A.tokens : 0, A.out_pitch, m0, n0);
+  const rsrc_t rest1 = tile_at<T>(static_cast<char*>(A.out1) + A.plane, kTwo ? A.tokens : 0, A.out_pitch, m0, n0);
   const rsrc_t from = tile_at<T>(A.in, kPull ? A.tokens : 0, A.in_pitch, m0, n0);
   // of the wave's first row
   const int out_pitch = (int)A.out_pitch * kSize, in_pitch = (int)A.in_pitch * kSize;
@@ -292,6 +426,7 @@ __device__ __forceinline__ void gate_store(const GateArgs& A, const typename P::
           float a, da;
           activate<kAct>(g, a, da);
           if constexpr (kPull) {
+            if constexpr (kScaled<typename P::Op>) y[q][e] *= scale;
             z[q][e] = y[q][e] * a;
             y[q][e] = y[q][e] * u * da;
           } else {
@@ -299,33 +434,59 @@ __device__ __forceinline__ void gate_store(const GateArgs& A, const typename P::
           }
         }
       if constexpr (kVec) {
-        Q::store(y[2 * p], y[2 * p + 1], to0, at, p, h, out_left);
-        if constexpr (kPull) Q::store(z[2 * p], z[2 * p + 1], to1, at, p, h, out_left);
+        const auto put = [&](float (&a)[4][4], rsrc_t to, rsrc_t rest) {
+          if constexpr (kTwo) {
+            Q::settle(a[2 * p]);
+            Q::settle(a[2 * p + 1]);
+          }
+          Q::store(a[2 * p], a[2 * p + 1], to, at, p, h, out_left);
+          if constexpr (kTwo) {
+            Q::rest(a[2 * p]);
+            Q::rest(a[2 * p + 1]);
+            Q::store(a[2 * p], a[2 * p + 1], rest, at, p, h, out_left);
+          }
+        };
+        put(y, to0, rest0);
         __builtin_amdgcn_sched_barrier(0);  // (few values at a time)
+        if constexpr (kPull) {
+          put(z, to1, rest1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     if constexpr (!kVec) {
+      const auto put = [&](const float (&a)[4][4], rsrc_t to) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) Q::box_in(box, lane, q, y[q]);
-      Q::box_store(box, lane, to0, out + mf * 32 * out_pitch, out_pitch, out_left);
-      if constexpr (kPull) {
+        for (int q = 0; q < 4; ++q) Q::box_in(box, lane, q, a[q]);
+        Q::box_store(box, lane, to, out + mf * 32 * out_pitch, out_pitch, out_left);
+      };
+      const auto put_all = [&](float (&a)[4][4], rsrc_t to, rsrc_t rest) {
+        if constexpr (kTwo) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) Q::box_in(box, lane, q, z[q]);
-        Q::box_store(box, lane, to1, out + mf * 32 * out_pitch, out_pitch, out_left);
-      }
+          for (int q = 0; q < 4; ++q) Q::settle(a[q]);
+        }
+        put(a, to);
+        if constexpr (kTwo) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) Q::rest(a[q]);
+          put(a, rest);
+        }
+      };
+      put_all(y, to0, rest0);
+      if constexpr (kPull) put_all(z, to1, rest1);
     }
   }
 }
 
 template <class P, bool kPull, bool kVec>
 __device__ __forceinline__ void by_act(const GateArgs& A, const typename P::Acc (&acc)[2][P::kMF],
-                                       int64_t m0, int64_t n0, char* box) {
+                                       int64_t m0, int64_t n0, char* box, float scale) {
   if (A.act == FMS_ACT_SILU)
-    gate_store<P, kPull, FMS_ACT_SILU, kVec>(A, acc, m0, n0, box);
+    gate_store<P, kPull, FMS_ACT_SILU, kVec>(A, acc, m0, n0, box, scale);
   else if (A.act == FMS_ACT_GELU)
-    gate_store<P, kPull, FMS_ACT_GELU, kVec>(A, acc, m0, n0, box);
+    gate_store<P, kPull, FMS_ACT_GELU, kVec>(A, acc, m0, n0, box, scale);
   else
-    gate_store<P, kPull, FMS_ACT_GELU_TANH, kVec>(A, acc, m0, n0, box);
+    gate_store<P, kPull, FMS_ACT_GELU_TANH, kVec>(A, acc, m0, n0, box, scale);
 }
 
 // Forward (kPull false): h.  Pullback: dg and du, their rows filled up with zeros to out_cols.
@@ -336,6 +497,12 @@ __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
   __shared__ __attribute__((aligned(16))) char lds[P::kLds + kBoxes<P>];
   char* const box = lds + P::kLds + (threadIdx.x >> 6) * Quads<typename P::Op>::kBox;
   const int tiles = A.tm * A.tn, mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  float scale = 1.0f;
+  if constexpr (kPull && kScaled<typename P::Op>) {
+    const int e = scale_exponent(A);
+    scale = ldexpf(1.0f, e);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *A.unscale = ldexpf(1.0f, -e);
+  }
   const auto place = [&](int j, int64_t& m0, int64_t& n0) {
     int im, in;
     tile_of(blockIdx.x + j * gridDim.x, A.tm, A.tn, im, in);
@@ -357,9 +524,9 @@ __global__ void __launch_bounds__(P::kThreads, 2) ffn_gate_kernel(GateArgs A) {
     int64_t m0, n0;
     place(j, m0, n0);
     if (!A.vec)
-      by_act<P, kPull, false>(A, acc, m0, n0, box);
+      by_act<P, kPull, false>(A, acc, m0, n0, box, scale);
     else
-      by_act<P, kPull, true>(A, acc, m0, n0, box);
+      by_act<P, kPull, true>(A, acc, m0, n0, box, scale);
   };
   P::run(mine, leg, after, lds);
 }
@@ -476,10 +643,14 @@ __global__ void __launch_bounds__(64 * kFewWaves) ffn_few_kernel(GateArgs A) {
 }
 
 // A product of the pullback.  Unit u of its tiles * splits * outputs: out[z] or, with splits,
-// a part of it over k, in fp32.
+// a part of it over k, in fp32.  With dg's planes first and du's after them, output z is the sum of planes
+// z segments .. (z + 1) segments - 1 times n[0] (dg's) or n[1] (du's).
 struct ProductArgs {
-  Matrix m[2], n[2];
-  int32_t segments;  // 2: out[0] = m0 n0 + m1 n1; 1: out[z] = m_z n_z
+  Matrix m;       // the first plane
+  int64_t plane;  // bytes to the next one
+  Matrix n[2];
+  const float* unscale;  // fp16: what the sums are multiplied with, or null
+  int32_t segments;
   int32_t outputs;
   int64_t bytes;                  // of a segment's k
   int32_t tm, tn, steps, splits;  // steps of all segments
@@ -494,7 +665,7 @@ struct ProductArgs {
 template <class P, class Q, bool kVec>
 __device__ __forceinline__ void product_store(const typename P::Acc (&acc)[2][P::kMF], void* out,
                                               int64_t rows, int64_t cols, int64_t pitch_, int64_t m0,
-                                              int64_t n0, char* box) {
+                                              int64_t n0, char* box, float unscale) {
   typedef typename Q::T T;
   const int lane = here(threadIdx.x & 63), wave = threadIdx.x >> 6, h = lane >> 5;
   const rsrc_t to = tile_at<T>(out, rows, pitch_, m0, n0);
@@ -508,7 +679,7 @@ __device__ __forceinline__ void product_store(const typename P::Acc (&acc)[2][P:
       const auto& c = acc[nf][mf];
       const auto quad = [&](int q, float (&a)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = c[4 * q + e];
+        for (int e = 0; e < 4; ++e) a[e] = kScaled<typename P::Op> ? c[4 * q + e] * unscale : c[4 * q + e];
       };
       float a[4], b[4];
       if constexpr (kVec) {
@@ -541,11 +712,15 @@ __device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, cha
   const int s1 = (int)((int64_t)A.steps * (split + 1) / A.splits);
   const int each = A.steps / A.segments;
   const int lo = each > 0 ? s0 / each : 0, hi = each > 0 ? (s1 - 1) / each : 0;
+  float unscale = 1.0f;
+  if constexpr (kScaled<typename P::Op>)
+    if (A.unscale) unscale = *A.unscale;
   const auto leg = [&](int j) {
-    const int s = lo + j, from = s0 - s * each, to = s1 - s * each;
+    const int s = lo + j, from = s0 - s * each, to = s1 - s * each, plane = z * A.segments + s;
     typename P::Legs l;
-    l.m[0] = z + s == 0 ? A.m[0] : A.m[1];
-    l.n[0] = z + s == 0 ? A.n[0] : A.n[1];
+    l.m[0] = A.m;
+    l.m[0].base += plane * A.plane;
+    l.n[0] = plane < kPlanes<typename P::Op> ? A.n[0] : A.n[1];
     l.m0 = m0;
     l.n0 = n0;
     l.first = from > 0 ? from : 0;
@@ -557,13 +732,13 @@ __device__ __forceinline__ void product_unit(const ProductArgs& A, int unit, cha
     if (A.splits > 1)
       product_store<P, Quads<OpF32>, true>(
           acc, A.parts + ((int64_t)split * A.outputs + z) * A.rows * A.part_pitch, A.rows, A.part_pitch,
-          A.part_pitch, m0, n0, box);
+          A.part_pitch, m0, n0, box, unscale);
     else if (A.vec)
       product_store<P, Quads<typename P::Op>, true>(acc, z == 0 ? A.out[0] : A.out[1], A.rows, A.cols,
-                                                    A.cols, m0, n0, box);
+                                                    A.cols, m0, n0, box, unscale);
     else
       product_store<P, Quads<typename P::Op>, false>(acc, z == 0 ? A.out[0] : A.out[1], A.rows, A.cols,
-                                                     A.cols, m0, n0, box);
+                                                     A.cols, m0, n0, box, unscale);
   };
   if (s0 < s1) {
     P::run(hi - lo + 1, leg, after, lds);
@@ -707,9 +882,9 @@ hipError_t place_inputs(const FfnArgs& a, const Inputs& in, char* ws, Matrix (&m
 template <class Op, bool kMRows, bool kNRows, int kParts>
 struct Shapes {
   // 256 x 256, 8 waves.  The pullback's products read dg and du from HBM and keep three
-  // shorter steps in flight (23040 x 1024 x 4096: 1490 us a training step, 1512 with one of 128
-  // bytes); the projections' operands come from the caches (290 us for 46080 x 768 x 2048, 315
-  // with shorter steps).
+  // shorter steps in flight (23040 x 1024 x 4096, with dg and du in one plane each: 1490 us a
+  // training step, 1512 with one step of 128 bytes); the projections' operands come from the
+  // caches (290 us for 46080 x 768 x 2048, 315 with shorter steps).
   typedef Product<Op, kMRows, kNRows, kParts, 2, 4, 4, kParts == 2 ? 128 : 64> Big;
   typedef Product<Op, kMRows, kNRows, kParts, 2, 2, 2> Small;  // 128 x 128, 4 waves
   typedef Product<Op, kMRows, kNRows, kParts, 2, 2, 1> Tiny;   // 64 x 128, 4 waves
@@ -763,9 +938,9 @@ bool few_tokens(const GateArgs& g, int esz) {
 template <class Op, bool kPull>
 hipError_t run_gate(const GateArgs& g, hipStream_t st) {
   if (g.tokens == 0 || g.out_cols == 0) return hipSuccess;
-  if (g.x.rowbytes == 0) {  // sums of nothing: h, dg and du are zero
-    return launch_pad(Op::kEsz, PadArgs{{g.out0, g.out1, nullptr}, {}, {g.tokens, g.out1 ? g.tokens : 0, 0},
-                                        0, g.out_pitch}, st);
+  if (g.x.rowbytes == 0) {  // sums of nothing: h is zero (and no one asks for the gradients)
+    return kPull ? hipErrorInvalidValue
+                 : launch_pad(Op::kEsz, PadArgs{{g.out0, nullptr, nullptr}, {}, {g.tokens, 0, 0}, 0, g.out_pitch}, st);
   }
   if constexpr (!kPull)
     if (few_tokens(g, Op::kEsz)) {
@@ -786,8 +961,9 @@ hipError_t run_gate(const GateArgs& g, hipStream_t st) {
 // One launch takes both, the longer units first, so that the shorter ones fill what the
 // longer leave idle; a product whose units would outlast the others is cut along k into parts
 // that a second kernel adds.  The choice is the least estimate over tile shapes and numbers of
-// parts, with the times measured on this card: of 23040 x 1024 x 4096 in bf16 the two
-// products take 750 us in one launch and 850 one after the other.
+// parts, with the times measured on this card: of 23040 x 1024 x 4096 in bf16 and one plane of dg
+// and du the two products take 750 us in one launch and 850 one after the other (two planes, in
+// one launch: 1430-1520).
 struct Cut {
   Shape shape;
   int w, x;  // splits of the weights' products and of dx
@@ -933,9 +1109,12 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
                     hipStream_t st) {
   const Inputs in = inputs_of(a);
   const int64_t pitch = round_up(a.hidden * Op::kEsz, 16);  // of dg and du
-  const int64_t each = round_up(a.tokens * pitch, 256);
+  const int64_t each = round_up(a.tokens * pitch, 256);     // a plane of them
+  constexpr int kDg = kPlanes<Op>;
+  const bool any = a.tokens > 0 && a.hidden > 0, scaled = kScaled<Op> && any;
+  // behind the planes the reciprocal of the power of two, and 256 bytes on the bound's parts
   Workspace ws(st);
-  hipError_t e = ws.take(in.bytes + 2 * each);
+  hipError_t e = ws.take(in.bytes + 2 * kDg * each + (scaled ? 256 + kMostBounds * (int64_t)sizeof(float2) : 0));
   if (e != hipSuccess) return e;
   Matrix m[3];
   e = place_inputs(a, in, ws.p, m, st);
@@ -946,16 +1125,30 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
   g.in_pitch = a.hidden;
   g.vec = whole_units(dh, a.hidden * Op::kEsz);
   g.out0 = dg;
-  g.out1 = dg + each;
+  g.out1 = dg + kDg * each;
+  g.plane = each;
   g.out_cols = g.out_pitch = pitch / Op::kEsz;
+  if constexpr (kScaled<Op>)
+    if (scaled) {
+      g.unscale = reinterpret_cast<float*>(dg + 2 * kDg * each);
+      float2* const bounds = reinterpret_cast<float2*>(dg + 2 * kDg * each + 256);
+      g.bounds = bounds;
+      const int64_t want = cdiv(a.tokens + 2 * a.hidden, kBoundWaves);
+      g.nbounds = (int32_t)(want < kMostBounds ? want : kMostBounds);
+      const BoundArgs b = {m[0], m[1], m[2], static_cast<const _Float16*>(dh), a.tokens, a.hidden, g.vec, bounds};
+      hipLaunchKernelGGL(ffn_bound_kernel, dim3((unsigned)g.nbounds), dim3(64 * kBoundWaves), 0, st,
+                         b);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
   e = run_gate<Op, true>(g, st);
   if (e != hipSuccess) return e;
-  const Matrix d[2] = {{dg, a.tokens, pitch, pitch}, {dg + each, a.tokens, pitch, pitch}};
   ProductArgs w = {}, x = {};
-  w.m[0] = d[0];
-  w.m[1] = d[1];
+  w.m = x.m = Matrix{dg, a.tokens, pitch, pitch};
+  w.plane = x.plane = each;
+  w.unscale = x.unscale = g.unscale;
   w.n[0] = w.n[1] = m[0];
-  w.segments = 1;
+  w.segments = kDg;
   w.outputs = 2;
   w.bytes = a.tokens * Op::kEsz;
   w.rows = a.hidden;
@@ -963,11 +1156,9 @@ hipError_t pullback(const FfnArgs& a, void* dx, void* dwg, void* dwu, const void
   w.out[0] = dwg;
   w.out[1] = dwu;
   w.vec = whole_units(dwg, a.dim * Op::kEsz) && whole_units(dwu, a.dim * Op::kEsz);
-  x.m[0] = d[0];
-  x.m[1] = d[1];
   x.n[0] = m[1];
   x.n[1] = m[2];
-  x.segments = 2;
+  x.segments = 2 * kDg;
   x.outputs = 1;
   x.bytes = pitch;
   x.rows = a.tokens;

@@ -11,7 +11,8 @@ pullback it is made of (``*_forward``, ``*_pullback``), all on the HIP kernels o
 
 Token states have the package's shapes ((T, dim) or (B, T, dim), any leading dimensions),
 weights are (hidden, dim) and (dim,), all in one feature type (float32, float16, bfloat16).
-Sums run in fp32 and each output is rounded once.  Arrays must be dense and on the device.
+Sums run in fp32 and each output is rounded once; what the pullbacks hold between their sums
+has more bits than the feature type.  Arrays must be dense and on the device.
 """
 from __future__ import annotations
 

@@ -460,8 +460,11 @@ fms_status fms_gated_ffn(int32_t dtype, void* h, const void* x, const void* wg, 
 /*
  * Its pullback for the cotangent dh (tokens, hidden): dx (tokens, dim), dwg and dwu
  * (hidden, dim), each overwritten in full.  dx, or dwg and dwu together, may be NULL when
- * not wanted.  The projections are computed again (nothing is kept from the forward); dg
- * and du are rounded once to `dtype` between the products.  Deterministic.
+ * not wanted.  The projections are computed again (nothing is kept from the forward).
+ * Between the products dg and du keep more than `dtype` holds: 16-bit types take two values
+ * for each, a rounding and what it left, and fp16 a power of two from a bound of the largest,
+ * so that no size of dh costs more than the outputs' own rounding.  The workspace holds them,
+ * 8 bytes a token and hidden unit in every type.  Deterministic.
  */
 fms_status fms_gated_ffn_pullback(int32_t dtype, void* dx, void* dwg, void* dwu, const void* dh,
                                   const void* x, const void* wg, const void* wu, int32_t act,
