@@ -26,6 +26,7 @@ MOMENT_BLOCK = 256
 _ADAMW_ENTRY = np.dtype([(k, "u8") for k in ("p", "m", "v", "master", "m_scale", "v_scale")]
                         + [("n", "i8"), ("p_dtype", "i8")])
 _numel, _address, _dtype = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.dtype.__get__
+_contiguous = torch.Tensor.is_contiguous
 _MOMENT_ENTRY = np.dtype([("codes", "u8"), ("scales", "u8"), ("values", "u8"), ("n", "i8"),
                           ("is_signed", "i8")])
 
@@ -82,12 +83,23 @@ def moment_values(moments, out=None):
     return out
 
 
+def _held(moment):
+    """A moment's memory under a handle that no one else has."""
+    if isinstance(moment, Moment8):
+        return Moment8(moment.codes.detach(), moment.scales.detach())
+    return moment.detach() if isinstance(moment, torch.Tensor) else moment
+
+
 class AdamW:
     """AdamW over a list of parameters.
 
     bits: 32 (float32 moments) or 8 (``Moment8``); masters: True to keep float32 copies of
     16-bit parameters, or a list of them (None where a parameter has none); moments: a pair
     of lists (m, v) to go on from, with ``step`` the steps already taken.
+
+    ``m``, ``v`` and ``masters`` are what the steps work on: for given ones, the memory that they
+    were given in, held from then on.  To restore them, copy into them.  A parameter, or one of
+    these, that is given other memory (``.data``, a Moment8's arrays) is stepped there.
 
     A step's number, rate and addresses are arguments of its kernels: captured in a graph it
     would repeat the same step."""
@@ -106,45 +118,109 @@ class AdamW:
         if len(set(map(id, self.params))) != len(self.params):
             raise ArgumentError("AdamW: a parameter is given twice")
         codes = [boundary.dtype_code(p) for p in self.params]
-        if moments is None:
-            if bits == 8:
-                moments = ([Moment8.zeros(p, True) for p in self.params],
-                           [Moment8.zeros(p, False) for p in self.params])
-            else:
-                moments = tuple([torch.zeros_like(p, dtype=torch.float32) for p in self.params]
-                                for _ in range(2))
-        self.m, self.v = tuple(moments[0]), tuple(moments[1])
+        if moments is not None:
+            moments = [map(_held, ms) for ms in moments]
+        elif bits == 8:
+            moments = ([Moment8.zeros(p, signed) for p in self.params] for signed in (True, False))
+        else:
+            moments = ([torch.zeros_like(p, dtype=torch.float32) for p in self.params] for _ in range(2))
+        self._m, self._v = map(tuple, moments)
         if masters is True:
             masters = [None if p.dtype == torch.float32 else p.detach().float() for p in self.params]
-        self.masters = (None,) * len(self.params) if not masters else tuple(masters)
-        if not len(self.params) == len(self.m) == len(self.v) == len(self.masters):
+        elif masters:
+            masters = map(_held, masters)
+        self._masters = tuple(masters) if masters else (None,) * len(self.params)
+        if not len(self.params) == len(self._m) == len(self._v) == len(self._masters):
             raise DimensionMismatch("AdamW: as many moments and masters as parameters")
-        # the table of the library, and what its addresses belong to
+        # Handles of the moments' and masters' memory once anyone else has seen them, and so can
+        # have moved them: None until then.
+        self._state_memory = None
+        # the table of the library
         self._numels, self._dtypes = [p.numel() for p in self.params], [p.dtype for p in self.params]
-        self._held = []
         self._table = np.zeros(len(self.params), _ADAMW_ENTRY)
         self._table["n"], self._table["p_dtype"] = self._numels, codes
-        for e, p, m, v, w in zip(self._table, self.params, self.m, self.v, self.masters):
-            self._place(e, p, m, v, w)
-        self._place_params()
+        self._home = boundary.stream_handle(self._device) if self.params else None
+        self._place()
 
-    def _place_params(self):
-        """Checks the parameters and notes where they lie.  Their memory is held until they are
-        seen elsewhere, so it is theirs as long as they are seen there."""
-        if ([p.numel() for p in self.params] != self._numels
-                or [p.dtype for p in self.params] != self._dtypes):
+    @property
+    def m(self):
+        self._show()
+        return self._m
+
+    @property
+    def v(self):
+        self._show()
+        return self._v
+
+    @property
+    def masters(self):
+        self._show()
+        return self._masters
+
+    def _show(self):
+        if self._state_memory is None:
+            self._state_memory = [t.detach() for t in self._arrays()]
+
+    def _state(self):
+        """The moments, masters and scales by their names in the library's table, None where a
+        parameter has none."""
+        m, v = self._m, self._v
+        eight = [isinstance(a, Moment8) for a in m]
+        if eight != [isinstance(a, Moment8) for a in v]:
+            raise ArgumentError("AdamW: both moments of a parameter in 32 or both in 8 bits")
+        if not any(eight):
+            none = (None,) * len(m)
+            return {"m": m, "v": v, "master": self._masters, "m_scale": none, "v_scale": none}
+        return {"m": [a.codes if e else a for a, e in zip(m, eight)],
+                "v": [a.codes if e else a for a, e in zip(v, eight)], "master": self._masters,
+                "m_scale": [a.scales if e else None for a, e in zip(m, eight)],
+                "v_scale": [a.scales if e else None for a, e in zip(v, eight)]}
+
+    def _arrays(self):
+        return [t for ts in self._state().values() for t in ts if t is not None]
+
+    def _check_state(self, state):
+        """Types and sizes of what _state gives."""
+        blocks = [-(-n // MOMENT_BLOCK) for n in self._numels]
+        eight = [s is not None for s in state["m_scale"]]
+        for name, ts in state.items():
+            code = {"m": torch.int8, "v": torch.uint8}.get(name)
+            for t, n, b, e in zip(ts, self._numels, blocks, eight):
+                if t is None:
+                    continue
+                if t.dtype != (code if code and e else torch.float32):
+                    raise ArgumentError("AdamW: moments are float32, or Moment8 with int8 codes for m and uint8 "
+                                        "codes for v; masters are float32")
+                if t.numel() != (b if name.endswith("scale") else n):
+                    raise DimensionMismatch("AdamW: moments and masters have their parameter's size")
+
+    def _place(self):
+        """Checks every array of a step and notes where it lies, in the library's plan.  The
+        memory of what can be moved is held until it is seen elsewhere, so it is the array's own
+        as long as that is seen there."""
+        params = self.params
+        if list(map(_numel, params)) != self._numels or list(map(_dtype, params)) != self._dtypes:
             raise DimensionMismatch("AdamW: a parameter has changed its size or eltype")
-        if self.params and boundary.require_device(*self.params) != self._device:
+        state = self._state()
+        arrays = [t for ts in state.values() for t in ts if t is not None]
+        if params and boundary.require_device_many(params, arrays) != self._device:
             raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
-        memory = [p.detach() for p in self.params]
+        self._check_state(state)
+        memory = [p.detach() for p in params]
         addresses = list(map(_address, memory))
         self._table["p"] = addresses
+        for name, ts in state.items():
+            self._table[name] = [0 if t is None else t.data_ptr() for t in ts]
         self._check_apart()
         plan = boundary.adamw_plan(self._table)
-        if self.params:
+        if params:
             self._device_plan = torch.from_numpy(plan).to(self._device)
-            self._plan_stream = boundary.stream_handle(self._device)
+            # streams that the memory of what the optimiser has made is safe on
+            self._streams = {boundary.stream_handle(self._device)} & {self._home}
         self._memory, self._addresses, self._plan = memory, addresses, plan  # (all checked)
+        self._state_at = list(map(_address, arrays))
+        if self._state_memory is not None:
+            self._state_memory = [t.detach() for t in arrays]
 
     def _check_apart(self):
         """A step writes every array from workgroups in no order: none may share memory."""
@@ -160,43 +236,26 @@ class AdamW:
         if (starts[1:] < ends[:-1]).any():
             raise ArgumentError("AdamW: parameters, moments and masters must not share memory")
 
-    def _place(self, e, p, m, v, master):
-        if isinstance(m, Moment8) != isinstance(v, Moment8):
-            raise ArgumentError("AdamW: both moments of a parameter in 32 or both in 8 bits")
-        if isinstance(m, Moment8):
-            boundary.require_device(p, m.codes, m.scales, v.codes, v.scales)
-            if m.codes.dtype != torch.int8 or v.codes.dtype != torch.uint8:
-                raise ArgumentError("AdamW: m has int8 codes and v uint8 codes")
-            e["m_scale"], e["v_scale"] = m.scales.data_ptr(), v.scales.data_ptr()
-            self._held += [m.scales, v.scales]
-            m, v = m.codes, v.codes
-        else:
-            boundary.require_device(p, m, v)
-            if m.dtype != torch.float32 or v.dtype != torch.float32:
-                raise ArgumentError("AdamW: moments are float32 or Moment8")
-        if not m.numel() == v.numel() == p.numel():
-            raise DimensionMismatch("AdamW: the moments have their parameter's size")
-        e["m"], e["v"] = m.data_ptr(), v.data_ptr()
-        self._held += [m, v, master]
-        if master is not None:
-            boundary.require_device(p, master)
-            if master.dtype != torch.float32:
-                raise ArgumentError("AdamW: masters are float32")
-            if master.numel() != p.numel():
-                raise DimensionMismatch("AdamW: a master has its parameter's size")
-            e["master"] = master.data_ptr()
+    def _moved(self):
+        """Whether an array does not lie where the plan has it."""
+        params = self.params
+        if (list(map(_address, params)) != self._addresses or list(map(_numel, params)) != self._numels
+                or not all(map(_contiguous, params))):
+            return True
+        # (444 that have been seen: 34 us of host time beside a step's 64)
+        return self._state_memory is not None and list(map(_address, self._arrays())) != self._state_at
 
     def step(self, grads=None, lr=None, grad_scale=1.0):
         """One step, in place.  grads: one per parameter, None to leave it as it is (default: the
         parameters' .grad); lr: instead of the optimiser's; grad_scale: multiplies the
-        gradients (loss scaling, clipping)."""
+        gradients (loss scaling, clipping).  Gradients are only read; they must not lie in the
+        memory of parameters, moments or masters."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise DimensionMismatch(f"{len(grads)} gradients for {len(self.params)} parameters")
         params, numels = self.params, self._numels
-        if (list(map(_address, params)) != self._addresses or list(map(_numel, params)) != numels
-                or not all(map(torch.Tensor.is_contiguous, params))):
-            self._place_params()
+        if self._moved():
+            self._place()
         addresses = np.zeros(len(params), np.uint64)
         keep = slice(None)
         if [g for g in grads if g is None]:
@@ -214,9 +273,13 @@ class AdamW:
         one_type = len(set(map(_dtype, grads))) == 1
         dtypes[keep] = (boundary.dtype_code(grads[0]) if one_type
                         else [boundary.dtype_code(g) for g in grads])
-        if boundary.stream_handle(self._device) != self._plan_stream:
-            # (its memory goes back to the stream it came from, past steps on this one)
-            self._device_plan.record_stream(torch.cuda.current_stream(self._device))
+        stream = boundary.stream_handle(self._device)
+        if stream not in self._streams:
+            # (memory goes back to the stream it came from, past steps on this one)
+            current = torch.cuda.current_stream(self._device)
+            for t in self._arrays() + [self._device_plan]:
+                t.record_stream(current)
+            self._streams.add(stream)
         boundary.adamw_step(self._plan, self._device_plan, addresses, dtypes, self.steps + 1,
                             self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay,
                             grad_scale, self._device)
@@ -225,15 +288,17 @@ class AdamW:
 
     def moment_values(self, out=None):
         """(m, v) as float32 lists; out: such a pair to write the values of 8-bit moments to."""
-        both = self.m + self.v
+        both = self._m + self._v
+        if not all(isinstance(m, Moment8) for m in both):
+            self._show()
         to = [None] * len(both) if out is None else list(out[0]) + list(out[1])
         at = [i for i, m in enumerate(both) if isinstance(m, Moment8)]
         got = moment_values([both[i] for i in at], None if out is None else [to[i] for i in at])
         values = list(both)
         for i, t in zip(at, got):
             values[i] = t
-        return values[:len(self.m)], values[len(self.m):]
+        return values[:len(self._m)], values[len(self._m):]
 
     def __repr__(self):
-        bits = "8" if self.m and isinstance(self.m[0], Moment8) else "32"
+        bits = "8" if self._m and isinstance(self._m[0], Moment8) else "32"
         return f"AdamW({len(self.params)} tensors, {bits}-bit moments, step {self.steps})"
