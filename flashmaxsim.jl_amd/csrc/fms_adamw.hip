@@ -4,7 +4,7 @@
 //   m = beta1 m + (1 - beta1) g
 //   v = beta2 v + (1 - beta2) (g * g)
 //   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
-// in fp32, every operation rounded by itself (the library is built without contraction), on
+// with t the tensor's own steps, in fp32, every operation rounded by itself (the library is built without contraction), on
 // the fp32 master where a tensor has one, else on the parameter.
 //
 // 8-bit moments: 256 neighbouring elements share an fp32 scale a, the largest magnitude among
@@ -19,12 +19,13 @@
 // with 8-bit moments.  A workgroup takes 2048 elements of one tensor, eight a lane, so that
 // half a wave holds a block of 8-bit moments.  What stays (parameters, moments, sizes, and which
 // tensor a workgroup belongs to) is read from the caller's plan in device memory; the gradients'
-// addresses travel as kernel arguments, 480 to a launch.  (With whole tables as arguments, 52 to a
+// addresses travel as kernel arguments, 480 to a launch, with up to 16 different t.  (With whole tables as arguments, 52 to a
 // launch, 148 tensors of 8 million elements took three launches and 68 us,
 // now one and 62; 64 million 8-bit elements in 12 tensors take 262 us with their values, 254 then.)
 #include "fms_adamw.hpp"
 
 #include <float.h>
+#include <math.h>
 
 #include "fms_device.hpp"
 
@@ -179,17 +180,33 @@ __device__ __forceinline__ bool aligned(P... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ...) & 15u) == 0;
 }
 
-constexpr int kTensors = 480;  // per launch: the arguments stay within 4 KiB
-constexpr int kTypeShift = 56;  // a gradient's address and, above it, its element type
+struct AdamWStep {
+  float beta1, rest1;  // and 1 - beta1
+  float beta2, rest2;
+  float eps;
+  float decay;  // 1 - lr * weight_decay
+  float grad_scale;
+};
+struct Correction {  // of a number of steps
+  float lr;          // lr / (1 - beta1^t)
+  float inv_bc2;     // 1 / sqrt(1 - beta2^t)
+};
+constexpr int kTensors = 480;     // per launch: the arguments stay within 4 KiB
+constexpr int kCorrections = 16;  // likewise
+// a gradient's address and, above it, its element type and which correction its tensor takes
+constexpr int kTypeShift = 56, kCorrectionShift = 58;
 struct Grads {
   uint64_t g[kTensors];  // 0: none
-  int32_t first;         // tensor of the launch
+  Correction c[kCorrections];
+  int32_t first;  // tensor of the launch
 };
+static_assert(FMS_BF16 < 1 << (kCorrectionShift - kTypeShift) && kCorrections <= 1 << (64 - kCorrectionShift),
+              "room above the address");
 static_assert(sizeof(Grads) + sizeof(AdamWStep) + 32 <= 4096, "kernel arguments");
 
 // Eight elements a lane from k on; whole half waves take part past the tensor's end.
 __device__ __forceinline__ void adamw_elements(const fms_adamw_tensor& t, const void* grad, int g_dtype,
-                                           const AdamWStep& S, int64_t k, bool vec) {
+                                           const AdamWStep& S, const Correction& c, int64_t k, bool vec) {
   const int64_t n = t.n;
   const bool codes = t.m_scale != nullptr;
   float g[kPer], p[kPer], m[kPer], v[kPer];
@@ -217,8 +234,8 @@ __device__ __forceinline__ void adamw_elements(const fms_adamw_tensor& t, const 
     const float gs = g[e] * S.grad_scale;
     m[e] = m[e] * S.beta1 + gs * S.rest1;
     v[e] = v[e] * S.beta2 + gs * gs * S.rest2;
-    const float den = sqrtf(v[e]) * S.inv_bc2 + S.eps;
-    p[e] = p[e] * S.decay - m[e] / den * S.lr;
+    const float den = sqrtf(v[e]) * c.inv_bc2 + S.eps;
+    p[e] = p[e] * S.decay - m[e] / den * c.lr;
   }
   if (t.master) store8(p, t.master, k, n, vec);
   store_typed(p, t.p, (int)t.p_dtype, k, n, vec);
@@ -273,8 +290,9 @@ __global__ void __launch_bounds__(256) adamw_kernel(const AdamWEntry* entries, c
   // (copied to scalar registers: what the stores below may alias would be read again after them)
   const AdamWEntry entry = uniform(entries[at]);
   const fms_adamw_tensor& t = entry.t;
-  adamw_elements(t, grad, (int)(g >> kTypeShift), S, (block - entry.first) * kChunk + threadIdx.x * kPer,
-                 aligned(t.p, grad, t.m, t.v, t.master));
+  const int type = (int)(g >> kTypeShift) & ((1 << (kCorrectionShift - kTypeShift)) - 1);
+  adamw_elements(t, grad, type, S, G.c[g >> kCorrectionShift],
+                 (block - entry.first) * kChunk + threadIdx.x * kPer, aligned(t.p, grad, t.m, t.v, t.master));
 }
 
 constexpr int kMoments = 92;
@@ -314,7 +332,19 @@ __global__ void __launch_bounds__(256) moment_values_kernel(Moments L) {
 int64_t adamw_blocks(const fms_adamw_tensor& t) { return (t.n + kChunk - 1) / kChunk; }
 
 hipError_t adamw_step(const AdamWPlan* plan, const void* device_plan, const void* const* grads,
-                      const int32_t* g_dtypes, const AdamWStep& s, hipStream_t stream) {
+                      const int32_t* g_dtypes, const AdamWRates& r, hipStream_t stream) {
+  AdamWStep s;
+  s.beta1 = (float)r.beta1;
+  s.rest1 = (float)(1.0 - r.beta1);
+  s.beta2 = (float)r.beta2;
+  s.rest2 = (float)(1.0 - r.beta2);
+  s.eps = (float)r.eps;
+  s.decay = (float)(1.0 - r.lr * r.weight_decay);
+  s.grad_scale = (float)r.grad_scale;
+  const auto correction = [&](int64_t t) {
+    return Correction{(float)(r.lr / (1.0 - pow(r.beta1, (double)t))),
+                      (float)(1.0 / sqrt(1.0 - pow(r.beta2, (double)t)))};
+  };
   const AdamWEntry* const entries = reinterpret_cast<const AdamWEntry*>(plan + 1);
   const AdamWEntry* const on_device =
       reinterpret_cast<const AdamWEntry*>(static_cast<const AdamWPlan*>(device_plan) + 1);
@@ -325,14 +355,24 @@ hipError_t adamw_step(const AdamWPlan* plan, const void* device_plan, const void
     Grads g;
     g.first = (int32_t)i;
     const int64_t first = entries[i].first;
-    int64_t last = first;
-    int n = 0;
+    int64_t last = first, counts[kCorrections];
+    int n = 0, ncounts = 0, at = 0;
     for (; i < plan->count && n < kTensors; ++i, ++n) {
       const int64_t end = entries[i].first + adamw_blocks(entries[i].t);
       if (n > 0 && end - first > kGrid) break;
-      last = end;
       g.g[n] = reinterpret_cast<uint64_t>(grads[i]);
-      if (g.g[n] != 0) g.g[n] |= (uint64_t)g_dtypes[i] << kTypeShift;
+      if (g.g[n] != 0) {
+        const int64_t t = r.steps ? r.steps[i] : r.step;
+        if (ncounts == 0 || counts[at] != t)
+          for (at = 0; at < ncounts && counts[at] != t;) ++at;
+        if (at == kCorrections) break;
+        if (at == ncounts) {
+          counts[ncounts] = t;
+          g.c[ncounts++] = correction(t);
+        }
+        g.g[n] |= (uint64_t)g_dtypes[i] << kTypeShift | (uint64_t)at << kCorrectionShift;
+      }
+      last = end;
     }
     if (last == first) continue;
     hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)(last - first)), dim3(256), 0, stream, on_device,

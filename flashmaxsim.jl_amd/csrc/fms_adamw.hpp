@@ -8,14 +8,12 @@
 
 namespace fms {
 
-struct AdamWStep {
-  float beta1, rest1;  // and 1 - beta1
-  float beta2, rest2;
-  float eps;
-  float decay;    // 1 - lr * weight_decay
-  float lr;       // lr / (1 - beta1^t)
-  float inv_bc2;  // 1 / sqrt(1 - beta2^t)
-  float grad_scale;
+// A step's numbers.  t, a tensor's own steps with this one, is steps[i], or `step` for all of
+// them where steps is null.
+struct AdamWRates {
+  double lr, beta1, beta2, eps, weight_decay, grad_scale;
+  int64_t step;
+  const int64_t* steps;
 };
 
 // A plan: this header, `count` entries, and for each workgroup of a step over all tensors the
@@ -29,7 +27,7 @@ struct AdamWEntry {
 };
 int64_t adamw_blocks(const fms_adamw_tensor& t);
 hipError_t adamw_step(const AdamWPlan* plan, const void* device_plan, const void* const* grads,
-                      const int32_t* g_dtypes, const AdamWStep& s, hipStream_t stream);
+                      const int32_t* g_dtypes, const AdamWRates& r, hipStream_t stream);
 hipError_t moment_values(int64_t count, const fms_moment8* moments, hipStream_t stream);
 
 }  // namespace fms

@@ -1175,29 +1175,38 @@ fms_status fms_adamw_plan(int64_t count, const fms_adamw_tensor* tensors, void* 
   return FMS_OK;
 }
 
+static fms_status adamw_run(const void* plan, const void* device_plan, const void* const* grads,
+                            const int32_t* g_dtypes, const AdamWRates& r, void* stream) {
+  // (negated: a NaN is refused too)
+  if (!(r.beta1 >= 0.0 && r.beta1 < 1.0 && r.beta2 >= 0.0 && r.beta2 < 1.0 && r.eps >= 0.0))
+    return FMS_EINVAL;
+  const AdamWPlan* const p = static_cast<const AdamWPlan*>(plan);
+  if (p->blocks == 0) return FMS_OK;
+  if (!device_plan || !grads || !g_dtypes) return FMS_EINVAL;
+  for (int64_t i = 0; i < p->count; ++i)
+    if (grads[i]) {
+      if (elem_bytes(g_dtypes[i]) == 0) return FMS_EUNSUPPORTED;
+      if (r.steps && r.steps[i] < 1) return FMS_EINVAL;
+    }
+  return from_hip(adamw_step(p, device_plan, grads, g_dtypes, r, as_stream(stream)));
+}
+
 fms_status fms_adamw_step(const void* plan, const void* device_plan, const void* const* grads,
                           const int32_t* g_dtypes, int64_t step, double lr, double beta1,
                           double beta2, double eps, double weight_decay, double grad_scale,
                           void* stream) {
   if (!plan || step < 1) return FMS_EINVAL;
-  // (negated: a NaN is refused too)
-  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return FMS_EINVAL;
-  const AdamWPlan* const p = static_cast<const AdamWPlan*>(plan);
-  if (p->blocks == 0) return FMS_OK;
-  if (!device_plan || !grads || !g_dtypes) return FMS_EINVAL;
-  for (int64_t i = 0; i < p->count; ++i)
-    if (grads[i] && elem_bytes(g_dtypes[i]) == 0) return FMS_EUNSUPPORTED;
-  AdamWStep s;
-  s.beta1 = (float)beta1;
-  s.rest1 = (float)(1.0 - beta1);
-  s.beta2 = (float)beta2;
-  s.rest2 = (float)(1.0 - beta2);
-  s.eps = (float)eps;
-  s.decay = (float)(1.0 - lr * weight_decay);
-  s.lr = (float)(lr / (1.0 - pow(beta1, (double)step)));
-  s.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
-  s.grad_scale = (float)grad_scale;
-  return from_hip(adamw_step(p, device_plan, grads, g_dtypes, s, as_stream(stream)));
+  return adamw_run(plan, device_plan, grads, g_dtypes,
+                   AdamWRates{lr, beta1, beta2, eps, weight_decay, grad_scale, step, nullptr}, stream);
+}
+
+fms_status fms_adamw_step_each(const void* plan, const void* device_plan, const void* const* grads,
+                               const int32_t* g_dtypes, const int64_t* steps, double lr, double beta1,
+                               double beta2, double eps, double weight_decay, double grad_scale,
+                               void* stream) {
+  if (!plan || (!steps && static_cast<const AdamWPlan*>(plan)->count > 0)) return FMS_EINVAL;
+  return adamw_run(plan, device_plan, grads, g_dtypes,
+                   AdamWRates{lr, beta1, beta2, eps, weight_decay, grad_scale, 1, steps}, stream);
 }
 
 fms_status fms_moment_values(int64_t count, const fms_moment8* moments, void* stream) {

@@ -83,6 +83,7 @@ SIGNATURES = {
     "fms_adamw_plan_bytes": [_i64, _p],
     "fms_adamw_plan": [_i64, _p, _p],
     "fms_adamw_step": [_p, _p, _p, _p, _i64, _d, _d, _d, _d, _d, _d, _p],
+    "fms_adamw_step_each": [_p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _p],
     "fms_moment_values": [_i64, _p, _p],
 }
 _RESTYPES = {

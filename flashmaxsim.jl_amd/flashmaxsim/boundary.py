@@ -765,12 +765,13 @@ def adamw_plan(table):
     return plan
 
 
-def adamw_step(plan, device_plan, grads, g_dtypes, step, lr, betas, eps, weight_decay, grad_scale, dev):
-    """One step over a plan and its copy on the device; grads and g_dtypes are numpy arrays of
-    the gradients' addresses (0: none) and element types, which the caller has checked."""
-    st = _lib.lib().fms_adamw_step(plan.ctypes.data, device_plan.data_ptr(), grads.ctypes.data,
-                                   g_dtypes.ctypes.data, step, lr, betas[0], betas[1], eps,
-                                   weight_decay, grad_scale, stream_handle(dev))
+def adamw_step(plan, device_plan, grads, g_dtypes, steps, lr, betas, eps, weight_decay, grad_scale, dev):
+    """One step over a plan and its copy on the device; grads, g_dtypes and steps are numpy arrays
+    of the gradients' addresses (0: none) and element types, which the caller has checked, and of
+    each tensor's number of steps with this one (int64)."""
+    st = _lib.lib().fms_adamw_step_each(plan.ctypes.data, device_plan.data_ptr(), grads.ctypes.data,
+                                        g_dtypes.ctypes.data, steps.ctypes.data, lr, betas[0], betas[1],
+                                        eps, weight_decay, grad_scale, stream_handle(dev))
     _lib.check(st, "adamw_step")
 
 

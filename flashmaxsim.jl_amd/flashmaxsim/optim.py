@@ -6,7 +6,7 @@ caller).  All tensors of a step go through one kernel, up to 480 a launch, in pl
     m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 
-in fp32.  With fp32 masters beside 16-bit parameters the step works on the masters and the
+with t the steps that the tensor itself has taken (those with a gradient for it), in fp32.  With fp32 masters beside 16-bit parameters the step works on the masters and the
 parameters become their roundings.
 
 8-bit moments (``Moment8``) hold a code for each element and an fp32 scale for every 256
@@ -95,7 +95,8 @@ class AdamW:
 
     bits: 32 (float32 moments) or 8 (``Moment8``); masters: True to keep float32 copies of
     16-bit parameters, or a list of them (None where a parameter has none); moments: a pair
-    of lists (m, v) to go on from, with ``step`` the steps already taken.
+    of lists (m, v) to go on from, with ``step`` the steps already taken, or the list of each
+    parameter's own (``tensor_steps``): a step without a gradient for it is none of its.
 
     ``m``, ``v`` and ``masters`` are what the steps work on: for given ones, the memory that they
     were given in, held from then on.  To restore them, copy into them.  A parameter, or one of
@@ -108,11 +109,15 @@ class AdamW:
                  masters=None, moments=None, step=0):
         self.params = list(params)
         self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
-        self.steps = int(step)
         if bits not in (8, 32):
             raise ArgumentError(f"moments are held in 32 or in 8 bits, got {bits!r}")
+        if np.ndim(step) and len(step) != len(self.params):
+            raise DimensionMismatch(f"{len(step)} numbers of steps for {len(self.params)} parameters")
+        self._tensor_steps = np.zeros(len(self.params), np.int64)
+        self._tensor_steps[:] = step
+        self._steps = int(np.max(step, initial=0))
         b1, b2 = self.betas
-        if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and self.steps >= 0):
+        if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0 and np.min(step, initial=0) >= 0):
             raise ArgumentError(f"AdamW: betas {self.betas}, eps {eps}, step {step}")
         self._device = boundary.require_device(*self.params)
         if len(set(map(id, self.params))) != len(self.params):
@@ -141,6 +146,21 @@ class AdamW:
         self._table["n"], self._table["p_dtype"] = self._numels, codes
         self._home = boundary.stream_handle(self._device) if self.params else None
         self._place()
+
+    @property
+    def steps(self):
+        """The steps taken; set, those of every tensor."""
+        return self._steps
+
+    @steps.setter
+    def steps(self, n):
+        self._steps = int(n)
+        self._tensor_steps[:] = self._steps
+
+    @property
+    def tensor_steps(self):
+        """The steps that each tensor has taken."""
+        return self._tensor_steps.tolist()
 
     @property
     def m(self):
@@ -280,10 +300,11 @@ class AdamW:
             for t in self._arrays() + [self._device_plan]:
                 t.record_stream(current)
             self._streams.add(stream)
-        boundary.adamw_step(self._plan, self._device_plan, addresses, dtypes, self.steps + 1,
+        boundary.adamw_step(self._plan, self._device_plan, addresses, dtypes, self._tensor_steps + 1,
                             self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay,
                             grad_scale, self._device)
-        self.steps += 1
+        self._steps += 1
+        self._tensor_steps[keep] += 1
         torch.autograd.graph.increment_version(params)
 
     def moment_values(self, out=None):

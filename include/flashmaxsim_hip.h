@@ -497,7 +497,7 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
                                    int64_t rows, int64_t dim, int64_t gate_rows, void* stream);
 
 /*
- * One AdamW step over many tensors at once, in place.  In fp32, t = step counted from 1:
+ * One AdamW step over many tensors at once, in place.  In fp32, t counted from 1:
  *   g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * With a master, p is computed from and to it, and the parameter is its rounding.  m and v
@@ -509,7 +509,12 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
  * bytes of host memory, of which the caller keeps a copy in device memory (16-byte aligned).
  * A step reads both and the gradients' addresses and element types, host arrays that are read
  * before the call returns; a NULL gradient leaves its tensor as it is.  One launch takes up
- * to 480 tensors.
+ * to 480 tensors.  No array that a step writes may share memory with another.
+ *
+ * t is a tensor's own number of steps, with this one.  fms_adamw_step has one for all tensors;
+ * where some had no gradient in earlier steps they have taken fewer, and
+ * fms_adamw_step_each takes an array of them, one a tensor (those without a gradient in this
+ * step are not read; a launch takes up to 16 different ones).
  */
 #define FMS_MOMENT_BLOCK 256
 typedef struct fms_adamw_tensor {
@@ -528,6 +533,10 @@ fms_status fms_adamw_step(const void* plan, const void* device_plan, const void*
                           const int32_t* g_dtypes, int64_t step, double lr, double beta1,
                           double beta2, double eps, double weight_decay, double grad_scale,
                           void* stream);
+fms_status fms_adamw_step_each(const void* plan, const void* device_plan, const void* const* grads,
+                               const int32_t* g_dtypes, const int64_t* steps, double lr, double beta1,
+                               double beta2, double eps, double weight_decay, double grad_scale,
+                               void* stream);
 
 /* The values of 8-bit moments, many at once: is_signed 1 for m's codes, 0 for v's. */
 typedef struct fms_moment8 {
