@@ -438,6 +438,12 @@ hipError_t workspace_alloc(void** ptr, size_t bytes, hipStream_t stream, bool ca
       return hipSuccess;
     }
   }
+  if (captured) {  // (a captured call's memory is lent or none)
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusActive;
+    const hipError_t e = hipStreamIsCapturing(stream, &cap);
+    if (e != hipSuccess) (void)hipGetLastError();
+    if (cap != hipStreamCaptureStatusNone) return e != hipSuccess ? e : hipErrorStreamCaptureUnsupported;
+  }
   int dev = 0;
   hipError_t e = stream_device(stream, &dev);
   if (e != hipSuccess) return e;

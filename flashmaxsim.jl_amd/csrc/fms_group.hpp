@@ -48,8 +48,8 @@ hipError_t stream_device(hipStream_t stream, int* dev);
 // Stream-ordered workspace from a library-owned memory pool of the stream's
 // device (created on first use, kept for the life of the process so repeated
 // calls do not return memory to the driver between synchronisations).
-// `captured`: the call may ask the lender under graph capture too, and the memory is the
-// graph's from then on.
+// `captured`: the call asks the lender under graph capture too, and the memory is the graph's
+// from then on; without a lender, or declined, it fails under capture and takes none of the pool.
 hipError_t workspace_alloc(void** ptr, size_t bytes, hipStream_t stream, bool captured = false);
 // This host thread's lender (null: none), asked first for every workspace outside graph
 // capture (and under it where the call says so); workspace_free of what it gave does nothing.

@@ -579,7 +579,8 @@ fms_status fms_debug_cross_lane(float* out, void* stream);
  * calling host thread (NULL: none, the default), may be asked several times by a
  * call, and is not asked while the stream is being captured -- except by the token
  * block's calls, which take no memory from the pool then: what it lends to a captured
- * call belongs to the graph as long as that is replayed (NULL fails the call).
+ * call belongs to the graph as long as that is replayed.  Where it lends none, or none is
+ * set, such a call returns FMS_EHIP and adds nothing to the graph.
  */
 typedef void* (*fms_workspace_lender)(int64_t bytes, void* stream);
 void fms_set_workspace_lender(fms_workspace_lender lender);
