@@ -787,6 +787,7 @@ function block_norm_pullback(dr::MaybeArray{T}, dn::MaybeArray{T}, x::ROCArray{T
     end
     like(a) = a === nothing ? nothing : similar(a)
     dx, df, dgate, dwpost, dwpre = similar(x), like(f), like(gate), like(wpost), like(wpre)
+    rows == 0 && dgate !== nothing && fill!(dgate, 0)  # the library writes a vector for gate_rows rows
     check(ccall((:fms_block_norm_pullback, libfms), Int32,
                 (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
                  Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Float32,

@@ -488,7 +488,8 @@ fms_status fms_block_norm(int32_t dtype, void* r, void* n, const void* x, const 
 /*
  * Its pullback for the cotangents dr and dn (either may be NULL: zero; dn only with
  * wpre).  dx and, where the input they belong to was given, df, dgate, dwpost and dwpre are
- * overwritten in full.  Deterministic.
+ * overwritten in full: dgate's rows / gate_rows vectors, so none for no rows, where a caller
+ * whose gate has one all the same clears its gradient.  Deterministic.
  */
 fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgate, void* dwpost,
                                    void* dwpre, const void* dr, const void* dn, const void* x,
