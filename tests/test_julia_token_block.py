@@ -15,4 +15,4 @@ def test_gate_gradient_of_no_rows_is_zero():
     shared gate has one."""
     pullback = body("block_norm_pullback")
     assert re.search(r"dgate\b.*=.*like\(gate\)", pullback)  # (uninitialised)
-    assert re.search(r"^\s*rows == 0 && dgate !== nothing && fill!\(dgate, 0\)$", pullback, re.M)
+    assert re.search(r"^\s*rows == 0 && dgate !== nothing && fill!\(dgate, 0\)\s*$", pullback, re.M)
