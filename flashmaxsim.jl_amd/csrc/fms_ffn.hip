@@ -53,7 +53,8 @@ struct OutOf<OpBF16> : OutBF16 {};
 template <>
 struct OutOf<OpF32> : OutF32 {};
 
-// act(g) in a, act'(g) in da.
+// act(g) in a, act'(g) in da.  With the hardware's exponential and reciprocal s is within about
+// 2 + |y| / 2 units of its last place; g's own rounding to fp32 moves an exponential of it by |g| / 2.
 template <int kAct>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
   float s, dy;
@@ -240,7 +241,9 @@ __device__ __forceinline__ int columns_left(int64_t cols, int64_t n0) {
 
 // Workgroup -> tile.  Workgroup ids go round robin over the 8 XCDs, each with an L2 of
 // its own: every XCD takes a contiguous run of tiles, and a run walks kGroupM row tiles
-// per column tile, so that the tiles in flight on an XCD share their operands.
+// per column tile, so that the tiles in flight on an XCD share their operands.  (In the
+// pullback's products a unit's number has its workgroup's residue only where the tiles, and the
+// units of the product before, are multiples of 8; otherwise neighbours part.)
 constexpr int kXcds = 8;
 constexpr int kGroupM = 8;
 __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in) {
@@ -881,7 +884,7 @@ hipError_t place_inputs(const FfnArgs& a, const Inputs& in, char* ws, Matrix (&m
 // The tile shapes by element size: wave grid and 32-row fragments per wave.
 template <class Op, bool kMRows, bool kNRows, int kParts>
 struct Shapes {
-  // 256 x 256, 8 waves.  The pullback's products read dg and du from HBM and keep three
+  // 256 x 256, 8 waves (the one that makes dg and du spills 7 registers).  The pullback's products read dg and du from HBM and keep three
   // shorter steps in flight (23040 x 1024 x 4096, with dg and du in one plane each: 1490 us a
   // training step, 1512 with one step of 128 bytes); the projections' operands come from the
   // caches (290 us for 46080 x 768 x 2048, 315 with shorter steps).
@@ -910,9 +913,10 @@ Shape gate_shape(int64_t rows, int64_t cols, int esz) {
   return cdiv(rows, 128) * cdiv(cols, 128) > 256 ? Shape::kSmall : Shape::kTiny;
 }
 
-// Eight hidden units a workgroup where sixteen would leave half the CUs without one (us at dim
-// 1024, one and 32 tokens: hidden 2048, 128 workgroups of sixteen, bf16 3.8 and 5.6 against 4.6
-// and 6.3, fp32 5.1 and 8.3 against 7.6 and 11.5; hidden 2560 bf16 5.0 and 8.6 against 4.6 and 6.4).
+// Eight hidden units a workgroup where sixteen would leave half the CUs without one (us in
+// replayed graphs, 0.4 to 0.8 less than in a kernel trace, at dim 1024, one and 32 tokens: hidden
+// 2048, 128 workgroups of sixteen, bf16 3.8 and 5.6 against 4.6 and 6.3, fp32 5.1 and 8.3 against
+// 7.6 and 11.5; hidden 2560 bf16 5.0 and 8.6 against 4.6 and 6.4).
 template <class Op, int kNT>
 hipError_t launch_few(const GateArgs& g, hipStream_t st) {
   const int64_t ny = cdiv(g.tokens, 16 * kNT);
@@ -925,8 +929,8 @@ hipError_t launch_few(const GateArgs& g, hipStream_t st) {
   return launch(ffn_few_kernel<Op, kNT, 16>, 16);
 }
 
-// Few tokens: against the 64-row tiles, whose time does not fall with the tokens (us at
-// 768 x 2048 / 1024 x 4096):
+// Few tokens: against the 64-row tiles, whose time does not fall with the tokens (us in replayed
+// graphs at 768 x 2048 / 1024 x 4096):
 //   16 bits: 1 token 3.7 / 4.7, 32 tokens 5.1 / 6.5, 64 tokens 6.9 / 8.9 (tiles 7.8 / 9.6;
 //   at dim 512 6.0 / 6.7 and 6.1 / 6.2, at dim 256 4.6 / 4.9 and 4.5 / 4.5);
 //   32 bits: 1 token 4.9 / 7.7, 128 tokens 16 / 34 (tiles 31 / 42), 256 tokens 31 / 67 (32 / 42).

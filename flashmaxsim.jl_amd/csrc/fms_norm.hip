@@ -17,6 +17,11 @@
 // registers, the mean first and then the squares around it.  The column sums over rows
 // stay in registers over a workgroup's rows and are joined in a fixed order: waves
 // through LDS, workgroups by a second kernel.
+//
+// That does not hold for the pullback of rows over 4096: a workgroup of sixteen waves has 128
+// registers a lane, and 235 to 354 of them spill to 532 to 832 bytes of scratch.  Measured
+// (with all inputs, one gate): 8192 rows of 4096 in bf16 forward 44 us and pullback 110, 4096 rows of
+// 8192 57 and 2785 (fp32: 102 and 1028), 2048 rows of 16384 49 and 1482 (103 and 620).
 #include "fms_norm.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
