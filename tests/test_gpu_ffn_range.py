@@ -115,3 +115,20 @@ def test_what_is_not_finite_stays_where_it_was(device, dtype, bad):
     check(dwu[hidden], want[2][hidden], dtype, "dwu")
     assert not torch.isfinite(dx[1]).any()
     assert not torch.isfinite(dwg[7]).any() and not torch.isfinite(dwu[7]).any()
+
+
+@pytest.mark.parametrize("shape", [(500, 100, 60), (300, 64, 136)], ids=str)
+def test_replayed_with_other_sizes(device, shape):
+    """A captured fp16 pullback finds the range of what it is replayed on."""
+    x, wg, wu, dh = make(device, *shape, torch.float16, dh=1.0)
+    d = dh.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fm.gated_ffn_pullback(d, x, wg, wu)
+    for scale in (1.0, 1e-5, 30.0, 0.0):
+        d.copy_(dh * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, fm.gated_ffn_pullback(d, x, wg, wu)))
+        for got, want in zip(out, exact(x, wg, wu, d, "silu")[0]):
+            check(got, want, torch.float16, scale)
