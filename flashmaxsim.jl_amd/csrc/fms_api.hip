@@ -14,6 +14,7 @@
 
 #include "../../include/flashmaxsim_hip.h"
 #include "fms_adamw.hpp"
+#include "fms_attn.hpp"
 #include "fms_backward.hpp"
 #include "fms_ffn.hpp"
 #include "fms_group.hpp"
@@ -1128,6 +1129,198 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
   g.dwpost = wpost ? dwpost : nullptr;
   g.dwpre = wpre ? dwpre : nullptr;
   return from_hip(norm_pullback(a, g, as_stream(stream)));
+}
+
+// ---- attention -------------------------------------------------------------------
+
+namespace {
+
+constexpr int64_t kAttnMaxTokens = (int64_t)1 << 29;
+
+fms_status attn_args(AttnArgs* out, int32_t dtype, const void* q, const void* k, const void* v,
+                     const int64_t* strides, const uint8_t* qmask, const uint8_t* kmask, const int32_t* cu_q,
+                     const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk, int64_t nq, int64_t nk,
+                     int64_t heads, int64_t kv_heads, int64_t dim, float scale, int32_t causal, int64_t window) {
+  if (elem_bytes(dtype) == 0) return FMS_EUNSUPPORTED;
+  if (seqs < 0 || tq < 0 || tk < 0 || heads < 0 || kv_heads < 0 || dim < 0) return FMS_EINVAL;
+  if ((causal & ~1) || window < -1) return FMS_EINVAL;
+  if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return FMS_EINVAL;
+  if ((cu_q == nullptr) != (cu_k == nullptr)) return FMS_EINVAL;
+  const bool ragged = cu_q != nullptr;
+  if (ragged && (qmask || kmask || nq < 0 || nk < 0)) return FMS_EINVAL;
+  if (dim > kAttnMaxDim) return FMS_EUNSUPPORTED;
+  if (tq >= kAttnMaxTokens || tk >= kAttnMaxTokens || seqs > kMaxTokens) return FMS_EUNSUPPORTED;
+  AttnArgs a = {};
+  a.dtype = dtype;
+  a.dim = (int32_t)dim;
+  const int64_t group = heads > 0 ? heads / kv_heads : 1;
+  // (rows of a unit are 32-bit, and their tokens found by a multiplication that is exact below this)
+  if (heads > kMaxTokens || tq * group * group >= kMaxTokens) return FMS_EUNSUPPORTED;
+  a.heads = (int32_t)heads;
+  a.kv_heads = (int32_t)kv_heads;
+  a.group = (int32_t)group;
+  a.group_inv = group > 1 ? (uint32_t)((((uint64_t)1 << 32) + group - 1) / group) : 0;
+  a.causal = causal;
+  a.window = window < kAttnMaxTokens ? (int32_t)window : (int32_t)kAttnMaxTokens;
+  a.scale = scale;
+  a.seqs = seqs;
+  a.tq = (int32_t)tq;
+  a.tk = (int32_t)tk;
+  a.nq = ragged ? nq : seqs * tq;
+  a.nk = ragged ? nk : seqs * tk;
+  if (a.nq > kMaxTokens || a.nk > kMaxTokens) return FMS_EUNSUPPORTED;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  const int64_t dense[9] = {tq * heads * dim,    heads * dim,    dim, tk * kv_heads * dim, kv_heads * dim, dim,
+                            tk * kv_heads * dim, kv_heads * dim, dim};
+  for (int i = 0; i < 9; ++i) {
+    const int64_t st = strides ? strides[i] : dense[i];
+    if (st < 0) return FMS_EINVAL;
+    (i < 3 ? a.qs : i < 6 ? a.ks : a.vs)[i % 3] = st;
+  }
+  a.qmask = qmask;
+  a.kmask = kmask;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  if (a.nq > 0 && heads > 0 && dim > 0 && seqs > 0 && !q) return FMS_EINVAL;
+  if (a.nk > 0 && kv_heads > 0 && dim > 0 && seqs > 0 && (!k || !v)) return FMS_EINVAL;
+  // pieces of work are counted in 32 bits
+  if (seqs * kv_heads > 0 &&
+      ((tq * group / 32 + 1) > kMaxTokens / 16 / (seqs * kv_heads) || (tk / 32 + 1) > kMaxTokens / 16 / (seqs * kv_heads)))
+    return FMS_EUNSUPPORTED;
+  *out = a;
+  return FMS_OK;
+}
+
+// Whether the kernels can read an array as it lies: whole 16-byte units, and 64 neighbouring tokens
+// of all heads within a buffer resource.
+bool attn_reads(const AttnArgs& a, const void* p, const int64_t (&st)[3], int64_t heads) {
+  const int64_t esz = elem_bytes(a.dtype), most = (int64_t)1 << 30;
+  if (!aligned16(p) || a.dim * esz % 16 != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] * esz % 16 != 0) return false;
+  return st[1] < most / esz / 64 && st[2] < most / esz / (heads > 0 ? heads : 1);
+}
+
+// Workspace of a call, in pieces, given back in stream order at its end.
+struct Pieces {
+  void* held[8];
+  int n = 0;
+  hipStream_t stream;
+  explicit Pieces(hipStream_t s) : stream(s) {}
+  ~Pieces() {
+    for (int i = 0; i < n; ++i) (void)workspace_free(held[i], stream);
+  }
+  hipError_t get(void** p, int64_t bytes) {
+    const hipError_t e = workspace_alloc(p, (size_t)(bytes < 256 ? 256 : bytes), stream, true);
+    if (e == hipSuccess) held[n++] = *p;
+    return e;
+  }
+};
+
+// Dense copies, zeros behind dim, of the arrays that the kernels cannot read as they lie.
+hipError_t attn_packed(AttnArgs* a, Pieces* w) {
+  const int64_t esz = elem_bytes(a->dtype), unit = 16 / esz;
+  const int64_t width = (a->dim + unit - 1) / unit * unit;
+  a->units = (int32_t)(width / unit);
+  struct One {
+    const void** p;
+    int64_t (*st)[3];
+    int64_t tokens, heads;
+  } all[3] = {{&a->q, &a->qs, a->tq, a->heads}, {&a->k, &a->ks, a->tk, a->kv_heads}, {&a->v, &a->vs, a->tk, a->kv_heads}};
+  for (int i = 0; i < 3; ++i) {
+    One& x = all[i];
+    if (attn_reads(*a, *x.p, *x.st, x.heads)) continue;
+    const int64_t rows = i == 0 ? a->nq : a->nk;
+    void* to;
+    hipError_t e = w->get(&to, rows * x.heads * width * esz);
+    if (e != hipSuccess) return e;
+    const bool ragged = a->cu_q != nullptr;
+    e = attn_pack(a->dtype, to, *x.p, *x.st, ragged ? 1 : a->seqs, ragged ? rows : x.tokens, x.heads, a->dim,
+                  (int32_t)width, w->stream);
+    if (e != hipSuccess) return e;
+    *x.p = to;
+    (*x.st)[0] = x.tokens * x.heads * width;
+    (*x.st)[1] = x.heads * width;
+    (*x.st)[2] = width;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const void* q, const void* k,
+                         const void* v, const int64_t* strides, const uint8_t* qmask, const uint8_t* kmask,
+                         const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk, int64_t nq,
+                         int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim, float scale, int32_t causal,
+                         int64_t window, void* stream) {
+  AttnArgs a;
+  const fms_status s = attn_args(&a, dtype, q, k, v, strides, qmask, kmask, cu_q, cu_k, seqs, tq, tk, nq, nk, heads,
+                                 kv_heads, dim, scale, causal, window);
+  if (s != FMS_OK) return s;
+  if (a.nq == 0 || heads == 0 || dim == 0) return FMS_OK;
+  if (!o || (dtype != FMS_F32 && (lse == nullptr) != (rest == nullptr))) return FMS_EINVAL;
+  const hipStream_t st = as_stream(stream);
+  hipError_t e = hipSuccess;
+  if (cu_q) e = attn_zero_gaps(dtype, o, cu_q, seqs, a.nq, tq, heads * dim, st);
+  if (cu_q && rest && dtype != FMS_F32 && e == hipSuccess)
+    e = attn_zero_gaps(dtype, rest, cu_q, seqs, a.nq, tq, heads * dim, st);
+  if (e != hipSuccess || seqs == 0 || tq == 0) return from_hip(e);
+  Pieces w(st);
+  e = attn_packed(&a, &w);
+  if (e == hipSuccess) e = attn_forward(a, AttnOut{o, lse, dtype == FMS_F32 ? nullptr : rest}, st);
+  return from_hip(e);
+}
+
+fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, const void* dout, const void* o,
+                                  const float* lse, const void* rest, const void* q, const void* k, const void* v,
+                                  const int64_t* strides, const uint8_t* qmask, const uint8_t* kmask,
+                                  const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk,
+                                  int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim, float scale,
+                                  int32_t causal, int64_t window, void* stream) {
+  AttnArgs a;
+  const fms_status s = attn_args(&a, dtype, q, k, v, strides, qmask, kmask, cu_q, cu_k, seqs, tq, tk, nq, nk, heads,
+                                 kv_heads, dim, scale, causal, window);
+  if (s != FMS_OK) return s;
+  if (dim == 0 || (a.nq == 0 && a.nk == 0) || heads == 0) return FMS_OK;
+  if (a.nq > 0 && (!dq || !dout || !o || !lse || (dtype != FMS_F32 && !rest))) return FMS_EINVAL;
+  if (a.nk > 0 && (!dk || !dv)) return FMS_EINVAL;
+  const hipStream_t st = as_stream(stream);
+  hipError_t e = hipSuccess;
+  if (cu_q) {
+    e = attn_zero_gaps(dtype, dq, cu_q, seqs, a.nq, tq, heads * dim, st);
+    if (e == hipSuccess) e = attn_zero_gaps(dtype, dk, cu_k, seqs, a.nk, tk, kv_heads * dim, st);
+    if (e == hipSuccess) e = attn_zero_gaps(dtype, dv, cu_k, seqs, a.nk, tk, kv_heads * dim, st);
+  }
+  if (e != hipSuccess || seqs == 0) return from_hip(e);
+  Pieces w(st);
+  AttnGrads g = {};
+  const int64_t rows = a.nq * heads, esz = elem_bytes(dtype);
+  void* p;
+  e = w.get(&p, rows * 4);
+  g.delta = static_cast<float*>(p);
+  if (e == hipSuccess && dtype == FMS_F16) {
+    e = w.get(&p, seqs * kv_heads * kAttnPeakParts * 8);
+    g.peaks = static_cast<float*>(p);
+  }
+  if (e == hipSuccess) e = attn_packed(&a, &w);
+  g.lse = lse;
+  g.dq = dq;
+  g.dk = dk;
+  g.dv = dv;
+  const int64_t width = a.units * (16 / esz), dense[3] = {0, heads * dim, dim};
+  const void* from[3] = {dout, o, dtype == FMS_F32 ? nullptr : rest};
+  const void** to[3] = {&g.dout, &g.o, &g.rest};
+  for (int i = 0; i < 3 && e == hipSuccess; ++i) {
+    *to[i] = from[i];
+    if (!from[i] || (width == dim && aligned16(from[i]))) continue;
+    e = w.get(&p, rows * width * esz);
+    if (e == hipSuccess) e = attn_pack(dtype, p, from[i], dense, 1, a.nq, heads, (int32_t)dim, (int32_t)width, st);
+    *to[i] = p;
+  }
+  if (e == hipSuccess) e = attn_pullback(a, g, st);
+  return from_hip(e);
 }
 
 // The workgroups of a step over all tensors; -1 and *status where a tensor is not valid.

@@ -1,0 +1,433 @@
+// fms_attn_back.hip -- the pullback of attention over heads.
+//
+// With p_ij as in the forward, computed again from q, k and the kept logarithms of its sums:
+//   dv_j = sum_i p_ij do_i                     dp_ij = do_i v_j
+//   ds_ij = p_ij (dp_ij - delta_i)             delta_i = sum_j p_ij dp_ij = do_i o_i
+//   dq_i = scale sum_j ds_ij k_j               dk_j = scale sum_i ds_ij q_i
+//
+// Two kernels, one with a wave's rows in registers and the keys passing by (dq), one with its keys
+// there and the rows passing by (dk, dv): seven products where one kernel would need five, but
+// each sum stays in registers, in fp32, in a fixed order, with no atomics and no partial sums in
+// memory; the heads that share a key head are rows of one run, so their sums are one too.
+//
+// delta takes o with what its rounding left (the forward keeps that): where one key has nearly all
+// the weight, dp - delta is a small difference of nearly equal terms.  p and ds are rounded once
+// to the feature type for their products, which costs about what rounding the results costs.
+// In fp16 both are scaled by powers of two: p by 2^15, dp - delta by a bound of its size from the
+// norms of do and v, so that neither small probabilities nor small cotangents lose their bits.
+#include "fms_attn.hpp"
+
+#include "../../include/flashmaxsim_hip.h"
+
+namespace fms {
+namespace attn {
+namespace {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// p in fp16 is held 2^15 times as large.
+template <class Op>
+constexpr float kShift = std::is_same<Op, OpF16>::value ? 15.0f : 0.0f;
+template <class Op>
+constexpr float kUnshift = std::is_same<Op, OpF16>::value ? 1.0f / 32768.0f : 1.0f;
+
+// A power of two that brings what is at most 2 sqrt(a) sqrt(b) below one (1 where that says nothing).
+__device__ __forceinline__ float scale_below_one(float a, float b) {
+  const float bound = 2.0f * sqrtf(a) * sqrtf(b);
+  if (!(bound > 1e-30f && bound < 1e30f)) return 1.0f;
+  int e;
+  frexpf(bound, &e);
+  return ldexpf(1.0f, -e);
+}
+
+// The values of a fragment as floats.  (fp32: the whole fragment is bit-cast before an element is
+// taken; element by element, this compiler shrinks the load behind it to its first word.)
+template <class Op>
+__device__ __forceinline__ float value(const u32x4& f, int e) {
+  if constexpr (Op::kEsz == 4) {
+    return __builtin_bit_cast(f32x4, f)[e];
+  } else {
+    typedef typename Elem<Op>::T T;
+    typedef T V __attribute__((ext_vector_type(8)));
+    return (float)__builtin_bit_cast(V, f)[e];
+  }
+}
+
+// Largest squared norms of a unit's v and do rows, in kAttnPeakParts parts.
+__global__ void __launch_bounds__(256) attn_peaks_kernel(AttnArgs A, AttnGrads G) {
+  __shared__ float lds[4][2];
+  const int64_t unit = blockIdx.x / kAttnPeakParts;
+  const int part = blockIdx.x % kAttnPeakParts;
+  const int64_t b = unit / A.kv_heads;
+  const int hk = (int)(unit % A.kv_heads);
+  const Span S = span_of(A, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sub = lane >> 3, in = lane & 7;  // eight lanes a row
+  float top[2] = {0.0f, 0.0f};
+  const int width = A.units * 8;
+  const auto norm = [&](const _Float16* p) {
+    float s = 0.0f;
+    typedef _Float16 V __attribute__((ext_vector_type(8)));
+    for (int d = in * 8; d < width; d += 64) {
+      const V v = *reinterpret_cast<const V*>(p + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (float)v[e] * (float)v[e];
+    }
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    s += __shfl_xor(s, 4);
+    return s;
+  };
+  const int step = kAttnPeakParts * 32, at = part * 32 + wave * 8 + sub;
+  const _Float16* v = static_cast<const _Float16*>(A.v) + seq_at(A.vs, A.cu_k, b, S.k0) + hk * A.vs[2];
+  for (int j = at; j < S.nk; j += step)
+    if (!A.kmask || A.kmask[b * A.tk + j]) top[0] = fmaxf(top[0], norm(v + j * A.vs[1]));
+  const _Float16* d = static_cast<const _Float16*>(G.dout) + S.q0 * A.heads * width;
+  for (int r = at; r < S.nq * A.group; r += step) {
+    const int t = token_of(r, A), head = hk * A.group + r - t * A.group;
+    if (!A.qmask || A.qmask[b * A.tq + t]) top[1] = fmaxf(top[1], norm(d + ((int64_t)t * A.heads + head) * width));
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    for (int o = 8; o < 64; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], o));
+    if (lane == 0) lds[wave][i] = top[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const int i = threadIdx.x;
+    G.peaks[(int64_t)blockIdx.x * 2 + i] = fmaxf(fmaxf(lds[0][i], lds[1][i]), fmaxf(lds[2][i], lds[3][i]));
+  }
+}
+__device__ __forceinline__ float peak(const float* peaks, int64_t unit, int which) {
+  float x = peaks[(unit * kAttnPeakParts + (threadIdx.x & (kAttnPeakParts - 1))) * 2 + which];
+#pragma unroll
+  for (int o = 1; o < kAttnPeakParts; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+
+template <class Op, int kD, int kWaves>
+__global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGrads G, int tiles, int64_t work) {
+  typedef Tile<Op, kD> T;
+  typedef typename Elem<Op>::T E;
+  constexpr int kThreads = kWaves * 64;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes];
+  __shared__ uint32_t words[kMaskSpan / 32];
+  const int64_t piece = piece_of(work);
+  if (piece >= work) return;
+  const int64_t unit = piece / tiles;
+  const int tile = A.causal ? tiles - 1 - (int)(piece % tiles) : (int)(piece % tiles);
+  const int64_t b = unit / A.kv_heads;
+  const int hk = (int)(unit % A.kv_heads);
+  const Span S = span_of(A, b);
+  const int nrows = S.nq * A.group;
+  const int row0 = tile * (32 * kWaves);
+  if (row0 >= nrows) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int h = lane >> 5;
+  const int row = row0 + wave * 32 + (lane & 31);
+  const int t = token_of(row, A), head = hk * A.group + row - t * A.group;
+  const bool there = row < nrows && (!A.qmask || A.qmask[b * A.tq + t]);
+  const Reach mine = there ? keys_of(t, S, A) : Reach{0, 0};
+  const int rlast = row0 + 32 * kWaves < nrows ? row0 + 32 * kWaves - 1 : nrows - 1;
+  const int first = keys_of(token_of(row0, A), S, A).lo / kRows * kRows;
+  const int last = keys_of(token_of(rlast, A), S, A).hi;
+  const Reach inner = common(mine);
+
+  const char* qrow = static_cast<const char*>(A.q) +
+                     (seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)t * A.qs[1] + (int64_t)head * A.qs[2]) * Op::kEsz;
+  const int64_t orow = ((S.q0 + t) * A.heads + head) * (int64_t)A.units * 16;
+  u32x4 q[T::kK], d[T::kK];
+  own_row<T>(q, qrow, there, A.units, h);
+  own_row<T>(d, static_cast<const char*>(G.dout) + orow, there, A.units, h);
+  float delta = 0.0f, norm = 0.0f;
+  {
+    u32x4 o[T::kK], rest[T::kK];
+    own_row<T>(o, static_cast<const char*>(G.o) + orow, there, A.units, h);
+    if constexpr (Op::kEsz == 2) own_row<T>(rest, static_cast<const char*>(G.rest) + orow, there, A.units, h);
+#pragma unroll
+    for (int kb = 0; kb < T::kK; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16 / Op::kEsz; ++e) {
+        const float x = value<Op>(d[kb], e);
+        float y = value<Op>(o[kb], e);
+        if constexpr (Op::kEsz == 2) y = __builtin_fmaf(value<Op>(rest[kb], e), 1.0f / kRestScale<Op>, y);
+        delta = __builtin_fmaf(x, y, delta);
+        if constexpr (kShift<Op> != 0.0f) norm = __builtin_fmaf(x, x, norm);
+      }
+    delta += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, delta), h));
+    if constexpr (kShift<Op> != 0.0f)
+      norm += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, norm), h));
+  }
+  const int64_t at = rows_at(A, b, hk, S.q0) + row;
+  if (h == 0 && row < nrows) G.delta[at] = delta;
+  float by = 1.0f;
+  if constexpr (kShift<Op> != 0.0f) by = scale_below_one(norm, peak(G.peaks, unit, 0));
+  const float c = fabsf(A.scale) * kLog2e;
+  const float off = there ? kShift<Op> - G.lse[at] : 0.0f;
+  if (A.scale < 0) negate<T>(q);
+
+  const char* kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
+  const char* vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
+  const int64_t kstep = A.ks[1] * Op::kEsz, vstep = A.vs[1] * Op::kEsz;
+  f32x16 acc[T::kBlocks];
+#pragma unroll
+  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
+
+  for (int span0 = first / kMaskSpan * kMaskSpan; span0 < last; span0 += kMaskSpan) {
+    const int from = first > span0 ? first : span0;
+    const int to = last < span0 + kMaskSpan ? last : span0 + kMaskSpan;
+    if (A.kmask) {
+      landed();
+      const uint8_t* km = A.kmask + b * A.tk;
+      mask_words<kThreads>(words, span0, S.nk, [&](int j) { return km[j] != 0; });
+      landed();
+    }
+    const auto bits_of = [&](int j0) -> uint32_t {
+      const uint32_t there = bits_between(0, to - j0);
+      return A.kmask && there ? rfl32(words[(j0 - span0) / 32]) & there : there;
+    };
+    const auto next = [&](int j0) {
+      while (j0 < to && !(bits_of(j0) | bits_of(j0 + 32))) j0 += kRows;
+      return j0;
+    };
+    const auto request = [&](int j0, int buffer) {
+      const uint32_t w0 = bits_of(j0), w1 = bits_of(j0 + 32);
+      const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
+      T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, ok);
+      T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, ok);
+    };
+    int j0 = next(from);
+    int buffer = 0;
+    if (j0 < to) request(j0, 0);
+    while (j0 < to) {
+      landed();
+      const int j1 = next(j0 + kRows);
+      if (j1 < to) request(j1, buffer ^ 1);
+      const char* const K = lds + buffer * 2 * T::kBytes;
+      const char* const V = K + T::kBytes;
+      const uint32_t w[2] = {bits_of(j0), bits_of(j0 + 32)};
+      const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && j0 >= inner.lo && j0 + kRows <= inner.hi;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x16 x = f32x16{}, y = f32x16{};
+#pragma unroll
+        for (int kb = 0; kb < T::kK; ++kb) {
+          x = mma<Op>(T::rows(K, 32 * half, kb, lane), q[kb], x);
+          y = mma<Op>(T::rows(V, 32 * half, kb, lane), d[kb], y);
+        }
+        float s[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, off)) * ((y[r] - delta) * by);
+        if (!whole_tile) {
+          const int j = j0 + 32 * half;
+          const uint32_t keep = (w[half] & bits_between(mine.lo - j, mine.hi - j)) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = (keep >> (8 * (r >> 2) + (r & 3))) & 1u ? s[r] : 0.0f;
+        }
+        constexpr int kPer = 32 / kGroups<Op>;
+#pragma unroll
+        for (int g = 0; g < kGroups<Op>; ++g) {
+          const u32x4 ds = operand<Op>(s, g);
+#pragma unroll
+          for (int i = 0; i < T::kBlocks; ++i)
+            acc[i] = mma<Op>(T::columns(K, 32 * half + kPer * g, i, lane), ds, acc[i]);
+        }
+      }
+      j0 = j1;
+      buffer ^= 1;
+    }
+  }
+  if (row >= nrows) return;
+  store_row<Op, T::kBlocks>(static_cast<E*>(G.dq) + ((S.q0 + t) * A.heads + head) * (int64_t)A.dim, acc,
+                            A.scale * kUnshift<Op> / by, A.dim, A.dim % 4 == 0 && aligned(G.dq), h);
+}
+
+template <class Op, int kD, int kWaves>
+__global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnGrads G, int tiles, int64_t work) {
+  typedef Tile<Op, kD> T;
+  typedef typename Elem<Op>::T E;
+  constexpr int kThreads = kWaves * 64;
+  constexpr int kBuffer = 2 * T::kBytes + 2 * kRows * 4;  // q, do, lse, delta
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
+  __shared__ uint32_t words[kMaskSpan / 32];
+  const int64_t piece = piece_of(work);
+  if (piece >= work) return;
+  const int64_t unit = piece / tiles;
+  const int tile = (int)(piece % tiles);  // (under a causal mask the first tiles have the most rows)
+  const int64_t b = unit / A.kv_heads;
+  const int hk = (int)(unit % A.kv_heads);
+  const Span S = span_of(A, b);
+  const int key0 = tile * (32 * kWaves);
+  if (key0 >= S.nk) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int h = lane >> 5;
+  const int key = key0 + wave * 32 + (lane & 31);
+  const bool there = key < S.nk && (!A.kmask || A.kmask[b * A.tk + key]);
+  const auto rows_of = [&](int j) {
+    Reach r = tokens_of(j, S, A);
+    r.lo *= A.group;
+    r.hi *= A.group;
+    return r;
+  };
+  const Reach mine = there ? rows_of(key) : Reach{0, 0};
+  const int klast = key0 + 32 * kWaves < S.nk ? key0 + 32 * kWaves - 1 : S.nk - 1;
+  const int first = rows_of(key0).lo / kRows * kRows;
+  const int last = rows_of(klast).hi;
+  const Reach inner = common(mine);
+
+  const int64_t kat = seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2] + (int64_t)key * A.ks[1];
+  const int64_t vat = seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2] + (int64_t)key * A.vs[1];
+  u32x4 k[T::kK], v[T::kK];
+  own_row<T>(k, static_cast<const char*>(A.k) + kat * Op::kEsz, there, A.units, h);
+  own_row<T>(v, static_cast<const char*>(A.v) + vat * Op::kEsz, there, A.units, h);
+  const float c = fabsf(A.scale) * kLog2e;
+  if (A.scale < 0) negate<T>(k);
+  float by = 1.0f;
+  if constexpr (kShift<Op> != 0.0f) by = scale_below_one(peak(G.peaks, unit, 1), peak(G.peaks, unit, 0));
+
+  const char* qbase = static_cast<const char*>(A.q) +
+                      (seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2]) * Op::kEsz;
+  const int64_t width = A.units * (16 / Op::kEsz);
+  const char* dbase = static_cast<const char*>(G.dout) + (S.q0 * A.heads + hk * A.group) * width * Op::kEsz;
+  const int64_t stat = rows_at(A, b, hk, S.q0);
+  f32x16 dk[T::kBlocks], dv[T::kBlocks];
+#pragma unroll
+  for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
+
+  for (int span0 = first / kMaskSpan * kMaskSpan; span0 < last; span0 += kMaskSpan) {
+    const int from = first > span0 ? first : span0;
+    const int to = last < span0 + kMaskSpan ? last : span0 + kMaskSpan;
+    if (A.qmask) {
+      landed();
+      const uint8_t* qm = A.qmask + b * A.tq;
+      mask_words<kThreads>(words, span0, S.nq * A.group, [&](int r) { return qm[token_of(r, A)] != 0; });
+      landed();
+    }
+    const auto bits_of = [&](int r0) -> uint32_t {
+      const uint32_t there = bits_between(0, to - r0);
+      return A.qmask && there ? rfl32(words[(r0 - span0) / 32]) & there : there;
+    };
+    const auto next = [&](int r0) {
+      while (r0 < to && !(bits_of(r0) | bits_of(r0 + 32))) r0 += kRows;
+      return r0;
+    };
+    const auto request = [&](int r0, int buffer) {
+      const uint32_t w0 = bits_of(r0), w1 = bits_of(r0 + 32);
+      const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
+      char* const base = lds + buffer * kBuffer;
+      T::template request_rows<kThreads>(base, qbase, A.qs[1], A.qs[2], A.units, r0, A, ok);
+      T::template request_rows<kThreads>(base + T::kBytes, dbase, A.heads * width, width, A.units, r0, A, ok);
+      if (wave < 2 || kWaves == 1) {
+#pragma unroll
+        for (int i = 0; i < (kWaves == 1 ? 2 : 1); ++i) {
+          const int which = kWaves == 1 ? i : wave;
+          const rsrc_t from_stat = make_rsrc_u((which ? G.delta : G.lse) + stat + r0, 0x7fffffffu);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(from_stat, (lds_ptr)(base + 2 * T::kBytes + which * kRows * 4), 4,
+                                                   r0 + lane < to ? lane * 4 : kFar, 0, 0, 0);
+        }
+      }
+    };
+    int r0 = next(from);
+    int buffer = 0;
+    if (r0 < to) request(r0, 0);
+    while (r0 < to) {
+      landed();
+      const int r1 = next(r0 + kRows);
+      if (r1 < to) request(r1, buffer ^ 1);
+      const char* const Q = lds + buffer * kBuffer;
+      const char* const D = Q + T::kBytes;
+      const float* const lse = reinterpret_cast<const float*>(D + T::kBytes);
+      const uint32_t w[2] = {bits_of(r0), bits_of(r0 + 32)};
+      const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && r0 >= inner.lo && r0 + kRows <= inner.hi;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x16 x = f32x16{}, y = f32x16{};
+#pragma unroll
+        for (int kb = 0; kb < T::kK; ++kb) {
+          x = mma<Op>(T::rows(Q, 32 * half, kb, lane), k[kb], x);
+          y = mma<Op>(T::rows(D, 32 * half, kb, lane), v[kb], y);
+        }
+        float p[16], ds[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + 32 * half + 8 * g + 4 * h);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(lse + kRows + 32 * half + 8 * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, kShift<Op> - l4[e]));
+            ds[r] = p[r] * ((y[r] - d4[e]) * by);
+          }
+        }
+        if (!whole_tile) {
+          const int r0h = r0 + 32 * half;
+          const uint32_t keep = (w[half] & bits_between(mine.lo - r0h, mine.hi - r0h)) >> (4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool in = (keep >> (8 * (r >> 2) + (r & 3))) & 1u;
+            p[r] = in ? p[r] : 0.0f;
+            ds[r] = in ? ds[r] : 0.0f;
+          }
+        }
+        constexpr int kPer = 32 / kGroups<Op>;
+#pragma unroll
+        for (int g = 0; g < kGroups<Op>; ++g) {
+          const u32x4 po = operand<Op>(p, g), so = operand<Op>(ds, g);
+#pragma unroll
+          for (int i = 0; i < T::kBlocks; ++i) {
+            dv[i] = mma<Op>(T::columns(D, 32 * half + kPer * g, i, lane), po, dv[i]);
+            dk[i] = mma<Op>(T::columns(Q, 32 * half + kPer * g, i, lane), so, dk[i]);
+          }
+        }
+      }
+      r0 = r1;
+      buffer ^= 1;
+    }
+  }
+  if (key >= S.nk) return;
+  const int64_t at = ((S.k0 + key) * A.kv_heads + hk) * (int64_t)A.dim;
+  const bool vec = A.dim % 4 == 0;
+  store_row<Op, T::kBlocks>(static_cast<E*>(G.dk) + at, dk, A.scale * kUnshift<Op> / by, A.dim, vec && aligned(G.dk), h);
+  store_row<Op, T::kBlocks>(static_cast<E*>(G.dv) + at, dv, kUnshift<Op>, A.dim, vec && aligned(G.dv), h);
+}
+
+template <class Op, int kD>
+hipError_t pullback_dim(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
+  constexpr int kWaves = 4;
+  const int64_t units = a.seqs * a.kv_heads;
+  if (std::is_same<Op, OpF16>::value)
+    hipLaunchKernelGGL(attn_peaks_kernel, dim3((unsigned)(units * kAttnPeakParts)), dim3(256), 0, stream, a, g);
+  {
+    const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), work = units * tiles;
+    if (work)
+      hipLaunchKernelGGL((attn_dq_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a,
+                         g, (int)tiles, work);
+  }
+  const int64_t tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles;
+  if (work)
+    hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
+                       (int)tiles, work);
+  return hipGetLastError();
+}
+template <class Op>
+hipError_t pullback_op(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
+  if (a.dim <= 32) return pullback_dim<Op, 32>(a, g, stream);
+  if (a.dim <= 64) return pullback_dim<Op, 64>(a, g, stream);
+  return pullback_dim<Op, 128>(a, g, stream);
+}
+
+}  // namespace
+}  // namespace attn
+
+hipError_t attn_pullback(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
+  switch (a.dtype) {
+    case FMS_F16: return attn::pullback_op<OpF16>(a, g, stream);
+    case FMS_BF16: return attn::pullback_op<OpBF16>(a, g, stream);
+    default: return attn::pullback_op<OpF32>(a, g, stream);
+  }
+}
+
+}  // namespace fms

@@ -27,6 +27,7 @@ package (Julia ``(dim, T, B)`` == torch ``(B, T, dim)``).
 | varlen_apply_pullback     | varlen_apply_pullback!   (packed.jl:449-485)         |
 | launch_gated_ffn, gated_ffn_apply_pullback     | (no reference method; block.py) |
 | launch_block_norm, block_norm_apply_pullback   | (no reference method; block.py) |
+| launch_attention, attention_apply_pullback     | (no reference method; encoder.py) |
 | adamw_step, moment_values                      | (no reference method; optim.py) |
 
 The pullbacks overwrite their gradient outputs in full (the reference
@@ -36,6 +37,7 @@ holds, since both strategies compute the same sums.
 """
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import numpy as np
@@ -755,6 +757,81 @@ def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, 
         kind, scale, eps, rows, dim, gate_rows, stream_handle(dev))
     if st:
         _lib.check(st, "block_norm_apply_pullback")
+
+
+# ---- encoder (no reference method) ------------------------------------------------------
+
+def _check_heads(q, k, v):
+    """Device, eltype and layout of the heads' arrays: any strides, a head's values contiguous."""
+    dtype, at = q.dtype, q.get_device()
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        if t is None:
+            continue
+        if at < 0 or t.get_device() != at:
+            require_device(q.new_empty(0), t.new_empty(0))  # (says what is wrong)
+        if t.dtype is not dtype:
+            raise ArgumentError(f"{what} must have the feature eltype {dtype}, got {t.dtype}")
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ArgumentError(f"{what}: the values of a head must be contiguous")
+    return q.device
+
+
+def _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k):
+    """The sizes and pointers that both attention calls take, after the checks of masks and cu."""
+    ragged = cu_q is not None
+    nq, heads, dim = q.shape[-3:]
+    nk, kv_heads = k.shape[-3:-1]
+    seqs = cu_q.numel() - 1 if ragged else (q.shape[0] if q.dim() == 4 else 1)
+    if ragged:
+        for cu, what in ((cu_q, "cu_q"), (cu_k, "cu_k")):
+            require_device(cu)
+            _cu(cu, what, seqs + 1)
+            if cu.device != dev:
+                raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+    else:
+        max_q, max_k = nq, nk
+        for m, what, n in ((qmask, "qmask", seqs * nq), (kmask, "kmask", seqs * nk)):
+            if m is not None:
+                require_device(m)
+                _maskn(m, what, n)
+                if m.device != dev:
+                    raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+    strides = None
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+        strides = (ctypes.c_int64 * 9)(*(n for t in (q, k, v)
+                                         for n in (t.stride(0) if t.dim() == 4 else 0, *t.stride()[-3:-1])))
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, ptr(qmask), ptr(kmask), ptr(cu_q),
+            ptr(cu_k), seqs, max_q, max_k, nq, nk, heads, kv_heads, dim)
+
+
+def launch_attention(o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, scale, causal,
+                     window):
+    """o <- attention of q over k and v; lse and rest (both or neither) keep what the pullback needs."""
+    dev = _check_heads(q, k, v)
+    _check_block(o, (q.shape, "o rest", (o, rest)))
+    args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
+    if lse is not None:
+        require_device(lse, o)
+        _buf(lse, "lse", torch.float32, q.shape[:-1].numel())
+    st = _call_with_workspace(_lib.lib().fms_attention, dev, dtype_code(q), o.data_ptr(), ptr(lse),
+                              ptr(rest), *args, scale, causal, window, stream_handle(dev))
+    if st:
+        _lib.check(st, "launch_attention")
+
+
+def attention_apply_pullback(dq, dk, dv, do, o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q,
+                             max_k, scale, causal, window):
+    """dq, dk, dv <- pullback of do; o, lse and rest are the forward's."""
+    dev = _check_heads(q, k, v)
+    _check_block(dq, (q.shape, "dq do o rest", (dq, do, o, rest)), (k.shape, "dk dv", (dk, dv)))
+    args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
+    require_device(lse, dq)
+    _buf(lse, "lse", torch.float32, q.shape[:-1].numel())
+    st = _call_with_workspace(_lib.lib().fms_attention_pullback, dev, dtype_code(q), dq.data_ptr(),
+                              dk.data_ptr(), dv.data_ptr(), do.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                              ptr(rest), *args, scale, causal, window, stream_handle(dev))
+    if st:
+        _lib.check(st, "attention_apply_pullback")
 
 
 def adamw_plan(table):

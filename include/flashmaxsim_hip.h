@@ -498,6 +498,52 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
                                    int64_t rows, int64_t dim, int64_t gate_rows, void* stream);
 
 /*
+ * Attention over heads of token states (heads of one token side by side):
+ *   o[i, h] = sum_j p_ij v[j, g],  p_ij = exp(scale q[i, h] k[j, g]) / sum_j exp(scale q[i, h] k[j, g])
+ * with g = h / (heads / kv_heads) the key head that query head h shares, over the keys j that count
+ * for i; o is zero where none does.  q (seqs, tq, heads, dim), k and v (seqs, tk, kv_heads, dim).
+ * `strides` holds nine element strides, of q's sequences, tokens and heads, then k's and v's
+ * (NULL: dense); the values of a head are contiguous.  o is dense.
+ *
+ * Which keys count:
+ *   - qmask (seqs, tq), kmask (seqs, tk), nullable: a query that is masked has none, a key that
+ *     is masked counts for none.  Rows behind a mask are not read.
+ *   - causal 1: j - (tk - tq) <= i (the last tokens are aligned).
+ *   - window >= 0: j - (tk - tq) is at most that far from i (-1: no window).
+ * Ragged sequences: cu_q and cu_k (seqs + 1, Int32, 1-based, both or neither; the same
+ * array for self-attention): q is (nq, heads, dim), k and v (nk, kv_heads, dim), sequence b has the
+ * token rows cu[b] .. cu[b + 1] - 1, tq and tk are the longest sequences' lengths, and sequence
+ * strides and masks are not used (masks NULL).  A longer sequence is cut to tq and tk; rows
+ * of no sequence give zeros.  nq and nk are not read for padded sequences.
+ *
+ * lse and rest, both or neither, keep what the pullback needs: lse seqs * tq * heads (ragged:
+ * nq * heads) floats, rest like o (what o's rounding left; not
+ * written, and may be NULL, for FMS_F32).  Values that count
+ * for some query of a sequence should be finite: under causal and window an infinite value also
+ * makes rows NaN that share a tile with it.  dim is at most 128, tq and tk are below 2^29.
+ */
+fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const void* q, const void* k,
+                         const void* v, const int64_t* strides, const uint8_t* qmask,
+                         const uint8_t* kmask, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs,
+                         int64_t tq, int64_t tk, int64_t nq, int64_t nk, int64_t heads,
+                         int64_t kv_heads, int64_t dim, float scale, int32_t causal, int64_t window,
+                         void* stream);
+
+/*
+ * Its pullback for the cotangent dout (dense, like o): dq, dk and dv, dense, overwritten in full.
+ * o, lse and rest are what fms_attention gave for the same arguments; the probabilities are
+ * computed again.  Cotangents of masked queries are not read.  Deterministic.
+ */
+fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, const void* dout,
+                                  const void* o, const float* lse, const void* rest, const void* q,
+                                  const void* k, const void* v, const int64_t* strides,
+                                  const uint8_t* qmask, const uint8_t* kmask, const int32_t* cu_q,
+                                  const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk,
+                                  int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                                  int64_t dim, float scale, int32_t causal, int64_t window,
+                                  void* stream);
+
+/*
  * One AdamW step over many tensors at once, in place.  In fp32, t counted from 1:
  *   g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
