@@ -16,12 +16,14 @@
 #include "fms_adamw.hpp"
 #include "fms_attn.hpp"
 #include "fms_backward.hpp"
+#include "fms_embed.hpp"
 #include "fms_ffn.hpp"
 #include "fms_group.hpp"
 #include "fms_inbatch.hpp"
 #include "fms_inbatch_split.hpp"
 #include "fms_misc.hpp"
 #include "fms_norm.hpp"
+#include "fms_rotary.hpp"
 #include "fms_topk.hpp"
 #include "fms_scan_decl.hpp"
 #include "fms_runs.hpp"
@@ -1321,6 +1323,122 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
   }
   if (e == hipSuccess) e = attn_pullback(a, g, st);
   return from_hip(e);
+}
+
+// ---- norm and rotation of heads, token lookup ----------------------------------------
+
+namespace {
+
+// Reports FMS_OK with *work = false where there is nothing to do.
+fms_status rotary_args(RotaryArgs* out, bool* work, int32_t dtype, const void* q, const void* k, const int64_t* strides,
+                       const float* table, const void* positions, int32_t position_bytes, int64_t position_seqs,
+                       const void* wq, const void* wk, int32_t kind, int32_t pairing, float eps, int64_t seqs,
+                       int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t turned,
+                       int64_t table_rows) {
+  *work = false;
+  if (elem_bytes(dtype) == 0) return FMS_EUNSUPPORTED;
+  if (kind != FMS_NORM_RMS && kind != FMS_NORM_LAYER) return FMS_EINVAL;
+  if (pairing != FMS_PAIR_HALVES && pairing != FMS_PAIR_NEIGHBOURS) return FMS_EINVAL;
+  if (seqs < 0 || tokens < 0 || heads < 0 || kv_heads < 0 || dim < 0 || turned < 0 || table_rows < 0) return FMS_EINVAL;
+  if (dim % 2 != 0 || turned % 2 != 0 || turned > dim) return FMS_EINVAL;
+  if (positions && position_bytes != 4 && position_bytes != 8) return FMS_EINVAL;
+  if (positions && position_seqs != 1 && position_seqs != seqs) return FMS_EINVAL;
+  if (!positions && table_rows < tokens && turned > 0) return FMS_EINVAL;
+  if (dim > kRotaryMaxDim) return FMS_EUNSUPPORTED;
+  if (heads + kv_heads > kMaxTokens || seqs > kMaxTokens || tokens > kMaxTokens || seqs * tokens > kMaxTokens)
+    return FMS_EUNSUPPORTED;
+  RotaryArgs a = {};
+  a.dtype = dtype;
+  a.kind = kind;
+  a.pairing = pairing;
+  a.dim = (int32_t)dim;
+  a.turned = (int32_t)turned;
+  a.eps = eps;
+  a.seqs = seqs;
+  a.tokens = tokens;
+  a.heads = (int32_t)heads;
+  a.kv_heads = (int32_t)kv_heads;
+  a.q = q;
+  a.k = k;
+  const int64_t dense[6] = {tokens * heads * dim, heads * dim, dim, tokens * kv_heads * dim, kv_heads * dim, dim};
+  for (int i = 0; i < 6; ++i) {
+    const int64_t st = strides ? strides[i] : dense[i];
+    if (st < 0) return FMS_EINVAL;
+    (i < 3 ? a.qs : a.ks)[i % 3] = st;
+  }
+  a.table = table;
+  a.table_rows = !positions && turned == 0 ? tokens : table_rows;  // (a table of nothing has every row)
+  a.positions = positions;
+  a.position_bytes = position_bytes;
+  a.position_seqs = position_seqs;
+  a.wq = wq;
+  a.wk = wk;
+  *out = a;
+  *work = seqs * tokens > 0 && heads + kv_heads > 0 && dim > 0;
+  if (!*work) return FMS_OK;
+  if ((heads > 0 && !q) || (kv_heads > 0 && !k) || (turned > 0 && table_rows > 0 && !table)) return FMS_EINVAL;
+  return FMS_OK;
+}
+
+fms_status embed_check(EmbedArgs* a, int32_t dtype, const void* ids, int32_t id_bytes, float scale, int64_t tokens,
+                       int64_t vocabulary, int64_t dim) {
+  if (elem_bytes(dtype) == 0) return FMS_EUNSUPPORTED;
+  if (tokens < 0 || vocabulary < 0 || dim < 0 || (id_bytes != 4 && id_bytes != 8)) return FMS_EINVAL;
+  if (tokens > kMaxTokens || vocabulary >= kMaxTokens || dim > ((int64_t)1 << 20)) return FMS_EUNSUPPORTED;
+  *a = EmbedArgs{dtype, id_bytes, ids, scale, tokens, vocabulary, dim};
+  return tokens > 0 && !ids ? FMS_EINVAL : FMS_OK;
+}
+
+}  // namespace
+
+fms_status fms_head_rotary(int32_t dtype, void* q_out, void* k_out, const void* q, const void* k,
+                           const int64_t* strides, const float* table, const void* positions, int32_t position_bytes,
+                           int64_t position_seqs, const void* wq, const void* wk, int32_t kind, int32_t pairing,
+                           float eps, int64_t seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
+                           int64_t turned, int64_t table_rows, void* stream) {
+  RotaryArgs a;
+  bool work;
+  const fms_status s = rotary_args(&a, &work, dtype, q, k, strides, table, positions, position_bytes, position_seqs, wq,
+                                   wk, kind, pairing, eps, seqs, tokens, heads, kv_heads, dim, turned, table_rows);
+  if (s != FMS_OK || !work) return s;
+  if ((heads > 0 && !q_out) || (kv_heads > 0 && !k_out)) return FMS_EINVAL;
+  return from_hip(rotary_forward(a, q_out, k_out, as_stream(stream)));
+}
+
+fms_status fms_head_rotary_pullback(int32_t dtype, void* dq, void* dk, void* dwq, void* dwk, const void* dq_out,
+                                    const void* dk_out, const void* q, const void* k, const int64_t* strides,
+                                    const float* table, const void* positions, int32_t position_bytes,
+                                    int64_t position_seqs, const void* wq, const void* wk, int32_t kind,
+                                    int32_t pairing, float eps, int64_t seqs, int64_t tokens, int64_t heads,
+                                    int64_t kv_heads, int64_t dim, int64_t turned, int64_t table_rows, void* stream) {
+  RotaryArgs a;
+  bool work;
+  const fms_status s = rotary_args(&a, &work, dtype, q, k, strides, table, positions, position_bytes, position_seqs, wq,
+                                   wk, kind, pairing, eps, seqs, tokens, heads, kv_heads, dim, turned, table_rows);
+  if (s != FMS_OK || dim == 0) return s;
+  if ((wq && !dwq) || (wk && !dwk)) return FMS_EINVAL;
+  if (work && ((heads > 0 && (!dq || !dq_out)) || (kv_heads > 0 && (!dk || !dk_out)))) return FMS_EINVAL;
+  if (!work) a.seqs = 0;  // the weights' gradients are zeros
+  return from_hip(rotary_pullback(a, RotaryGrads{dq_out, dk_out, dq, dk, wq ? dwq : nullptr, wk ? dwk : nullptr},
+                                  as_stream(stream)));
+}
+
+fms_status fms_embed_tokens(int32_t dtype, void* e, const void* ids, int32_t id_bytes, const void* weight, float scale,
+                            int64_t tokens, int64_t vocabulary, int64_t dim, void* stream) {
+  EmbedArgs a;
+  const fms_status s = embed_check(&a, dtype, ids, id_bytes, scale, tokens, vocabulary, dim);
+  if (s != FMS_OK || tokens == 0 || dim == 0) return s;
+  if (!e || (vocabulary > 0 && !weight)) return FMS_EINVAL;
+  return from_hip(embed_forward(a, e, weight, as_stream(stream)));
+}
+
+fms_status fms_embed_tokens_pullback(int32_t dtype, void* dweight, const void* de, const void* ids, int32_t id_bytes,
+                                     float scale, int64_t tokens, int64_t vocabulary, int64_t dim, void* stream) {
+  EmbedArgs a;
+  const fms_status s = embed_check(&a, dtype, ids, id_bytes, scale, tokens, vocabulary, dim);
+  if (s != FMS_OK || vocabulary == 0 || dim == 0) return s;
+  if (!dweight || (tokens > 0 && !de)) return FMS_EINVAL;
+  return from_hip(embed_pullback(a, dweight, de, as_stream(stream)));
 }
 
 // The workgroups of a step over all tensors; -1 and *status where a tensor is not valid.

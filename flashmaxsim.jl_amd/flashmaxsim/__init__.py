@@ -20,7 +20,9 @@ from .boundary import (inbatch_device_scan, launch_candidates_scan, launch_int8_
                        launch_int8_pair_scan, launch_int8_paired_scan, launch_packed_scan,
                        launch_pair_scan, launch_paired_scan, launch_varlen_scan,
                        tensor_cores_active)
-from .encoder import AttentionKept, attention, attention_forward, attention_pullback
+from .encoder import (AttentionKept, attention, attention_forward, attention_pullback, embed_tokens,
+                      embed_tokens_forward, embed_tokens_pullback, head_rotary, head_rotary_forward,
+                      head_rotary_pullback, rotary_table)
 from .errors import ArgumentError, DimensionMismatch, HIPError, UnsupportedError
 from .forward import (candidates_forward, inbatch_forward, int8_candidates_forward,
                       int8_pair_forward, int8_paired_forward, packed_forward,
@@ -41,6 +43,8 @@ __all__ = [
     "pair_pullback", "paired_pullback", "inbatch_pullback", "candidates_pullback",
     "packed_pullback", "varlen_pullback", "rrule", "MaxSimFunction",
     "gated_ffn", "gated_ffn_forward", "gated_ffn_pullback",
+    "embed_tokens", "embed_tokens_forward", "embed_tokens_pullback", "rotary_table",
+    "head_rotary", "head_rotary_forward", "head_rotary_pullback",
     "attention", "attention_forward", "attention_pullback", "AttentionKept",
     "block_norm", "block_norm_forward", "block_norm_pullback", "AdamW", "Moment8", "moment_values",
     "launch_pair_scan", "launch_paired_scan", "launch_candidates_scan", "inbatch_device_scan",

@@ -82,6 +82,11 @@ SIGNATURES = {
                                 _i64, _i64, _i64, _p],
     "fms_attention": [_i32] + [_p] * 11 + [_i64] * 8 + [_f, _i32, _i64, _p],
     "fms_attention_pullback": [_i32] + [_p] * 15 + [_i64] * 8 + [_f, _i32, _i64, _p],
+    "fms_head_rotary": [_i32] + [_p] * 7 + [_i32, _i64, _p, _p, _i32, _i32, _f] + [_i64] * 7 + [_p],
+    "fms_head_rotary_pullback": ([_i32] + [_p] * 11 + [_i32, _i64, _p, _p, _i32, _i32, _f] + [_i64] * 7
+                                 + [_p]),
+    "fms_embed_tokens": [_i32, _p, _p, _i32, _p, _f, _i64, _i64, _i64, _p],
+    "fms_embed_tokens_pullback": [_i32, _p, _p, _p, _i32, _f, _i64, _i64, _i64, _p],
     "fms_adamw_plan_bytes": [_i64, _p],
     "fms_adamw_plan": [_i64, _p, _p],
     "fms_adamw_step": [_p, _p, _p, _p, _i64, _d, _d, _d, _d, _d, _d, _p],

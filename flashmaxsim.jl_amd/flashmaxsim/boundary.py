@@ -28,6 +28,8 @@ package (Julia ``(dim, T, B)`` == torch ``(B, T, dim)``).
 | launch_gated_ffn, gated_ffn_apply_pullback     | (no reference method; block.py) |
 | launch_block_norm, block_norm_apply_pullback   | (no reference method; block.py) |
 | launch_attention, attention_apply_pullback     | (no reference method; encoder.py) |
+| launch_head_rotary, head_rotary_apply_pullback | (no reference method; encoder.py) |
+| launch_embed_tokens, embed_tokens_apply_pullback | (no reference method; encoder.py) |
 | adamw_step, moment_values                      | (no reference method; optim.py) |
 
 The pullbacks overwrite their gradient outputs in full (the reference
@@ -761,7 +763,7 @@ def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, 
 
 # ---- encoder (no reference method) ------------------------------------------------------
 
-def _check_heads(q, k, v):
+def _check_heads(q, k, v=None):
     """Device, eltype and layout of the heads' arrays: any strides, a head's values contiguous."""
     dtype, at = q.dtype, q.get_device()
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
@@ -832,6 +834,97 @@ def attention_apply_pullback(dq, dk, dv, do, o, lse, rest, q, k, v, qmask, kmask
                               ptr(rest), *args, scale, causal, window, stream_handle(dev))
     if st:
         _lib.check(st, "attention_apply_pullback")
+
+
+def _rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps):
+    """The arguments that both calls take from the heads on, after the checks of the others."""
+    seqs = q.shape[0] if q.dim() == 4 else 1
+    tokens, heads, dim = q.shape[-3:]
+    kv_heads = 0 if k is None else k.shape[-2]
+    require_device(table, positions, wq, wk)
+    if table.dtype != torch.float32:
+        raise ArgumentError(f"table must be float32, got {table.dtype}")
+    if table.dim() != 2 or table.shape[1] > dim or table.shape[1] % 2:
+        raise DimensionMismatch(f"table must be (positions, turned), turned even and at most {dim}: "
+                                f"got {tuple(table.shape)}")
+    if positions is None:
+        if table.shape[0] < tokens and table.shape[1]:
+            raise DimensionMismatch(f"table has {table.shape[0]} positions for {tokens} tokens")
+    elif positions.dtype not in (torch.int32, torch.int64):
+        raise ArgumentError("positions must be Int32 or Int64")
+    elif positions.shape != q.shape[:-2] and positions.shape != q.shape[-3:-2]:
+        raise DimensionMismatch(f"positions must be (tokens,) or one for each token: got "
+                                f"{tuple(positions.shape)} for {tuple(q.shape)}")
+    for w, what in ((wq, "q_weight"), (wk, "k_weight")):
+        if w is not None and w.dtype != q.dtype:
+            raise ArgumentError(f"{what} must have the feature eltype {q.dtype}, got {w.dtype}")
+        if w is not None and w.shape != q.shape[-1:]:
+            raise DimensionMismatch(f"{what} must have the shape ({dim},), got {tuple(w.shape)}")
+    for t in (table, positions, wq, wk):
+        if t is not None and t.device != dev:
+            raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+    strides = None
+    if not (q.is_contiguous() and (k is None or k.is_contiguous())):
+        strides = (ctypes.c_int64 * 6)(*(n for t in (q, q if k is None else k)
+                                         for n in (t.stride(0) if t.dim() == 4 else 0, *t.stride()[-3:-1])))
+    return (q.data_ptr(), ptr(k), strides, table.data_ptr(), ptr(positions),
+            4 if positions is None else positions.element_size(),
+            seqs if positions is not None and positions.dim() == 2 else 1, ptr(wq), ptr(wk), kind, pairing, eps,
+            seqs, tokens, heads, kv_heads, dim, table.shape[1], table.shape[0])
+
+
+def launch_head_rotary(q_out, k_out, q, k, table, positions, wq, wk, kind, pairing, eps):
+    """q_out, k_out <- norm and rotation of the heads of q and k (k, k_out may be None)."""
+    dev = _check_heads(q, k)
+    _check_block(q_out, (q.shape, "q_out", (q_out,)), (None if k is None else k.shape, "k_out", (k_out,)))
+    st = _lib.lib().fms_head_rotary(dtype_code(q), q_out.data_ptr(), ptr(k_out),
+                                    *_rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps),
+                                    stream_handle(dev))
+    if st:
+        _lib.check(st, "launch_head_rotary")
+
+
+def head_rotary_apply_pullback(dq, dk, dwq, dwk, dq_out, dk_out, q, k, table, positions, wq, wk, kind,
+                               pairing, eps):
+    dev = _check_heads(q, k)
+    _check_block(dq, (q.shape, "dq dq_out", (dq, dq_out)),
+                 (None if k is None else k.shape, "dk dk_out", (dk, dk_out)),
+                 (q.shape[-1:], "dq_weight dk_weight", (dwq, dwk)))
+    st = _call_with_workspace(
+        _lib.lib().fms_head_rotary_pullback, dev, dtype_code(q), dq.data_ptr(), ptr(dk), ptr(dwq), ptr(dwk),
+        dq_out.data_ptr(), ptr(dk_out), *_rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps),
+        stream_handle(dev))
+    if st:
+        _lib.check(st, "head_rotary_apply_pullback")
+
+
+def _check_ids(ids):
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ArgumentError("ids must be Int32 or Int64")
+
+
+def launch_embed_tokens(e, ids, weight, scale):
+    """e <- scale * weight[ids - 1]."""
+    dev = require_device(e, ids, weight)
+    _check_ids(ids)
+    _check_block(weight, (weight.shape, "weight", (weight,)), ((*ids.shape, weight.shape[1]), "e", (e,)))
+    st = _lib.lib().fms_embed_tokens(dtype_code(weight), e.data_ptr(), ids.data_ptr(), ids.element_size(),
+                                     weight.data_ptr(), scale, ids.numel(), weight.shape[0], weight.shape[1],
+                                     stream_handle(dev))
+    if st:
+        _lib.check(st, "launch_embed_tokens")
+
+
+def embed_tokens_apply_pullback(dweight, de, ids, scale):
+    """dweight <- scale * sums of de's rows by id."""
+    dev = require_device(dweight, de, ids)
+    _check_ids(ids)
+    _check_block(dweight, ((*ids.shape, dweight.shape[1]), "de", (de,)))
+    st = _call_with_workspace(_lib.lib().fms_embed_tokens_pullback, dev, dtype_code(dweight),
+                              dweight.data_ptr(), de.data_ptr(), ids.data_ptr(), ids.element_size(), scale,
+                              ids.numel(), dweight.shape[0], dweight.shape[1], stream_handle(dev))
+    if st:
+        _lib.check(st, "embed_tokens_apply_pullback")
 
 
 def adamw_plan(table):

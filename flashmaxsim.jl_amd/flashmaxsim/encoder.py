@@ -1,9 +1,12 @@
-"""Operators of an encoder's layers around the token block: attention.
+"""Operators of an encoder's layers around the token block: token lookup, the norm and rotation of
+queries and keys, attention.
 
 With the token block's operators they make the token states that ``maxsim`` scores out of token
 ids.  (Extension: the reference starts from finished embeddings.)  As in ``block``, each comes as
 a verb that torch autograd records and as the forward and pullback it is made of:
 
+    e = embed_tokens(ids, weight, scale)         rows of the table, scaled
+    q, k = head_rotary(q, k, table, ...)         norm of each head, and its rotation by position
     o = attention(q, k, v, qmask, kmask, ...)    softmax(scale q k^T) v over heads, one kernel
 
 The heads of a token lie side by side: q is (B, T, heads, dim) or (T, heads, dim), k and v the
@@ -19,8 +22,137 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import boundary
-from .block import _cotangent
+from .block import NORMS, _code, _cotangent
 from .errors import ArgumentError, DimensionMismatch
+
+PAIRINGS = ("halves", "neighbours")
+
+
+# ---- token lookup --------------------------------------------------------------------------
+
+def embed_tokens_forward(ids, weight, scale=1.0):
+    """e (*ids.shape, dim) = scale * weight[ids - 1]; see ``embed_tokens``."""
+    if weight.dim() != 2:
+        raise DimensionMismatch("embed_tokens takes a table (vocabulary, dim)")
+    e = weight.new_empty((*ids.shape, weight.shape[1]))
+    boundary.launch_embed_tokens(e, ids, weight, float(scale))
+    return e
+
+
+def embed_tokens_pullback(de, ids, vocabulary, scale=1.0):
+    """dweight (vocabulary, dim) for the cotangent de (*ids.shape, dim): every row written."""
+    if de.dim() != ids.dim() + 1 or vocabulary < 0:
+        raise DimensionMismatch(f"de must be ids' shape and dim: got {tuple(de.shape)} for {tuple(ids.shape)}")
+    dweight = de.new_empty((vocabulary, de.shape[-1]))
+    boundary.embed_tokens_apply_pullback(dweight, de.contiguous(), ids, float(scale))
+    return dweight
+
+
+class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale):
+        ctx.save_for_backward(ids)
+        ctx.args = weight.shape[0], scale
+        return embed_tokens_forward(ids, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, de):
+        return None, embed_tokens_pullback(de, ctx.saved_tensors[0], *ctx.args), None
+
+
+def embed_tokens(ids, weight, scale=1.0):
+    """scale * weight[ids - 1], recorded by autograd: ids (Int32 or Int64, any shape) are 1-based rows of
+    weight (vocabulary, dim), as every index of the package.  An id outside 1 .. vocabulary gives
+    zeros and takes no part in the gradient; 0 pads.  The gradient is the whole table's, its sums in
+    fp32 and in the order of the tokens."""
+    return _EmbedTokens.apply(ids, weight, scale)
+
+
+# ---- norm and rotation of heads --------------------------------------------------------------
+
+def rotary_table(positions, turned, base=10000.0, device=None):
+    """(positions, turned) float32 for ``head_rotary``: row p, counted from 0, has the cosines and then the
+    sines of p * base ** (-2 i / turned), i < turned / 2.  The angles are computed in 64 bits, in
+    32 far positions would be off by much of a turn."""
+    if positions < 0 or turned < 0 or turned % 2:
+        raise ArgumentError("rotary_table takes counts >= 0, turned even")
+    i = torch.arange(turned // 2, dtype=torch.float64, device=device)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * base ** (-2.0 / max(turned, 1) * i)
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def _rotary_codes(q, k, kind, pairing):
+    if q.dim() not in (3, 4):
+        raise DimensionMismatch("head_rotary takes q (B, T, heads, dim) or (T, heads, dim)")
+    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
+        raise DimensionMismatch(f"k {tuple(k.shape)} must have q's tokens and dim: q is {tuple(q.shape)}")
+    if q.shape[-1] % 2:
+        raise DimensionMismatch(f"head_rotary takes heads of an even number of values, got {q.shape[-1]}")
+    return _code(kind, NORMS, "kind"), _code(pairing, PAIRINGS, "pairing")
+
+
+def _dense_like(t):
+    return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def head_rotary_forward(q, k, table, positions=None, *, q_weight=None, k_weight=None, kind="rms",
+                        pairing="halves", eps=1e-6):
+    """(q, k) with each head normed and rotated, dense; see ``head_rotary``."""
+    codes = _rotary_codes(q, k, kind, pairing)
+    out = _dense_like(q), _dense_like(k)
+    boundary.launch_head_rotary(*out, q, k, table, positions, q_weight, k_weight, *codes, float(eps))
+    return out
+
+
+def head_rotary_pullback(dq_out, dk_out, q, k, table, positions=None, *, q_weight=None, k_weight=None,
+                         kind="rms", pairing="halves", eps=1e-6):
+    """(dq, dk, dq_weight, dk_weight) for the cotangents of both outputs (None: zero); None for what was not
+    given."""
+    codes = _rotary_codes(q, k, kind, pairing)
+    cotangents = []
+    for d, like, what in ((dq_out, q, "dq_out"), (dk_out, k, "dk_out")):
+        d = None if like is None else _cotangent(d, like.shape, like, what)
+        if d is None and like is not None:
+            d = torch.zeros(like.shape, dtype=like.dtype, device=like.device)
+        cotangents.append(d)
+    grads = [_dense_like(t) for t in (q, k, q_weight, k_weight)]
+    boundary.head_rotary_apply_pullback(*grads, *cotangents, q, k, table, positions, q_weight, k_weight,
+                                        *codes, float(eps))
+    return tuple(grads)
+
+
+class _HeadRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, table, positions, args):
+        ctx.save_for_backward(q, k, q_weight, k_weight, table, positions)
+        ctx.args = args
+        ctx.set_materialize_grads(False)
+        return head_rotary_forward(q, k, table, positions, q_weight=q_weight, k_weight=k_weight, **args)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
+        grads = head_rotary_pullback(dq, dk, q, k, table, positions, q_weight=q_weight, k_weight=k_weight,
+                                     **ctx.args)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 3
+
+
+def head_rotary(q, k, table, positions=None, *, q_weight=None, k_weight=None, kind="rms", pairing="halves",
+                eps=1e-6):
+    """(q, k) with each head normed and then rotated by its token's position, recorded by autograd.
+
+    q (B, T, heads, dim), k (B, T, kv_heads, dim) or None, or both without B.  A head is normed over its
+    values (kind "rms" or "layer") and multiplied by its weight (dim,); without a weight it is only
+    rotated.  table (P, turned), as ``rotary_table`` makes it, has the cosines and sines of the first
+    ``turned`` values of a head, taken in pairs (i, i + turned / 2) ("halves") or (2 i, 2 i + 1)
+    ("neighbours"); the other values are not rotated.  positions, (T,) or (B, T), Int32 or Int64, are
+    1-based rows of the table, token t takes row t without them.  A position that is none of the
+    table's (0, say, for padding) gives zeros and takes no part in the gradients.  dim is even and
+    at most 512."""
+    args = dict(kind=kind, pairing=pairing, eps=eps)
+    return _HeadRotary.apply(q, k, q_weight, k_weight, table, positions, args)
 
 
 # ---- attention -----------------------------------------------------------------------------

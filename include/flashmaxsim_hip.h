@@ -81,6 +81,10 @@ typedef int32_t fms_status;
 #define FMS_NORM_RMS 0   /* a / sqrt(mean(a^2) + eps) */
 #define FMS_NORM_LAYER 1 /* (a - mean(a)) / sqrt(mean((a - mean(a))^2) + eps) */
 
+/* Which values of a head fms_head_rotary turns together. */
+#define FMS_PAIR_HALVES 0     /* i and i + turned / 2 */
+#define FMS_PAIR_NEIGHBOURS 1 /* 2 i and 2 i + 1 */
+
 /* Human-readable text for a status code (static storage). */
 const char* fms_status_string(fms_status s);
 
@@ -542,6 +546,56 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
                                   int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
                                   int64_t dim, float scale, int32_t causal, int64_t window,
                                   void* stream);
+
+/*
+ * The norm of each head of queries and keys and their rotation by position, in one pass:
+ *   n = norm(x) * w  over the dim values of a head (x itself without w)
+ *   y_a = n_a cos - n_b sin, y_b = n_b cos + n_a sin  for the pairs of the first `turned` values,
+ * the other values are n.  q (seqs, tokens, heads, dim) and k (seqs, tokens, kv_heads, dim, NULL with
+ * kv_heads 0), with six element strides of q's and k's sequences, tokens and heads (NULL: dense;
+ * a head's values are contiguous); q_out and k_out are dense.  table (table_rows, turned) has the
+ * turned / 2 cosines of a position, then its sines.  positions (position_seqs, tokens), Int32 or
+ * Int64 (position_bytes), are 1-based rows of the table, of one sequence for all or of each
+ * (position_seqs 1 or seqs); NULL: token t takes row t, and the table has tokens rows at least.  A token
+ * whose position is none of the table's rows (0, say, for padding) gives zeros.  wq, wk
+ * (dim,) may be NULL.  dim and turned are even, dim at most 512.
+ */
+fms_status fms_head_rotary(int32_t dtype, void* q_out, void* k_out, const void* q, const void* k,
+                           const int64_t* strides, const float* table, const void* positions,
+                           int32_t position_bytes, int64_t position_seqs, const void* wq,
+                           const void* wk, int32_t kind, int32_t pairing, float eps, int64_t seqs,
+                           int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
+                           int64_t turned, int64_t table_rows, void* stream);
+
+/*
+ * Its pullback for the cotangents dq_out and dk_out (dense): dq, dk (dense), and dwq and dwk where the
+ * weight was given, overwritten in full; no gradient for the table.  Deterministic.
+ */
+fms_status fms_head_rotary_pullback(int32_t dtype, void* dq, void* dk, void* dwq, void* dwk,
+                                    const void* dq_out, const void* dk_out, const void* q,
+                                    const void* k, const int64_t* strides, const float* table,
+                                    const void* positions, int32_t position_bytes,
+                                    int64_t position_seqs, const void* wq, const void* wk,
+                                    int32_t kind, int32_t pairing, float eps, int64_t seqs,
+                                    int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
+                                    int64_t turned, int64_t table_rows, void* stream);
+
+/*
+ * Rows of a table by token: e[t] = scale * weight[ids[t] - 1].  ids (tokens,) Int32 or Int64
+ * (id_bytes), 1-based; an id outside 1 .. vocabulary (0, say, for padding) gives zeros.
+ * weight (vocabulary, dim), e (tokens, dim).
+ */
+fms_status fms_embed_tokens(int32_t dtype, void* e, const void* ids, int32_t id_bytes,
+                            const void* weight, float scale, int64_t tokens, int64_t vocabulary,
+                            int64_t dim, void* stream);
+
+/*
+ * Its pullback: dweight (vocabulary, dim), overwritten in full, = scale * the sums of the cotangent
+ * de's rows by id, in fp32 and in the order of the tokens.  Deterministic.
+ */
+fms_status fms_embed_tokens_pullback(int32_t dtype, void* dweight, const void* de, const void* ids,
+                                     int32_t id_bytes, float scale, int64_t tokens,
+                                     int64_t vocabulary, int64_t dim, void* stream);
 
 /*
  * One AdamW step over many tensors at once, in place.  In fp32, t counted from 1:
