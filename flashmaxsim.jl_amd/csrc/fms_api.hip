@@ -1158,6 +1158,8 @@ fms_status attn_args(AttnArgs* out, int32_t dtype, const void* q, const void* k,
   const int64_t group = heads > 0 ? heads / kv_heads : 1;
   // (rows of a unit are 32-bit, and their tokens found by a multiplication that is exact below this)
   if (heads > kMaxTokens || tq * group * group >= kMaxTokens) return FMS_EUNSUPPORTED;
+  // (a wave's rows of a dense array are within one buffer resource)
+  if (heads * kAttnMaxDim * 4 * 64 >= kMaxSeqBytes) return FMS_EUNSUPPORTED;
   a.heads = (int32_t)heads;
   a.kv_heads = (int32_t)kv_heads;
   a.group = (int32_t)group;

@@ -22,33 +22,39 @@ namespace {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// What the splits of a row leave for their join: sums of values, maximum and sum.
+// Where a row's keys are split among workgroups: what each leaves for the join.
 struct Parts {
-  float* acc;   // (piece, value, row) pieces of 32 rows
-  float* stat;  // (piece, 2, row)
+  float* acc;   // (piece, row of the tile, value): sums of values
+  float* stat;  // (piece, row of the tile, 2): maximum and sum
   int splits;
-  int keys;  // of a split
+  int keys;  // of a split, a multiple of kRows
 };
+
+// p in fp16 is held 2^10 times as large, so that small ones keep their bits.
+template <class Op>
+constexpr float kShift = std::is_same<Op, OpF16>::value ? 10.0f : 0.0f;
+
+// A score's factor, to base 2.  (Not zero, so that a masked score's -inf stays that.)
+__device__ __forceinline__ float factor(const AttnArgs& A) { return fmaxf(fabsf(A.scale) * kLog2e, 1e-30f); }
 
 template <class Op, int kD, int kWaves, bool kSplit>
 __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, AttnOut out, Parts P,
-                                                                   int tiles, int64_t work) {
+                                                                   uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
   typedef typename Elem<Op>::T E;
   constexpr int kThreads = kWaves * 64;
-  // p in fp16 is held 2^10 times as large, so that small ones keep their bits
-  constexpr float kShift = std::is_same<Op, OpF16>::value ? 10.0f : 0.0f;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes];
-  __shared__ uint32_t words[kMaskSpan / 32];
-  const int64_t piece = piece_of(work);
+  // (one array: beside a second one the compiler waits for all loads into LDS before it reads there)
+  __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes + kMaskSpan / 8];
+  uint32_t* const words = reinterpret_cast<uint32_t*>(lds + 4 * T::kBytes);
+  const uint32_t piece = piece_of(work);
   if (piece >= work) return;
-  const int split = kSplit ? (int)(piece % P.splits) : 0;
-  const int64_t whole = kSplit ? piece / P.splits : piece;
-  const int64_t unit = whole / tiles;
+  const uint32_t whole = kSplit ? piece / (uint32_t)P.splits : piece;
+  const int split = (int)(piece - whole * (kSplit ? (uint32_t)P.splits : 1u));
+  const uint32_t unit = whole / tiles;
   // (under a causal mask the last tiles have the most keys: they start first)
-  const int tile = A.causal ? tiles - 1 - (int)(whole % tiles) : (int)(whole % tiles);
-  const int64_t b = unit / A.kv_heads;
-  const int hk = (int)(unit % A.kv_heads);
+  const int tile = (int)(A.causal ? tiles - 1 - (whole - unit * tiles) : whole - unit * tiles);
+  const int64_t b = unit / (uint32_t)A.kv_heads;
+  const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
   const int nrows = S.nq * A.group;
   const int row0 = tile * (32 * kWaves);
@@ -57,25 +63,32 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int h = lane >> 5;
   const int row = row0 + wave * 32 + (lane & 31);
-  const int t = token_of(row, A), head = hk * A.group + row - t * A.group;
+  const int t = token_of(row, A), head = row - t * A.group;  // (of the key head's)
+  const int wt = token_of(row0 + wave * 32, A);              // the wave's first token
+  u32x4 q[T::kK];
+  own_row<T>(q, wave_rows<Op>(A.q, seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2], wt, A.qs[1]),
+             row < nrows ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar, A.units, h);
   const bool there = row < nrows && (!A.qmask || A.qmask[b * A.tq + t]);
-  Reach mine = there ? keys_of(t, S, A) : Reach{0, 0};
-  // of the whole workgroup (reaches grow with the token), and of all of this wave's rows
-  const int rlast = row0 + 32 * kWaves < nrows ? row0 + 32 * kWaves - 1 : nrows - 1;
-  int first = keys_of(token_of(row0, A), S, A).lo / kRows * kRows;
-  int last = keys_of(token_of(rlast, A), S, A).hi;
+  // the keys that count for this row by position, and for the workgroup (reaches grow with the token)
+  const Reach mine = keys_of(t, S, A);
+  const auto reach = [&](int r) { return keys_of(token_of(r < nrows ? r : nrows - 1, A), S, A); };
+  int first = reach(row0).lo / kRows * kRows, last = reach(row0 + 32 * kWaves - 1).hi;
   if constexpr (kSplit) {
     const int from = split * P.keys;
     first = first > from ? first : from;
     last = last < from + P.keys ? last : from + P.keys;
   }
-  const Reach inner = common(mine);
-
-  const char* qrow = static_cast<const char*>(A.q) +
-                     (seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)t * A.qs[1] + (int64_t)head * A.qs[2]) * Op::kEsz;
-  u32x4 q[T::kK];
-  own_row<T>(q, qrow, there, A.units, h);
-  const float c = fabsf(A.scale) * kLog2e;
+  // (the masks' bits, the queries and their mask are on their way together)
+  Rows keys = {words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
+  const auto gather = [&] {
+    const uint8_t* km = A.kmask + b * A.tk;
+    keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
+  };
+  if (keys.given && first < last) gather();
+  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no keys are read)
+  if (A.qmask) clear_unless<T>(q, there);
+  const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
+  const float c = factor(A);
   if (A.scale < 0) negate<T>(q);
   const char* kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
   const char* vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
@@ -86,38 +99,35 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
   float m = -INFINITY, l = 0.0f;
 
-  for (int span0 = first / kMaskSpan * kMaskSpan; span0 < last; span0 += kMaskSpan) {
-    const int from = first > span0 ? first : span0;
-    const int to = last < span0 + kMaskSpan ? last : span0 + kMaskSpan;
-    if (A.kmask) {
+  for (bool more = false; keys.span0 < last; keys.span0 += kMaskSpan, more = true) {
+    const int from = first > keys.span0 ? first : keys.span0;
+    const int to = last < keys.span0 + kMaskSpan ? last : keys.span0 + kMaskSpan;
+    keys.to = to;
+    if (more) {  // (every wave is through with the words, and with the buffers)
       landed();
-      const uint8_t* km = A.kmask + b * A.tk;
-      mask_words<kThreads>(words, span0, S.nk, [&](int j) { return km[j] != 0; });
+      if (keys.given) gather();
       landed();
     }
-    const auto bits_of = [&](int j0) -> uint32_t {  // of keys j0 .. j0 + 31, which may end the keys
-      const uint32_t there = bits_between(0, to - j0);
-      return A.kmask && there ? rfl32(words[(j0 - span0) / 32]) & there : there;
-    };
-    const auto next = [&](int j0) {  // the first tile from j0 on that has keys
-      while (j0 < to && !(bits_of(j0) | bits_of(j0 + 32))) j0 += kRows;
-      return j0;
-    };
     const auto request = [&](int j0, int buffer) {
-      const uint32_t w0 = bits_of(j0), w1 = bits_of(j0 + 32);
+      const uint32_t w0 = keys.bits(j0), w1 = keys.bits(j0 + 32);
       const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
       T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, ok);
       T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, ok);
     };
-    int j0 = next(from);
+    int j0 = keys.next(from);
     int buffer = 0;
     if (j0 < to) request(j0, 0);
     while (j0 < to) {
       landed();
-      const int j1 = next(j0 + kRows);
+      const int j1 = keys.next(j0 + kRows);
       if (j1 < to) request(j1, buffer ^ 1);
       const char* const K = lds + buffer * 2 * T::kBytes;
       const char* const V = K + T::kBytes;
+      const bool none = j0 >= wide.any.hi || j0 + kRows <= wide.any.lo;
+      const int now = j0;
+      j0 = j1;
+      buffer ^= 1;
+      if (none) continue;  // (none of this wave's rows reaches here)
       float s[2][16];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -127,17 +137,16 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[half][r] = x[r];
       }
-      const uint32_t w0 = bits_of(j0), w1 = bits_of(j0 + 32);
-      const bool whole_tile = (w0 & w1) == 0xffffffffu && j0 >= inner.lo && j0 + kRows <= inner.hi;
+      const uint32_t w0 = keys.bits(now), w1 = keys.bits(now + 32);
+      const bool whole_tile = (w0 & w1) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
       uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
       if (!whole_tile) {
-        keep[0] = (w0 & bits_between(mine.lo - j0, mine.hi - j0)) >> (4 * h);
-        keep[1] = (w1 & bits_between(mine.lo - j0 - 32, mine.hi - j0 - 32)) >> (4 * h);
+        keep[0] = (w0 & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
+        keep[1] = (w1 & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[half][r] = (keep[half] >> (8 * (r >> 2) + (r & 3))) & 1u ? s[half][r] : -INFINITY;
+          for (int r = 0; r < 16; ++r) s[half][r] = masked(s[half][r], keep[half], r, -INFINITY);
       }
       // (NaN scores are ignored here and make p, and with it the row, NaN)
       float top = m;
@@ -155,18 +164,17 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
           for (int r = 0; r < 16; ++r) acc[i][r] *= by;
         m = top;
       }
-      const float off = m == -INFINITY ? 0.0f : kShift - m * c;
+      const float base = m == -INFINITY ? 0.0f : m, off = kShift<Op> - base * c;
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
-      if (!whole_tile) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[half][r] = (keep[half] >> (8 * (r >> 2) + (r & 3))) & 1u ? s[half][r] : 0.0f;
-      }
+        for (int r = 0; r < 16; ++r) {
+          // (fp32: exactly 1 at the maximum; where p is rounded to 16 bits the cheaper form is that, too)
+          if constexpr (Op::kEsz == 4)
+            s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
+          else
+            s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
+        }
       float sum[2] = {0.0f, 0.0f};
       constexpr int kPer = 32 / kGroups<Op>;
 #pragma unroll
@@ -180,29 +188,35 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
             acc[i] = mma<Op>(T::columns(V, 32 * half + kPer * g, i, lane), p, acc[i]);
         }
       l += sum[0] + sum[1];
-      j0 = j1;
-      buffer ^= 1;
     }
+  }
+  if (A.qmask && !there) {
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
   }
   // both halves of the wave summed other keys of the same row
   l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
+  if (row >= nrows) return;
   if constexpr (kSplit) {
-    float* to = P.acc + (piece * (kWaves * 32 * kD) + wave * 32 * kD);
+    const int64_t slot = (int64_t)piece * (32 * kWaves) + wave * 32 + (lane & 31);
+    float* to = P.acc + slot * kD;
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) to[(32 * i + acc_row(r, h)) * 32 + (lane & 31)] = acc[i][r];
-    float* st = P.stat + (piece * kWaves + wave) * 64;
-    st[lane] = h ? l : m;
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * h) =
+            f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+    P.stat[slot * 2 + h] = h ? l : m;
     return;
   }
-  if (row >= nrows) return;
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   const bool vec = A.dim % 4 == 0 && aligned(out.o) && aligned(out.rest);
-  const int64_t at = ((S.q0 + t) * A.heads + head) * (int64_t)A.dim;
-  store_row<Op, T::kBlocks>(static_cast<E*>(out.o) + at, acc, inv, A.dim, vec, h);
+  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
+  const int at = row_at<Op>(t - wt, width, head, A.dim);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, inv, A.dim, vec, h);
   if (out.lse && h == 0)
-    out.lse[rows_at(A, b, hk, S.q0) + row] = l > 0.0f || l != l ? m * c + __builtin_amdgcn_logf(l) - kShift : -INFINITY;
+    out.lse[rows_at(A, b, hk, S.q0) + row] = l > 0.0f || l != l ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
   if (Op::kEsz == 2 && out.rest) {
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i)
@@ -211,8 +225,58 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
         const float o = acc[i][r] * inv;
         acc[i][r] = (o - (float)(E)o) * kRestScale<Op>;
       }
-    store_row<Op, T::kBlocks>(static_cast<E*>(out.rest) + at, acc, 1.0f, A.dim, vec, h);
+    store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, start, wt, width), at, acc, 1.0f, A.dim, vec, h);
   }
+}
+
+// The splits of row blockIdx.x (of units * most rows), joined by the four waves of a workgroup.
+template <class Op, int kD, int kWaves>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs A, AttnOut out, Parts P, int tiles, int most) {
+  typedef typename Elem<Op>::T E;
+  constexpr int kPer = (kD + 63) / 64;
+  __shared__ float lds[4][kD + 1];
+  const int64_t unit = blockIdx.x / most;
+  const int row = (int)(blockIdx.x % most);
+  const int64_t b = unit / A.kv_heads;
+  const int hk = (int)(unit % A.kv_heads);
+  const Span S = span_of(A, b);
+  if (row >= S.nq * A.group) return;
+  const int tile = row / (32 * kWaves), r = row % (32 * kWaves);
+  const int64_t whole = unit * tiles + (A.causal ? tiles - 1 - tile : tile);
+  const auto slot = [&](int s) { return (whole * P.splits + s) * (32 * kWaves) + r; };
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  float m = -INFINITY;
+  for (int s = lane; s < P.splits; s += 64) m = fmaxf(m, P.stat[slot(s) * 2]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float c = factor(A), base = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[kPer] = {};
+#pragma unroll 4
+  for (int s = wave; s < P.splits; s += 4) {
+    const float* st = P.stat + slot(s) * 2;
+    const float by = __builtin_amdgcn_exp2f((st[0] - base) * c);
+    l += by * st[1];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (lane + 64 * i < kD) acc[i] += by * P.acc[slot(s) * kD + lane + 64 * i];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (lane + 64 * i < kD) lds[wave][lane + 64 * i] = acc[i];
+  if (lane == 0) lds[wave][kD] = l;
+  __syncthreads();
+  l = (lds[0][kD] + lds[1][kD]) + (lds[2][kD] + lds[3][kD]);
+  const bool any = l > 0.0f || l != l;
+  const float inv = any ? 1.0f / l : 0.0f;
+  const int t = token_of(row, A), head = hk * A.group + row - t * A.group;
+  const int64_t at = ((S.q0 + t) * A.heads + head) * (int64_t)A.dim;
+  for (int d = threadIdx.x; d < A.dim; d += 256) {
+    const float o = ((lds[0][d] + lds[1][d]) + (lds[2][d] + lds[3][d])) * inv;
+    static_cast<E*>(out.o)[at + d] = (E)o;
+    if (Op::kEsz == 2 && out.rest) static_cast<E*>(out.rest)[at + d] = (E)((o - (float)(E)o) * kRestScale<Op>);
+  }
+  if (out.lse && threadIdx.x == 0)
+    out.lse[rows_at(A, b, hk, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
 }
 
 template <class E>
@@ -257,9 +321,32 @@ hipError_t by_type(int32_t dtype, F&& f) {
 template <class Op, int kD, int kWaves>
 hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {
   const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), units = a.seqs * a.kv_heads;
-  const int64_t work = units * tiles;
-  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0,
-                     stream, a, out, Parts{}, (int)tiles, work);
+  // Few workgroups of many keys each leave most of the card idle: their keys are split, 256 to a
+  // workgroup at least, until there are two to a CU (16 heads on 4 of 128 values in bf16, one token, 32768
+  // keys: 1414 us in 4 workgroups, SPLITUS in 512).
+  const int64_t pieces = units * tiles, wanted = pieces <= 128 ? 512 / pieces : 1;
+  const int64_t keys = (cdiv(a.tk, wanted) + 255) / 256 * 256;
+  if (a.tk > keys) {
+    Parts p;
+    p.splits = (int)cdiv(a.tk, keys);
+    p.keys = (int)keys;
+    const int64_t slots = pieces * p.splits * (32 * kWaves);
+    void* mem;
+    hipError_t e = workspace_alloc(&mem, (size_t)(slots * (kD + 2) * 4), stream, true);
+    if (e != hipSuccess) return e;
+    p.acc = static_cast<float*>(mem);
+    p.stat = p.acc + slots * kD;
+    hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, true>), dim3(piece_blocks(pieces * p.splits)),
+                       dim3(kWaves * 64), 0, stream, a, out, p, (uint32_t)tiles, (uint32_t)(pieces * p.splits));
+    const int most = a.tq * a.group;
+    hipLaunchKernelGGL((attn_join_kernel<Op, kD, kWaves>), dim3((unsigned)(units * most)), dim3(256), 0, stream, a,
+                       out, p, (int)tiles, most);
+    e = hipGetLastError();
+    const hipError_t ef = workspace_free(mem, stream);
+    return e != hipSuccess ? e : ef;
+  }
+  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(pieces)), dim3(kWaves * 64), 0,
+                     stream, a, out, Parts{}, (uint32_t)tiles, (uint32_t)pieces);
   return hipGetLastError();
 }
 

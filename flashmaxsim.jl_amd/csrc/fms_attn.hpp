@@ -124,9 +124,9 @@ __device__ __forceinline__ int token_of(int row, const AttnArgs& A) {
 
 // The workgroup's place in `work` pieces: each XCD takes a contiguous run of them, so that
 // what neighbouring pieces share is in one L2.
-__device__ __forceinline__ int64_t piece_of(int64_t work) {
-  const int64_t per = (work + 7) / 8;
-  return (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+// (below 2^31 of them, so that the divisions behind it are short ones)
+__device__ __forceinline__ uint32_t piece_of(uint32_t work) {
+  return (blockIdx.x & 7) * ((work + 7) / 8) + (blockIdx.x >> 3);
 }
 inline unsigned piece_blocks(int64_t work) { return (unsigned)((work + 7) / 8 * 8); }
 
@@ -146,7 +146,7 @@ __device__ __forceinline__ Reach keys_of(int token, const Span& s, const AttnArg
   return r;
 }
 __device__ __forceinline__ Reach tokens_of(int key, const Span& s, const AttnArgs& A) {
-  const int pos = key - (s.nk - s.nq);
+  const int pos = key - (s.nk - s.nq);  // the token beside the key
   Reach r = {0, s.nq};
   if (A.window >= 0) {
     if (pos - A.window > 0) r.lo = pos - A.window;
@@ -157,15 +157,14 @@ __device__ __forceinline__ Reach tokens_of(int key, const Span& s, const AttnArg
   if (r.hi < r.lo) r.hi = r.lo;
   return r;
 }
-// What the lanes of a wave have in common of their reaches.
-__device__ __forceinline__ Reach common(Reach r) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_xor(r.lo, o), y = __shfl_xor(r.hi, o);
-    r.lo = x > r.lo ? x : r.lo;
-    r.hi = y < r.hi ? y : r.hi;
-  }
-  return {uniform(r.lo), uniform(r.hi)};
+// Reaches grow with the token (or key), so those of a wave's 32 follow from its first and last: what all have in
+// common, and what any has.  (A masked row or key counts too: it was read as zeros, and its
+// result is made zero at the end.)
+struct Reaches {
+  Reach all, any;
+};
+__device__ __forceinline__ Reaches reaches(const Reach& first, const Reach& last, bool some) {
+  return {{last.lo, first.hi}, {some ? first.lo : 0, some ? last.hi : 0}};
 }
 
 // ---- tiles in LDS --------------------------------------------------------------------------
@@ -328,14 +327,21 @@ __device__ __forceinline__ float add_operand(const u32x4& p, float c) {
 template <class Op>
 constexpr int kGroups = Op::kEsz == 4 ? 4 : 2;  // operands of 32 rows
 
-// Lane's own row as a second operand for `rows`: units 2 kb + half of it, straight from memory.
+// What lies behind a mask may be anything: zero.
 template <class T>
-__device__ __forceinline__ void own_row(u32x4 (&f)[T::kK], const char* row, bool ok, int units, int h) {
+__device__ __forceinline__ void clear_unless(u32x4 (&f)[T::kK], bool there) {
 #pragma unroll
-  for (int kb = 0; kb < T::kK; ++kb) {
-    f[kb] = u32x4{0, 0, 0, 0};
-    if (ok && 2 * kb + h < units) f[kb] = *reinterpret_cast<const u32x4*>(row + (2 * kb + h) * 16);
-  }
+  for (int kb = 0; kb < T::kK; ++kb)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[kb][e] = there ? f[kb][e] : 0u;
+}
+
+// Lane's own row as a second operand for `rows`: units 2 kb + half of it, straight from memory, `at` bytes
+// into the resource (kFar: zeros).  (Loads behind a branch would wait for one another.)
+template <class T>
+__device__ __forceinline__ void own_row(u32x4 (&f)[T::kK], rsrc_t from, int at, int units, int h) {
+#pragma unroll
+  for (int kb = 0; kb < T::kK; ++kb) f[kb] = buf_load16(from, 2 * kb + h < units ? at + (2 * kb + h) * 16 : kFar);
 }
 
 // A negative scale: the same scores from the other sign.
@@ -354,20 +360,45 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
 }
 
-// The mask bits of rows first .. first + kMaskSpan - 1, 32 to a word.  keep(row): is it there, and
-// does its mask have it.  All threads of the workgroup call it.
-template <int kThreads, class Keep>
-__device__ __forceinline__ void mask_words(uint32_t* words, int first, int n, Keep&& keep) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int left = n - first, most = left < kMaskSpan ? left : kMaskSpan;
-  for (int r = wave * 64; r < (most + 63) / 64 * 64; r += kThreads) {
-    const uint64_t bits = __ballot(r + lane < most && keep(first + r + lane));
-    if (lane == 0) {
-      words[r / 32] = (uint32_t)bits;
-      words[r / 32 + 1] = (uint32_t)(bits >> 32);
+// v where register r's row is in `keep` (shifted to the lane's half), else what: two instructions, and
+// no compare whose result a select would wait for.
+__device__ __forceinline__ float masked(float v, uint32_t keep, int r, float what) {
+  const int bit = 8 * (r >> 2) + (r & 3);
+  const uint32_t all = (uint32_t)((int32_t)(keep << (31 - bit)) >> 31);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & all) | (__builtin_bit_cast(uint32_t, what) & ~all));
+}
+
+// Which rows (keys, or query rows) of a stretch are there: `to` ends them, a mask leaves some out.  Masks
+// are held as bits in LDS, kMaskSpan rows at a time.
+struct Rows {
+  uint32_t* words;
+  bool given;  // a mask
+  int span0, to;
+
+  // The mask bits of rows from span0 on, below n; keep(row): its mask has it.  All threads call it.
+  template <int kThreads, class Keep>
+  __device__ __forceinline__ void gather(int n, Keep&& keep) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int left = n - span0, most = left < kMaskSpan ? left : kMaskSpan;
+    for (int r = wave * 64; r < (most + 63) / 64 * 64; r += kThreads) {
+      const uint64_t bits = __ballot(r + lane < most && keep(span0 + r + lane));
+      if (lane == 0) {
+        words[r / 32] = (uint32_t)bits;
+        words[r / 32 + 1] = (uint32_t)(bits >> 32);
+      }
     }
   }
-}
+  // Of rows r0 .. r0 + 31.
+  __device__ __forceinline__ uint32_t bits(int r0) const {
+    const uint32_t in = bits_between(0, to - r0);
+    return given && in ? rfl32(words[(r0 - span0) / 32]) & in : in;
+  }
+  // The first tile from r0 on that has any.
+  __device__ __forceinline__ int next(int r0) const {
+    while (given && r0 < to && !(bits(r0) | bits(r0 + 32))) r0 += kRows;
+    return r0;
+  }
+};
 
 // All that this wave has asked for has landed, and so has every other wave's.
 __device__ __forceinline__ void landed() {
@@ -378,11 +409,11 @@ __device__ __forceinline__ void landed() {
   asm volatile("" ::: "memory");
 }
 
-// A lane's accumulators (its row; values 32 b + 8 (r / 4) + 4 h + r % 4) to the row `out` of
-// `dim` values, times `by`.  vec: rows are whole groups of four, aligned to them.
+// A lane's accumulators (values 32 b + 8 (r / 4) + 4 h + r % 4 of its row) times `by` to its row of `dim` values,
+// `at` bytes into the resource (kFar: nowhere).  vec: rows are whole groups of four, aligned to them.
 template <class Op, int kBlocks>
-__device__ __forceinline__ void store_row(typename Elem<Op>::T* out, const f32x16 (&acc)[kBlocks], float by,
-                                          int dim, bool vec, int h) {
+__device__ __forceinline__ void store_row(rsrc_t to, int at, const f32x16 (&acc)[kBlocks], float by, int dim, bool vec,
+                                          int h) {
   typedef typename Elem<Op>::T T;
   typedef T V4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -390,19 +421,40 @@ __device__ __forceinline__ void store_row(typename Elem<Op>::T* out, const f32x1
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * b + 8 * g + 4 * h;
-      if (vec) {
-        if (d < dim) {
-          V4 x;
+      V4 x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = (T)(acc[b][4 * g + e] * by);
-          *reinterpret_cast<V4*>(out + d) = x;
-        }
+      for (int e = 0; e < 4; ++e) x[e] = (T)(acc[b][4 * g + e] * by);
+      if (vec) {
+        const int off = d < dim ? at + d * Op::kEsz : kFar;
+        if constexpr (Op::kEsz == 2)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), to, off, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), to, off, 0, 0);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < dim) out[d + e] = (T)(acc[b][4 * g + e] * by);
+        for (int e = 0; e < 4; ++e) {
+          const int off = d + e < dim ? at + (d + e) * Op::kEsz : kFar;
+          const T y = x[e];
+          if constexpr (Op::kEsz == 2)
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), to, off, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), to, off, 0, 0);
+        }
       }
     }
+}
+
+// The rows of a wave, 32 from row `first` on, in an array of tokens `token` and heads `head` elements apart:
+// the resource starts at the first row's token, `start` elements into the array being the
+// unit's token 0 and its first head.
+template <class Op>
+__device__ __forceinline__ rsrc_t wave_rows(const void* p, int64_t start, int first_token, int64_t token) {
+  return make_rsrc_u(static_cast<const char*>(p) + (start + first_token * token) * Op::kEsz, 0x7fffffffu);
+}
+// Where a row lies in it.
+template <class Op>
+__device__ __forceinline__ int row_at(int tokens, int64_t token, int heads, int64_t head) {
+  return (tokens * (int)token + heads * (int)head) * Op::kEsz;
 }
 
 }  // namespace attn

@@ -53,6 +53,15 @@ __device__ __forceinline__ float value(const u32x4& f, int e) {
   }
 }
 
+// x[i][i] for i = lane % 32, in both halves of the wave.
+__device__ __forceinline__ float diagonal(const f32x16& x, int lane) {
+  const int i = lane & 31, r = 4 * (i >> 3) + (i & 3);
+  float v = x[0];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) v = r == j ? x[j] : v;
+  return __shfl(v, i + 32 * ((i >> 2) & 1));
+}
+
 // Largest squared norms of a unit's v and do rows, in kAttnPeakParts parts.
 __global__ void __launch_bounds__(256) attn_peaks_kernel(AttnArgs A, AttnGrads G) {
   __shared__ float lds[4][2];
@@ -106,18 +115,17 @@ __device__ __forceinline__ float peak(const float* peaks, int64_t unit, int whic
 }
 
 template <class Op, int kD, int kWaves>
-__global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGrads G, int tiles, int64_t work) {
+__global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGrads G, uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
-  typedef typename Elem<Op>::T E;
   constexpr int kThreads = kWaves * 64;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes];
-  __shared__ uint32_t words[kMaskSpan / 32];
-  const int64_t piece = piece_of(work);
+  __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes + kMaskSpan / 8];  // (one array: as forward)
+  uint32_t* const words = reinterpret_cast<uint32_t*>(lds + 4 * T::kBytes);
+  const uint32_t piece = piece_of(work);
   if (piece >= work) return;
-  const int64_t unit = piece / tiles;
-  const int tile = A.causal ? tiles - 1 - (int)(piece % tiles) : (int)(piece % tiles);
-  const int64_t b = unit / A.kv_heads;
-  const int hk = (int)(unit % A.kv_heads);
+  const uint32_t unit = piece / tiles;
+  const int tile = (int)(A.causal ? tiles - 1 - (piece - unit * tiles) : piece - unit * tiles);
+  const int64_t b = unit / (uint32_t)A.kv_heads;
+  const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
   const int nrows = S.nq * A.group;
   const int row0 = tile * (32 * kWaves);
@@ -126,45 +134,65 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int h = lane >> 5;
   const int row = row0 + wave * 32 + (lane & 31);
-  const int t = token_of(row, A), head = hk * A.group + row - t * A.group;
+  const int t = token_of(row, A), head = row - t * A.group;  // (of the key head's)
+  const int wt = token_of(row0 + wave * 32, A);              // the wave's first token
+  const int64_t at = rows_at(A, b, hk, S.q0) + row;
+  u32x4 q[T::kK], d[T::kK], o[T::kK], rest[T::kK];
+  own_row<T>(q, wave_rows<Op>(A.q, seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2], wt, A.qs[1]),
+             row < nrows ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar, A.units, h);
+  {
+    const int64_t dim = A.units * (16 / Op::kEsz), width = A.heads * dim;
+    const int64_t start = S.q0 * width + (int64_t)hk * A.group * dim;
+    const int place = row < nrows ? row_at<Op>(t - wt, width, head, dim) : kFar;
+    own_row<T>(d, wave_rows<Op>(G.dout, start, wt, width), place, A.units, h);
+    own_row<T>(o, wave_rows<Op>(G.o, start, wt, width), place, A.units, h);
+    if constexpr (Op::kEsz == 2) own_row<T>(rest, wave_rows<Op>(G.rest, start, wt, width), place, A.units, h);
+  }
+  const float lse = row < nrows ? G.lse[at] : 0.0f;
   const bool there = row < nrows && (!A.qmask || A.qmask[b * A.tq + t]);
-  const Reach mine = there ? keys_of(t, S, A) : Reach{0, 0};
-  const int rlast = row0 + 32 * kWaves < nrows ? row0 + 32 * kWaves - 1 : nrows - 1;
-  const int first = keys_of(token_of(row0, A), S, A).lo / kRows * kRows;
-  const int last = keys_of(token_of(rlast, A), S, A).hi;
-  const Reach inner = common(mine);
-
-  const char* qrow = static_cast<const char*>(A.q) +
-                     (seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)t * A.qs[1] + (int64_t)head * A.qs[2]) * Op::kEsz;
-  const int64_t orow = ((S.q0 + t) * A.heads + head) * (int64_t)A.units * 16;
-  u32x4 q[T::kK], d[T::kK];
-  own_row<T>(q, qrow, there, A.units, h);
-  own_row<T>(d, static_cast<const char*>(G.dout) + orow, there, A.units, h);
+  const Reach mine = keys_of(t, S, A);
+  const auto reach = [&](int r) { return keys_of(token_of(r < nrows ? r : nrows - 1, A), S, A); };
+  const int first = reach(row0).lo / kRows * kRows;
+  int last = reach(row0 + 32 * kWaves - 1).hi;
+  Rows keys = {words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
+  const auto gather = [&] {
+    const uint8_t* km = A.kmask + b * A.tk;
+    keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
+  };
+  if (keys.given && first < last) gather();
+  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no keys are read)
+  if (A.qmask) {
+    clear_unless<T>(q, there);
+    clear_unless<T>(d, there);  // (o and rest are zeros there)
+  }
+  const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
   float delta = 0.0f, norm = 0.0f;
   {
-    u32x4 o[T::kK], rest[T::kK];
-    own_row<T>(o, static_cast<const char*>(G.o) + orow, there, A.units, h);
-    if constexpr (Op::kEsz == 2) own_row<T>(rest, static_cast<const char*>(G.rest) + orow, there, A.units, h);
+    // by the same products as dp below, of which the diagonal is wanted: a row that sees one key has
+    // o = v, and dp - delta is then zero and not a rounding
+    f32x16 x = f32x16{};
 #pragma unroll
-    for (int kb = 0; kb < T::kK; ++kb)
+    for (int kb = 0; kb < T::kK; ++kb) x = mma<Op>(o[kb], d[kb], x);
+    delta = diagonal(x, lane);
+    if constexpr (Op::kEsz == 2) {
+      x = f32x16{};
 #pragma unroll
-      for (int e = 0; e < 16 / Op::kEsz; ++e) {
-        const float x = value<Op>(d[kb], e);
-        float y = value<Op>(o[kb], e);
-        if constexpr (Op::kEsz == 2) y = __builtin_fmaf(value<Op>(rest[kb], e), 1.0f / kRestScale<Op>, y);
-        delta = __builtin_fmaf(x, y, delta);
-        if constexpr (kShift<Op> != 0.0f) norm = __builtin_fmaf(x, x, norm);
-      }
-    delta += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, delta), h));
-    if constexpr (kShift<Op> != 0.0f)
+      for (int kb = 0; kb < T::kK; ++kb) x = mma<Op>(rest[kb], d[kb], x);
+      delta += diagonal(x, lane) * (1.0f / kRestScale<Op>);
+    }
+    if constexpr (kShift<Op> != 0.0f) {
+#pragma unroll
+      for (int kb = 0; kb < T::kK; ++kb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) norm = __builtin_fmaf(value<Op>(d[kb], e), value<Op>(d[kb], e), norm);
       norm += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, norm), h));
+    }
   }
-  const int64_t at = rows_at(A, b, hk, S.q0) + row;
   if (h == 0 && row < nrows) G.delta[at] = delta;
   float by = 1.0f;
   if constexpr (kShift<Op> != 0.0f) by = scale_below_one(norm, peak(G.peaks, unit, 0));
   const float c = fabsf(A.scale) * kLog2e;
-  const float off = there ? kShift<Op> - G.lse[at] : 0.0f;
+  const float off = lse > -INFINITY ? kShift<Op> - lse : 0.0f;  // (no key counts: nothing to make infinite)
   if (A.scale < 0) negate<T>(q);
 
   const char* kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
@@ -174,40 +202,37 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
 #pragma unroll
   for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
 
-  for (int span0 = first / kMaskSpan * kMaskSpan; span0 < last; span0 += kMaskSpan) {
-    const int from = first > span0 ? first : span0;
-    const int to = last < span0 + kMaskSpan ? last : span0 + kMaskSpan;
-    if (A.kmask) {
+  for (bool more = false; keys.span0 < last; keys.span0 += kMaskSpan, more = true) {
+    const int from = first > keys.span0 ? first : keys.span0;
+    const int to = last < keys.span0 + kMaskSpan ? last : keys.span0 + kMaskSpan;
+    keys.to = to;
+    if (more) {  // (every wave is through with the words, and with the buffers)
       landed();
-      const uint8_t* km = A.kmask + b * A.tk;
-      mask_words<kThreads>(words, span0, S.nk, [&](int j) { return km[j] != 0; });
+      if (keys.given) gather();
       landed();
     }
-    const auto bits_of = [&](int j0) -> uint32_t {
-      const uint32_t there = bits_between(0, to - j0);
-      return A.kmask && there ? rfl32(words[(j0 - span0) / 32]) & there : there;
-    };
-    const auto next = [&](int j0) {
-      while (j0 < to && !(bits_of(j0) | bits_of(j0 + 32))) j0 += kRows;
-      return j0;
-    };
     const auto request = [&](int j0, int buffer) {
-      const uint32_t w0 = bits_of(j0), w1 = bits_of(j0 + 32);
+      const uint32_t w0 = keys.bits(j0), w1 = keys.bits(j0 + 32);
       const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
       T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, ok);
       T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, ok);
     };
-    int j0 = next(from);
+    int j0 = keys.next(from);
     int buffer = 0;
     if (j0 < to) request(j0, 0);
     while (j0 < to) {
       landed();
-      const int j1 = next(j0 + kRows);
+      const int j1 = keys.next(j0 + kRows);
       if (j1 < to) request(j1, buffer ^ 1);
       const char* const K = lds + buffer * 2 * T::kBytes;
       const char* const V = K + T::kBytes;
-      const uint32_t w[2] = {bits_of(j0), bits_of(j0 + 32)};
-      const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && j0 >= inner.lo && j0 + kRows <= inner.hi;
+      const bool none = j0 >= wide.any.hi || j0 + kRows <= wide.any.lo;
+      const int now = j0;
+      j0 = j1;
+      buffer ^= 1;
+      if (none) continue;  // (none of this wave's rows reaches here)
+      const uint32_t w[2] = {keys.bits(now), keys.bits(now + 32)};
+      const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f32x16 x = f32x16{}, y = f32x16{};
@@ -221,10 +246,10 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
         for (int r = 0; r < 16; ++r)
           s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, off)) * ((y[r] - delta) * by);
         if (!whole_tile) {
-          const int j = j0 + 32 * half;
+          const int j = now + 32 * half;
           const uint32_t keep = (w[half] & bits_between(mine.lo - j, mine.hi - j)) >> (4 * h);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = (keep >> (8 * (r >> 2) + (r & 3))) & 1u ? s[r] : 0.0f;
+          for (int r = 0; r < 16; ++r) s[r] = masked(s[r], keep, r, 0.0f);
         }
         constexpr int kPer = 32 / kGroups<Op>;
 #pragma unroll
@@ -235,29 +260,30 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
             acc[i] = mma<Op>(T::columns(K, 32 * half + kPer * g, i, lane), ds, acc[i]);
         }
       }
-      j0 = j1;
-      buffer ^= 1;
     }
   }
   if (row >= nrows) return;
-  store_row<Op, T::kBlocks>(static_cast<E*>(G.dq) + ((S.q0 + t) * A.heads + head) * (int64_t)A.dim, acc,
+  if (A.qmask && !there)
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
+  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), row_at<Op>(t - wt, width, head, A.dim), acc,
                             A.scale * kUnshift<Op> / by, A.dim, A.dim % 4 == 0 && aligned(G.dq), h);
 }
 
 template <class Op, int kD, int kWaves>
-__global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnGrads G, int tiles, int64_t work) {
+__global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnGrads G, uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
-  typedef typename Elem<Op>::T E;
   constexpr int kThreads = kWaves * 64;
   constexpr int kBuffer = 2 * T::kBytes + 2 * kRows * 4;  // q, do, lse, delta
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
-  __shared__ uint32_t words[kMaskSpan / 32];
-  const int64_t piece = piece_of(work);
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer + kMaskSpan / 8];
+  uint32_t* const words = reinterpret_cast<uint32_t*>(lds + 2 * kBuffer);
+  const uint32_t piece = piece_of(work);
   if (piece >= work) return;
-  const int64_t unit = piece / tiles;
-  const int tile = (int)(piece % tiles);  // (under a causal mask the first tiles have the most rows)
-  const int64_t b = unit / A.kv_heads;
-  const int hk = (int)(unit % A.kv_heads);
+  const uint32_t unit = piece / tiles;
+  const int tile = (int)(piece - unit * tiles);  // (under a causal mask the first tiles have the most rows)
+  const int64_t b = unit / (uint32_t)A.kv_heads;
+  const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
   const int key0 = tile * (32 * kWaves);
   if (key0 >= S.nk) return;
@@ -265,24 +291,34 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int h = lane >> 5;
   const int key = key0 + wave * 32 + (lane & 31);
+  const int wkey = key0 + wave * 32;  // the wave's first
+  u32x4 k[T::kK], v[T::kK];
+  own_row<T>(k, wave_rows<Op>(A.k, seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2], wkey, A.ks[1]),
+             key < S.nk ? row_at<Op>(key - wkey, A.ks[1], 0, 0) : kFar, A.units, h);
+  own_row<T>(v, wave_rows<Op>(A.v, seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2], wkey, A.vs[1]),
+             key < S.nk ? row_at<Op>(key - wkey, A.vs[1], 0, 0) : kFar, A.units, h);
   const bool there = key < S.nk && (!A.kmask || A.kmask[b * A.tk + key]);
-  const auto rows_of = [&](int j) {
-    Reach r = tokens_of(j, S, A);
+  const auto reach = [&](int j) {  // in rows
+    Reach r = tokens_of(j < S.nk ? j : S.nk - 1, S, A);
     r.lo *= A.group;
     r.hi *= A.group;
     return r;
   };
-  const Reach mine = there ? rows_of(key) : Reach{0, 0};
-  const int klast = key0 + 32 * kWaves < S.nk ? key0 + 32 * kWaves - 1 : S.nk - 1;
-  const int first = rows_of(key0).lo / kRows * kRows;
-  const int last = rows_of(klast).hi;
-  const Reach inner = common(mine);
-
-  const int64_t kat = seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2] + (int64_t)key * A.ks[1];
-  const int64_t vat = seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2] + (int64_t)key * A.vs[1];
-  u32x4 k[T::kK], v[T::kK];
-  own_row<T>(k, static_cast<const char*>(A.k) + kat * Op::kEsz, there, A.units, h);
-  own_row<T>(v, static_cast<const char*>(A.v) + vat * Op::kEsz, there, A.units, h);
+  const Reach mine = reach(key);
+  const int first = reach(key0).lo / kRows * kRows;
+  int last = reach(key0 + 32 * kWaves - 1).hi;
+  Rows rows = {words, A.qmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
+  const auto gather = [&] {
+    const uint8_t* qm = A.qmask + b * A.tq;
+    rows.gather<kThreads>(S.nq * A.group, [&](int r) { return qm[token_of(r, A)] != 0; });
+  };
+  if (rows.given && first < last) gather();
+  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no rows are read)
+  if (A.kmask) {
+    clear_unless<T>(k, there);
+    clear_unless<T>(v, there);
+  }
+  const Reaches wide = reaches(reach(key0 + wave * 32), reach(key0 + wave * 32 + 31), __any(there));
   const float c = fabsf(A.scale) * kLog2e;
   if (A.scale < 0) negate<T>(k);
   float by = 1.0f;
@@ -297,25 +333,17 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
 #pragma unroll
   for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
 
-  for (int span0 = first / kMaskSpan * kMaskSpan; span0 < last; span0 += kMaskSpan) {
-    const int from = first > span0 ? first : span0;
-    const int to = last < span0 + kMaskSpan ? last : span0 + kMaskSpan;
-    if (A.qmask) {
+  for (bool more = false; rows.span0 < last; rows.span0 += kMaskSpan, more = true) {
+    const int from = first > rows.span0 ? first : rows.span0;
+    const int to = last < rows.span0 + kMaskSpan ? last : rows.span0 + kMaskSpan;
+    rows.to = to;
+    if (more) {  // (every wave is through with the words, and with the buffers)
       landed();
-      const uint8_t* qm = A.qmask + b * A.tq;
-      mask_words<kThreads>(words, span0, S.nq * A.group, [&](int r) { return qm[token_of(r, A)] != 0; });
+      if (rows.given) gather();
       landed();
     }
-    const auto bits_of = [&](int r0) -> uint32_t {
-      const uint32_t there = bits_between(0, to - r0);
-      return A.qmask && there ? rfl32(words[(r0 - span0) / 32]) & there : there;
-    };
-    const auto next = [&](int r0) {
-      while (r0 < to && !(bits_of(r0) | bits_of(r0 + 32))) r0 += kRows;
-      return r0;
-    };
     const auto request = [&](int r0, int buffer) {
-      const uint32_t w0 = bits_of(r0), w1 = bits_of(r0 + 32);
+      const uint32_t w0 = rows.bits(r0), w1 = rows.bits(r0 + 32);
       const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
       char* const base = lds + buffer * kBuffer;
       T::template request_rows<kThreads>(base, qbase, A.qs[1], A.qs[2], A.units, r0, A, ok);
@@ -330,18 +358,23 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
         }
       }
     };
-    int r0 = next(from);
+    int r0 = rows.next(from);
     int buffer = 0;
     if (r0 < to) request(r0, 0);
     while (r0 < to) {
       landed();
-      const int r1 = next(r0 + kRows);
+      const int r1 = rows.next(r0 + kRows);
       if (r1 < to) request(r1, buffer ^ 1);
       const char* const Q = lds + buffer * kBuffer;
       const char* const D = Q + T::kBytes;
       const float* const lse = reinterpret_cast<const float*>(D + T::kBytes);
-      const uint32_t w[2] = {bits_of(r0), bits_of(r0 + 32)};
-      const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && r0 >= inner.lo && r0 + kRows <= inner.hi;
+      const bool none = r0 >= wide.any.hi || r0 + kRows <= wide.any.lo;
+      const int now = r0;
+      r0 = r1;
+      buffer ^= 1;
+      if (none) continue;  // (no row here reaches this wave's keys)
+      const uint32_t w[2] = {rows.bits(now), rows.bits(now + 32)};
+      const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f32x16 x = f32x16{}, y = f32x16{};
@@ -363,13 +396,12 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
           }
         }
         if (!whole_tile) {
-          const int r0h = r0 + 32 * half;
+          const int r0h = now + 32 * half;
           const uint32_t keep = (w[half] & bits_between(mine.lo - r0h, mine.hi - r0h)) >> (4 * h);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const bool in = (keep >> (8 * (r >> 2) + (r & 3))) & 1u;
-            p[r] = in ? p[r] : 0.0f;
-            ds[r] = in ? ds[r] : 0.0f;
+            p[r] = masked(p[r], keep, r, 0.0f);
+            ds[r] = masked(ds[r], keep, r, 0.0f);
           }
         }
         constexpr int kPer = 32 / kGroups<Op>;
@@ -383,15 +415,19 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
           }
         }
       }
-      r0 = r1;
-      buffer ^= 1;
     }
   }
   if (key >= S.nk) return;
-  const int64_t at = ((S.k0 + key) * A.kv_heads + hk) * (int64_t)A.dim;
+  if (A.kmask && !there)
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
+  const int64_t wide_row = (int64_t)A.kv_heads * A.dim, start = S.k0 * wide_row + (int64_t)hk * A.dim;
+  const int at = row_at<Op>(key - wkey, wide_row, 0, 0);
   const bool vec = A.dim % 4 == 0;
-  store_row<Op, T::kBlocks>(static_cast<E*>(G.dk) + at, dk, A.scale * kUnshift<Op> / by, A.dim, vec && aligned(G.dk), h);
-  store_row<Op, T::kBlocks>(static_cast<E*>(G.dv) + at, dv, kUnshift<Op>, A.dim, vec && aligned(G.dv), h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, A.scale * kUnshift<Op> / by, A.dim,
+                            vec && aligned(G.dk), h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, kUnshift<Op>, A.dim,
+                            vec && aligned(G.dv), h);
 }
 
 template <class Op, int kD>
@@ -404,12 +440,12 @@ hipError_t pullback_dim(const AttnArgs& a, const AttnGrads& g, hipStream_t strea
     const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), work = units * tiles;
     if (work)
       hipLaunchKernelGGL((attn_dq_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a,
-                         g, (int)tiles, work);
+                         g, (uint32_t)tiles, (uint32_t)work);
   }
   const int64_t tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles;
   if (work)
     hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
-                       (int)tiles, work);
+                       (uint32_t)tiles, (uint32_t)work);
   return hipGetLastError();
 }
 template <class Op>

@@ -100,6 +100,27 @@ def test_long_mask(dtype, device):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,d,causal,window", [
+    (1, 1, 5000, 4, 1, 128, False, None), (2, 1, 3001, 2, 2, 64, True, None), (1, 40, 2500, 6, 2, 32, True, 300),
+    (1, 130, 1100, 1, 1, 96, False, 5), (1, 1, 257, 1, 1, 64, False, None), (1, 2, 4096, 1, 1, 20, False, 0),
+])
+def test_split(dtype, B, Tq, Tk, H, Hk, d, causal, window, device):
+    """Few rows and many keys: the keys are split among workgroups, some of which have none that count."""
+    q, k, v, do = inputs((B, Tq, H, d), (B, Tk, Hk, d), dtype, device, seed=Tk)
+    padded(q, k, v, do, causal=causal, window=window)
+    mask = torch.zeros(B, Tk, dtype=torch.bool, device=device)
+    mask[0, 100:180] = True
+    k[~mask] = float("nan")
+    padded(q, k, v, do, kmask=mask, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_split_ragged(dtype, device):
+    ragged([1, 0, 3], [3000, 700, 0], 4, 2, 64, dtype, device)
+    ragged([2, 2], [1200, 5], 2, 2, 64, dtype, device, causal=True, front=1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
 def test_scale(dtype, scale, device):
     padded(*inputs((1, 70, 2, 64), (1, 100, 1, 64), dtype, device, size=0.5), scale=scale, causal=True)
