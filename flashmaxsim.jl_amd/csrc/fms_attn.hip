@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   constexpr int kThreads = kWaves * 64;
   // (one array: beside a second one the compiler waits for all loads into LDS before it reads there)
   __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes + kMaskSpan / 8];
-  uint32_t* const words = reinterpret_cast<uint32_t*>(lds + 4 * T::kBytes);
+  uint64_t* const words = reinterpret_cast<uint64_t*>(lds + 4 * T::kBytes);
   const uint32_t piece = piece_of(work);
   if (piece >= work) return;
   const uint32_t whole = kSplit ? piece / (uint32_t)P.splits : piece;
@@ -85,7 +85,20 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
     keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
   };
   if (keys.given && first < last) gather();
-  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no keys are read)
+  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
+  const int at = row < nrows ? row_at<Op>(t - wt, width, head, A.dim) : kFar;
+  const bool vec = whole_units(out.o, A.dim, Op::kEsz) && whole_units(out.rest, A.dim, Op::kEsz);
+  const int64_t stat = rows_at(A, b, hk, S.q0) + row;
+  f32x16 acc[T::kBlocks];
+#pragma unroll
+  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
+  if (!__syncthreads_or(there) && !kSplit) {  // padding: zeros, and nothing is read
+    store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, 0.0f, A.dim, vec, h);
+    if (Op::kEsz == 2 && out.rest)
+      store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, start, wt, width), at, acc, 0.0f, A.dim, vec, h);
+    if (out.lse && h == 0 && row < nrows) out.lse[stat] = -INFINITY;
+    return;
+  }
   if (A.qmask) clear_unless<T>(q, there);
   const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
   const float c = factor(A);
@@ -94,9 +107,6 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   const char* vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
   const int64_t kstep = A.ks[1] * Op::kEsz, vstep = A.vs[1] * Op::kEsz;
 
-  f32x16 acc[T::kBlocks];
-#pragma unroll
-  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
   float m = -INFINITY, l = 0.0f;
 
   for (bool more = false; keys.span0 < last; keys.span0 += kMaskSpan, more = true) {
@@ -108,24 +118,25 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
       if (keys.given) gather();
       landed();
     }
-    const auto request = [&](int j0, int buffer) {
-      const uint32_t w0 = keys.bits(j0), w1 = keys.bits(j0 + 32);
-      const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
-      T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, ok);
-      T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, ok);
+    const auto request = [&](int j0, uint64_t bits, int buffer) {
+      T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, bits);
+      T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, bits);
     };
-    int j0 = keys.next(from);
+    uint64_t bits, bits1;  // of this tile, and of the next
+    int j0 = keys.next(from, bits);
     int buffer = 0;
-    if (j0 < to) request(j0, 0);
+    if (j0 < to) request(j0, bits, 0);
     while (j0 < to) {
       landed();
-      const int j1 = keys.next(j0 + kRows);
-      if (j1 < to) request(j1, buffer ^ 1);
+      const int j1 = keys.next(j0 + kRows, bits1);
+      if (j1 < to) request(j1, bits1, buffer ^ 1);
       const char* const K = lds + buffer * 2 * T::kBytes;
       const char* const V = K + T::kBytes;
       const bool none = j0 >= wide.any.hi || j0 + kRows <= wide.any.lo;
       const int now = j0;
+      const uint64_t in = bits;
       j0 = j1;
+      bits = bits1;
       buffer ^= 1;
       if (none) continue;  // (none of this wave's rows reaches here)
       float s[2][16];
@@ -137,12 +148,11 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[half][r] = x[r];
       }
-      const uint32_t w0 = keys.bits(now), w1 = keys.bits(now + 32);
-      const bool whole_tile = (w0 & w1) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
+      const bool whole_tile = in == ~0ull && now >= wide.all.lo && now + kRows <= wide.all.hi;
       uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
       if (!whole_tile) {
-        keep[0] = (w0 & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
-        keep[1] = (w1 & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
+        keep[0] = ((uint32_t)in & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
+        keep[1] = ((uint32_t)(in >> 32) & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -197,8 +207,8 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   }
   // both halves of the wave summed other keys of the same row
   l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
-  if (row >= nrows) return;
   if constexpr (kSplit) {
+    if (row >= nrows) return;
     const int64_t slot = (int64_t)piece * (32 * kWaves) + wave * 32 + (lane & 31);
     float* to = P.acc + slot * kD;
 #pragma unroll
@@ -211,12 +221,9 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
     return;
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  const bool vec = A.dim % 4 == 0 && aligned(out.o) && aligned(out.rest);
-  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
-  const int at = row_at<Op>(t - wt, width, head, A.dim);
   store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, inv, A.dim, vec, h);
-  if (out.lse && h == 0)
-    out.lse[rows_at(A, b, hk, S.q0) + row] = l > 0.0f || l != l ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
+  if (out.lse && h == 0 && row < nrows)
+    out.lse[stat] = l > 0.0f || l != l ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
   if (Op::kEsz == 2 && out.rest) {
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i)

@@ -186,25 +186,25 @@ struct Tile {
   }
   static constexpr int loads(int threads) { return kBytes / 16 / threads; }
 
-  // Rows as they lie: key / value tokens `stride` bytes apart from `base` on.  ok(row): the row is read.
-  template <int kThreads, class Ok>
+  // Rows as they lie: key / value tokens `stride` bytes apart from `base` on; those not in `bits` are zeros.
+  template <int kThreads>
   __device__ static __forceinline__ void request(char* lds, const char* base, int stride, int units,
-                                                 Ok&& ok) {
+                                                 uint64_t bits) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const rsrc_t from = make_rsrc_u(base, 0x7fffffffu);
 #pragma unroll
     for (int i = 0; i < loads(kThreads); ++i) {
       const int u = i * kThreads + tid, row = u / kUnits, unit = (u % kUnits) ^ mix(row);
-      const int at = unit < units && ok(row) ? row * stride + unit * 16 : kFar;
+      const int at = unit < units && (bits >> row & 1) ? row * stride + unit * 16 : kFar;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(lds + (i * kThreads + wave * 64) * 16), 16,
                                                at, 0, 0, 0);
     }
   }
   // Query rows row0 .. row0 + kRows - 1 of a unit; base is the unit's token 0, its tokens `token`
   // and heads `head_step` elements apart.
-  template <int kThreads, class Ok>
+  template <int kThreads>
   __device__ static __forceinline__ void request_rows(char* lds, const char* base, int64_t token, int64_t head_step,
-                                                      int units, int row0, const AttnArgs& A, Ok&& ok) {
+                                                      int units, int row0, const AttnArgs& A, uint64_t bits) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int t0 = token_of(row0, A);
     const rsrc_t from = make_rsrc_u(base + (int64_t)t0 * token * Op::kEsz, 0x7fffffffu);
@@ -213,7 +213,7 @@ struct Tile {
     for (int i = 0; i < loads(kThreads); ++i) {
       const int u = i * kThreads + tid, row = u / kUnits, unit = (u % kUnits) ^ mix(row);
       const int t = token_of(row0 + row, A), head = row0 + row - t * A.group;
-      const int at = unit < units && ok(row) ? (t - t0) * ts + head * hs + unit * 16 : kFar;
+      const int at = unit < units && (bits >> row & 1) ? (t - t0) * ts + head * hs + unit * 16 : kFar;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(lds + (i * kThreads + wave * 64) * 16), 16,
                                                at, 0, 0, 0);
     }
@@ -351,7 +351,9 @@ __device__ __forceinline__ void negate(u32x4 (&f)[T::kK]) {
   for (int kb = 0; kb < T::kK; ++kb) f[kb] ^= T::Op::kEsz == 4 ? 0x80000000u : 0x80008000u;
 }
 
-__device__ __forceinline__ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+__device__ __forceinline__ bool whole_units(const void* p, int dim, int esz) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && dim * esz % 16 == 0;
+}
 
 // Bits lo .. hi - 1 of 32 (bounds anywhere).
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
@@ -369,9 +371,10 @@ __device__ __forceinline__ float masked(float v, uint32_t keep, int r, float wha
 }
 
 // Which rows (keys, or query rows) of a stretch are there: `to` ends them, a mask leaves some out.  Masks
-// are held as bits in LDS, kMaskSpan rows at a time.
+// are held as bits in LDS, kMaskSpan rows at a time, 64 to a word: a tile's.
+static_assert(kRows == 64, "a word of mask bits is a tile");
 struct Rows {
-  uint32_t* words;
+  uint64_t* words;
   bool given;  // a mask
   int span0, to;
 
@@ -380,22 +383,19 @@ struct Rows {
   __device__ __forceinline__ void gather(int n, Keep&& keep) const {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int left = n - span0, most = left < kMaskSpan ? left : kMaskSpan;
-    for (int r = wave * 64; r < (most + 63) / 64 * 64; r += kThreads) {
+    for (int r = wave * 64; r < most; r += kThreads) {
       const uint64_t bits = __ballot(r + lane < most && keep(span0 + r + lane));
-      if (lane == 0) {
-        words[r / 32] = (uint32_t)bits;
-        words[r / 32 + 1] = (uint32_t)(bits >> 32);
-      }
+      if (lane == 0) words[r / 64] = bits;
     }
   }
-  // Of rows r0 .. r0 + 31.
-  __device__ __forceinline__ uint32_t bits(int r0) const {
-    const uint32_t in = bits_between(0, to - r0);
-    return given && in ? rfl32(words[(r0 - span0) / 32]) & in : in;
-  }
-  // The first tile from r0 on that has any.
-  __device__ __forceinline__ int next(int r0) const {
-    while (given && r0 < to && !(bits(r0) | bits(r0 + 32))) r0 += kRows;
+  // The first tile from r0 on that has any rows (`to` or past it: none), and which.
+  __device__ __forceinline__ int next(int r0, uint64_t& bits) const {
+    bits = 0;
+    for (; r0 < to; r0 += kRows) {
+      bits = r0 + kRows <= to ? ~0ull : (1ull << (to - r0)) - 1;
+      if (given) bits &= rfl64(words[(r0 - span0) / 64]);
+      if (bits) break;
+    }
     return r0;
   }
 };
@@ -410,31 +410,44 @@ __device__ __forceinline__ void landed() {
 }
 
 // A lane's accumulators (values 32 b + 8 (r / 4) + 4 h + r % 4 of its row) times `by` to its row of `dim` values,
-// `at` bytes into the resource (kFar: nowhere).  vec: rows are whole groups of four, aligned to them.
+// `at` bytes into the resource (kFar: nowhere).  units: rows are whole units of 16 bytes, aligned to them.
+// All lanes of the wave call it.
 template <class Op, int kBlocks>
-__device__ __forceinline__ void store_row(rsrc_t to, int at, const f32x16 (&acc)[kBlocks], float by, int dim, bool vec,
+__device__ __forceinline__ void store_row(rsrc_t to, int at, const f32x16 (&acc)[kBlocks], float by, int dim, bool units,
                                           int h) {
   typedef typename Elem<Op>::T T;
   typedef T V4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * b + 8 * g + 4 * h;
-      V4 x;
+    for (int g = 0; g < 4; g += 2) {
+      V4 x[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (T)(acc[b][4 * g + e] * by);
-      if (vec) {
-        const int off = d < dim ? at + d * Op::kEsz : kFar;
-        if constexpr (Op::kEsz == 2)
-          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), to, off, 0, 0);
-        else
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), to, off, 0, 0);
-      } else {
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = (T)(acc[b][4 * (g + i) + e] * by);
+      if constexpr (Op::kEsz == 2) if (units) {
+        // the halves of the wave trade: half 0 has all of group g's eight values, half 1 all of g + 1's
+        const u32x2 lo = __builtin_bit_cast(u32x2, x[0]), hi = __builtin_bit_cast(u32x2, x[1]);
+        const auto s0 = __builtin_amdgcn_permlane32_swap(lo[0], hi[0], false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(lo[1], hi[1], false, false);
+        const int d = 32 * b + 8 * (g + h);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, to,
+                                               d < dim ? at + d * Op::kEsz : kFar, 0, 0);
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = 32 * b + 8 * (g + i) + 4 * h;
+        if constexpr (Op::kEsz == 4) if (units) {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), to,
+                                                 d < dim ? at + d * Op::kEsz : kFar, 0, 0);
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int off = d + e < dim ? at + (d + e) * Op::kEsz : kFar;
-          const T y = x[e];
+          const T y = x[i][e];
           if constexpr (Op::kEsz == 2)
             __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), to, off, 0, 0);
           else

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   typedef Tile<Op, kD> T;
   constexpr int kThreads = kWaves * 64;
   __shared__ __attribute__((aligned(1024))) char lds[4 * T::kBytes + kMaskSpan / 8];  // (one array: as forward)
-  uint32_t* const words = reinterpret_cast<uint32_t*>(lds + 4 * T::kBytes);
+  uint64_t* const words = reinterpret_cast<uint64_t*>(lds + 4 * T::kBytes);
   const uint32_t piece = piece_of(work);
   if (piece >= work) return;
   const uint32_t unit = piece / tiles;
@@ -153,14 +153,24 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   const Reach mine = keys_of(t, S, A);
   const auto reach = [&](int r) { return keys_of(token_of(r < nrows ? r : nrows - 1, A), S, A); };
   const int first = reach(row0).lo / kRows * kRows;
-  int last = reach(row0 + 32 * kWaves - 1).hi;
+  const int last = reach(row0 + 32 * kWaves - 1).hi;
   Rows keys = {words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
   const auto gather = [&] {
     const uint8_t* km = A.kmask + b * A.tk;
     keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
   };
   if (keys.given && first < last) gather();
-  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no keys are read)
+  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
+  const int to_row = row < nrows ? row_at<Op>(t - wt, width, head, A.dim) : kFar;
+  const bool vec = whole_units(G.dq, A.dim, Op::kEsz);
+  f32x16 acc[T::kBlocks];
+#pragma unroll
+  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
+  if (!__syncthreads_or(there)) {  // padding: zeros, and no keys are read
+    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), to_row, acc, 0.0f, A.dim, vec, h);
+    if (h == 0 && row < nrows) G.delta[at] = 0.0f;
+    return;
+  }
   if (A.qmask) {
     clear_unless<T>(q, there);
     clear_unless<T>(d, there);  // (o and rest are zeros there)
@@ -198,9 +208,6 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   const char* kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
   const char* vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
   const int64_t kstep = A.ks[1] * Op::kEsz, vstep = A.vs[1] * Op::kEsz;
-  f32x16 acc[T::kBlocks];
-#pragma unroll
-  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
 
   for (bool more = false; keys.span0 < last; keys.span0 += kMaskSpan, more = true) {
     const int from = first > keys.span0 ? first : keys.span0;
@@ -211,27 +218,27 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
       if (keys.given) gather();
       landed();
     }
-    const auto request = [&](int j0, int buffer) {
-      const uint32_t w0 = keys.bits(j0), w1 = keys.bits(j0 + 32);
-      const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
-      T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, ok);
-      T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, ok);
+    const auto request = [&](int j0, uint64_t bits, int buffer) {
+      T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, bits);
+      T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, bits);
     };
-    int j0 = keys.next(from);
+    uint64_t bits, bits1;  // of this tile, and of the next
+    int j0 = keys.next(from, bits);
     int buffer = 0;
-    if (j0 < to) request(j0, 0);
+    if (j0 < to) request(j0, bits, 0);
     while (j0 < to) {
       landed();
-      const int j1 = keys.next(j0 + kRows);
-      if (j1 < to) request(j1, buffer ^ 1);
+      const int j1 = keys.next(j0 + kRows, bits1);
+      if (j1 < to) request(j1, bits1, buffer ^ 1);
       const char* const K = lds + buffer * 2 * T::kBytes;
       const char* const V = K + T::kBytes;
       const bool none = j0 >= wide.any.hi || j0 + kRows <= wide.any.lo;
       const int now = j0;
+      const uint32_t w[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
       j0 = j1;
+      bits = bits1;
       buffer ^= 1;
       if (none) continue;  // (none of this wave's rows reaches here)
-      const uint32_t w[2] = {keys.bits(now), keys.bits(now + 32)};
       const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -262,13 +269,11 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
       }
     }
   }
-  if (row >= nrows) return;
   if (A.qmask && !there)
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
-  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), row_at<Op>(t - wt, width, head, A.dim), acc,
-                            A.scale * kUnshift<Op> / by, A.dim, A.dim % 4 == 0 && aligned(G.dq), h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), to_row, acc, A.scale * kUnshift<Op> / by, A.dim, vec,
+                            h);
 }
 
 template <class Op, int kD, int kWaves>
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   constexpr int kThreads = kWaves * 64;
   constexpr int kBuffer = 2 * T::kBytes + 2 * kRows * 4;  // q, do, lse, delta
   __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer + kMaskSpan / 8];
-  uint32_t* const words = reinterpret_cast<uint32_t*>(lds + 2 * kBuffer);
+  uint64_t* const words = reinterpret_cast<uint64_t*>(lds + 2 * kBuffer);
   const uint32_t piece = piece_of(work);
   if (piece >= work) return;
   const uint32_t unit = piece / tiles;
@@ -306,14 +311,24 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   };
   const Reach mine = reach(key);
   const int first = reach(key0).lo / kRows * kRows;
-  int last = reach(key0 + 32 * kWaves - 1).hi;
+  const int last = reach(key0 + 32 * kWaves - 1).hi;
   Rows rows = {words, A.qmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
   const auto gather = [&] {
     const uint8_t* qm = A.qmask + b * A.tq;
     rows.gather<kThreads>(S.nq * A.group, [&](int r) { return qm[token_of(r, A)] != 0; });
   };
   if (rows.given && first < last) gather();
-  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no rows are read)
+  const int64_t wide_row = (int64_t)A.kv_heads * A.dim, start = S.k0 * wide_row + (int64_t)hk * A.dim;
+  const int at = key < S.nk ? row_at<Op>(key - wkey, wide_row, 0, 0) : kFar;
+  const bool vec_k = whole_units(G.dk, A.dim, Op::kEsz), vec_v = whole_units(G.dv, A.dim, Op::kEsz);
+  f32x16 dk[T::kBlocks], dv[T::kBlocks];
+#pragma unroll
+  for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
+  if (!__syncthreads_or(there)) {  // padding: zeros, and no rows are read
+    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, 0.0f, A.dim, vec_k, h);
+    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, 0.0f, A.dim, vec_v, h);
+    return;
+  }
   if (A.kmask) {
     clear_unless<T>(k, there);
     clear_unless<T>(v, there);
@@ -329,9 +344,6 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   const int64_t width = A.units * (16 / Op::kEsz);
   const char* dbase = static_cast<const char*>(G.dout) + (S.q0 * A.heads + hk * A.group) * width * Op::kEsz;
   const int64_t stat = rows_at(A, b, hk, S.q0);
-  f32x16 dk[T::kBlocks], dv[T::kBlocks];
-#pragma unroll
-  for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
 
   for (bool more = false; rows.span0 < last; rows.span0 += kMaskSpan, more = true) {
     const int from = first > rows.span0 ? first : rows.span0;
@@ -342,12 +354,10 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
       if (rows.given) gather();
       landed();
     }
-    const auto request = [&](int r0, int buffer) {
-      const uint32_t w0 = rows.bits(r0), w1 = rows.bits(r0 + 32);
-      const auto ok = [&](int r) { return ((r < 32 ? w0 : w1) >> (r & 31) & 1u) != 0; };
+    const auto request = [&](int r0, uint64_t bits, int buffer) {
       char* const base = lds + buffer * kBuffer;
-      T::template request_rows<kThreads>(base, qbase, A.qs[1], A.qs[2], A.units, r0, A, ok);
-      T::template request_rows<kThreads>(base + T::kBytes, dbase, A.heads * width, width, A.units, r0, A, ok);
+      T::template request_rows<kThreads>(base, qbase, A.qs[1], A.qs[2], A.units, r0, A, bits);
+      T::template request_rows<kThreads>(base + T::kBytes, dbase, A.heads * width, width, A.units, r0, A, bits);
       if (wave < 2 || kWaves == 1) {
 #pragma unroll
         for (int i = 0; i < (kWaves == 1 ? 2 : 1); ++i) {
@@ -358,22 +368,24 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
         }
       }
     };
-    int r0 = rows.next(from);
+    uint64_t bits, bits1;  // of this tile, and of the next
+    int r0 = rows.next(from, bits);
     int buffer = 0;
-    if (r0 < to) request(r0, 0);
+    if (r0 < to) request(r0, bits, 0);
     while (r0 < to) {
       landed();
-      const int r1 = rows.next(r0 + kRows);
-      if (r1 < to) request(r1, buffer ^ 1);
+      const int r1 = rows.next(r0 + kRows, bits1);
+      if (r1 < to) request(r1, bits1, buffer ^ 1);
       const char* const Q = lds + buffer * kBuffer;
       const char* const D = Q + T::kBytes;
       const float* const lse = reinterpret_cast<const float*>(D + T::kBytes);
       const bool none = r0 >= wide.any.hi || r0 + kRows <= wide.any.lo;
       const int now = r0;
+      const uint32_t w[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
       r0 = r1;
+      bits = bits1;
       buffer ^= 1;
       if (none) continue;  // (no row here reaches this wave's keys)
-      const uint32_t w[2] = {rows.bits(now), rows.bits(now + 32)};
       const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -417,17 +429,12 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
       }
     }
   }
-  if (key >= S.nk) return;
   if (A.kmask && !there)
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
-  const int64_t wide_row = (int64_t)A.kv_heads * A.dim, start = S.k0 * wide_row + (int64_t)hk * A.dim;
-  const int at = row_at<Op>(key - wkey, wide_row, 0, 0);
-  const bool vec = A.dim % 4 == 0;
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, A.scale * kUnshift<Op> / by, A.dim,
-                            vec && aligned(G.dk), h);
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, kUnshift<Op>, A.dim,
-                            vec && aligned(G.dv), h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, A.scale * kUnshift<Op> / by, A.dim, vec_k,
+                            h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, kUnshift<Op>, A.dim, vec_v, h);
 }
 
 template <class Op, int kD>

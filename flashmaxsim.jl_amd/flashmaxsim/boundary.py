@@ -763,58 +763,69 @@ def block_norm_apply_pullback(dx, df, dgate, dwpost, dwpre, dr, dn, x, f, gate, 
 
 # ---- encoder (no reference method) ------------------------------------------------------
 
-def _check_heads(q, k, v=None):
+def _heads(*arrays):
     """Device, eltype and layout of the heads' arrays: any strides, a head's values contiguous."""
+    q = arrays[0]
     dtype, at = q.dtype, q.get_device()
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        if t is None:
-            continue
-        if at < 0 or t.get_device() != at:
-            require_device(q.new_empty(0), t.new_empty(0))  # (says what is wrong)
-        if t.dtype is not dtype:
-            raise ArgumentError(f"{what} must have the feature eltype {dtype}, got {t.dtype}")
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            raise ArgumentError(f"{what}: the values of a head must be contiguous")
+    good = at >= 0
+    for t in arrays:
+        good = good and t.get_device() == at and t.dtype is dtype and (t.stride(-1) == 1 or t.shape[-1] <= 1)
+    if not good:
+        for t, what in zip(arrays, "qkv"):
+            require_device(q.new_empty(0), t.new_empty(0))  # (says what is wrong; they need not be dense)
+            if t.dtype != dtype:
+                raise ArgumentError(f"{what} must have the feature eltype {dtype}, got {t.dtype}")
+            if t.stride(-1) != 1 and t.shape[-1] > 1:
+                raise ArgumentError(f"{what}: the values of a head must be contiguous")
     return q.device
+
+
+def _dense_strides(*arrays):
+    """None where all are dense, else the element strides of sequences, tokens and heads of each."""
+    if all([t.is_contiguous() for t in arrays]):
+        return None
+    out = []
+    for t in arrays:
+        st = t.stride()
+        out += (0, *st[:2]) if len(st) == 3 else st[:3]
+    return (ctypes.c_int64 * len(out))(*out)
+
+
+def _beside(t, dev):
+    """t is a dense array on the device, or None."""
+    if t is not None and not (t.get_device() == dev.index and t.is_contiguous()):
+        require_device(t)
+        raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+    return t
 
 
 def _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k):
     """The sizes and pointers that both attention calls take, after the checks of masks and cu."""
-    ragged = cu_q is not None
-    nq, heads, dim = q.shape[-3:]
+    *lead, nq, heads, dim = q.shape
     nk, kv_heads = k.shape[-3:-1]
-    seqs = cu_q.numel() - 1 if ragged else (q.shape[0] if q.dim() == 4 else 1)
-    if ragged:
-        for cu, what in ((cu_q, "cu_q"), (cu_k, "cu_k")):
-            require_device(cu)
-            _cu(cu, what, seqs + 1)
-            if cu.device != dev:
-                raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
+    if cu_q is not None:
+        seqs = cu_q.numel() - 1
+        _cu(_beside(cu_q, dev), "cu_q", seqs + 1)
+        _cu(_beside(cu_k, dev), "cu_k", seqs + 1)
     else:
+        seqs = lead[0] if lead else 1
         max_q, max_k = nq, nk
-        for m, what, n in ((qmask, "qmask", seqs * nq), (kmask, "kmask", seqs * nk)):
-            if m is not None:
-                require_device(m)
-                _maskn(m, what, n)
-                if m.device != dev:
-                    raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
-    strides = None
-    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
-        strides = (ctypes.c_int64 * 9)(*(n for t in (q, k, v)
-                                         for n in (t.stride(0) if t.dim() == 4 else 0, *t.stride()[-3:-1])))
-    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, ptr(qmask), ptr(kmask), ptr(cu_q),
-            ptr(cu_k), seqs, max_q, max_k, nq, nk, heads, kv_heads, dim)
+        if qmask is not None:
+            _maskn(_beside(qmask, dev), "qmask", seqs * nq)
+        if kmask is not None:
+            _maskn(_beside(kmask, dev), "kmask", seqs * nk)
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), _dense_strides(q, k, v), ptr(qmask), ptr(kmask),
+            ptr(cu_q), ptr(cu_k), seqs, max_q, max_k, nq, nk, heads, kv_heads, dim)
 
 
 def launch_attention(o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, scale, causal,
                      window):
     """o <- attention of q over k and v; lse and rest (both or neither) keep what the pullback needs."""
-    dev = _check_heads(q, k, v)
+    dev = _heads(q, k, v)
     _check_block(o, (q.shape, "o rest", (o, rest)))
     args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
     if lse is not None:
-        require_device(lse, o)
-        _buf(lse, "lse", torch.float32, q.shape[:-1].numel())
+        _buf(_beside(lse, dev), "lse", torch.float32, q.shape[:-1].numel())
     st = _call_with_workspace(_lib.lib().fms_attention, dev, dtype_code(q), o.data_ptr(), ptr(lse),
                               ptr(rest), *args, scale, causal, window, stream_handle(dev))
     if st:
@@ -824,11 +835,10 @@ def launch_attention(o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max
 def attention_apply_pullback(dq, dk, dv, do, o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q,
                              max_k, scale, causal, window):
     """dq, dk, dv <- pullback of do; o, lse and rest are the forward's."""
-    dev = _check_heads(q, k, v)
+    dev = _heads(q, k, v)
     _check_block(dq, (q.shape, "dq do o rest", (dq, do, o, rest)), (k.shape, "dk dv", (dk, dv)))
     args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
-    require_device(lse, dq)
-    _buf(lse, "lse", torch.float32, q.shape[:-1].numel())
+    _buf(_beside(lse, dev), "lse", torch.float32, q.shape[:-1].numel())
     st = _call_with_workspace(_lib.lib().fms_attention_pullback, dev, dtype_code(q), dq.data_ptr(),
                               dk.data_ptr(), dv.data_ptr(), do.data_ptr(), o.data_ptr(), lse.data_ptr(),
                               ptr(rest), *args, scale, causal, window, stream_handle(dev))
@@ -838,44 +848,43 @@ def attention_apply_pullback(dq, dk, dv, do, o, lse, rest, q, k, v, qmask, kmask
 
 def _rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps):
     """The arguments that both calls take from the heads on, after the checks of the others."""
-    seqs = q.shape[0] if q.dim() == 4 else 1
-    tokens, heads, dim = q.shape[-3:]
-    kv_heads = 0 if k is None else k.shape[-2]
-    require_device(table, positions, wq, wk)
-    if table.dtype != torch.float32:
+    *lead, heads, dim = shape = q.shape
+    tokens, seqs = lead[-1], lead[0] if len(lead) == 2 else 1
+    rows, turned = table.shape if table.dim() == 2 else (-1, 0)
+    _beside(table, dev)
+    if table.dtype is not torch.float32:
         raise ArgumentError(f"table must be float32, got {table.dtype}")
-    if table.dim() != 2 or table.shape[1] > dim or table.shape[1] % 2:
+    if rows < 0 or turned > dim or turned % 2:
         raise DimensionMismatch(f"table must be (positions, turned), turned even and at most {dim}: "
                                 f"got {tuple(table.shape)}")
+    id_bytes, placed = 4, 1
     if positions is None:
-        if table.shape[0] < tokens and table.shape[1]:
-            raise DimensionMismatch(f"table has {table.shape[0]} positions for {tokens} tokens")
-    elif positions.dtype not in (torch.int32, torch.int64):
-        raise ArgumentError("positions must be Int32 or Int64")
-    elif positions.shape != q.shape[:-2] and positions.shape != q.shape[-3:-2]:
-        raise DimensionMismatch(f"positions must be (tokens,) or one for each token: got "
-                                f"{tuple(positions.shape)} for {tuple(q.shape)}")
+        if rows < tokens and turned:
+            raise DimensionMismatch(f"table has {rows} positions for {tokens} tokens")
+    else:
+        _beside(positions, dev)
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ArgumentError("positions must be Int32 or Int64")
+        if positions.shape != shape[:-2] and positions.shape != shape[-3:-2]:
+            raise DimensionMismatch(f"positions must be (tokens,) or one for each token: got "
+                                    f"{tuple(positions.shape)} for {tuple(shape)}")
+        id_bytes, placed = positions.element_size(), seqs if positions.dim() == 2 else 1
     for w, what in ((wq, "q_weight"), (wk, "k_weight")):
-        if w is not None and w.dtype != q.dtype:
+        if w is None:
+            continue
+        _beside(w, dev)
+        if w.dtype is not q.dtype:
             raise ArgumentError(f"{what} must have the feature eltype {q.dtype}, got {w.dtype}")
-        if w is not None and w.shape != q.shape[-1:]:
+        if w.shape != shape[-1:]:
             raise DimensionMismatch(f"{what} must have the shape ({dim},), got {tuple(w.shape)}")
-    for t in (table, positions, wq, wk):
-        if t is not None and t.device != dev:
-            raise ArgumentError("FlashMaxSim requires colocated arrays (same device)")
-    strides = None
-    if not (q.is_contiguous() and (k is None or k.is_contiguous())):
-        strides = (ctypes.c_int64 * 6)(*(n for t in (q, q if k is None else k)
-                                         for n in (t.stride(0) if t.dim() == 4 else 0, *t.stride()[-3:-1])))
-    return (q.data_ptr(), ptr(k), strides, table.data_ptr(), ptr(positions),
-            4 if positions is None else positions.element_size(),
-            seqs if positions is not None and positions.dim() == 2 else 1, ptr(wq), ptr(wk), kind, pairing, eps,
-            seqs, tokens, heads, kv_heads, dim, table.shape[1], table.shape[0])
+    return (q.data_ptr(), ptr(k), _dense_strides(q, q if k is None else k), table.data_ptr(), ptr(positions),
+            id_bytes, placed, ptr(wq), ptr(wk), kind, pairing, eps, seqs, tokens, heads,
+            0 if k is None else k.shape[-2], dim, turned, rows)
 
 
 def launch_head_rotary(q_out, k_out, q, k, table, positions, wq, wk, kind, pairing, eps):
     """q_out, k_out <- norm and rotation of the heads of q and k (k, k_out may be None)."""
-    dev = _check_heads(q, k)
+    dev = _heads(q) if k is None else _heads(q, k)
     _check_block(q_out, (q.shape, "q_out", (q_out,)), (None if k is None else k.shape, "k_out", (k_out,)))
     st = _lib.lib().fms_head_rotary(dtype_code(q), q_out.data_ptr(), ptr(k_out),
                                     *_rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps),
@@ -886,7 +895,7 @@ def launch_head_rotary(q_out, k_out, q, k, table, positions, wq, wk, kind, pairi
 
 def head_rotary_apply_pullback(dq, dk, dwq, dwk, dq_out, dk_out, q, k, table, positions, wq, wk, kind,
                                pairing, eps):
-    dev = _check_heads(q, k)
+    dev = _heads(q) if k is None else _heads(q, k)
     _check_block(dq, (q.shape, "dq dq_out", (dq, dq_out)),
                  (None if k is None else k.shape, "dk dk_out", (dk, dk_out)),
                  (q.shape[-1:], "dq_weight dk_weight", (dwq, dwk)))
@@ -898,31 +907,33 @@ def head_rotary_apply_pullback(dq, dk, dwq, dwk, dq_out, dk_out, q, k, table, po
         _lib.check(st, "head_rotary_apply_pullback")
 
 
-def _check_ids(ids):
+def _ids(ids, dev):
+    """The ids' bytes, after their checks."""
+    _beside(ids, dev)
     if ids.dtype not in (torch.int32, torch.int64):
         raise ArgumentError("ids must be Int32 or Int64")
+    return ids.element_size()
 
 
 def launch_embed_tokens(e, ids, weight, scale):
     """e <- scale * weight[ids - 1]."""
-    dev = require_device(e, ids, weight)
-    _check_ids(ids)
-    _check_block(weight, (weight.shape, "weight", (weight,)), ((*ids.shape, weight.shape[1]), "e", (e,)))
-    st = _lib.lib().fms_embed_tokens(dtype_code(weight), e.data_ptr(), ids.data_ptr(), ids.element_size(),
-                                     weight.data_ptr(), scale, ids.numel(), weight.shape[0], weight.shape[1],
-                                     stream_handle(dev))
+    rows, dim = weight.shape
+    dev = _check_block(weight, ((*ids.shape, dim), "e", (e,)))
+    id_bytes = _ids(ids, dev)
+    st = _lib.lib().fms_embed_tokens(dtype_code(weight), e.data_ptr(), ids.data_ptr(), id_bytes,
+                                     weight.data_ptr(), scale, ids.numel(), rows, dim, stream_handle(dev))
     if st:
         _lib.check(st, "launch_embed_tokens")
 
 
 def embed_tokens_apply_pullback(dweight, de, ids, scale):
     """dweight <- scale * sums of de's rows by id."""
-    dev = require_device(dweight, de, ids)
-    _check_ids(ids)
-    _check_block(dweight, ((*ids.shape, dweight.shape[1]), "de", (de,)))
+    rows, dim = dweight.shape
+    dev = _check_block(dweight, ((*ids.shape, dim), "de", (de,)))
+    id_bytes = _ids(ids, dev)
     st = _call_with_workspace(_lib.lib().fms_embed_tokens_pullback, dev, dtype_code(dweight),
-                              dweight.data_ptr(), de.data_ptr(), ids.data_ptr(), ids.element_size(), scale,
-                              ids.numel(), dweight.shape[0], dweight.shape[1], stream_handle(dev))
+                              dweight.data_ptr(), de.data_ptr(), ids.data_ptr(), id_bytes, scale, ids.numel(),
+                              rows, dim, stream_handle(dev))
     if st:
         _lib.check(st, "embed_tokens_apply_pullback")
 

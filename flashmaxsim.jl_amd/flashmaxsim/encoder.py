@@ -83,17 +83,18 @@ def rotary_table(positions, turned, base=10000.0, device=None):
 
 
 def _rotary_codes(q, k, kind, pairing):
-    if q.dim() not in (3, 4):
+    qs = q.shape
+    if len(qs) not in (3, 4):
         raise DimensionMismatch("head_rotary takes q (B, T, heads, dim) or (T, heads, dim)")
-    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
-        raise DimensionMismatch(f"k {tuple(k.shape)} must have q's tokens and dim: q is {tuple(q.shape)}")
-    if q.shape[-1] % 2:
-        raise DimensionMismatch(f"head_rotary takes heads of an even number of values, got {q.shape[-1]}")
+    if k is not None and (k.dim() != len(qs) or k.shape[:-2] != qs[:-2] or k.shape[-1] != qs[-1]):
+        raise DimensionMismatch(f"k {tuple(k.shape)} must have q's tokens and dim: q is {tuple(qs)}")
+    if qs[-1] % 2:
+        raise DimensionMismatch(f"head_rotary takes heads of an even number of values, got {qs[-1]}")
     return _code(kind, NORMS, "kind"), _code(pairing, PAIRINGS, "pairing")
 
 
 def _dense_like(t):
-    return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return None if t is None else t.new_empty(t.shape)
 
 
 def head_rotary_forward(q, k, table, positions=None, *, q_weight=None, k_weight=None, kind="rms",
@@ -166,46 +167,51 @@ class AttentionKept(NamedTuple):
 
 def _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, window, scale):
     """Shapes of the heads and the options as the boundary takes them (it checks the rest)."""
-    if q.dim() not in (3, 4) or k.dim() != q.dim() or v.shape != k.shape:
+    qs, ks = q.shape, k.shape
+    n = len(qs)
+    if n not in (3, 4) or len(ks) != n or v.shape != ks:
         raise DimensionMismatch("attention takes q (B, Tq, heads, dim) and k, v (B, Tk, kv_heads, dim), "
                                 "or all of them without B")
-    if q.shape[-1] != k.shape[-1] or q.shape[:-3] != k.shape[:-3]:
-        raise DimensionMismatch(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch or dim")
-    if k.shape[-2] == 0 and q.shape[-2] > 0 or k.shape[-2] > 0 and q.shape[-2] % k.shape[-2]:
-        raise DimensionMismatch(f"{q.shape[-2]} query heads cannot share {k.shape[-2]} key heads evenly")
-    if (cu_q is None) != (cu_k is None):
-        raise ArgumentError("ragged attention needs cu_q and cu_k (the same one for self-attention)")
-    if cu_q is not None:
-        if q.dim() != 3:
+    if qs[-1] != ks[-1] or n == 4 and qs[0] != ks[0]:
+        raise DimensionMismatch(f"q {tuple(qs)} and k {tuple(ks)} differ in batch or dim")
+    if qs[-2] != ks[-2] and (not ks[-2] or qs[-2] % ks[-2]):
+        raise DimensionMismatch(f"{qs[-2]} query heads cannot share {ks[-2]} key heads evenly")
+    if cu_q is None and cu_k is None:
+        if max_q is not None or max_k is not None:
+            raise ArgumentError("max_q and max_k go with cu_q and cu_k")
+        max_q = max_k = 0
+    else:
+        if cu_q is None or cu_k is None:
+            raise ArgumentError("ragged attention needs cu_q and cu_k (the same one for self-attention)")
+        if n != 3:
             raise DimensionMismatch("ragged attention takes token rows (tokens, heads, dim)")
         if qmask is not None or kmask is not None:
             raise ArgumentError("masks go with padded sequences, not with cu_q and cu_k")
-        max_q = q.shape[0] if max_q is None else int(max_q)
-        max_k = k.shape[0] if max_k is None else int(max_k)
+        max_q = qs[0] if max_q is None else int(max_q)
+        max_k = ks[0] if max_k is None else int(max_k)
         if max_q < 0 or max_k < 0:
             raise ArgumentError("max_q and max_k must be >= 0")
-    elif max_q is not None or max_k is not None:
-        raise ArgumentError("max_q and max_k go with cu_q and cu_k")
-    if window is not None and window < 0:
+    if window is None:
+        window = -1
+    elif window < 0:
         raise ArgumentError("window must be >= 0, or None")
     if scale is None:
-        scale = max(q.shape[-1], 1) ** -0.5
-    return (qmask, kmask, cu_q, cu_k, max_q or 0, max_k or 0, float(scale), 1 if causal else 0,
-            -1 if window is None else int(window))
+        scale = qs[-1] ** -0.5 if qs[-1] else 1.0
+    return qmask, kmask, cu_q, cu_k, max_q, max_k, float(scale), 1 if causal else 0, int(window)
 
 
 def attention_forward(q, k, v, qmask=None, kmask=None, *, cu_q=None, cu_k=None, max_q=None, max_k=None,
                       causal=False, window=None, scale=None, keep=False):
     """o (q's shape), dense; with ``keep`` (o, kept) for ``attention_pullback``.  See ``attention``."""
     options = _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, window, scale)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = q.new_empty(q.shape)
     lse = rest = None
     if keep:
         *lead, tokens, heads, _ = q.shape
         shared = k.shape[-2]
         lse = torch.empty((*lead, shared, tokens * (heads // max(shared, 1))), dtype=torch.float32,
                           device=q.device)
-        rest = None if q.dtype == torch.float32 else torch.empty_like(o)
+        rest = None if q.dtype is torch.float32 else q.new_empty(q.shape)
     boundary.launch_attention(o, lse, rest, q, k, v, *options)
     return (o, AttentionKept(lse, rest)) if keep else o
 
@@ -218,7 +224,7 @@ def attention_pullback(do, q, k, v, o, kept, qmask=None, kmask=None, *, cu_q=Non
     do = _cotangent(do, q.shape, q, "do")
     if do is None:
         raise DimensionMismatch("do: missing")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     boundary.attention_apply_pullback(dq, dk, dv, do, o, kept.lse, kept.rest, q, k, v, *options)
     return dq, dk, dv
 
