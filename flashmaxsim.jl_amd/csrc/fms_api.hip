@@ -1209,7 +1209,7 @@ bool attn_reads(const AttnArgs& a, const void* p, const int64_t (&st)[3], int64_
 
 // Workspace of a call, in pieces, given back in stream order at its end.
 struct Pieces {
-  void* held[8];
+  void* held[16];
   int n = 0;
   hipStream_t stream;
   explicit Pieces(hipStream_t s) : stream(s) {}
@@ -1252,6 +1252,21 @@ hipError_t attn_packed(AttnArgs* a, Pieces* w) {
   return hipSuccess;
 }
 
+// Where the kernels write a dense result: itself, or workspace with rows of whole units.
+hipError_t attn_place(const AttnArgs& a, Pieces* w, void* result, int64_t rows, int64_t heads, void** at) {
+  const int64_t esz = elem_bytes(a.dtype), bytes = a.units * 16;
+  *at = result;
+  if (bytes == a.dim * esz && aligned16(result)) return hipSuccess;
+  return w->get(at, rows * heads * bytes);
+}
+// And from there to the result.
+hipError_t attn_unpack(const AttnArgs& a, void* result, const void* at, int64_t rows, int64_t heads,
+                       hipStream_t stream) {
+  if (at == result) return hipSuccess;
+  const int64_t width = a.units * (16 / elem_bytes(a.dtype)), strides[3] = {0, heads * width, width};
+  return attn_pack(a.dtype, result, at, strides, 1, rows, heads, a.dim, a.dim, stream);
+}
+
 }  // namespace
 
 fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const void* q, const void* k,
@@ -1266,14 +1281,21 @@ fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const v
   if (a.nq == 0 || heads == 0 || dim == 0) return FMS_OK;
   if (!o || (dtype != FMS_F32 && (lse == nullptr) != (rest == nullptr))) return FMS_EINVAL;
   const hipStream_t st = as_stream(stream);
-  hipError_t e = hipSuccess;
-  if (cu_q) e = attn_zero_gaps(dtype, o, cu_q, seqs, a.nq, tq, heads * dim, st);
-  if (cu_q && rest && dtype != FMS_F32 && e == hipSuccess)
-    e = attn_zero_gaps(dtype, rest, cu_q, seqs, a.nq, tq, heads * dim, st);
-  if (e != hipSuccess || seqs == 0 || tq == 0) return from_hip(e);
   Pieces w(st);
-  e = attn_packed(&a, &w);
-  if (e == hipSuccess) e = attn_forward(a, AttnOut{o, lse, dtype == FMS_F32 ? nullptr : rest}, st);
+  AttnOut out = {};
+  out.lse = lse;
+  hipError_t e = hipSuccess;
+  if (seqs > 0 && tq > 0) {
+    if (e == hipSuccess) e = attn_packed(&a, &w);
+    if (e == hipSuccess) e = attn_place(a, &w, o, a.nq, heads, &out.o);
+    if (e == hipSuccess && dtype != FMS_F32 && rest) e = attn_place(a, &w, rest, a.nq, heads, &out.rest);
+    if (e == hipSuccess) e = attn_forward(a, out, st);
+    if (e == hipSuccess) e = attn_unpack(a, o, out.o, a.nq, heads, st);
+    if (e == hipSuccess && out.rest) e = attn_unpack(a, rest, out.rest, a.nq, heads, st);
+  }
+  if (cu_q && e == hipSuccess) e = attn_zero_gaps(dtype, o, cu_q, seqs, a.nq, tq, heads * dim, st);
+  if (cu_q && e == hipSuccess && rest && dtype != FMS_F32)
+    e = attn_zero_gaps(dtype, rest, cu_q, seqs, a.nq, tq, heads * dim, st);
   return from_hip(e);
 }
 
@@ -1291,39 +1313,43 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
   if (a.nq > 0 && (!dq || !dout || !o || !lse || (dtype != FMS_F32 && !rest))) return FMS_EINVAL;
   if (a.nk > 0 && (!dk || !dv)) return FMS_EINVAL;
   const hipStream_t st = as_stream(stream);
+  Pieces w(st);
+  AttnGrads g = {};
   hipError_t e = hipSuccess;
-  if (cu_q) {
+  if (seqs > 0) {
+    const int64_t rows = a.nq * heads, esz = elem_bytes(dtype);
+    void* p;
+    e = w.get(&p, rows * 4);
+    g.delta = static_cast<float*>(p);
+    if (e == hipSuccess && dtype == FMS_F16) {
+      e = w.get(&p, seqs * kv_heads * kAttnPeakParts * 8);
+      g.peaks = static_cast<float*>(p);
+    }
+    if (e == hipSuccess) e = attn_packed(&a, &w);
+    g.lse = lse;
+    const int64_t width = a.units * (16 / esz), dense[3] = {0, heads * dim, dim};
+    const void* from[3] = {dout, o, dtype == FMS_F32 ? nullptr : rest};
+    const void** to[3] = {&g.dout, &g.o, &g.rest};
+    for (int i = 0; i < 3 && e == hipSuccess; ++i) {
+      *to[i] = from[i];
+      if (!from[i] || (width == dim && aligned16(from[i]))) continue;
+      e = w.get(&p, rows * width * esz);
+      if (e == hipSuccess) e = attn_pack(dtype, p, from[i], dense, 1, a.nq, heads, (int32_t)dim, (int32_t)width, st);
+      *to[i] = p;
+    }
+    if (e == hipSuccess) e = attn_place(a, &w, dq, a.nq, heads, &g.dq);
+    if (e == hipSuccess) e = attn_place(a, &w, dk, a.nk, kv_heads, &g.dk);
+    if (e == hipSuccess) e = attn_place(a, &w, dv, a.nk, kv_heads, &g.dv);
+    if (e == hipSuccess) e = attn_pullback(a, g, st);
+    if (e == hipSuccess) e = attn_unpack(a, dq, g.dq, a.nq, heads, st);
+    if (e == hipSuccess) e = attn_unpack(a, dk, g.dk, a.nk, kv_heads, st);
+    if (e == hipSuccess) e = attn_unpack(a, dv, g.dv, a.nk, kv_heads, st);
+  }
+  if (cu_q && e == hipSuccess) {
     e = attn_zero_gaps(dtype, dq, cu_q, seqs, a.nq, tq, heads * dim, st);
     if (e == hipSuccess) e = attn_zero_gaps(dtype, dk, cu_k, seqs, a.nk, tk, kv_heads * dim, st);
     if (e == hipSuccess) e = attn_zero_gaps(dtype, dv, cu_k, seqs, a.nk, tk, kv_heads * dim, st);
   }
-  if (e != hipSuccess || seqs == 0) return from_hip(e);
-  Pieces w(st);
-  AttnGrads g = {};
-  const int64_t rows = a.nq * heads, esz = elem_bytes(dtype);
-  void* p;
-  e = w.get(&p, rows * 4);
-  g.delta = static_cast<float*>(p);
-  if (e == hipSuccess && dtype == FMS_F16) {
-    e = w.get(&p, seqs * kv_heads * kAttnPeakParts * 8);
-    g.peaks = static_cast<float*>(p);
-  }
-  if (e == hipSuccess) e = attn_packed(&a, &w);
-  g.lse = lse;
-  g.dq = dq;
-  g.dk = dk;
-  g.dv = dv;
-  const int64_t width = a.units * (16 / esz), dense[3] = {0, heads * dim, dim};
-  const void* from[3] = {dout, o, dtype == FMS_F32 ? nullptr : rest};
-  const void** to[3] = {&g.dout, &g.o, &g.rest};
-  for (int i = 0; i < 3 && e == hipSuccess; ++i) {
-    *to[i] = from[i];
-    if (!from[i] || (width == dim && aligned16(from[i]))) continue;
-    e = w.get(&p, rows * width * esz);
-    if (e == hipSuccess) e = attn_pack(dtype, p, from[i], dense, 1, a.nq, heads, (int32_t)dim, (int32_t)width, st);
-    *to[i] = p;
-  }
-  if (e == hipSuccess) e = attn_pullback(a, g, st);
   return from_hip(e);
 }
 

@@ -38,8 +38,8 @@ constexpr float kShift = std::is_same<Op, OpF16>::value ? 10.0f : 0.0f;
 __device__ __forceinline__ float factor(const AttnArgs& A) { return fmaxf(fabsf(A.scale) * kLog2e, 1e-30f); }
 
 template <class Op, int kD, int kWaves, bool kSplit>
-__global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, AttnOut out, Parts P,
-                                                                   uint32_t tiles, uint32_t work) {
+__global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) attn_forward_kernel(AttnArgs A, AttnOut out, Parts P,
+                                                                   int chunk, uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
   typedef typename Elem<Op>::T E;
   constexpr int kThreads = kWaves * 64;
@@ -53,8 +53,10 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   const uint32_t unit = whole / tiles;
   // (under a causal mask the last tiles have the most keys: they start first)
   const int tile = (int)(A.causal ? tiles - 1 - (whole - unit * tiles) : whole - unit * tiles);
-  const int64_t b = unit / (uint32_t)A.kv_heads;
-  const int hk = (int)(unit % (uint32_t)A.kv_heads);
+  // `chunk` neighbouring key heads, of which kv_heads is a multiple
+  const uint32_t chunks = (uint32_t)A.kv_heads / (uint32_t)chunk;
+  const int64_t b = unit / chunks;
+  const int hk = (int)(unit % chunks) * chunk;  // the first
   const Span S = span_of(A, b);
   const int nrows = S.nq * A.group;
   const int row0 = tile * (32 * kWaves);
@@ -65,10 +67,15 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
   const int row = row0 + wave * 32 + (lane & 31);
   const int t = token_of(row, A), head = row - t * A.group;  // (of the key head's)
   const int wt = token_of(row0 + wave * 32, A);              // the wave's first token
-  u32x4 q[T::kK];
-  own_row<T>(q, wave_rows<Op>(A.q, seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2], wt, A.qs[1]),
-             row < nrows ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar, A.units, h);
   const bool there = row < nrows && (!A.qmask || A.qmask[b * A.tq + t]);
+  // (rows behind a mask are not read: zeros, as their results are)
+  u32x4 q[T::kK];
+  const int64_t qstart = seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2];
+  const int qat = there ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar;
+  const auto load_q = [&](int u) {
+    own_row<T>(q, wave_rows<Op>(A.q, qstart + (int64_t)u * A.group * A.qs[2], wt, A.qs[1]), qat, A.units, h);
+  };
+  load_q(0);
   // the keys that count for this row by position, and for the workgroup (reaches grow with the token)
   const Reach mine = keys_of(t, S, A);
   const auto reach = [&](int r) { return keys_of(token_of(r < nrows ? r : nrows - 1, A), S, A); };
@@ -78,67 +85,91 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
     first = first > from ? first : from;
     last = last < from + P.keys ? last : from + P.keys;
   }
-  // (the masks' bits, the queries and their mask are on their way together)
-  Rows keys = {words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
-  const auto gather = [&] {
+  Walk walk = {{words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0}, first, last, chunk, 0, 0, 0};
+  const auto gather = [&](const Rows& keys) {
     const uint8_t* km = A.kmask + b * A.tk;
     keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
   };
-  if (keys.given && first < last) gather();
-  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
-  const int at = row < nrows ? row_at<Op>(t - wt, width, head, A.dim) : kFar;
-  const bool vec = whole_units(out.o, A.dim, Op::kEsz) && whole_units(out.rest, A.dim, Op::kEsz);
-  const int64_t stat = rows_at(A, b, hk, S.q0) + row;
+  if (walk.rows.given && first < last) gather(walk.rows);
+  const bool some = __syncthreads_or(there);
+
+  const int64_t dim = A.units * (16 / Op::kEsz), width = A.heads * dim;
+  const int64_t start = S.q0 * width + hk * A.group * dim;
+  const int at = row < nrows ? row_at<Op>(t - wt, width, head, dim) : kFar;
+  const float c = factor(A);
   f32x16 acc[T::kBlocks];
+  float m = -INFINITY, l = 0.0f;
+  const auto clear = [&] {
 #pragma unroll
-  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
-  if (!__syncthreads_or(there) && !kSplit) {  // padding: zeros, and nothing is read
-    store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, 0.0f, A.dim, vec, h);
-    if (Op::kEsz == 2 && out.rest)
-      store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, start, wt, width), at, acc, 0.0f, A.dim, vec, h);
-    if (out.lse && h == 0 && row < nrows) out.lse[stat] = -INFINITY;
+    for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
+    m = -INFINITY;
+    l = 0.0f;
+  };
+  // What unit u's rows summed, to memory.
+  const auto finish = [&](int u) {
+    // both halves of the wave summed other keys of the same row
+    l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
+    if constexpr (kSplit) {
+      if (row >= nrows) return;
+      const int64_t slot = (int64_t)piece * (32 * kWaves) + wave * 32 + (lane & 31);
+      float* to = P.acc + slot * kD;
+#pragma unroll
+      for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * h) =
+              f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+      P.stat[slot * 2 + h] = h ? l : m;
+    } else {
+      const bool any = l > 0.0f || l != l;
+      const float inv = any ? 1.0f / l : 0.0f;
+      const int64_t to = start + u * A.group * dim;
+      store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, to, wt, width), at, acc, inv, A.units, h);
+      if (out.lse && h == 0 && row < nrows)
+        out.lse[rows_at(A, b, hk + u, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
+      if (Op::kEsz == 2 && out.rest) {
+#pragma unroll
+        for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float o = acc[i][r] * inv;
+            acc[i][r] = (o - (float)(E)o) * kRestScale<Op>;
+          }
+        store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, to, wt, width), at, acc, 1.0f, A.units, h);
+      }
+    }
+  };
+  clear();
+  if (!some || !walk.begin(gather)) {  // no row, or no key, that counts: zeros
+    for (int u = 0; u < chunk; ++u) finish(u);
     return;
   }
-  if (A.qmask) clear_unless<T>(q, there);
   const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
-  const float c = factor(A);
-  if (A.scale < 0) negate<T>(q);
-  const char* kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
-  const char* vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
-  const int64_t kstep = A.ks[1] * Op::kEsz, vstep = A.vs[1] * Op::kEsz;
-
-  float m = -INFINITY, l = 0.0f;
-
-  for (bool more = false; keys.span0 < last; keys.span0 += kMaskSpan, more = true) {
-    const int from = first > keys.span0 ? first : keys.span0;
-    const int to = last < keys.span0 + kMaskSpan ? last : keys.span0 + kMaskSpan;
-    keys.to = to;
-    if (more) {  // (every wave is through with the words, and with the buffers)
-      landed();
-      if (keys.given) gather();
-      landed();
-    }
-    const auto request = [&](int j0, uint64_t bits, int buffer) {
-      T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * kstep, (int)kstep, A.units, bits);
-      T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * vstep, (int)vstep, A.units, bits);
-    };
-    uint64_t bits, bits1;  // of this tile, and of the next
-    int j0 = keys.next(from, bits);
-    int buffer = 0;
-    if (j0 < to) request(j0, bits, 0);
-    while (j0 < to) {
-      landed();
-      const int j1 = keys.next(j0 + kRows, bits1);
-      if (j1 < to) request(j1, bits1, buffer ^ 1);
-      const char* const K = lds + buffer * 2 * T::kBytes;
-      const char* const V = K + T::kBytes;
-      const bool none = j0 >= wide.any.hi || j0 + kRows <= wide.any.lo;
-      const int now = j0;
-      const uint64_t in = bits;
-      j0 = j1;
-      bits = bits1;
-      buffer ^= 1;
-      if (none) continue;  // (none of this wave's rows reaches here)
+  const char* const kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
+  const char* const vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
+  const auto request = [&](const Walk& w, int buffer) {
+    T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + (w.u * A.ks[2] + w.at * A.ks[1]) * Op::kEsz,
+                                  (int)A.ks[1] * Op::kEsz, A.units, w.bits);
+    T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes,
+                                  vbase + (w.u * A.vs[2] + w.at * A.vs[1]) * Op::kEsz, (int)A.vs[1] * Op::kEsz, A.units,
+                                  w.bits);
+  };
+  int buffer = 0;
+  request(walk, 0);
+  for (int u = 0; u < chunk; ++u) {
+    clear();
+    if (A.scale < 0) negate<T>(q);
+    while (walk.u == u) {
+    landed();
+    const Walk next = walk.next(gather);
+    if (next.u < chunk) request(next, buffer ^ 1);
+    const char* const K = lds + buffer * 2 * T::kBytes;
+    const char* const V = K + T::kBytes;
+    const int now = walk.at;
+    const uint64_t in = walk.bits;
+    walk = next;
+    buffer ^= 1;
+    if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
       float s[2][16];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -199,40 +230,9 @@ __global__ void __launch_bounds__(kWaves * 64) attn_forward_kernel(AttnArgs A, A
         }
       l += sum[0] + sum[1];
     }
-  }
-  if (A.qmask && !there) {
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
-  }
-  // both halves of the wave summed other keys of the same row
-  l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
-  if constexpr (kSplit) {
-    if (row >= nrows) return;
-    const int64_t slot = (int64_t)piece * (32 * kWaves) + wave * 32 + (lane & 31);
-    float* to = P.acc + slot * kD;
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * h) =
-            f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
-    P.stat[slot * 2 + h] = h ? l : m;
-    return;
-  }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, inv, A.dim, vec, h);
-  if (out.lse && h == 0 && row < nrows)
-    out.lse[stat] = l > 0.0f || l != l ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
-  if (Op::kEsz == 2 && out.rest) {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float o = acc[i][r] * inv;
-        acc[i][r] = (o - (float)(E)o) * kRestScale<Op>;
-      }
-    store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, start, wt, width), at, acc, 1.0f, A.dim, vec, h);
+    if (A.qmask && !there) clear();
+    finish(u);
+    if (u + 1 < chunk) load_q(u + 1);
   }
 }
 
@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs A, AttnOut out,
   const bool any = l > 0.0f || l != l;
   const float inv = any ? 1.0f / l : 0.0f;
   const int t = token_of(row, A), head = hk * A.group + row - t * A.group;
-  const int64_t at = ((S.q0 + t) * A.heads + head) * (int64_t)A.dim;
-  for (int d = threadIdx.x; d < A.dim; d += 256) {
+  const int dim = A.units * (16 / Op::kEsz);
+  const int64_t at = ((S.q0 + t) * A.heads + head) * (int64_t)dim;
+  for (int d = threadIdx.x; d < dim; d += 256) {
     const float o = ((lds[0][d] + lds[1][d]) + (lds[2][d] + lds[3][d])) * inv;
     static_cast<E*>(out.o)[at + d] = (E)o;
     if (Op::kEsz == 2 && out.rest) static_cast<E*>(out.rest)[at + d] = (E)((o - (float)(E)o) * kRestScale<Op>);
@@ -344,7 +345,7 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
     p.acc = static_cast<float*>(mem);
     p.stat = p.acc + slots * kD;
     hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, true>), dim3(piece_blocks(pieces * p.splits)),
-                       dim3(kWaves * 64), 0, stream, a, out, p, (uint32_t)tiles, (uint32_t)(pieces * p.splits));
+                       dim3(kWaves * 64), 0, stream, a, out, p, 1, (uint32_t)tiles, (uint32_t)(pieces * p.splits));
     const int most = a.tq * a.group;
     hipLaunchKernelGGL((attn_join_kernel<Op, kD, kWaves>), dim3((unsigned)(units * most)), dim3(256), 0, stream, a,
                        out, p, (int)tiles, most);
@@ -352,8 +353,9 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
     const hipError_t ef = workspace_free(mem, stream);
     return e != hipSuccess ? e : ef;
   }
-  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(pieces)), dim3(kWaves * 64), 0,
-                     stream, a, out, Parts{}, (uint32_t)tiles, (uint32_t)pieces);
+  const int chunk = attn_chunk(a, pieces);
+  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(pieces / chunk)),
+                     dim3(kWaves * 64), 0, stream, a, out, Parts{}, chunk, (uint32_t)tiles, (uint32_t)(pieces / chunk));
   return hipGetLastError();
 }
 
@@ -400,6 +402,13 @@ hipError_t attn_zero_gaps(int32_t dtype, void* out, const int32_t* cu, int64_t s
     hipLaunchKernelGGL((attn::attn_gap_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream,
                        static_cast<uint16_t*>(out), cu, seqs, rows, most, width);
   return hipGetLastError();
+}
+
+int attn_chunk(const AttnArgs& a, int64_t pieces) {
+  int chunk = 1;
+  for (int n = 2; n <= a.kv_heads && pieces / n >= 2048; ++n)
+    if (a.kv_heads % n == 0) chunk = n;
+  return chunk;
 }
 
 hipError_t attn_forward(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {

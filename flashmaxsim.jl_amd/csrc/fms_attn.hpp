@@ -23,7 +23,7 @@ namespace fms {
 struct AttnArgs {
   int32_t dtype;  // FMS_F32, FMS_F16, FMS_BF16
   int32_t dim;    // values of a head
-  int32_t units;  // 16-byte units of a head's row in q, k and v as the kernels read them
+  int32_t units;  // 16-byte units of a head's row as the kernels read and write it (dim, made whole units)
   int32_t heads, kv_heads, group;
   uint32_t group_inv;  // ceil(2^32 / group), 0 for a group of one
   int32_t causal;
@@ -40,7 +40,7 @@ struct AttnArgs {
 
 constexpr int64_t kAttnMaxDim = 128;
 
-// o (token rows, heads, dim); lse (seqs, kv_heads, tq * group) or ragged (kv_heads, nq * group),
+// o (token rows, heads, whole units of dim, 16-byte aligned); lse (seqs, kv_heads, tq * group) or ragged (kv_heads, nq * group),
 // base-2 logarithms of the rows' sums, and rest, what o's rounding left (16-bit types): both null
 // where no pullback follows.
 struct AttnOut {
@@ -69,6 +69,10 @@ hipError_t attn_pack(int32_t dtype, void* to, const void* from, const int64_t* s
 // Zeros for token rows of (rows, width) that no sequence covers.
 hipError_t attn_zero_gaps(int32_t dtype, void* out, const int32_t* cu, int64_t seqs, int64_t rows,
                           int64_t most, int64_t width, hipStream_t stream);
+
+// How many neighbouring key heads a workgroup takes: as many as leave two rounds of workgroups (four to a
+// CU), so that the start of the next head's work hides behind this one's.
+int attn_chunk(const AttnArgs& a, int64_t pieces);
 
 // ---- device --------------------------------------------------------------------------------
 
@@ -253,6 +257,10 @@ struct Tile {
   }
 };
 
+// Waves of a SIMD that the registers should leave room for: as many as the LDS does.
+template <class Op, int kD, int kWaves>
+constexpr int kSimdWaves = kWaves < 4 ? 1 : kD * Op::kEsz <= 128 ? 4 : kD * Op::kEsz <= 256 ? 2 : 1;
+
 template <class Op>
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
   if constexpr (Op::kEsz == 4) {
@@ -327,19 +335,11 @@ __device__ __forceinline__ float add_operand(const u32x4& p, float c) {
 template <class Op>
 constexpr int kGroups = Op::kEsz == 4 ? 4 : 2;  // operands of 32 rows
 
-// What lies behind a mask may be anything: zero.
-template <class T>
-__device__ __forceinline__ void clear_unless(u32x4 (&f)[T::kK], bool there) {
-#pragma unroll
-  for (int kb = 0; kb < T::kK; ++kb)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[kb][e] = there ? f[kb][e] : 0u;
-}
-
 // Lane's own row as a second operand for `rows`: units 2 kb + half of it, straight from memory, `at` bytes
 // into the resource (kFar: zeros).  (Loads behind a branch would wait for one another.)
 template <class T>
 __device__ __forceinline__ void own_row(u32x4 (&f)[T::kK], rsrc_t from, int at, int units, int h) {
+  asm volatile("" : "+v"(at), "+v"(h));  // (offsets are computed here, not kept in registers around a loop)
 #pragma unroll
   for (int kb = 0; kb < T::kK; ++kb) f[kb] = buf_load16(from, 2 * kb + h < units ? at + (2 * kb + h) * 16 : kFar);
 }
@@ -349,10 +349,6 @@ template <class T>
 __device__ __forceinline__ void negate(u32x4 (&f)[T::kK]) {
 #pragma unroll
   for (int kb = 0; kb < T::kK; ++kb) f[kb] ^= T::Op::kEsz == 4 ? 0x80000000u : 0x80008000u;
-}
-
-__device__ __forceinline__ bool whole_units(const void* p, int dim, int esz) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && dim * esz % 16 == 0;
 }
 
 // Bits lo .. hi - 1 of 32 (bounds anywhere).
@@ -375,7 +371,7 @@ __device__ __forceinline__ float masked(float v, uint32_t keep, int r, float wha
 static_assert(kRows == 64, "a word of mask bits is a tile");
 struct Rows {
   uint64_t* words;
-  bool given;  // a mask
+  bool given;  // a mask (without one there is one span)
   int span0, to;
 
   // The mask bits of rows from span0 on, below n; keep(row): its mask has it.  All threads call it.
@@ -409,14 +405,63 @@ __device__ __forceinline__ void landed() {
   asm volatile("" ::: "memory");
 }
 
-// A lane's accumulators (values 32 b + 8 (r / 4) + 4 h + r % 4 of its row) times `by` to its row of `dim` values,
-// `at` bytes into the resource (kFar: nowhere).  units: rows are whole units of 16 bytes, aligned to them.
-// All lanes of the wave call it.
+// The tiles of a workgroup, one after the other: of each of its `units` units (neighbouring key heads of a
+// sequence, alike in their masks), those of [first, last) that have rows.  While one is worked on the
+// next is on its way, across units too: the start of a short sequence's next head costs no wait.
+// gather(rows) fills the words from rows.span0 on; those of `first` are there when begin() is called.
+struct Walk {
+  Rows rows;
+  int first, last, units;
+  int u, at;       // the current tile: unit, first row
+  uint64_t bits;   // and its rows
+
+  template <class Gather>
+  __device__ __forceinline__ void move(int span0, Gather&& gather) {
+    landed();  // (every wave is through with the words)
+    rows.span0 = span0;
+    rows.to = last - span0 < kMaskSpan ? last : span0 + kMaskSpan;
+    gather(rows);
+    landed();
+  }
+  // False: there are none.
+  template <class Gather>
+  __device__ __forceinline__ bool begin(Gather&& gather) {
+    u = 0;
+    rows.to = rows.given && last - rows.span0 > kMaskSpan ? rows.span0 + kMaskSpan : last;
+    at = rows.next(first, bits);
+    while (at >= rows.to && rows.to < last) {
+      move(rows.span0 + kMaskSpan, gather);
+      at = rows.next(rows.span0, bits);
+    }
+    return at < rows.to;
+  }
+  // What comes after the current tile; its unit is `units` where nothing does.
+  template <class Gather>
+  __device__ __forceinline__ Walk next(Gather&& gather) const {
+    Walk w = *this;
+    w.at = w.rows.next(at + kRows, w.bits);
+    while (w.at >= w.rows.to) {
+      if (w.rows.to < last) {
+        w.move(w.rows.span0 + kMaskSpan, gather);
+        w.at = w.rows.next(w.rows.span0, w.bits);
+      } else {
+        if (++w.u == units) break;
+        const int span0 = first / kMaskSpan * kMaskSpan;
+        if (rows.given && w.rows.span0 != span0) w.move(span0, gather);
+        w.at = w.rows.next(first, w.bits);
+      }
+    }
+    return w;
+  }
+};
+
+// A lane's accumulators (values 32 b + 8 (r / 4) + 4 h + r % 4 of its row) times `by` to its row of `units` 16-byte
+// units, `at` bytes into the resource (kFar: nowhere).  All lanes of the wave call it.
 template <class Op, int kBlocks>
-__device__ __forceinline__ void store_row(rsrc_t to, int at, const f32x16 (&acc)[kBlocks], float by, int dim, bool units,
-                                          int h) {
+__device__ __forceinline__ void store_row(rsrc_t to, int at, const f32x16 (&acc)[kBlocks], float by, int units, int h) {
   typedef typename Elem<Op>::T T;
   typedef T V4 __attribute__((ext_vector_type(4)));
+  asm volatile("" : "+v"(at), "+v"(h));  // (as own_row)
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
@@ -426,32 +471,18 @@ __device__ __forceinline__ void store_row(rsrc_t to, int at, const f32x16 (&acc)
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[i][e] = (T)(acc[b][4 * (g + i) + e] * by);
-      if constexpr (Op::kEsz == 2) if (units) {
+      if constexpr (Op::kEsz == 2) {
         // the halves of the wave trade: half 0 has all of group g's eight values, half 1 all of g + 1's
         const u32x2 lo = __builtin_bit_cast(u32x2, x[0]), hi = __builtin_bit_cast(u32x2, x[1]);
         const auto s0 = __builtin_amdgcn_permlane32_swap(lo[0], hi[0], false, false);
         const auto s1 = __builtin_amdgcn_permlane32_swap(lo[1], hi[1], false, false);
-        const int d = 32 * b + 8 * (g + h);
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, to,
-                                               d < dim ? at + d * Op::kEsz : kFar, 0, 0);
-        continue;
-      }
+        const int u = 4 * b + g + h;
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{s0[0], s1[0], s0[1], s1[1]}, to, u < units ? at + u * 16 : kFar, 0, 0);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int d = 32 * b + 8 * (g + i) + 4 * h;
-        if constexpr (Op::kEsz == 4) if (units) {
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), to,
-                                                 d < dim ? at + d * Op::kEsz : kFar, 0, 0);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int off = d + e < dim ? at + (d + e) * Op::kEsz : kFar;
-          const T y = x[i][e];
-          if constexpr (Op::kEsz == 2)
-            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), to, off, 0, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), to, off, 0, 0);
+        for (int i = 0; i < 2; ++i) {
+          const int u = 8 * b + 2 * (g + i) + h;
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), to, u < units ? at + u * 16 : kFar, 0, 0);
         }
       }
     }

@@ -137,19 +137,18 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   const int t = token_of(row, A), head = row - t * A.group;  // (of the key head's)
   const int wt = token_of(row0 + wave * 32, A);              // the wave's first token
   const int64_t at = rows_at(A, b, hk, S.q0) + row;
-  u32x4 q[T::kK], d[T::kK], o[T::kK], rest[T::kK];
-  own_row<T>(q, wave_rows<Op>(A.q, seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2], wt, A.qs[1]),
-             row < nrows ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar, A.units, h);
-  {
-    const int64_t dim = A.units * (16 / Op::kEsz), width = A.heads * dim;
-    const int64_t start = S.q0 * width + (int64_t)hk * A.group * dim;
-    const int place = row < nrows ? row_at<Op>(t - wt, width, head, dim) : kFar;
-    own_row<T>(d, wave_rows<Op>(G.dout, start, wt, width), place, A.units, h);
-    own_row<T>(o, wave_rows<Op>(G.o, start, wt, width), place, A.units, h);
-    if constexpr (Op::kEsz == 2) own_row<T>(rest, wave_rows<Op>(G.rest, start, wt, width), place, A.units, h);
-  }
   const float lse = row < nrows ? G.lse[at] : 0.0f;
   const bool there = row < nrows && (!A.qmask || A.qmask[b * A.tq + t]);
+  u32x4 q[T::kK], d[T::kK], o[T::kK], rest[T::kK];
+  own_row<T>(q, wave_rows<Op>(A.q, seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2], wt, A.qs[1]),
+             there ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar, A.units, h);
+  const int64_t dim = A.units * (16 / Op::kEsz), width = A.heads * dim;
+  const int64_t start = S.q0 * width + hk * A.group * dim;
+  const int place = row < nrows ? row_at<Op>(t - wt, width, head, dim) : kFar;
+  const int from = there ? place : kFar;  // (rows behind a mask are not read: zeros, as their results are)
+  own_row<T>(d, wave_rows<Op>(G.dout, start, wt, width), from, A.units, h);
+  own_row<T>(o, wave_rows<Op>(G.o, start, wt, width), from, A.units, h);
+  if constexpr (Op::kEsz == 2) own_row<T>(rest, wave_rows<Op>(G.rest, start, wt, width), from, A.units, h);
   const Reach mine = keys_of(t, S, A);
   const auto reach = [&](int r) { return keys_of(token_of(r < nrows ? r : nrows - 1, A), S, A); };
   const int first = reach(row0).lo / kRows * kRows;
@@ -160,20 +159,13 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
     keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
   };
   if (keys.given && first < last) gather();
-  const int64_t width = (int64_t)A.heads * A.dim, start = S.q0 * width + (int64_t)hk * A.group * A.dim;
-  const int to_row = row < nrows ? row_at<Op>(t - wt, width, head, A.dim) : kFar;
-  const bool vec = whole_units(G.dq, A.dim, Op::kEsz);
   f32x16 acc[T::kBlocks];
 #pragma unroll
   for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
   if (!__syncthreads_or(there)) {  // padding: zeros, and no keys are read
-    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), to_row, acc, 0.0f, A.dim, vec, h);
+    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), place, acc, 0.0f, A.units, h);
     if (h == 0 && row < nrows) G.delta[at] = 0.0f;
     return;
-  }
-  if (A.qmask) {
-    clear_unless<T>(q, there);
-    clear_unless<T>(d, there);  // (o and rest are zeros there)
   }
   const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
   float delta = 0.0f, norm = 0.0f;
@@ -272,7 +264,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   if (A.qmask && !there)
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), to_row, acc, A.scale * kUnshift<Op> / by, A.dim, vec,
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), place, acc, A.scale * kUnshift<Op> / by, A.units,
                             h);
 }
 
@@ -297,12 +289,12 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   const int h = lane >> 5;
   const int key = key0 + wave * 32 + (lane & 31);
   const int wkey = key0 + wave * 32;  // the wave's first
-  u32x4 k[T::kK], v[T::kK];
-  own_row<T>(k, wave_rows<Op>(A.k, seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2], wkey, A.ks[1]),
-             key < S.nk ? row_at<Op>(key - wkey, A.ks[1], 0, 0) : kFar, A.units, h);
-  own_row<T>(v, wave_rows<Op>(A.v, seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2], wkey, A.vs[1]),
-             key < S.nk ? row_at<Op>(key - wkey, A.vs[1], 0, 0) : kFar, A.units, h);
   const bool there = key < S.nk && (!A.kmask || A.kmask[b * A.tk + key]);
+  u32x4 k[T::kK], v[T::kK];  // (keys behind a mask are not read: zeros, as their results are)
+  own_row<T>(k, wave_rows<Op>(A.k, seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2], wkey, A.ks[1]),
+             there ? row_at<Op>(key - wkey, A.ks[1], 0, 0) : kFar, A.units, h);
+  own_row<T>(v, wave_rows<Op>(A.v, seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2], wkey, A.vs[1]),
+             there ? row_at<Op>(key - wkey, A.vs[1], 0, 0) : kFar, A.units, h);
   const auto reach = [&](int j) {  // in rows
     Reach r = tokens_of(j < S.nk ? j : S.nk - 1, S, A);
     r.lo *= A.group;
@@ -318,20 +310,16 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
     rows.gather<kThreads>(S.nq * A.group, [&](int r) { return qm[token_of(r, A)] != 0; });
   };
   if (rows.given && first < last) gather();
-  const int64_t wide_row = (int64_t)A.kv_heads * A.dim, start = S.k0 * wide_row + (int64_t)hk * A.dim;
+  const int64_t width = A.units * (16 / Op::kEsz);
+  const int64_t wide_row = A.kv_heads * width, start = S.k0 * wide_row + hk * width;
   const int at = key < S.nk ? row_at<Op>(key - wkey, wide_row, 0, 0) : kFar;
-  const bool vec_k = whole_units(G.dk, A.dim, Op::kEsz), vec_v = whole_units(G.dv, A.dim, Op::kEsz);
   f32x16 dk[T::kBlocks], dv[T::kBlocks];
 #pragma unroll
   for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
   if (!__syncthreads_or(there)) {  // padding: zeros, and no rows are read
-    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, 0.0f, A.dim, vec_k, h);
-    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, 0.0f, A.dim, vec_v, h);
+    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, 0.0f, A.units, h);
+    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, 0.0f, A.units, h);
     return;
-  }
-  if (A.kmask) {
-    clear_unless<T>(k, there);
-    clear_unless<T>(v, there);
   }
   const Reaches wide = reaches(reach(key0 + wave * 32), reach(key0 + wave * 32 + 31), __any(there));
   const float c = fabsf(A.scale) * kLog2e;
@@ -341,7 +329,6 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
 
   const char* qbase = static_cast<const char*>(A.q) +
                       (seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2]) * Op::kEsz;
-  const int64_t width = A.units * (16 / Op::kEsz);
   const char* dbase = static_cast<const char*>(G.dout) + (S.q0 * A.heads + hk * A.group) * width * Op::kEsz;
   const int64_t stat = rows_at(A, b, hk, S.q0);
 
@@ -432,9 +419,8 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   if (A.kmask && !there)
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, A.scale * kUnshift<Op> / by, A.dim, vec_k,
-                            h);
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, kUnshift<Op>, A.dim, vec_v, h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, A.scale * kUnshift<Op> / by, A.units, h);
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, kUnshift<Op>, A.units, h);
 }
 
 template <class Op, int kD>
