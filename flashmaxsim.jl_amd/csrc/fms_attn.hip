@@ -85,13 +85,13 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
     first = first > from ? first : from;
     last = last < from + P.keys ? last : from + P.keys;
   }
-  Walk walk = {{words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0}, first, last, chunk, 0, 0, 0};
-  const auto gather = [&](const Rows& keys) {
+  Rows keys = {words, A.kmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
+  const auto gather = [&] {
     const uint8_t* km = A.kmask + b * A.tk;
     keys.gather<kThreads>(S.nk, [&](int j) { return km[j] != 0; });
   };
-  if (walk.rows.given && first < last) gather(walk.rows);
-  const bool some = __syncthreads_or(there);
+  if (keys.given && first < last) gather();
+  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no keys are read)
 
   const int64_t dim = A.units * (16 / Op::kEsz), width = A.heads * dim;
   const int64_t start = S.q0 * width + hk * A.group * dim;
@@ -139,37 +139,42 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
       }
     }
   };
-  clear();
-  if (!some || !walk.begin(gather)) {  // no row, or no key, that counts: zeros
-    for (int u = 0; u < chunk; ++u) finish(u);
-    return;
-  }
   const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
   const char* const kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
   const char* const vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
-  const auto request = [&](const Walk& w, int buffer) {
-    T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + (w.u * A.ks[2] + w.at * A.ks[1]) * Op::kEsz,
-                                  (int)A.ks[1] * Op::kEsz, A.units, w.bits);
-    T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes,
-                                  vbase + (w.u * A.vs[2] + w.at * A.vs[1]) * Op::kEsz, (int)A.vs[1] * Op::kEsz, A.units,
-                                  w.bits);
+  const auto request = [&](int u, int j0, uint64_t bits, int buffer) {
+    T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + (u * A.ks[2] + j0 * A.ks[1]) * Op::kEsz,
+                                  (int)A.ks[1] * Op::kEsz, A.units, bits);
+    T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + (u * A.vs[2] + j0 * A.vs[1]) * Op::kEsz,
+                                  (int)A.vs[1] * Op::kEsz, A.units, bits);
   };
+  // While a tile is worked on the next is on its way, a next head's first one too.  (Several heads
+  // only where one span holds the keys' mask: they are alike in what counts.)
+  uint64_t bits0;
+  keys.end(last);
+  const int j00 = keys.next(first, bits0);
   int buffer = 0;
-  request(walk, 0);
+  if (j00 < keys.to) request(0, j00, bits0, 0);
   for (int u = 0; u < chunk; ++u) {
     clear();
     if (A.scale < 0) negate<T>(q);
-    while (walk.u == u) {
-    landed();
-    const Walk next = walk.next(gather);
-    if (next.u < chunk) request(next, buffer ^ 1);
-    const char* const K = lds + buffer * 2 * T::kBytes;
-    const char* const V = K + T::kBytes;
-    const int now = walk.at;
-    const uint64_t in = walk.bits;
-    walk = next;
-    buffer ^= 1;
-    if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
+    int j0 = j00;
+    uint64_t bits = bits0;
+    for (;;) {
+    while (j0 < keys.to) {
+      landed();
+      uint64_t bits1;
+      const int j1 = keys.next(j0 + kRows, bits1);
+      const bool same = j1 < keys.to;
+      if (same || u + 1 < chunk) request(same ? u : u + 1, same ? j1 : j00, same ? bits1 : bits0, buffer ^ 1);
+      const char* const K = lds + buffer * 2 * T::kBytes;
+      const char* const V = K + T::kBytes;
+      const int now = j0;
+      const uint64_t in = bits;
+      j0 = j1;
+      bits = bits1;
+      buffer ^= 1;
+      if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
       float s[2][16];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -229,6 +234,15 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
             acc[i] = mma<Op>(T::columns(V, 32 * half + kPer * g, i, lane), p, acc[i]);
         }
       l += sum[0] + sum[1];
+    }
+      if (keys.to >= last) break;
+      landed();  // (every wave is through with the words, and with the buffers)
+      keys.span0 += kMaskSpan;
+      keys.end(last);
+      gather();
+      landed();
+      j0 = keys.next(keys.span0, bits);
+      if (j0 < keys.to) request(u, j0, bits, buffer);
     }
     if (A.qmask && !there) clear();
     finish(u);
@@ -406,6 +420,7 @@ hipError_t attn_zero_gaps(int32_t dtype, void* out, const int32_t* cu, int64_t s
 
 int attn_chunk(const AttnArgs& a, int64_t pieces) {
   int chunk = 1;
+  if (a.kmask && a.tk > attn::kMaskSpan) return 1;
   for (int n = 2; n <= a.kv_heads && pieces / n >= 2048; ++n)
     if (a.kv_heads % n == 0) chunk = n;
   return chunk;

@@ -374,6 +374,8 @@ struct Rows {
   bool given;  // a mask (without one there is one span)
   int span0, to;
 
+  // Sets `to`: the rows end at `last`, or with the span.
+  __device__ __forceinline__ void end(int last) { to = given && last - span0 > kMaskSpan ? span0 + kMaskSpan : last; }
   // The mask bits of rows from span0 on, below n; keep(row): its mask has it.  All threads call it.
   template <int kThreads, class Keep>
   __device__ __forceinline__ void gather(int n, Keep&& keep) const {
@@ -404,56 +406,6 @@ __device__ __forceinline__ void landed() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
 }
-
-// The tiles of a workgroup, one after the other: of each of its `units` units (neighbouring key heads of a
-// sequence, alike in their masks), those of [first, last) that have rows.  While one is worked on the
-// next is on its way, across units too: the start of a short sequence's next head costs no wait.
-// gather(rows) fills the words from rows.span0 on; those of `first` are there when begin() is called.
-struct Walk {
-  Rows rows;
-  int first, last, units;
-  int u, at;       // the current tile: unit, first row
-  uint64_t bits;   // and its rows
-
-  template <class Gather>
-  __device__ __forceinline__ void move(int span0, Gather&& gather) {
-    landed();  // (every wave is through with the words)
-    rows.span0 = span0;
-    rows.to = last - span0 < kMaskSpan ? last : span0 + kMaskSpan;
-    gather(rows);
-    landed();
-  }
-  // False: there are none.
-  template <class Gather>
-  __device__ __forceinline__ bool begin(Gather&& gather) {
-    u = 0;
-    rows.to = rows.given && last - rows.span0 > kMaskSpan ? rows.span0 + kMaskSpan : last;
-    at = rows.next(first, bits);
-    while (at >= rows.to && rows.to < last) {
-      move(rows.span0 + kMaskSpan, gather);
-      at = rows.next(rows.span0, bits);
-    }
-    return at < rows.to;
-  }
-  // What comes after the current tile; its unit is `units` where nothing does.
-  template <class Gather>
-  __device__ __forceinline__ Walk next(Gather&& gather) const {
-    Walk w = *this;
-    w.at = w.rows.next(at + kRows, w.bits);
-    while (w.at >= w.rows.to) {
-      if (w.rows.to < last) {
-        w.move(w.rows.span0 + kMaskSpan, gather);
-        w.at = w.rows.next(w.rows.span0, w.bits);
-      } else {
-        if (++w.u == units) break;
-        const int span0 = first / kMaskSpan * kMaskSpan;
-        if (rows.given && w.rows.span0 != span0) w.move(span0, gather);
-        w.at = w.rows.next(first, w.bits);
-      }
-    }
-    return w;
-  }
-};
 
 // A lane's accumulators (values 32 b + 8 (r / 4) + 4 h + r % 4 of its row) times `by` to its row of `units` 16-byte
 // units, `at` bytes into the resource (kFar: nowhere).  All lanes of the wave call it.
