@@ -312,22 +312,24 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(E* to, const E* from, in
   }
 }
 
-// One wave a token row.
+// A thread a token row finds whether a sequence covers it; the wave clears those of its 64 that none does.
 template <class E>
 __global__ void __launch_bounds__(256) attn_gap_kernel(E* out, const int32_t* cu, int64_t seqs, int64_t rows,
                                                        int64_t most, int64_t width) {
-  const int64_t stride = (int64_t)gridDim.x * 4;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += stride) {
-    // the last sequence that starts at r or before
-    int64_t a = 0, e = seqs;  // cu[a] - 1 <= r < cu[e] - 1, as if cu[seqs] were past all
-    const bool before = seqs == 0 || r < (int64_t)cu[0] - 1;
-    while (!before && e - a > 1) {
+  const int64_t r0 = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63u), r = r0 + (threadIdx.x & 63);
+  bool gap = r < rows;
+  if (gap && seqs > 0 && r >= (int64_t)cu[0] - 1) {
+    int64_t a = 0, e = seqs;  // the last sequence that starts at r or before is in [a, e)
+    while (e - a > 1) {
       const int64_t mid = (a + e) / 2;
       if ((int64_t)cu[mid] - 1 <= r) a = mid;
       else e = mid;
     }
-    if (!before && r < (int64_t)cu[a + 1] - 1 && r - ((int64_t)cu[a] - 1) < most) continue;
-    for (int64_t i = threadIdx.x & 63; i < width; i += 64) out[r * width + i] = (E)0;
+    gap = !(r < (int64_t)cu[a + 1] - 1 && r - ((int64_t)cu[a] - 1) < most);
+  }
+  for (uint64_t left = __ballot(gap); left; left &= left - 1) {
+    E* const row = out + (r0 + __builtin_ctzll(left)) * width;
+    for (int64_t i = threadIdx.x & 63; i < width; i += 64) row[i] = (E)0;
   }
 }
 
@@ -375,7 +377,8 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
 
 template <class Op, int kD>
 hipError_t forward_dim(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {
-  if ((int64_t)a.tq * a.group <= 32) return forward_waves<Op, kD, 1>(a, out, stream);
+  const int64_t rows = (int64_t)a.tq * a.group;
+  if (rows <= 32) return forward_waves<Op, kD, 1>(a, out, stream);
   return forward_waves<Op, kD, 4>(a, out, stream);
 }
 
@@ -408,7 +411,7 @@ hipError_t attn_pack(int32_t dtype, void* to, const void* from, const int64_t* s
 hipError_t attn_zero_gaps(int32_t dtype, void* out, const int32_t* cu, int64_t seqs, int64_t rows, int64_t most,
                           int64_t width, hipStream_t stream) {
   if (rows == 0 || width == 0) return hipSuccess;
-  const int64_t blocks = attn::cdiv(rows, 4) < 8192 ? attn::cdiv(rows, 4) : 8192;
+  const int64_t blocks = attn::cdiv(rows, 256);
   if (dtype == FMS_F32)
     hipLaunchKernelGGL((attn::attn_gap_kernel<uint32_t>), dim3((unsigned)blocks), dim3(256), 0, stream,
                        static_cast<uint32_t*>(out), cu, seqs, rows, most, width);

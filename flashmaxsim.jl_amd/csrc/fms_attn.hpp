@@ -273,6 +273,10 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
   }
 }
 
+// What was asked for above stays above: reads are under way before the work that hides them.  (Left to itself the
+// compiler puts each fragment's read right before its product, which waits for it.)
+__device__ __forceinline__ void asked() { __builtin_amdgcn_sched_barrier(0); }
+
 template <class Op>
 struct Elem {
   typedef float T;

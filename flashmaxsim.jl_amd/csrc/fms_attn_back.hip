@@ -18,6 +18,7 @@
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
+#include "fms_group.hpp"
 
 namespace fms {
 namespace attn {
@@ -268,8 +269,11 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
                             h);
 }
 
+// `splits` workgroups share the rows of a tile of keys; with more than one their sums go to `parts`:
+// (split, dk or dv, unit, key, value).
 template <class Op, int kD, int kWaves>
-__global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnGrads G, uint32_t tiles, uint32_t work) {
+__global__ void __launch_bounds__(kWaves * 64, 1)
+    attn_dkv_kernel(AttnArgs A, AttnGrads G, float* parts, uint32_t splits, uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
   constexpr int kThreads = kWaves * 64;
   constexpr int kBuffer = 2 * T::kBytes + 2 * kRows * 4;  // q, do, lse, delta
@@ -277,8 +281,9 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   uint64_t* const words = reinterpret_cast<uint64_t*>(lds + 2 * kBuffer);
   const uint32_t piece = piece_of(work);
   if (piece >= work) return;
-  const uint32_t unit = piece / tiles;
-  const int tile = (int)(piece - unit * tiles);  // (under a causal mask the first tiles have the most rows)
+  const uint32_t shared = piece / splits, split = piece - shared * splits;
+  const uint32_t unit = shared / tiles;
+  const int tile = (int)(shared - unit * tiles);  // (under a causal mask the first tiles have the most rows)
   const int64_t b = unit / (uint32_t)A.kv_heads;
   const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
@@ -302,8 +307,14 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
     return r;
   };
   const Reach mine = reach(key);
-  const int first = reach(key0).lo / kRows * kRows;
-  const int last = reach(key0 + 32 * kWaves - 1).hi;
+  int first = reach(key0).lo / kRows * kRows;
+  int last = reach(key0 + 32 * kWaves - 1).hi;
+  if (splits > 1) {  // an equal share of the row tiles that this tile of keys reaches
+    const int64_t n = last > first ? (last - first + kRows - 1) / kRows : 0;
+    const int end = first + (int)(n * (split + 1) / splits) * kRows;
+    first += (int)(n * split / splits) * kRows;
+    last = end < last ? end : last;
+  }
   Rows rows = {words, A.qmask != nullptr, first / kMaskSpan * kMaskSpan, 0};
   const auto gather = [&] {
     const uint8_t* qm = A.qmask + b * A.tq;
@@ -316,11 +327,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   f32x16 dk[T::kBlocks], dv[T::kBlocks];
 #pragma unroll
   for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
-  if (!__syncthreads_or(there)) {  // padding: zeros, and no rows are read
-    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, 0.0f, A.units, h);
-    store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, 0.0f, A.units, h);
-    return;
-  }
+  if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no rows are read)
   const Reaches wide = reaches(reach(key0 + wave * 32), reach(key0 + wave * 32 + 31), __any(there));
   const float c = fabsf(A.scale) * kLog2e;
   if (A.scale < 0) negate<T>(k);
@@ -374,14 +381,38 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
       buffer ^= 1;
       if (none) continue;  // (no row here reaches this wave's keys)
       const bool whole_tile = (w[0] & w[1]) == 0xffffffffu && now >= wide.all.lo && now + kRows <= wide.all.hi;
+      // fragments: of the rows by values, and (two groups in turn) of the values by rows
+      // (wide 16-bit heads only, whose registers leave room for one wave of a SIMD: 1317 -> 1077 us for 8192 causal
+      // tokens, 16 heads on 4 of 128 in bf16; narrow ones have other waves to hide a read behind, 165 -> 180
+      // us for 48 ragged documents, 12 heads of 64 in fp16, and 32-bit ones no registers left)
+      constexpr bool kAhead = Op::kEsz == 2 && kD > 64;
+      u32x4 fq[T::kK], fd[T::kK], cq[2][T::kBlocks], cd[2][T::kBlocks];
+      const auto read_rows = [&](int half) {
+#pragma unroll
+        for (int kb = 0; kb < T::kK; ++kb) {
+          fq[kb] = T::rows(Q, 32 * half, kb, lane);
+          fd[kb] = T::rows(D, 32 * half, kb, lane);
+        }
+      };
+      constexpr int kPer = 32 / kGroups<Op>;
+      const auto read_columns = [&](int half, int g) {
+#pragma unroll
+        for (int i = 0; i < T::kBlocks; ++i) {
+          cd[g & 1][i] = T::columns(D, 32 * half + kPer * g, i, lane);
+          cq[g & 1][i] = T::columns(Q, 32 * half + kPer * g, i, lane);
+        }
+      };
+      if (kAhead) read_rows(0);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        if (kAhead) asked();
         f32x16 x = f32x16{}, y = f32x16{};
 #pragma unroll
         for (int kb = 0; kb < T::kK; ++kb) {
-          x = mma<Op>(T::rows(Q, 32 * half, kb, lane), k[kb], x);
-          y = mma<Op>(T::rows(D, 32 * half, kb, lane), v[kb], y);
+          x = mma<Op>(kAhead ? fq[kb] : T::rows(Q, 32 * half, kb, lane), k[kb], x);
+          y = mma<Op>(kAhead ? fd[kb] : T::rows(D, 32 * half, kb, lane), v[kb], y);
         }
+        if (kAhead) read_columns(half, 0);
         float p[16], ds[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -396,21 +427,23 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
         }
         if (!whole_tile) {
           const int r0h = now + 32 * half;
-          const uint32_t keep = (w[half] & bits_between(mine.lo - r0h, mine.hi - r0h)) >> (4 * h);
+          const uint32_t keep = ((half ? w[1] : w[0]) & bits_between(mine.lo - r0h, mine.hi - r0h)) >> (4 * h);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             p[r] = masked(p[r], keep, r, 0.0f);
             ds[r] = masked(ds[r], keep, r, 0.0f);
           }
         }
-        constexpr int kPer = 32 / kGroups<Op>;
+        if (kAhead && half == 0) read_rows(1);
 #pragma unroll
         for (int g = 0; g < kGroups<Op>; ++g) {
+          if (kAhead && g + 1 < kGroups<Op>) read_columns(half, g + 1);
+          if (kAhead) asked();
           const u32x4 po = operand<Op>(p, g), so = operand<Op>(ds, g);
 #pragma unroll
           for (int i = 0; i < T::kBlocks; ++i) {
-            dv[i] = mma<Op>(T::columns(D, 32 * half + kPer * g, i, lane), po, dv[i]);
-            dk[i] = mma<Op>(T::columns(Q, 32 * half + kPer * g, i, lane), so, dk[i]);
+            dv[i] = mma<Op>(kAhead ? cd[g & 1][i] : T::columns(D, 32 * half + kPer * g, i, lane), po, dv[i]);
+            dk[i] = mma<Op>(kAhead ? cq[g & 1][i] : T::columns(Q, 32 * half + kPer * g, i, lane), so, dk[i]);
           }
         }
       }
@@ -419,27 +452,103 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dkv_kernel(AttnArgs A, AttnG
   if (A.kmask && !there)
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, A.scale * kUnshift<Op> / by, A.units, h);
+  const float by_k = A.scale * kUnshift<Op> / by;
+  if (splits > 1) {
+    if (key >= S.nk) return;
+    const int64_t units = A.seqs * A.kv_heads;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float* const to = parts + (((int64_t)(split * 2 + which) * units + unit) * A.tk + key) * kD;
+      const float scale = which ? kUnshift<Op> : by_k;
+#pragma unroll
+      for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = (which ? dv[i][4 * g + e] : dk[i][4 * g + e]) * scale;
+          *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * h) = x;
+        }
+    }
+    return;
+  }
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dk, start, wkey, wide_row), at, dk, by_k, A.units, h);
   store_row<Op, T::kBlocks>(wave_rows<Op>(G.dv, start, wkey, wide_row), at, dv, kUnshift<Op>, A.units, h);
+}
+
+// The splits' sums of dk (blockIdx.y 0) and dv (1), four values a thread.
+template <class Op, int kD>
+__global__ void __launch_bounds__(256) attn_dkv_join_kernel(AttnArgs A, AttnGrads G, const float* parts, int splits) {
+  typedef typename Elem<Op>::T E;
+  typedef E V4 __attribute__((ext_vector_type(4)));
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / (kD / 4);  // (unit, key)
+  const int d = (int)(i % (kD / 4)) * 4, width = A.units * (16 / Op::kEsz);
+  const int64_t rows = A.seqs * A.kv_heads * A.tk;
+  const uint32_t unit = row / (uint32_t)A.tk, key = row - unit * (uint32_t)A.tk;
+  if (row >= rows || d >= width) return;
+  const int64_t b = unit / (uint32_t)A.kv_heads;
+  const int hk = (int)(unit % (uint32_t)A.kv_heads);
+  const Span S = span_of(A, b);
+  if ((int)key >= S.nk) return;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j = 0; j < splits; ++j) s += *reinterpret_cast<const f32x4*>(parts + ((j * 2 + blockIdx.y) * rows + row) * kD + d);
+  V4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = (E)s[e];
+  *reinterpret_cast<V4*>(static_cast<E*>(blockIdx.y ? G.dv : G.dk) + ((S.k0 + key) * A.kv_heads + hk) * width + d) = x;
+}
+
+// (Four waves a workgroup: two, where four leave CUs idle, gain nothing -- 16 sequences of 237 queries and 301 keys, 6
+// heads of 48 in fp32, dq 38 us with four and 41 with two, dk and dv 42 and 45.)
+constexpr int kWaves = 4;
+
+template <class Op, int kD>
+hipError_t launch_dq(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
+  const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), work = a.seqs * a.kv_heads * tiles;
+  if (work)
+    hipLaunchKernelGGL((attn_dq_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
+                       (uint32_t)tiles, (uint32_t)work);
+  return hipGetLastError();
+}
+
+template <class Op, int kD>
+hipError_t launch_dkv(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
+  const int64_t units = a.seqs * a.kv_heads;
+  const int64_t tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles;
+  if (!work) return hipGetLastError();
+  // Few workgroups of many rows each: the rows are shared out, eight tiles of them to a workgroup at
+  // least, until there are four workgroups to a CU.  (Their sums cost 2 * 4 bytes a value and split, twice;
+  // 8192 causal tokens, 16 heads on 4 of 128 in bf16: 1583 us unsplit, SPLITUS in four.)
+  int64_t splits = 1024 / work;
+  const int64_t most = cdiv((int64_t)a.tq * a.group, kRows) / 8;
+  if (splits > most) splits = most;
+  if (splits > 8) splits = 8;
+  if (splits <= 1) {
+    hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
+                       static_cast<float*>(nullptr), 1u, (uint32_t)tiles, (uint32_t)work);
+    return hipGetLastError();
+  }
+  void* mem;
+  const int64_t rows = units * a.tk;
+  hipError_t e = workspace_alloc(&mem, (size_t)(splits * 2 * rows * kD * 4), stream, true);
+  if (e != hipSuccess) return e;
+  float* const parts = static_cast<float*>(mem);
+  hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work * splits)), dim3(kWaves * 64), 0, stream,
+                     a, g, parts, (uint32_t)splits, (uint32_t)tiles, (uint32_t)(work * splits));
+  hipLaunchKernelGGL((attn_dkv_join_kernel<Op, kD>), dim3((unsigned)cdiv(rows * (kD / 4), 256), 2), dim3(256), 0, stream,
+                     a, g, static_cast<const float*>(parts), (int)splits);
+  e = hipGetLastError();
+  const hipError_t ef = workspace_free(mem, stream);
+  return e != hipSuccess ? e : ef;
 }
 
 template <class Op, int kD>
 hipError_t pullback_dim(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
-  constexpr int kWaves = 4;
   const int64_t units = a.seqs * a.kv_heads;
   if (std::is_same<Op, OpF16>::value)
     hipLaunchKernelGGL(attn_peaks_kernel, dim3((unsigned)(units * kAttnPeakParts)), dim3(256), 0, stream, a, g);
-  {
-    const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), work = units * tiles;
-    if (work)
-      hipLaunchKernelGGL((attn_dq_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a,
-                         g, (uint32_t)tiles, (uint32_t)work);
-  }
-  const int64_t tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles;
-  if (work)
-    hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
-                       (uint32_t)tiles, (uint32_t)work);
-  return hipGetLastError();
+  const hipError_t e = launch_dq<Op, kD>(a, g, stream);
+  return e != hipSuccess ? e : launch_dkv<Op, kD>(a, g, stream);
 }
 template <class Op>
 hipError_t pullback_op(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
