@@ -23,7 +23,7 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int kRun = 64;              // tokens of an id that one wave adds up
 constexpr int kMapBits = 1 << 18;     // tokens whose bits are held at a time
-constexpr int kHotThreads = 1024, kHotRows = 128;  // rows of dW that a workgroup looks through
+constexpr int kHotThreads = 1024, kHotBlocks = 64;  // workgroups (of sixteen units) that share the longer runs
 
 template <class T_, int kU_>
 struct Unit {
@@ -61,17 +61,24 @@ __global__ void __launch_bounds__(256) embed_forward_kernel(EmbedArgs A, typenam
   }
 }
 
-// A wave a row of dW: rows without tokens, and with at most kRun.
+__global__ void embed_zero_kernel(uint32_t* hots) { *hots = 0u; }
+
+// A wave a row of dW: rows without tokens, and with at most kRun.  The others are listed, in any order: a row's sum
+// is its own.
 template <class U>
 __global__ void __launch_bounds__(256) embed_rows_kernel(EmbedArgs A, typename U::T* dweight, const typename U::T* de,
-                                                         const PairRef* order, const uint32_t* ends, int units) {
+                                                         const PairRef* order, const uint32_t* ends, int units,
+                                                         uint32_t* hots, uint32_t* hot) {
   typedef typename U::T T;
   typedef typename U::V V;
   constexpr int kPer = 2, kAtOnce = 4;  // units a lane holds, tokens whose rows are read at once
   const int lane = threadIdx.x & 63;
   for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < A.vocabulary; v += (int64_t)gridDim.x * 4) {
     const uint32_t s = rfl32(v ? ends[v - 1] : 0u), run = rfl32(ends[v]) - s;
-    if (run > (uint32_t)kRun) continue;
+    if (run > (uint32_t)kRun) {
+      if (lane == 0) hot[atomicAdd(hots, 1u)] = (uint32_t)v;
+      continue;
+    }
     int token = 0;
     if (run > 0) token = order ? order[s + ((uint32_t)lane < run ? lane : 0)].p : 0;
     if (run > 1) {
@@ -115,35 +122,23 @@ __global__ void __launch_bounds__(256) embed_rows_kernel(EmbedArgs A, typename U
   }
 }
 
-// Rows of more than kRun tokens among kHotRows neighbouring ones; blockIdx.y: sixteen units of them.
+// The listed rows, sixteen units of them (blockIdx.y).
 template <class U>
 __global__ void __launch_bounds__(kHotThreads) embed_hot_kernel(EmbedArgs A, typename U::T* dweight,
                                                                 const typename U::T* de, const PairRef* order,
-                                                                const uint32_t* ends, int units) {
+                                                                const uint32_t* ends, int units, const uint32_t* hots,
+                                                                const uint32_t* hot) {
   typedef typename U::T T;
   typedef typename U::V V;
   __shared__ uint32_t map[kMapBits / 32];
   __shared__ float sums[64][16][U::kU];
-  __shared__ int hot[kHotRows], hots;
   const int tid = threadIdx.x;
-  const int64_t v0 = (int64_t)blockIdx.x * kHotRows;
-  if (tid < 64) {  // (one wave, so that the list is in order)
-    int before = 0;
-    for (int r = tid; r < kHotRows; r += 64) {
-      const int64_t v = v0 + r;
-      const bool is = v < A.vocabulary && ends[v] - (v ? ends[v - 1] : 0u) > (uint32_t)kRun;
-      const uint64_t all = __ballot(is);
-      if (is) hot[before + __popcll(all & ((1ull << tid) - 1))] = r;
-      before += __popcll(all);
-    }
-    if (tid == 0) hots = before;
-  }
-  __syncthreads();
   const int group = tid >> 4, lane = tid & 15;
   const int u = blockIdx.y * 16 + lane;
   const bool in = u < units;
-  for (int i = 0; i < hots; ++i) {
-    const int64_t v = v0 + hot[i];
+  const uint32_t n = *hots;
+  for (uint32_t i = blockIdx.x; i < n; i += kHotBlocks) {
+    const int64_t v = hot[i];
     const uint32_t s = v ? ends[v - 1] : 0u, e = ends[v];
     float acc[U::kU] = {};
     for (int64_t w0 = 0; w0 < A.n; w0 += kMapBits) {
@@ -156,26 +151,26 @@ __global__ void __launch_bounds__(kHotThreads) embed_hot_kernel(EmbedArgs A, typ
         if (p >= 0 && p < bits) atomicOr(&map[p / 32], 1u << (p & 31));
       }
       __syncthreads();
-      // this group's words, four tokens at a time
+      // this group's words, eight tokens at a time
       int w = (int)((int64_t)words * group / 64);
       const int end = (int)((int64_t)words * (group + 1) / 64);
       uint32_t left = w < end ? map[w] : 0u;
       while (w < end) {
-        int t[4];
+        int t[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
           while (left == 0u && w < end) left = ++w < end ? map[w] : 0u;
           t[j] = w < end ? w * 32 + __builtin_ctz(left) : -1;
           left &= left - 1;
         }
-        V x[4];
+        V x[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
           x[j] = V{};
           if (t[j] >= 0 && in) x[j] = *reinterpret_cast<const V*>(de + (w0 + t[j]) * A.dim + u * U::kU);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
           for (int k = 0; k < U::kU; ++k) acc[k] += (float)x[j][k];
       }
@@ -183,11 +178,20 @@ __global__ void __launch_bounds__(kHotThreads) embed_hot_kernel(EmbedArgs A, typ
 #pragma unroll
     for (int k = 0; k < U::kU; ++k) sums[group][lane][k] = acc[k];
     __syncthreads();
-    for (int k = tid; k < 16 * U::kU; k += kHotThreads) {
-      const int unit = blockIdx.y * 16 + k / U::kU;
+    // sixteen threads a value, four groups each, and then the sixteen
+    constexpr int kValues = 16 * U::kU;
+    for (int k = tid; k < kValues * 16; k += kHotThreads) {
+      const int value = k % kValues, part = k / kValues;
+      float* const s0 = &sums[part * 4][0][0] + value;
+      *s0 = (s0[0] + s0[kValues]) + (s0[2 * kValues] + s0[3 * kValues]);
+    }
+    __syncthreads();
+    if (tid < kValues) {
+      const int unit = blockIdx.y * 16 + tid / U::kU;
       float total = 0.0f;
-      for (int g = 0; g < 64; ++g) total += sums[g][k / U::kU][k % U::kU];
-      if (unit < units) dweight[v * A.dim + unit * U::kU + k % U::kU] = (T)(total * A.scale);
+#pragma unroll
+      for (int g = 0; g < 64; g += 4) total += (&sums[g][0][0])[tid];
+      if (unit < units) dweight[v * A.dim + unit * U::kU + tid % U::kU] = (T)(total * A.scale);
     }
     __syncthreads();
   }
@@ -222,8 +226,14 @@ hipError_t embed_forward(const EmbedArgs& a, void* e, const void* weight, hipStr
 
 hipError_t embed_pullback(const EmbedArgs& a, void* dweight, const void* de, hipStream_t stream) {
   void* mem = nullptr;
-  hipError_t e = workspace_alloc(&mem, group_workspace_bytes(a.n, a.vocabulary), stream, true);
+  // the sort's workspace, then the count and list of the longer runs
+  const size_t sort = (group_workspace_bytes(a.n, a.vocabulary) + 255) / 256 * 256;
+  hipError_t e = workspace_alloc(&mem, sort + 256 + (size_t)(a.n / (kRun + 1)) * 4, stream, true);
   if (e != hipSuccess) return e;
+  uint32_t* const hots = reinterpret_cast<uint32_t*>(static_cast<char*>(mem) + sort);
+  uint32_t* const hot = hots + 64;
+  const bool runs = a.n > kRun;
+  if (runs) hipLaunchKernelGGL(embed_zero_kernel, dim3(1), dim3(1), 0, stream, hots);
   const PairRef* order = nullptr;
   const uint32_t* ends = nullptr;
   e = group_pairs_by_document(a.ids, a.id_bytes == 8, a.n, a.vocabulary, mem, &order, &ends, stream);
@@ -233,11 +243,11 @@ hipError_t embed_pullback(const EmbedArgs& a, void* dweight, const void* de, hip
       typedef typename U::T T;
       const int64_t units = a.dim / U::kU, rows = cdiv(a.vocabulary, 4), most = 16384;
       hipLaunchKernelGGL((embed_rows_kernel<U>), dim3((unsigned)(rows < most ? rows : most)), dim3(256), 0, stream, a,
-                         static_cast<T*>(dweight), static_cast<const T*>(de), order, ends, (int)units);
-      if (a.n > kRun)
-        hipLaunchKernelGGL((embed_hot_kernel<U>), dim3((unsigned)cdiv(a.vocabulary, kHotRows), (unsigned)cdiv(units, 16)),
+                         static_cast<T*>(dweight), static_cast<const T*>(de), order, ends, (int)units, hots, hot);
+      if (runs)
+        hipLaunchKernelGGL((embed_hot_kernel<U>), dim3(kHotBlocks, (unsigned)cdiv(units, 16)),
                            dim3(kHotThreads), 0, stream, a, static_cast<T*>(dweight), static_cast<const T*>(de), order,
-                           ends, (int)units);
+                           ends, (int)units, static_cast<const uint32_t*>(hots), static_cast<const uint32_t*>(hot));
       return hipGetLastError();
     });
   const hipError_t ef = workspace_free(mem, stream);
