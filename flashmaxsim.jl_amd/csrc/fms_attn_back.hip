@@ -511,44 +511,42 @@ hipError_t launch_dq(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) 
   return hipGetLastError();
 }
 
+// Few workgroups of many rows each: the rows of a tile of keys are shared out, eight tiles of them to a
+// workgroup at least, until there are four workgroups to a CU.  (Their sums cost 2 * 4 bytes a value and
+// split, written and read; 8192 causal tokens, 16 heads on 4 of 128 in bf16, fragments read where they are
+// used: 1583 us unsplit, 1290 + 23 for the join in four.)
+int64_t dkv_splits(const AttnArgs& a) {
+  const int64_t work = a.seqs * a.kv_heads * cdiv(a.tk, 32 * kWaves);
+  const int64_t most = cdiv((int64_t)a.tq * a.group, kRows) / 8, wanted = work ? 1024 / work : 1;
+  const int64_t n = wanted < most ? wanted : most;
+  return n < 1 ? 1 : n > 8 ? 8 : n;
+}
+
 template <class Op, int kD>
-hipError_t launch_dkv(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
-  const int64_t units = a.seqs * a.kv_heads;
-  const int64_t tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles;
-  if (!work) return hipGetLastError();
-  // Few workgroups of many rows each: the rows are shared out, eight tiles of them to a workgroup at
-  // least, until there are four workgroups to a CU.  (Their sums cost 2 * 4 bytes a value and split, twice;
-  // 8192 causal tokens, 16 heads on 4 of 128 in bf16: 1583 us unsplit, SPLITUS in four.)
-  int64_t splits = 1024 / work;
-  const int64_t most = cdiv((int64_t)a.tq * a.group, kRows) / 8;
-  if (splits > most) splits = most;
-  if (splits > 8) splits = 8;
-  if (splits <= 1) {
-    hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
-                       static_cast<float*>(nullptr), 1u, (uint32_t)tiles, (uint32_t)work);
-    return hipGetLastError();
-  }
-  void* mem;
-  const int64_t rows = units * a.tk;
-  hipError_t e = workspace_alloc(&mem, (size_t)(splits * 2 * rows * kD * 4), stream, true);
-  if (e != hipSuccess) return e;
-  float* const parts = static_cast<float*>(mem);
-  hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work * splits)), dim3(kWaves * 64), 0, stream,
-                     a, g, parts, (uint32_t)splits, (uint32_t)tiles, (uint32_t)(work * splits));
-  hipLaunchKernelGGL((attn_dkv_join_kernel<Op, kD>), dim3((unsigned)cdiv(rows * (kD / 4), 256), 2), dim3(256), 0, stream,
-                     a, g, static_cast<const float*>(parts), (int)splits);
-  e = hipGetLastError();
-  const hipError_t ef = workspace_free(mem, stream);
-  return e != hipSuccess ? e : ef;
+hipError_t launch_dkv(const AttnArgs& a, const AttnGrads& g, float* parts, int64_t splits, hipStream_t stream) {
+  const int64_t units = a.seqs * a.kv_heads, tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles * splits;
+  if (!work) return hipSuccess;
+  hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
+                     parts, (uint32_t)splits, (uint32_t)tiles, (uint32_t)work);
+  if (splits > 1)
+    hipLaunchKernelGGL((attn_dkv_join_kernel<Op, kD>), dim3((unsigned)cdiv(units * a.tk * (kD / 4), 256), 2), dim3(256),
+                       0, stream, a, g, static_cast<const float*>(parts), (int)splits);
+  return hipGetLastError();
 }
 
 template <class Op, int kD>
 hipError_t pullback_dim(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
-  const int64_t units = a.seqs * a.kv_heads;
+  const int64_t units = a.seqs * a.kv_heads, splits = dkv_splits(a);
+  void* parts = nullptr;  // (before anything is launched: a captured call without workspace adds nothing)
+  hipError_t e = hipSuccess;
+  if (splits > 1) e = workspace_alloc(&parts, (size_t)(splits * 2 * units * a.tk * kD * 4), stream, true);
+  if (e != hipSuccess) return e;
   if (std::is_same<Op, OpF16>::value)
     hipLaunchKernelGGL(attn_peaks_kernel, dim3((unsigned)(units * kAttnPeakParts)), dim3(256), 0, stream, a, g);
-  const hipError_t e = launch_dq<Op, kD>(a, g, stream);
-  return e != hipSuccess ? e : launch_dkv<Op, kD>(a, g, stream);
+  e = launch_dq<Op, kD>(a, g, stream);
+  if (e == hipSuccess) e = launch_dkv<Op, kD>(a, g, static_cast<float*>(parts), splits, stream);
+  const hipError_t ef = parts ? workspace_free(parts, stream) : hipSuccess;
+  return e != hipSuccess ? e : ef;
 }
 template <class Op>
 hipError_t pullback_op(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {

@@ -35,7 +35,8 @@
 # extension module: packed_multi_scan (nq queries against one PackedSeq in
 # one pass), topk (the k best scores of every query column),
 # load_int8_index (an Int8Index read from its at-rest file), and the operators
-# of a token block: gated_ffn, gated_ffn_pullback, block_norm, block_norm_pullback.
+# of a token block and of an encoder's layers around it: gated_ffn, block_norm,
+# embed_tokens, head_rotary and attention, each with its *_pullback, and rotary_table.
 #
 # Score buffers.  Every scan entry point writes Float32 partials and scores.
 # The reference allocates them as dot_accum(T) / score_eltype(T)
@@ -798,6 +799,222 @@ function block_norm_pullback(dr::MaybeArray{T}, dn::MaybeArray{T}, x::ROCArray{T
                 stream_ptr()),
           "block norm pullback")
     dx, df, dgate, dwpost, dwpre
+end
+
+# ---- encoder -----------------------------------------------------------------------
+# What turns token ids into the states that the token block takes.  The heads of a token lie
+# side by side: q (dim, heads, T, B) or (dim, heads, T).
+
+const MaybePositions = Union{ROCArray{Int32}, ROCArray{Int64}, Nothing}
+const TokenIds = Union{ROCArray{Int32}, ROCArray{Int64}}
+const MaybeCu = Union{ROCVector{Int32}, Nothing}
+const PAIRINGS = Dict(:halves => Int32(0), :neighbours => Int32(1))
+id_bytes_of(x) = x === nothing ? Int32(4) : Int32(sizeof(eltype(x)))
+
+"""
+    embed_tokens(ids, weight; scale = 1) -> e (dim, size(ids)...)
+
+`scale .* weight[:, ids]`; an id outside `1:size(weight, 2)` (0, say, for padding) gives zeros.
+"""
+function embed_tokens(ids::TokenIds, weight::ROCMatrix{T}; scale = 1) where {T<:AnyFeature}
+    require_gfx950("token lookup")
+    dim, vocabulary = size(weight)
+    e = similar(weight, dim, size(ids)...)
+    check(ccall((:fms_embed_tokens, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Ptr{Cvoid}, Float32, Int64, Int64, Int64,
+                 Ptr{Cvoid}),
+                dtype_code(T), dptr(e), dptr(ids), id_bytes_of(ids), dptr(weight), Float32(scale),
+                length(ids), vocabulary, dim, stream_ptr()),
+          "token lookup")
+    e
+end
+
+"""
+    embed_tokens_pullback(de, ids, vocabulary; scale = 1) -> dweight (dim, vocabulary)
+"""
+function embed_tokens_pullback(de::ROCArray{T}, ids::TokenIds, vocabulary::Integer;
+                               scale = 1) where {T<:AnyFeature}
+    require_gfx950("token lookup pullback")
+    size(de)[2:end] == size(ids) || throw(DimensionMismatch("de"))
+    dim = size(de, 1)
+    dweight = similar(de, dim, vocabulary)
+    check(ccall((:fms_embed_tokens_pullback, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Float32, Int64, Int64, Int64,
+                 Ptr{Cvoid}),
+                dtype_code(T), dptr(dweight), dptr(de), dptr(ids), id_bytes_of(ids), Float32(scale),
+                length(ids), vocabulary, dim, stream_ptr()),
+          "token lookup pullback")
+    dweight
+end
+
+"""
+    rotary_table(positions, turned; base = 10000) -> (turned, positions) Float32
+
+For `head_rotary`: column p has the cosines and then the sines of (p - 1) base^(-2 i / turned),
+i = 0 ... turned / 2 - 1, their angles computed in 64 bits.
+"""
+function rotary_table(positions::Integer, turned::Integer; base = 10000)
+    iseven(turned) || throw(ArgumentError("turned must be even"))
+    angle = [(p - 1) * Float64(base)^(-2 * i / turned) for i in 0:(turned ÷ 2 - 1), p in 1:positions]
+    ROCArray(Float32.(vcat(cos.(angle), sin.(angle))))
+end
+
+# The sizes that both calls take: sequences, tokens, heads of q and k, a head's values, what is turned, the table's rows.
+function rotary_sizes(q, k, table, positions, wq, wk)
+    ndims(q) in (3, 4) || throw(DimensionMismatch("q must be (dim, heads, T) or (dim, heads, T, B)"))
+    dim, heads, tokens = size(q, 1), size(q, 2), size(q, 3)
+    k === nothing || (size(k, 1) == dim && size(k)[3:end] == size(q)[3:end]) ||
+        throw(DimensionMismatch("k must have q's tokens and dim"))
+    turned, table_rows = size(table)
+    (iseven(dim) && iseven(turned) && turned <= dim) || throw(DimensionMismatch("dim and turned"))
+    positions === nothing ? (table_rows >= tokens || turned == 0 || throw(DimensionMismatch("table"))) :
+        (size(positions) == size(q)[3:end] || size(positions) == (tokens,) ||
+         throw(DimensionMismatch("positions")))
+    for w in (wq, wk)
+        w === nothing || length(w) == dim || throw(DimensionMismatch("norm weights"))
+    end
+    seqs = size(q, 4)
+    placed = positions !== nothing && ndims(positions) == 2 ? seqs : 1
+    seqs, tokens, heads, k === nothing ? 0 : size(k, 2), dim, turned, table_rows, placed
+end
+
+"""
+    head_rotary(q, k, table, positions = nothing; wq, wk, kind = :rms, pairing = :halves, eps = 1f-6)
+        -> (q, k)
+
+Each head normed over its values (`kind` :rms or :layer; only with its weight) and rotated by its token's
+position, in one pass.  `positions` are 1-based columns of the table, (T,) or (T, B); token t takes column
+t without them; one that is none of the table's gives zeros.  `k` may be nothing.
+"""
+function head_rotary(q::ROCArray{T}, k::MaybeArray{T}, table::ROCMatrix{Float32},
+                     positions::MaybePositions = nothing; wq::MaybeVector{T} = nothing,
+                     wk::MaybeVector{T} = nothing, kind::Symbol = :rms, pairing::Symbol = :halves,
+                     eps = 1.0f-6) where {T<:AnyFeature}
+    require_gfx950("head rotary")
+    seqs, tokens, heads, kv_heads, dim, turned, table_rows, placed =
+        rotary_sizes(q, k, table, positions, wq, wk)
+    q_out, k_out = similar(q), k === nothing ? nothing : similar(k)
+    check(ccall((:fms_head_rotary, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Int32, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int32, Float32, Int64, Int64,
+                 Int64, Int64, Int64, Int64, Int64, Ptr{Cvoid}),
+                dtype_code(T), dptr(q_out), dptr(k_out), dptr(q), dptr(k), C_NULL, dptr(table),
+                dptr(positions), id_bytes_of(positions), placed, dptr(wq), dptr(wk),
+                named(NORMS, kind, "norm"), named(PAIRINGS, pairing, "pairing"), Float32(eps), seqs,
+                tokens, heads, kv_heads, dim, turned, table_rows, stream_ptr()),
+          "head rotary")
+    q_out, k_out
+end
+
+"""
+    head_rotary_pullback(dq_out, dk_out, q, k, table, positions = nothing; ...) -> (dq, dk, dwq, dwk)
+"""
+function head_rotary_pullback(dq_out::ROCArray{T}, dk_out::MaybeArray{T}, q::ROCArray{T},
+                              k::MaybeArray{T}, table::ROCMatrix{Float32},
+                              positions::MaybePositions = nothing; wq::MaybeVector{T} = nothing,
+                              wk::MaybeVector{T} = nothing, kind::Symbol = :rms,
+                              pairing::Symbol = :halves, eps = 1.0f-6) where {T<:AnyFeature}
+    require_gfx950("head rotary pullback")
+    seqs, tokens, heads, kv_heads, dim, turned, table_rows, placed =
+        rotary_sizes(q, k, table, positions, wq, wk)
+    same_size(dq_out, q, "dq_out")
+    (k === nothing) == (dk_out === nothing) || throw(DimensionMismatch("dk_out"))
+    k === nothing || same_size(dk_out, k, "dk_out")
+    like(a) = a === nothing ? nothing : similar(a)
+    dq, dk, dwq, dwk = similar(q), like(k), like(wq), like(wk)
+    check(ccall((:fms_head_rotary_pullback, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int32, Int64, Ptr{Cvoid},
+                 Ptr{Cvoid}, Int32, Int32, Float32, Int64, Int64, Int64, Int64, Int64, Int64, Int64,
+                 Ptr{Cvoid}),
+                dtype_code(T), dptr(dq), dptr(dk), dptr(dwq), dptr(dwk), dptr(dq_out), dptr(dk_out),
+                dptr(q), dptr(k), C_NULL, dptr(table), dptr(positions), id_bytes_of(positions), placed,
+                dptr(wq), dptr(wk), named(NORMS, kind, "norm"), named(PAIRINGS, pairing, "pairing"),
+                Float32(eps), seqs, tokens, heads, kv_heads, dim, turned, table_rows, stream_ptr()),
+          "head rotary pullback")
+    dq, dk, dwq, dwk
+end
+
+# Sequences, their most tokens, all token rows, heads and values of an attention call.
+function attention_sizes(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
+    same_size(k, v, "k and v")
+    ndims(q) == ndims(k) && ndims(q) in (3, 4) && size(q, 1) == size(k, 1) && size(q, 4) == size(k, 4) ||
+        throw(DimensionMismatch("q must be (dim, heads, T) or (dim, heads, T, B), k and v alike"))
+    heads, kv_heads, nq, nk = size(q, 2), size(k, 2), size(q, 3), size(k, 3)
+    heads == kv_heads || (kv_heads > 0 && heads % kv_heads == 0) || throw(DimensionMismatch("heads"))
+    (cu_q === nothing) == (cu_k === nothing) || throw(ArgumentError("cu_q and cu_k go together"))
+    if cu_q === nothing
+        qmask === nothing || length(qmask) == nq * size(q, 4) || throw(DimensionMismatch("qmask"))
+        kmask === nothing || length(kmask) == nk * size(k, 4) || throw(DimensionMismatch("kmask"))
+        return size(q, 4), nq, nk, nq, nk, heads, kv_heads, size(q, 1)
+    end
+    ndims(q) == 3 && qmask === nothing && kmask === nothing && length(cu_q) == length(cu_k) >= 1 ||
+        throw(DimensionMismatch("ragged attention takes token rows, two cu and no masks"))
+    length(cu_q) - 1, something(max_q, nq), something(max_k, nk), nq, nk, heads, kv_heads, size(q, 1)
+end
+
+"""
+    attention(q, k, v, qmask = nothing, kmask = nothing; cu_q, cu_k, max_q, max_k, causal = false,
+              window = -1, scale = dim^-0.5, keep = false) -> o, or (o, (lse, rest)) with `keep`
+
+`softmax(scale q'k) v` over heads; q (dim, heads, T, B), k and v with as many or fewer heads, masks (T, B).
+Ragged sequences: token rows (dim, heads, N) with `PackedSeq`'s 1-based `cu`.  A query sees keys that
+are not behind it (`causal`) and at most `window` tokens away (-1: any); one that sees none gives zeros.
+"""
+function attention(q::ROCArray{T}, k::ROCArray{T}, v::ROCArray{T},
+                   qmask::Union{ROCArray{Bool}, Nothing} = nothing,
+                   kmask::Union{ROCArray{Bool}, Nothing} = nothing; cu_q::MaybeCu = nothing,
+                   cu_k::MaybeCu = nothing, max_q = nothing, max_k = nothing, causal::Bool = false,
+                   window::Integer = -1, scale = nothing, keep::Bool = false) where {T<:AnyFeature}
+    require_gfx950("attention")
+    seqs, tq, tk, nq, nk, heads, kv_heads, dim =
+        attention_sizes(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
+    o = similar(q)
+    lse = keep ? similar(q, Float32, size(q)[2:end]) : nothing
+    rest = keep && T !== Float32 ? similar(q) : nothing
+    check(ccall((:fms_attention, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64,
+                 Int64, Int64, Int64, Int64, Float32, Int32, Int64, Ptr{Cvoid}),
+                dtype_code(T), dptr(o), dptr(lse), dptr(rest), dptr(q), dptr(k), dptr(v), C_NULL,
+                dptr(qmask), dptr(kmask), dptr(cu_q), dptr(cu_k), seqs, tq, tk, nq, nk, heads, kv_heads,
+                dim, Float32(something(scale, max(dim, 1)^-0.5)), Int32(causal), window, stream_ptr()),
+          "attention")
+    keep ? (o, (lse, rest)) : o
+end
+
+"""
+    attention_pullback(dout, q, k, v, o, kept, qmask = nothing, kmask = nothing; ...) -> (dq, dk, dv)
+
+`o` and `kept` are what `attention(...; keep = true)` gave for the same arguments.
+"""
+function attention_pullback(dout::ROCArray{T}, q::ROCArray{T}, k::ROCArray{T}, v::ROCArray{T},
+                            o::ROCArray{T}, kept::Tuple,
+                            qmask::Union{ROCArray{Bool}, Nothing} = nothing,
+                            kmask::Union{ROCArray{Bool}, Nothing} = nothing; cu_q::MaybeCu = nothing,
+                            cu_k::MaybeCu = nothing, max_q = nothing, max_k = nothing,
+                            causal::Bool = false, window::Integer = -1,
+                            scale = nothing) where {T<:AnyFeature}
+    require_gfx950("attention pullback")
+    seqs, tq, tk, nq, nk, heads, kv_heads, dim =
+        attention_sizes(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
+    same_size(dout, q, "dout")
+    same_size(o, q, "o")
+    lse, rest = kept
+    length(lse) == length(q) ÷ max(dim, 1) || throw(DimensionMismatch("lse"))
+    T === Float32 || same_size(rest, q, "rest")
+    dq, dk, dv = similar(q), similar(k), similar(v)
+    check(ccall((:fms_attention_pullback, libfms), Int32,
+                (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Float32,
+                 Int32, Int64, Ptr{Cvoid}),
+                dtype_code(T), dptr(dq), dptr(dk), dptr(dv), dptr(dout), dptr(o), dptr(lse), dptr(rest),
+                dptr(q), dptr(k), dptr(v), C_NULL, dptr(qmask), dptr(kmask), dptr(cu_q), dptr(cu_k),
+                seqs, tq, tk, nq, nk, heads, kv_heads, dim,
+                Float32(something(scale, max(dim, 1)^-0.5)), Int32(causal), window, stream_ptr()),
+          "attention pullback")
+    dq, dk, dv
 end
 
 # ---- Int8Index at rest -------------------------------------------------------------
