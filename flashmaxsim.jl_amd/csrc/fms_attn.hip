@@ -4,11 +4,9 @@
 // over the keys j that count for row i (masks, causal, window); 0 where none does.
 //
 // One pass over the keys: a running maximum m and sum l per row, and what was summed so far
-// rescaled where m grows.  Scores, m, l and the sums of values are fp32; p is rounded once to
-// the feature type for its product with v, which costs about what rounding o costs, and l is the
-// sum of the p as rounded: o is then a mean of the values with weights that are a little off, and the
-// pullback's delta, do . o, is off by no more than those weights' share of ds.  (p is at most 1
-// and exactly 1 at the maximum, so a row that attends to one key is exact.)
+// rescaled where m grows.  Scores, p, m, l and the sums of values are fp32; in 16-bit types p goes
+// into its product with v as two values, a rounding and what it left.  (p is at most 1 and exactly 1
+// at the maximum.)
 #include <cmath>
 
 #include "fms_attn.hpp"
@@ -161,80 +159,83 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
     int j0 = j00;
     uint64_t bits = bits0;
     for (;;) {
-    while (j0 < keys.to) {
-      landed();
-      uint64_t bits1;
-      const int j1 = keys.next(j0 + kRows, bits1);
-      const bool same = j1 < keys.to;
-      if (same || u + 1 < chunk) request(same ? u : u + 1, same ? j1 : j00, same ? bits1 : bits0, buffer ^ 1);
-      const char* const K = lds + buffer * 2 * T::kBytes;
-      const char* const V = K + T::kBytes;
-      const int now = j0;
-      const uint64_t in = bits;
-      j0 = j1;
-      bits = bits1;
-      buffer ^= 1;
-      if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
-      float s[2][16];
+      while (j0 < keys.to) {
+        landed();
+        uint64_t bits1;
+        const int j1 = keys.next(j0 + kRows, bits1);
+        const bool same = j1 < keys.to;
+        if (same || u + 1 < chunk) request(same ? u : u + 1, same ? j1 : j00, same ? bits1 : bits0, buffer ^ 1);
+        const char* const K = lds + buffer * 2 * T::kBytes;
+        const char* const V = K + T::kBytes;
+        const int now = j0;
+        const uint64_t in = bits;
+        j0 = j1;
+        bits = bits1;
+        buffer ^= 1;
+        if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
+        float s[2][16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        f32x16 x = f32x16{};
+        for (int half = 0; half < 2; ++half) {
+          f32x16 x = f32x16{};
 #pragma unroll
-        for (int kb = 0; kb < T::kK; ++kb) x = mma<Op>(T::rows(K, 32 * half, kb, lane), q[kb], x);
+          for (int kb = 0; kb < T::kK; ++kb) x = mma<Op>(T::rows(K, 32 * half, kb, lane), q[kb], x);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[half][r] = x[r];
-      }
-      const bool whole_tile = in == ~0ull && now >= wide.all.lo && now + kRows <= wide.all.hi;
-      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-      if (!whole_tile) {
-        keep[0] = ((uint32_t)in & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
-        keep[1] = ((uint32_t)(in >> 32) & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
+          for (int r = 0; r < 16; ++r) s[half][r] = x[r];
+        }
+        const bool whole_tile = in == ~0ull && now >= wide.all.lo && now + kRows <= wide.all.hi;
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        if (!whole_tile) {
+          keep[0] = ((uint32_t)in & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
+          keep[1] = ((uint32_t)(in >> 32) & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[half][r] = masked(s[half][r], keep[half], r, -INFINITY);
+        }
+        // (NaN scores are ignored here and make p, and with it the row, NaN)
+        float top = m;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[half][r] = masked(s[half][r], keep[half], r, -INFINITY);
-      }
-      // (NaN scores are ignored here and make p, and with it the row, NaN)
-      float top = m;
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) top = max3_ieee(s[half][r], s[half][r + 1], top);
-      top = merge_halves_max(top);
-      if (__any(top > m)) {
-        const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
-        l *= by;
-#pragma unroll
-        for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][r] *= by;
-        m = top;
-      }
-      const float base = m == -INFINITY ? 0.0f : m, off = kShift<Op> - base * c;
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          // (fp32: exactly 1 at the maximum; where p is rounded to 16 bits the cheaper form is that, too)
-          if constexpr (Op::kEsz == 4)
-            s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
-          else
-            s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
-        }
-      float sum[2] = {0.0f, 0.0f};
-      constexpr int kPer = 32 / kGroups<Op>;
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int g = 0; g < kGroups<Op>; ++g) {
-          const u32x4 p = operand<Op>(s[half], g);
-          sum[half] = add_operand<Op>(p, sum[half]);
+          for (int r = 0; r < 16; r += 2) top = max3_ieee(s[half][r], s[half][r + 1], top);
+        top = merge_halves_max(top);
+        if (__any(top > m)) {
+          const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
+          l *= by;
 #pragma unroll
           for (int i = 0; i < T::kBlocks; ++i)
-            acc[i] = mma<Op>(T::columns(V, 32 * half + kPer * g, i, lane), p, acc[i]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][r] *= by;
+          m = top;
         }
-      l += sum[0] + sum[1];
-    }
+        const float base = m == -INFINITY ? 0.0f : m, off = kShift<Op> - base * c;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            // (fp32: exactly 1 at the maximum; where p is rounded to 16 bits the cheaper form is that, too)
+            if constexpr (Op::kEsz == 4)
+              s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
+            else
+              s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
+          }
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum[half] += s[half][r];
+        l += sum[0] + sum[1];
+        constexpr int kPer = 32 / kGroups<Op>;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int g = 0; g < kGroups<Op>; ++g) {
+            const Operand<Op> p = operand<Op>(s[half], g);
+#pragma unroll
+            for (int i = 0; i < T::kBlocks; ++i)
+              acc[i] = mma(T::columns(V, 32 * half + kPer * g, i, lane), p, acc[i]);
+          }
+      }
       if (keys.to >= last) break;
       landed();  // (every wave is through with the words, and with the buffers)
       keys.span0 += kMaskSpan;

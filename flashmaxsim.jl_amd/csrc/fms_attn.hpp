@@ -257,9 +257,10 @@ struct Tile {
   }
 };
 
-// Waves of a SIMD that the registers should leave room for: as many as the LDS does.
+// Waves of a SIMD that the forward's registers should leave room for: as many as the LDS does, or one less where it
+// would have to spill some (64 values in 16 bits: 56 us against 84 for 128 x 180 tokens of 16 heads).
 template <class Op, int kD, int kWaves>
-constexpr int kSimdWaves = kWaves < 4 ? 1 : kD * Op::kEsz <= 128 ? 4 : kD * Op::kEsz <= 256 ? 2 : 1;
+constexpr int kSimdWaves = kWaves < 4 ? 1 : kD * Op::kEsz <= 128 ? 3 : kD * Op::kEsz <= 256 ? 2 : 1;
 
 template <class Op>
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
@@ -295,46 +296,38 @@ template <class Op>
 constexpr float kRestScale = std::is_same<Op, OpF16>::value ? 2048.0f : 1.0f;
 
 // Registers 8 j .. 8 j + 7 (16-bit; 4 j .. 4 j + 3 in 32 bits) of a lane's values as the second
-// operand of the product that `columns` feeds.  16-bit: rounded once, here.
+// operand of the product that `columns` feeds.  16-bit: two values for each, a rounding and what it left, so that a
+// product's terms have twice the feature type's bits: with the rounding alone the sums would be 1.4 times as far
+// off as their own rounding takes them, and more where a few terms make them up.
 template <class Op>
-__device__ __forceinline__ u32x4 operand(const float (&v)[16], int j) {
+struct Operand {
+  u32x4 hi, lo;
+};
+template <class Op>
+__device__ __forceinline__ Operand<Op> operand(const float (&v)[16], int j) {
+  Operand<Op> x;
   if constexpr (Op::kEsz == 4) {
-    return u32x4{__builtin_bit_cast(uint32_t, v[4 * j]), __builtin_bit_cast(uint32_t, v[4 * j + 1]),
-                 __builtin_bit_cast(uint32_t, v[4 * j + 2]), __builtin_bit_cast(uint32_t, v[4 * j + 3])};
+    x.hi = __builtin_bit_cast(u32x4, f32x4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]});
   } else {
     typedef typename Elem<Op>::T T;
     typedef T V __attribute__((ext_vector_type(8)));
-    V x;
+    V hi, lo;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (T)v[8 * j + e];
-    return __builtin_bit_cast(u32x4, x);
+    for (int e = 0; e < 8; ++e) hi[e] = (T)v[8 * j + e];
+    x.hi = __builtin_bit_cast(u32x4, hi);
+    asm volatile("" : "+v"(x.hi));  // (settled: what it left is of these bits, however they were rounded)
+    hi = __builtin_bit_cast(V, x.hi);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = (T)(v[8 * j + e] - (float)hi[e]);
+    x.lo = __builtin_bit_cast(u32x4, lo);
   }
+  return x;
 }
-// c plus the sum of such an operand's values (as rounded).
 template <class Op>
-__device__ __forceinline__ float add_operand(const u32x4& p, float c) {
-  if constexpr (Op::kEsz == 4) {
-    const f32x4 v = __builtin_bit_cast(f32x4, p);
-    return c + ((v[0] + v[1]) + (v[2] + v[3]));
-  } else {
-    // (pairs are taken from the vector of values: out of the words, this compiler takes the first
-    // word four times)
-    typedef typename Elem<Op>::T T;
-    typedef T V8 __attribute__((ext_vector_type(8)));
-    typedef T V2 __attribute__((ext_vector_type(2)));
-    const V8 v = __builtin_bit_cast(V8, p);
-    const V2 one = {(T)1.0f, (T)1.0f};
-    const V2 pair[4] = {__builtin_shufflevector(v, v, 0, 1), __builtin_shufflevector(v, v, 2, 3),
-                        __builtin_shufflevector(v, v, 4, 5), __builtin_shufflevector(v, v, 6, 7)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<Op, OpF16>::value)
-        c = __builtin_amdgcn_fdot2(pair[i], one, c, false);
-      else
-        c = __builtin_amdgcn_fdot2_f32_bf16(pair[i], one, c, false);
-    }
-    return c;
-  }
+__device__ __forceinline__ f32x16 mma(u32x4 a, const Operand<Op>& b, f32x16 acc) {
+  acc = mma<Op>(a, b.hi, acc);
+  if constexpr (Op::kEsz == 2) acc = mma<Op>(a, b.lo, acc);
+  return acc;
 }
 template <class Op>
 constexpr int kGroups = Op::kEsz == 4 ? 4 : 2;  // operands of 32 rows

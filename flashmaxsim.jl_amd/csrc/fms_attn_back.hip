@@ -11,10 +11,10 @@
 // memory; the heads that share a key head are rows of one run, so their sums are one too.
 //
 // delta takes o with what its rounding left (the forward keeps that): where one key has nearly all
-// the weight, dp - delta is a small difference of nearly equal terms.  p and ds are rounded once
-// to the feature type for their products, which costs about what rounding the results costs.
-// In fp16 both are scaled by powers of two: p by 2^15, dp - delta by a bound of its size from the
-// norms of do and v, so that neither small probabilities nor small cotangents lose their bits.
+// the weight, dp - delta is a small difference of nearly equal terms.  In 16-bit types p and ds go into their
+// products as two values each, a rounding and what it left, and in fp16 both are scaled by powers of
+// two: p by 2^15, dp - delta by a bound of its size from the norms of do and v, so that neither small
+// probabilities nor small cotangents lose their bits.
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
@@ -254,10 +254,10 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
         constexpr int kPer = 32 / kGroups<Op>;
 #pragma unroll
         for (int g = 0; g < kGroups<Op>; ++g) {
-          const u32x4 ds = operand<Op>(s, g);
+          const Operand<Op> ds = operand<Op>(s, g);
 #pragma unroll
           for (int i = 0; i < T::kBlocks; ++i)
-            acc[i] = mma<Op>(T::columns(K, 32 * half + kPer * g, i, lane), ds, acc[i]);
+            acc[i] = mma(T::columns(K, 32 * half + kPer * g, i, lane), ds, acc[i]);
         }
       }
     }
@@ -439,11 +439,11 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
         for (int g = 0; g < kGroups<Op>; ++g) {
           if (kAhead && g + 1 < kGroups<Op>) read_columns(half, g + 1);
           if (kAhead) asked();
-          const u32x4 po = operand<Op>(p, g), so = operand<Op>(ds, g);
+          const Operand<Op> po = operand<Op>(p, g), so = operand<Op>(ds, g);
 #pragma unroll
           for (int i = 0; i < T::kBlocks; ++i) {
-            dv[i] = mma<Op>(kAhead ? cd[g & 1][i] : T::columns(D, 32 * half + kPer * g, i, lane), po, dv[i]);
-            dk[i] = mma<Op>(kAhead ? cq[g & 1][i] : T::columns(Q, 32 * half + kPer * g, i, lane), so, dk[i]);
+            dv[i] = mma(kAhead ? cd[g & 1][i] : T::columns(D, 32 * half + kPer * g, i, lane), po, dv[i]);
+            dk[i] = mma(kAhead ? cq[g & 1][i] : T::columns(Q, 32 * half + kPer * g, i, lane), so, dk[i]);
           }
         }
       }

@@ -43,8 +43,9 @@ def reference(q, k, v, keep, scale, do=None):
     size = (abs(scale) * (Q.abs() @ K.abs().transpose(1, 2).contiguous())).masked_fill(~keep, 0.0)
     rows = size.amax(-1, keepdim=True)
     off = unit * ((d + 4) * rows + 16) * 2 + unit * (nk + 64)
-    # p in its product: rounded to the feature type; small fp16 ones on a grid of 2^-24, scaled by 2^10 or more
-    rough = half if q.dtype != torch.float32 else 0.0
+    # p in its product: in 16 bits a rounding and what it left, itself rounded; small fp16 ones on a grid of 2^-24,
+    # scaled by 2^10 or more
+    rough = half * half if q.dtype != torch.float32 else 0.0
     grid = 2.0 ** -35 if q.dtype == torch.float16 else 0.0
     o = p @ V
     mass = p @ V.abs()
@@ -55,12 +56,12 @@ def reference(q, k, v, keep, scale, do=None):
         dp = D @ V.transpose(1, 2).contiguous()
         delta = (p * dp).sum(-1, keepdim=True)
         ds = p * (dp - delta)
-        # dp and delta are fp32 sums; delta's o has what its rounding left, to the square of the rounding,
-        # and the rounding of its p: half a step of each p's share of delta, which is its ds
+        # dp and delta are fp32 sums; delta's o has what its rounding left, to the square of the rounding, and the
+        # error of its p
         dp_size = D.abs() @ V.abs().transpose(1, 2).contiguous()
         delta_size = (p * dp_size).sum(-1, keepdim=True)
         delta_off = ((unit * (d + nk + 64) + 4 * half * half) * delta_size + off * delta_size
-                     + rough * 1.01 * ds.abs().sum(-1, keepdim=True)
+                     + rough * 1.01 * delta_size
                      + grid * dp_size.sum(-1, keepdim=True))
         if q.dtype == torch.float32:
             delta_off = delta_off + half * delta_size  # (o is rounded to fp32 there)
@@ -72,9 +73,6 @@ def reference(q, k, v, keep, scale, do=None):
         sums = unit * (nq * group + nk + 64)
         dv_size = p.transpose(1, 2).contiguous() @ D.abs()
         dv_off = (off.amax(1, keepdim=True) + rough * 1.01 + sums) * dv_size + grid * D.abs().sum(1, keepdim=True)
-        # (the sum of a row is of its p as rounded: in the pullback all p of a row are off alike)
-        ds_off = ds_off + rough * 1.01 * ds.abs()
-        dv_off = dv_off + rough * 1.01 * dv_size
         dq_off = abs(scale) * ((ds_off + sums * ds.abs()) @ K.abs())
         dk_off = abs(scale) * ((ds_off + sums * ds.abs()).transpose(1, 2).contiguous() @ Q.abs())
         share = lambda t: t.view(Hk, group, *t.shape[1:]).sum(1)  # noqa: E731
