@@ -1293,9 +1293,11 @@ fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const v
     if (e == hipSuccess) e = attn_unpack(a, o, out.o, a.nq, heads, st);
     if (e == hipSuccess && out.rest) e = attn_unpack(a, rest, out.rest, a.nq, heads, st);
   }
-  if (cu_q && e == hipSuccess) e = attn_zero_gaps(dtype, o, cu_q, seqs, a.nq, tq, heads * dim, st);
-  if (cu_q && e == hipSuccess && rest && dtype != FMS_F32)
-    e = attn_zero_gaps(dtype, rest, cu_q, seqs, a.nq, tq, heads * dim, st);
+  if (cu_q && e == hipSuccess) {
+    AttnGaps gaps = {{{o, cu_q, a.nq, tq, heads * dim}, {rest, cu_q, a.nq, tq, heads * dim}}, 1, seqs};
+    if (rest && dtype != FMS_F32) gaps.n = 2;
+    e = attn_zero_gaps(dtype, gaps, st);
+  }
   return from_hip(e);
 }
 
@@ -1345,11 +1347,9 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
     if (e == hipSuccess) e = attn_unpack(a, dk, g.dk, a.nk, kv_heads, st);
     if (e == hipSuccess) e = attn_unpack(a, dv, g.dv, a.nk, kv_heads, st);
   }
-  if (cu_q && e == hipSuccess) {
-    e = attn_zero_gaps(dtype, dq, cu_q, seqs, a.nq, tq, heads * dim, st);
-    if (e == hipSuccess) e = attn_zero_gaps(dtype, dk, cu_k, seqs, a.nk, tk, kv_heads * dim, st);
-    if (e == hipSuccess) e = attn_zero_gaps(dtype, dv, cu_k, seqs, a.nk, tk, kv_heads * dim, st);
-  }
+  if (cu_q && e == hipSuccess)
+    e = attn_zero_gaps(dtype, {{{dq, cu_q, a.nq, tq, heads * dim}, {dk, cu_k, a.nk, tk, kv_heads * dim},
+                                {dv, cu_k, a.nk, tk, kv_heads * dim}}, 3, seqs}, st);
   return from_hip(e);
 }
 

@@ -7,6 +7,7 @@
 // rescaled where m grows.  Scores, p, m, l and the sums of values are fp32; in 16-bit types p goes
 // into its product with v as two values, a rounding and what it left.  (p is at most 1 and exactly 1
 // at the maximum.)
+#include <algorithm>
 #include <cmath>
 
 #include "fms_attn.hpp"
@@ -36,8 +37,8 @@ constexpr float kShift = std::is_same<Op, OpF16>::value ? 10.0f : 0.0f;
 __device__ __forceinline__ float factor(const AttnArgs& A) { return fmaxf(fabsf(A.scale) * kLog2e, 1e-30f); }
 
 template <class Op, int kD, int kWaves, bool kSplit>
-__global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) attn_forward_kernel(AttnArgs A, AttnOut out, Parts P,
-                                                                   int chunk, uint32_t tiles, uint32_t work) {
+__global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
+    attn_forward_kernel(AttnArgs A, AttnOut out, Parts P, uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
   typedef typename Elem<Op>::T E;
   constexpr int kThreads = kWaves * 64;
@@ -51,10 +52,8 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
   const uint32_t unit = whole / tiles;
   // (under a causal mask the last tiles have the most keys: they start first)
   const int tile = (int)(A.causal ? tiles - 1 - (whole - unit * tiles) : whole - unit * tiles);
-  // `chunk` neighbouring key heads, of which kv_heads is a multiple
-  const uint32_t chunks = (uint32_t)A.kv_heads / (uint32_t)chunk;
-  const int64_t b = unit / chunks;
-  const int hk = (int)(unit % chunks) * chunk;  // the first
+  const int64_t b = unit / (uint32_t)A.kv_heads;
+  const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
   const int nrows = S.nq * A.group;
   const int row0 = tile * (32 * kWaves);
@@ -70,10 +69,8 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
   u32x4 q[T::kK];
   const int64_t qstart = seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2];
   const int qat = there ? row_at<Op>(t - wt, A.qs[1], head, A.qs[2]) : kFar;
-  const auto load_q = [&](int u) {
-    own_row<T>(q, wave_rows<Op>(A.q, qstart + (int64_t)u * A.group * A.qs[2], wt, A.qs[1]), qat, A.units, h);
-  };
-  load_q(0);
+  own_row<T>(q, wave_rows<Op>(A.q, qstart, wt, A.qs[1]), qat, A.units, h);
+  if (A.scale < 0) negate<T>(q);
   // the keys that count for this row by position, and for the workgroup (reaches grow with the token)
   const Reach mine = keys_of(t, S, A);
   const auto reach = [&](int r) { return keys_of(token_of(r < nrows ? r : nrows - 1, A), S, A); };
@@ -97,157 +94,145 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>)) att
   const float c = factor(A);
   f32x16 acc[T::kBlocks];
   float m = -INFINITY, l = 0.0f;
-  const auto clear = [&] {
+#pragma unroll
+  for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
+  const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
+  const char* const kbase =
+      static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
+  const char* const vbase =
+      static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
+  const auto request = [&](int j0, uint64_t bits, int buffer) {
+    T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + j0 * A.ks[1] * Op::kEsz,
+                                  (int)A.ks[1] * Op::kEsz, A.units, bits);
+    T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + j0 * A.vs[1] * Op::kEsz,
+                                  (int)A.vs[1] * Op::kEsz, A.units, bits);
+  };
+  // (While a tile is worked on the next is on its way.)
+  uint64_t bits;
+  keys.end(last);
+  int j0 = keys.next(first, bits), buffer = 0;
+  if (j0 < keys.to) request(j0, bits, 0);
+  for (;;) {
+    while (j0 < keys.to) {
+      landed();
+      uint64_t bits1;
+      const int j1 = keys.next(j0 + kRows, bits1);
+      if (j1 < keys.to) request(j1, bits1, buffer ^ 1);
+      const char* const K = lds + buffer * 2 * T::kBytes;
+      const char* const V = K + T::kBytes;
+      const int now = j0;
+      const uint64_t in = bits;
+      j0 = j1;
+      bits = bits1;
+      buffer ^= 1;
+      if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
+      float s[2][16];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x16 x = f32x16{};
+#pragma unroll
+        for (int kb = 0; kb < T::kK; ++kb) x = mma<Op>(T::rows(K, 32 * half, kb, lane), q[kb], x);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[half][r] = x[r];
+      }
+      const bool whole_tile = in == ~0ull && now >= wide.all.lo && now + kRows <= wide.all.hi;
+      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+      if (!whole_tile) {
+        keep[0] = ((uint32_t)in & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
+        keep[1] = ((uint32_t)(in >> 32) & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[half][r] = masked(s[half][r], keep[half], r, -INFINITY);
+      }
+      // (NaN scores are ignored here and make p, and with it the row, NaN)
+      float top = m;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) top = max3_ieee(s[half][r], s[half][r + 1], top);
+      top = merge_halves_max(top);
+      if (__any(top > m)) {
+        const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
+        l *= by;
+#pragma unroll
+        for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] *= by;
+        m = top;
+      }
+      const float base = m == -INFINITY ? 0.0f : m, off = kShift<Op> - base * c;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          // (fp32: exactly 1 at the maximum; where p is rounded to 16 bits the cheaper form is that, too)
+          if constexpr (Op::kEsz == 4)
+            s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
+          else
+            s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
+        }
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[half] += s[half][r];
+      l += sum[0] + sum[1];
+      constexpr int kPer = 32 / kGroups<Op>;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int g = 0; g < kGroups<Op>; ++g) {
+          const Operand<Op> p = operand<Op>(s[half], g);
+#pragma unroll
+          for (int i = 0; i < T::kBlocks; ++i)
+            acc[i] = mma(T::columns(V, 32 * half + kPer * g, i, lane), p, acc[i]);
+        }
+    }
+    if (keys.to >= last) break;
+    landed();  // (every wave is through with the words, and with the buffers)
+    keys.span0 += kMaskSpan;
+    keys.end(last);
+    gather();
+    landed();
+    j0 = keys.next(keys.span0, bits);
+    if (j0 < keys.to) request(j0, bits, buffer);
+  }
+  if (A.qmask && !there) {
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
     m = -INFINITY;
     l = 0.0f;
-  };
-  // What unit u's rows summed, to memory.
-  const auto finish = [&](int u) {
-    // both halves of the wave summed other keys of the same row
-    l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
-    if constexpr (kSplit) {
-      if (row >= nrows) return;
-      const int64_t slot = (int64_t)piece * (32 * kWaves) + wave * 32 + (lane & 31);
-      float* to = P.acc + slot * kD;
+  }
+  // both halves of the wave summed other keys of the same row
+  l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
+  if constexpr (kSplit) {
+    if (row >= nrows) return;
+    const int64_t slot = (int64_t)piece * (32 * kWaves) + wave * 32 + (lane & 31);
+    float* to = P.acc + slot * kD;
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * h) =
+            f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+    P.stat[slot * 2 + h] = h ? l : m;
+  } else {
+    const bool any = l > 0.0f || l != l;
+    const float inv = any ? 1.0f / l : 0.0f;
+    store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, inv, A.units, h);
+    if (out.lse && h == 0 && row < nrows)
+      out.lse[rows_at(A, b, hk, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
+    if (Op::kEsz == 2 && out.rest) {
 #pragma unroll
       for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * h) =
-              f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
-      P.stat[slot * 2 + h] = h ? l : m;
-    } else {
-      const bool any = l > 0.0f || l != l;
-      const float inv = any ? 1.0f / l : 0.0f;
-      const int64_t to = start + u * A.group * dim;
-      store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, to, wt, width), at, acc, inv, A.units, h);
-      if (out.lse && h == 0 && row < nrows)
-        out.lse[rows_at(A, b, hk + u, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
-      if (Op::kEsz == 2 && out.rest) {
-#pragma unroll
-        for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float o = acc[i][r] * inv;
-            acc[i][r] = (o - (float)(E)o) * kRestScale<Op>;
-          }
-        store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, to, wt, width), at, acc, 1.0f, A.units, h);
-      }
+        for (int r = 0; r < 16; ++r) {
+          const float o = acc[i][r] * inv;
+          acc[i][r] = (o - (float)(E)o) * kRestScale<Op>;
+        }
+      store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, start, wt, width), at, acc, 1.0f, A.units, h);
     }
-  };
-  const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
-  const char* const kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
-  const char* const vbase = static_cast<const char*>(A.v) + (seq_at(A.vs, A.cu_k, b, S.k0) + (int64_t)hk * A.vs[2]) * Op::kEsz;
-  const auto request = [&](int u, int j0, uint64_t bits, int buffer) {
-    T::template request<kThreads>(lds + buffer * 2 * T::kBytes, kbase + (u * A.ks[2] + j0 * A.ks[1]) * Op::kEsz,
-                                  (int)A.ks[1] * Op::kEsz, A.units, bits);
-    T::template request<kThreads>(lds + (buffer * 2 + 1) * T::kBytes, vbase + (u * A.vs[2] + j0 * A.vs[1]) * Op::kEsz,
-                                  (int)A.vs[1] * Op::kEsz, A.units, bits);
-  };
-  // While a tile is worked on the next is on its way, a next head's first one too.  (Several heads
-  // only where one span holds the keys' mask: they are alike in what counts.)
-  uint64_t bits0;
-  keys.end(last);
-  const int j00 = keys.next(first, bits0);
-  int buffer = 0;
-  if (j00 < keys.to) request(0, j00, bits0, 0);
-  for (int u = 0; u < chunk; ++u) {
-    clear();
-    if (A.scale < 0) negate<T>(q);
-    int j0 = j00;
-    uint64_t bits = bits0;
-    for (;;) {
-      while (j0 < keys.to) {
-        landed();
-        uint64_t bits1;
-        const int j1 = keys.next(j0 + kRows, bits1);
-        const bool same = j1 < keys.to;
-        if (same || u + 1 < chunk) request(same ? u : u + 1, same ? j1 : j00, same ? bits1 : bits0, buffer ^ 1);
-        const char* const K = lds + buffer * 2 * T::kBytes;
-        const char* const V = K + T::kBytes;
-        const int now = j0;
-        const uint64_t in = bits;
-        j0 = j1;
-        bits = bits1;
-        buffer ^= 1;
-        if (now >= wide.any.hi || now + kRows <= wide.any.lo) continue;  // (none of this wave's rows reaches here)
-        float s[2][16];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          f32x16 x = f32x16{};
-#pragma unroll
-          for (int kb = 0; kb < T::kK; ++kb) x = mma<Op>(T::rows(K, 32 * half, kb, lane), q[kb], x);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[half][r] = x[r];
-        }
-        const bool whole_tile = in == ~0ull && now >= wide.all.lo && now + kRows <= wide.all.hi;
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (!whole_tile) {
-          keep[0] = ((uint32_t)in & bits_between(mine.lo - now, mine.hi - now)) >> (4 * h);
-          keep[1] = ((uint32_t)(in >> 32) & bits_between(mine.lo - now - 32, mine.hi - now - 32)) >> (4 * h);
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[half][r] = masked(s[half][r], keep[half], r, -INFINITY);
-        }
-        // (NaN scores are ignored here and make p, and with it the row, NaN)
-        float top = m;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int r = 0; r < 16; r += 2) top = max3_ieee(s[half][r], s[half][r + 1], top);
-        top = merge_halves_max(top);
-        if (__any(top > m)) {
-          const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
-          l *= by;
-#pragma unroll
-          for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][r] *= by;
-          m = top;
-        }
-        const float base = m == -INFINITY ? 0.0f : m, off = kShift<Op> - base * c;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            // (fp32: exactly 1 at the maximum; where p is rounded to 16 bits the cheaper form is that, too)
-            if constexpr (Op::kEsz == 4)
-              s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
-            else
-              s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
-          }
-        float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sum[half] += s[half][r];
-        l += sum[0] + sum[1];
-        constexpr int kPer = 32 / kGroups<Op>;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int g = 0; g < kGroups<Op>; ++g) {
-            const Operand<Op> p = operand<Op>(s[half], g);
-#pragma unroll
-            for (int i = 0; i < T::kBlocks; ++i)
-              acc[i] = mma(T::columns(V, 32 * half + kPer * g, i, lane), p, acc[i]);
-          }
-      }
-      if (keys.to >= last) break;
-      landed();  // (every wave is through with the words, and with the buffers)
-      keys.span0 += kMaskSpan;
-      keys.end(last);
-      gather();
-      landed();
-      j0 = keys.next(keys.span0, bits);
-      if (j0 < keys.to) request(u, j0, bits, buffer);
-    }
-    if (A.qmask && !there) clear();
-    finish(u);
-    if (u + 1 < chunk) load_q(u + 1);
   }
 }
 
@@ -313,24 +298,25 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(E* to, const E* from, in
   }
 }
 
-// A thread a token row finds whether a sequence covers it; the wave clears those of its 64 that none does.
+// A thread a token row finds whether a sequence covers it; the wave clears those of its 64 that none does.  All
+// results of a call in one launch (blockIdx.y): one is 4 us, nearly all of it latency.
 template <class E>
-__global__ void __launch_bounds__(256) attn_gap_kernel(E* out, const int32_t* cu, int64_t seqs, int64_t rows,
-                                                       int64_t most, int64_t width) {
+__global__ void __launch_bounds__(256) attn_gap_kernel(AttnGaps gaps) {
+  const AttnGaps::Result& x = gaps.of[blockIdx.y];
   const int64_t r0 = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63u), r = r0 + (threadIdx.x & 63);
-  bool gap = r < rows;
-  if (gap && seqs > 0 && r >= (int64_t)cu[0] - 1) {
-    int64_t a = 0, e = seqs;  // the last sequence that starts at r or before is in [a, e)
+  bool gap = r < x.rows;
+  if (gap && gaps.seqs > 0 && r >= (int64_t)x.cu[0] - 1) {
+    int64_t a = 0, e = gaps.seqs;  // the last sequence that starts at r or before is in [a, e)
     while (e - a > 1) {
       const int64_t mid = (a + e) / 2;
-      if ((int64_t)cu[mid] - 1 <= r) a = mid;
+      if ((int64_t)x.cu[mid] - 1 <= r) a = mid;
       else e = mid;
     }
-    gap = !(r < (int64_t)cu[a + 1] - 1 && r - ((int64_t)cu[a] - 1) < most);
+    gap = !(r < (int64_t)x.cu[a + 1] - 1 && r - ((int64_t)x.cu[a] - 1) < x.most);
   }
   for (uint64_t left = __ballot(gap); left; left &= left - 1) {
-    E* const row = out + (r0 + __builtin_ctzll(left)) * width;
-    for (int64_t i = threadIdx.x & 63; i < width; i += 64) row[i] = (E)0;
+    E* const row = static_cast<E*>(x.out) + (r0 + __builtin_ctzll(left)) * x.width;
+    for (int64_t i = threadIdx.x & 63; i < x.width; i += 64) row[i] = (E)0;
   }
 }
 
@@ -348,7 +334,7 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
   const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), units = a.seqs * a.kv_heads;
   // Few workgroups of many keys each leave most of the card idle: their keys are split, 256 to a
   // workgroup at least, until there are two to a CU (16 heads on 4 of 128 values in bf16, one token, 32768
-  // keys: 1414 us in 4 workgroups, SPLITUS in 512).
+  // keys: 1414 us in 4 workgroups, 20 and 5 for the join in 512).
   const int64_t pieces = units * tiles, wanted = pieces <= 128 ? 512 / pieces : 1;
   const int64_t keys = (cdiv(a.tk, wanted) + 255) / 256 * 256;
   if (a.tk > keys) {
@@ -362,7 +348,7 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
     p.acc = static_cast<float*>(mem);
     p.stat = p.acc + slots * kD;
     hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, true>), dim3(piece_blocks(pieces * p.splits)),
-                       dim3(kWaves * 64), 0, stream, a, out, p, 1, (uint32_t)tiles, (uint32_t)(pieces * p.splits));
+                       dim3(kWaves * 64), 0, stream, a, out, p, (uint32_t)tiles, (uint32_t)(pieces * p.splits));
     const int most = a.tq * a.group;
     hipLaunchKernelGGL((attn_join_kernel<Op, kD, kWaves>), dim3((unsigned)(units * most)), dim3(256), 0, stream, a,
                        out, p, (int)tiles, most);
@@ -370,9 +356,8 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
     const hipError_t ef = workspace_free(mem, stream);
     return e != hipSuccess ? e : ef;
   }
-  const int chunk = attn_chunk(a, pieces);
-  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(pieces / chunk)),
-                     dim3(kWaves * 64), 0, stream, a, out, Parts{}, chunk, (uint32_t)tiles, (uint32_t)(pieces / chunk));
+  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(pieces)), dim3(kWaves * 64), 0,
+                     stream, a, out, Parts{}, (uint32_t)tiles, (uint32_t)pieces);
   return hipGetLastError();
 }
 
@@ -409,25 +394,16 @@ hipError_t attn_pack(int32_t dtype, void* to, const void* from, const int64_t* s
   return hipGetLastError();
 }
 
-hipError_t attn_zero_gaps(int32_t dtype, void* out, const int32_t* cu, int64_t seqs, int64_t rows, int64_t most,
-                          int64_t width, hipStream_t stream) {
-  if (rows == 0 || width == 0) return hipSuccess;
-  const int64_t blocks = attn::cdiv(rows, 256);
+hipError_t attn_zero_gaps(int32_t dtype, const AttnGaps& gaps, hipStream_t stream) {
+  int64_t rows = 0;
+  for (int i = 0; i < gaps.n; ++i) rows = std::max(rows, gaps.of[i].width ? gaps.of[i].rows : 0);
+  if (rows == 0) return hipSuccess;
+  const dim3 blocks((unsigned)attn::cdiv(rows, 256), (unsigned)gaps.n);
   if (dtype == FMS_F32)
-    hipLaunchKernelGGL((attn::attn_gap_kernel<uint32_t>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                       static_cast<uint32_t*>(out), cu, seqs, rows, most, width);
+    hipLaunchKernelGGL((attn::attn_gap_kernel<uint32_t>), blocks, dim3(256), 0, stream, gaps);
   else
-    hipLaunchKernelGGL((attn::attn_gap_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                       static_cast<uint16_t*>(out), cu, seqs, rows, most, width);
+    hipLaunchKernelGGL((attn::attn_gap_kernel<uint16_t>), blocks, dim3(256), 0, stream, gaps);
   return hipGetLastError();
-}
-
-int attn_chunk(const AttnArgs& a, int64_t pieces) {
-  int chunk = 1;
-  if (a.kmask && a.tk > attn::kMaskSpan) return 1;
-  for (int n = 2; n <= a.kv_heads && pieces / n >= 2048; ++n)
-    if (a.kv_heads % n == 0) chunk = n;
-  return chunk;
 }
 
 hipError_t attn_forward(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {

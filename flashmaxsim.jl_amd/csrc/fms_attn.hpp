@@ -66,13 +66,17 @@ hipError_t attn_pullback(const AttnArgs& a, const AttnGrads& g, hipStream_t stre
 // rows x heads x dim -> dense rows x heads x packed_dim, zeros behind dim
 hipError_t attn_pack(int32_t dtype, void* to, const void* from, const int64_t* strides, int64_t seqs,
                      int64_t tokens, int64_t heads, int32_t dim, int32_t packed_dim, hipStream_t stream);
-// Zeros for token rows of (rows, width) that no sequence covers.
-hipError_t attn_zero_gaps(int32_t dtype, void* out, const int32_t* cu, int64_t seqs, int64_t rows,
-                          int64_t most, int64_t width, hipStream_t stream);
-
-// How many neighbouring key heads a workgroup takes: as many as leave two rounds of workgroups (four to a
-// CU), so that the start of the next head's work hides behind this one's.
-int attn_chunk(const AttnArgs& a, int64_t pieces);
+// Zeros for the token rows of some results that no sequence covers.
+struct AttnGaps {
+  struct Result {
+    void* out;
+    const int32_t* cu;
+    int64_t rows, most, width;  // token rows, the longest sequence, values of a row
+  } of[3];
+  int n;
+  int64_t seqs;
+};
+hipError_t attn_zero_gaps(int32_t dtype, const AttnGaps& gaps, hipStream_t stream);
 
 // ---- device --------------------------------------------------------------------------------
 
@@ -257,10 +261,10 @@ struct Tile {
   }
 };
 
-// Waves of a SIMD that the forward's registers should leave room for: as many as the LDS does, or one less where it
-// would have to spill some (64 values in 16 bits: 56 us against 84 for 128 x 180 tokens of 16 heads).
+// Waves of a SIMD that the forward's registers should leave room for: as many as the LDS does.  (256 documents of up
+// to 180 tokens, 12 heads of 64 in bf16: 61 us with four, 71 with three, though four spill a few registers.)
 template <class Op, int kD, int kWaves>
-constexpr int kSimdWaves = kWaves < 4 ? 1 : kD * Op::kEsz <= 128 ? 3 : kD * Op::kEsz <= 256 ? 2 : 1;
+constexpr int kSimdWaves = kWaves < 4 ? 1 : kD * Op::kEsz <= 128 ? 4 : kD * Op::kEsz <= 256 ? 2 : 1;
 
 template <class Op>
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 acc) {
