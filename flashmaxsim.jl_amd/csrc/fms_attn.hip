@@ -7,6 +7,22 @@
 // rescaled where m grows.  Scores, p, m, l and the sums of values are fp32; in 16-bit types p goes
 // into its product with v as two values, a rounding and what it left.  (p is at most 1 and exactly 1
 // at the maximum.)
+//
+// The rows of a key head's group of query heads are one run, row = token * group + head, 32 to a wave: a
+// tile of 64 keys in LDS serves all of them.  The scores are formed transposed, K Q^T, so that a lane
+// has half the keys of one row: maximum and sum are a lane's own but for one exchange, and p lies as
+// the product with v wants it.  v is read by columns through the transposing LDS read.  While a tile is
+// worked on the next is on its way into LDS.  Masked rows and keys are not loaded, tiles in which no
+// key counts are skipped.
+//
+// What bounds it, as measured:
+//   256 documents of up to 180 tokens, masked, 12 heads of 64, bf16: 62 us.  Exponentials and
+//     conversions (about 8 instructions a score, one of them at a quarter of the rate) cost more cycles than
+//     the products.
+//   8192 causal tokens, 16 heads on 4 of 128, bf16: 555 us, three products' work (p in two values), 0.74
+//     PFLOP/s of it; one rounding of p took 440, and results 1.4 times as far off.
+//   one token on 32768 keys, 16 heads on 4 of 128, bf16: 20 us and 5 for the join, 67 MB at 3.4 TB/s:
+//     512 workgroups of a wave have four tiles each, and wait for the first.
 #include <algorithm>
 #include <cmath>
 

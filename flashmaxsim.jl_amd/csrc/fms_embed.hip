@@ -3,7 +3,9 @@
 //   e[t] = scale * W[id_t],   dW[v] = scale * sum of de[t] over the tokens t with id_t = v
 //
 // Bound by memory: the lookup writes every e once (its reads repeat), the gradient reads every de once
-// and writes all of dW.  For the gradient the tokens are grouped by id (the candidate scans'
+// and writes all of dW (128 x 180 tokens, 70 % of them real, 32768 rows
+// of 1024 in bf16: lookup 11 us; gradient 31 for the sort, whose short kernels are latency, 25 for the
+// rows, 14 for the longer runs).  For the gradient the tokens are grouped by id (the candidate scans'
 // counting sort, whose atomics stay in LDS); a wave takes a row of dW and adds its tokens' rows in
 // fp32 and in the order of the tokens, which it restores first (the sort leaves a group's order
 // open), so the sums are the same every time.  Ids of more than 64 tokens (a text's most frequent

@@ -6,7 +6,8 @@
 //   dw = sum d * x^,  dx = i (d w - [mean(d w)] - x^ mean(d w x^))
 // with x^ = norm(x) and i = 1 / sqrt(..) computed again from x.
 //
-// Bound by memory: forward moves 2 values an element, the pullback 3.  A wave takes a token: its
+// Bound by memory: forward moves 2 values an element, the pullback 3 (128 x 180 tokens of 16 and 16 heads
+// of 64 in bf16: 41 us at 4.6 TB/s, 66 at 4.3, and 4 for the join).  A wave takes a token: its
 // cosines and sines stay in registers while the token's heads, queries' and keys' alike, pass by,
 // as many at a time as fit (a head of 64 16-bit values takes four lanes).  A lane holds both
 // values of its pairs, so that the rotation needs no exchange, and the norm's sums run over the
@@ -360,7 +361,9 @@ hipError_t rotary_pullback(const RotaryArgs& a, const RotaryGrads& g, hipStream_
   return by_share(a, vec, [&](auto share, int lanes) {
     typedef decltype(share) S;
     typedef typename S::T T;
-    const int64_t want = cdiv(a.seqs * a.tokens, 4), most = 1024;
+    // (three to a CU, as many as the largest share's registers let in: 66 us for the header's case, 81 with four, whose
+    // last quarter runs by itself, 78 with two)
+    const int64_t want = cdiv(a.seqs * a.tokens, 4), most = 768;
     const int64_t blocks = want < most ? want : most;
     const bool weights = g.dwq || g.dwk;
     void* parts = nullptr;
