@@ -16,11 +16,12 @@
 // key counts are skipped.
 //
 // What bounds it, as measured:
-//   256 documents of up to 180 tokens, masked, 12 heads of 64, bf16: 62 us.  Exponentials and
-//     conversions (about 8 instructions a score, one of them at a quarter of the rate) cost more cycles than
-//     the products.
-//   8192 causal tokens, 16 heads on 4 of 128, bf16: 555 us, three products' work (p in two values), 0.74
-//     PFLOP/s of it; one rounding of p took 440, and results 1.4 times as far off.
+//   256 documents of up to 180 tokens, masked, 12 heads of 64, bf16: 62 us.  Vector
+//     instructions (about 8 a score, one of them at a quarter of the rate) are issued in 52 % of the cycles, the
+//     matrix cores busy in 11 %: a workgroup has one to three tiles, whose first loads and last stores
+//     other workgroups of the CU hide in part.
+//   8192 causal tokens, 16 heads on 4 of 128, bf16: 560 us, three products' work (p in two values), 0.73
+//     PFLOP/s of it, matrix cores busy in 54 % of the cycles, vector units in 57; one rounding of p took 440, and results 1.4 times as far off.
 //   one token on 32768 keys, 16 heads on 4 of 128, bf16: 20 us and 5 for the join, 67 MB at 3.4 TB/s:
 //     512 workgroups of a wave have four tiles each, and wait for the first.
 #include <algorithm>

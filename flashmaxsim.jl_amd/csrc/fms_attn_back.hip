@@ -16,16 +16,18 @@
 // two: p by 2^15, dp - delta by a bound of its size from the norms of do and v, so that neither small
 // probabilities nor small cotangents lose their bits.
 //
-// What bounds it, as measured: the matrix cores, which few waves a SIMD (three in the first kernel and two in the
-// second for 16-bit heads of 64, two and one for 128: accumulators and operands) do not keep fed.
-//   128 documents of up to 180 tokens, masked, 16 heads of 64, bf16: dq 62 us, dk and dv 84.
-//   48 ragged documents of up to 1999 tokens, window 64, 12 heads of 64, fp16: norms 28, dq 143, dk and dv 191;
-//     tiles on the window's edge are half empty.
-//   8192 causal tokens, 16 heads on 4 of 128, bf16: dq 645 (four products' work, 0.85 PFLOP/s), dk and dv 1310 and
-//     23 (six, 0.63 PFLOP/s).  With p and ds rounded once 530 and 1077; gradients were then 1.4 to 1.5 times as far off
-//     as their own rounding takes them.
-//   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 40 and 43, the path of the longest
-//     sequence's workgroups (fp32 products of 64 values run at about an eighth of the 16-bit rate).
+// What bounds it, as measured (matrix cores busy, vector instructions issued, of the cycles):
+//   128 documents of up to 180 tokens, masked, 16 heads of 64, bf16: dq 62 us (13 %, 35 %), dk and dv 84 (12 %,
+//     37 %).  One to three tiles a workgroup: its loads at the start and its stores at the end, which three
+//     and two waves a SIMD (accumulators and operands) hide in part.
+//   48 ragged documents of up to 1999 tokens, window 64, 12 heads of 64, fp16: norms 28, dq 142 (20 %, 46 %), dk and dv
+//     188 (20 %, 47 %); tiles on the window's edge are half empty.
+//   8192 causal tokens, 16 heads on 4 of 128, bf16: dq 645 (63 %, 46 %; four products' work, 0.85 PFLOP/s), dk and
+//     dv 1310 and 23 for the join (42 %, 41 %; six, 0.63 PFLOP/s), with one wave a SIMD, whose exponentials nothing else
+//     hides.  With p and ds rounded once 530 and 1077; gradients were then 1.4 to 1.5 times as far off as
+//     their own rounding takes them.
+//   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 40 (47 %) and 43 (43 %): the path of the
+//     longest sequence's workgroups, one wave a SIMD; fp32 products run at about an eighth of the rate.
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"

@@ -136,7 +136,7 @@ def _norm(normalize) -> int:
 # from the caching allocator on the call's stream and go back to it, to be reused
 # in stream order, when the call returns.  Whatever _lend declines, and every
 # allocation under graph capture, comes from the library's pool.  (The token block's
-# calls are lent memory under capture too: torch's allocator takes it from the graph's own.)
+# and the encoder's calls are lent memory under capture too: torch's allocator takes it from the graph's own.)
 
 class _Call:
     """The call a thread is in: its device and the pieces lent to it."""

@@ -679,8 +679,9 @@ fms_status fms_debug_cross_lane(float* out, void* stream);
  * owner may reuse it in stream order from then on.  The lender belongs to the
  * calling host thread (NULL: none, the default), may be asked several times by a
  * call, and is not asked while the stream is being captured -- except by the token
- * block's calls, which take no memory from the pool then: what it lends to a captured
- * call belongs to the graph as long as that is replayed.  Where it lends none, or none is
+ * block's and the encoder's calls (gated feed-forward, norms, AdamW; attention, head norm
+ * and rotation, token lookup), which take no memory from the pool then: what it lends to a
+ * captured call belongs to the graph as long as that is replayed.  Where it lends none, or none is
  * set, such a call returns FMS_EHIP and adds nothing to the graph.
  */
 typedef void* (*fms_workspace_lender)(int64_t bytes, void* stream);
