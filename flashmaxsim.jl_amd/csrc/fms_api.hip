@@ -1146,7 +1146,7 @@ fms_status attn_args(AttnArgs* out, int32_t dtype, const void* q, const void* k,
   if (elem_bytes(dtype) == 0) return FMS_EUNSUPPORTED;
   if (seqs < 0 || tq < 0 || tk < 0 || heads < 0 || kv_heads < 0 || dim < 0) return FMS_EINVAL;
   if ((causal & ~1) || window < -1) return FMS_EINVAL;
-  if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0)) return FMS_EINVAL;
+  if ((heads == 0) != (kv_heads == 0) || (heads > 0 && heads % kv_heads != 0)) return FMS_EINVAL;
   if ((cu_q == nullptr) != (cu_k == nullptr)) return FMS_EINVAL;
   const bool ragged = cu_q != nullptr;
   if (ragged && (qmask || kmask || nq < 0 || nk < 0)) return FMS_EINVAL;

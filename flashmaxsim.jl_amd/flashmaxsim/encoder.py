@@ -165,6 +165,9 @@ class AttentionKept(NamedTuple):
     rest: torch.Tensor | None
 
 
+_MOST = 1 << 40  # more than any length or window: what passes 64 bits would lose its upper ones on the way
+
+
 def _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, window, scale):
     """Shapes of the heads and the options as the boundary takes them (it checks the rest)."""
     qs, ks = q.shape, k.shape
@@ -174,7 +177,7 @@ def _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, 
                                 "or all of them without B")
     if qs[-1] != ks[-1] or n == 4 and qs[0] != ks[0]:
         raise DimensionMismatch(f"q {tuple(qs)} and k {tuple(ks)} differ in batch or dim")
-    if qs[-2] != ks[-2] and (not ks[-2] or qs[-2] % ks[-2]):
+    if qs[-2] != ks[-2] and (not ks[-2] or not qs[-2] or qs[-2] % ks[-2]):
         raise DimensionMismatch(f"{qs[-2]} query heads cannot share {ks[-2]} key heads evenly")
     if cu_q is None and cu_k is None:
         if max_q is not None or max_k is not None:
@@ -187,8 +190,8 @@ def _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, 
             raise DimensionMismatch("ragged attention takes token rows (tokens, heads, dim)")
         if qmask is not None or kmask is not None:
             raise ArgumentError("masks go with padded sequences, not with cu_q and cu_k")
-        max_q = qs[0] if max_q is None else int(max_q)
-        max_k = ks[0] if max_k is None else int(max_k)
+        max_q = qs[0] if max_q is None else min(int(max_q), _MOST)
+        max_k = ks[0] if max_k is None else min(int(max_k), _MOST)
         if max_q < 0 or max_k < 0:
             raise ArgumentError("max_q and max_k must be >= 0")
     if window is None:
@@ -197,7 +200,7 @@ def _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, 
         raise ArgumentError("window must be >= 0, or None")
     if scale is None:
         scale = qs[-1] ** -0.5 if qs[-1] else 1.0
-    return qmask, kmask, cu_q, cu_k, max_q, max_k, float(scale), 1 if causal else 0, int(window)
+    return qmask, kmask, cu_q, cu_k, max_q, max_k, float(scale), 1 if causal else 0, min(int(window), _MOST)
 
 
 def attention_forward(q, k, v, qmask=None, kmask=None, *, cu_q=None, cu_k=None, max_q=None, max_k=None,

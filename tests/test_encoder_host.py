@@ -24,7 +24,7 @@ def pullback(L, dtype=1, dq=1, dk=1, dv=1, dout=1, o=1, lse=1, rest=1, tq=8, tk=
 
 
 @pytest.mark.parametrize("args,expect", [
-    (dict(dtype=9), EUNSUP), (dict(tq=-1), EINVAL), (dict(heads=3), EINVAL), (dict(kv_heads=0), EINVAL),
+    (dict(dtype=9), EUNSUP), (dict(tq=-1), EINVAL), (dict(heads=3), EINVAL), (dict(kv_heads=0), EINVAL), (dict(heads=0), EINVAL),
     (dict(causal=2), EINVAL), (dict(window=-2), EINVAL), (dict(cu_q=1), EINVAL), (dict(cu_k=1), EINVAL),
     (dict(cu_q=1, cu_k=1, nq=-1), EINVAL), (dict(cu_q=1, cu_k=1, qmask=1), EINVAL), (dict(dim=129), EUNSUP),
     (dict(tq=1 << 29), EUNSUP), (dict(tk=1 << 29), EUNSUP), (dict(seqs=1 << 31), EUNSUP),
@@ -89,3 +89,10 @@ def test_host_arrays_are_refused():
                  lambda: fm.embed_tokens_pullback(torch.zeros(3, 8), ids, 5)):
         with pytest.raises(fm.ArgumentError):
             call()
+
+
+def test_heads_are_refused():
+    """Key heads that no query head shares: their gradients would be nobody's."""
+    for h, hk in ((0, 2), (2, 0), (3, 2)):
+        with pytest.raises(fm.DimensionMismatch):
+            fm.attention_forward(torch.zeros(1, 4, h, 32), torch.zeros(1, 5, hk, 32), torch.zeros(1, 5, hk, 32))

@@ -304,3 +304,23 @@ def test_refusals(device):
     for error, arrays, options in bad:
         with pytest.raises(error):
             fm.attention_forward(*arrays, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Tq,Tk", [(0, 5), (5, 0), (0, 0)])
+def test_no_tokens(dtype, Tq, Tk, device):
+    """Without queries the keys' gradients are zero, without keys the results are."""
+    q, k, v, do = inputs((2, Tq, 4, 48), (2, Tk, 2, 48), dtype, device)
+    o, kept = fm.attention_forward(q, k, v, keep=True)
+    for t, like in zip((o, *fm.attention_pullback(do, q, k, v, o, kept)), (q, q, k, v)):
+        assert t.shape == like.shape and not t.any()
+
+
+def test_sizes_past_64_bits(device):
+    q, k, v, do = inputs((70, 2, 32), (70, 2, 32), torch.bfloat16, device)
+    cu = torch.tensor([1, 31, 71], dtype=torch.int32, device=device)
+    whole = fm.attention_forward(q, k, v, cu_q=cu, cu_k=cu)
+    for args in (dict(window=10 ** 30), dict(window=2 ** 64)):
+        assert torch.equal(fm.attention_forward(q, k, v, cu_q=cu, cu_k=cu, **args), whole)
+    with pytest.raises(fm.UnsupportedError):
+        fm.attention_forward(q, k, v, cu_q=cu, cu_k=cu, max_q=2 ** 64 + 70, max_k=70)
