@@ -19,7 +19,7 @@
 // What bounds it, as measured (matrix cores busy, vector instructions issued, of the cycles):
 //   128 documents of up to 180 tokens, masked, 16 heads of 64, bf16: dq 62 us (13 %, 35 %), dk and dv 84 (12 %,
 //     37 %).  One to three tiles a workgroup: its loads at the start and its stores at the end, which three
-//     and two waves a SIMD (accumulators and operands) hide in part.
+//     and two waves a SIMD (accumulators and operands) hide in part.  (dq with four: 84, twenty registers spill.)
 //   48 ragged documents of up to 1999 tokens, window 64, 12 heads of 64, fp16: norms 28, dq 142 (20 %, 46 %), dk and dv
 //     188 (20 %, 47 %); tiles on the window's edge are half empty.
 //   8192 causal tokens, 16 heads on 4 of 128, bf16: dq 645 (63 %, 46 %; four products' work, 0.85 PFLOP/s), dk and
