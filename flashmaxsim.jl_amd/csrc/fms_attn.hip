@@ -5,8 +5,7 @@
 //
 // One pass over the keys: a running maximum m and sum l per row, and what was summed so far
 // rescaled where m grows.  Scores, p, m, l and the sums of values are fp32; in 16-bit types p goes
-// into its product with v as two values, a rounding and what it left.  (p is at most 1 and exactly 1
-// at the maximum.)
+// into its product with v as two values, a rounding and what it left.
 //
 // The rows of a key head's group of query heads are one run, row = token * group + head, 32 to a wave: a
 // tile of 64 keys in LDS serves all of them.  The scores are formed transposed, K Q^T, so that a lane
@@ -183,7 +182,8 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          // (fp32: exactly 1 at the maximum; where p is rounded to 16 bits the cheaper form is that, too)
+          // (fp32: exactly 1 at the maximum.  16-bit: off by what m c was rounded by, for all of a row alike,
+          // in the logarithm of the sum too, so that it cancels)
           if constexpr (Op::kEsz == 4)
             s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
           else
