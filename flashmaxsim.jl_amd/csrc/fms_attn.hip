@@ -177,18 +177,14 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
           for (int r = 0; r < 16; ++r) acc[i][r] *= by;
         m = top;
       }
-      const float base = m == -INFINITY ? 0.0f : m, off = kShift<Op> - base * c;
+      const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          // (fp32: exactly 1 at the maximum.  16-bit: off by what m c was rounded by, for all of a row alike,
-          // in the logarithm of the sum too, so that it cancels)
-          if constexpr (Op::kEsz == 4)
-            s[half][r] = __builtin_amdgcn_exp2f((s[half][r] - base) * c);
-          else
-            s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r], c, off));
-        }
+        for (int r = 0; r < 16; ++r)
+          // (The maximum goes before the factor: p is exactly 1 there, so a row that sees one key has that key's
+          // value, and of large scores too the difference is what counts.)
+          s[half][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[half][r] - base, c, kShift<Op>));
       float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int half = 0; half < 2; ++half)
