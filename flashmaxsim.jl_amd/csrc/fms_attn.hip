@@ -233,17 +233,22 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
   } else {
     const bool any = l > 0.0f || l != l;
     const float inv = any ? 1.0f / l : 0.0f;
-    store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, inv, A.units, h);
+    // (the quotient is settled before it is rounded: fp16's rounding could be of the product in full, and what it left
+    // of the product in 32 bits, which near a tie is a step away)
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= inv;
+      asm volatile("" : "+v"(acc[i]));
+    }
+    store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, 1.0f, A.units, h);
     if (out.lse && h == 0 && row < nrows)
       out.lse[rows_at(A, b, hk, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
     if (Op::kEsz == 2 && out.rest) {
 #pragma unroll
       for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float o = acc[i][r] * inv;
-          acc[i][r] = (o - (float)(E)o) * kRestScale<Op>;
-        }
+        for (int r = 0; r < 16; ++r) acc[i][r] = (acc[i][r] - (float)(E)acc[i][r]) * kRestScale<Op>;
       store_row<Op, T::kBlocks>(wave_rows<Op>(out.rest, start, wt, width), at, acc, 1.0f, A.units, h);
     }
   }
@@ -292,7 +297,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs A, AttnOut out,
   const int dim = A.units * (16 / Op::kEsz);
   const int64_t at = ((S.q0 + t) * A.heads + head) * (int64_t)dim;
   for (int d = threadIdx.x; d < dim; d += 256) {
-    const float o = ((lds[0][d] + lds[1][d]) + (lds[2][d] + lds[3][d])) * inv;
+    float o = ((lds[0][d] + lds[1][d]) + (lds[2][d] + lds[3][d])) * inv;
+    asm volatile("" : "+v"(o));  // (settled, as in the kernel above)
     static_cast<E*>(out.o)[at + d] = (E)o;
     if (Op::kEsz == 2 && out.rest) static_cast<E*>(out.rest)[at + d] = (E)((o - (float)(E)o) * kRestScale<Op>);
   }
