@@ -1269,7 +1269,7 @@ hipError_t attn_unpack(const AttnArgs& a, void* result, const void* at, int64_t 
 
 }  // namespace
 
-fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const void* q, const void* k,
+fms_status fms_attention(int32_t dtype, void* o, float* top, void* rest, const void* q, const void* k,
                          const void* v, const int64_t* strides, const uint8_t* qmask, const uint8_t* kmask,
                          const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk, int64_t nq,
                          int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim, float scale, int32_t causal,
@@ -1279,11 +1279,11 @@ fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const v
                                  kv_heads, dim, scale, causal, window);
   if (s != FMS_OK) return s;
   if (a.nq == 0 || heads == 0 || dim == 0) return FMS_OK;
-  if (!o || (dtype != FMS_F32 && (lse == nullptr) != (rest == nullptr))) return FMS_EINVAL;
+  if (!o || (dtype != FMS_F32 && (top == nullptr) != (rest == nullptr))) return FMS_EINVAL;
   const hipStream_t st = as_stream(stream);
   Pieces w(st);
   AttnOut out = {};
-  out.lse = lse;
+  out.top = top;
   hipError_t e = hipSuccess;
   if (seqs > 0 && tq > 0) {
     if (e == hipSuccess) e = attn_packed(&a, &w);
@@ -1302,7 +1302,7 @@ fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const v
 }
 
 fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, const void* dout, const void* o,
-                                  const float* lse, const void* rest, const void* q, const void* k, const void* v,
+                                  const float* top, const void* rest, const void* q, const void* k, const void* v,
                                   const int64_t* strides, const uint8_t* qmask, const uint8_t* kmask,
                                   const int32_t* cu_q, const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk,
                                   int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim, float scale,
@@ -1312,7 +1312,7 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
                                  kv_heads, dim, scale, causal, window);
   if (s != FMS_OK) return s;
   if (dim == 0 || (a.nq == 0 && a.nk == 0) || heads == 0) return FMS_OK;
-  if (a.nq > 0 && (!dq || !dout || !o || !lse || (dtype != FMS_F32 && !rest))) return FMS_EINVAL;
+  if (a.nq > 0 && (!dq || !dout || !o || !top || (dtype != FMS_F32 && !rest))) return FMS_EINVAL;
   if (a.nk > 0 && (!dk || !dv)) return FMS_EINVAL;
   const hipStream_t st = as_stream(stream);
   Pieces w(st);
@@ -1321,14 +1321,15 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
   if (seqs > 0) {
     const int64_t rows = a.nq * heads, esz = elem_bytes(dtype);
     void* p;
-    e = w.get(&p, rows * 4);
+    e = w.get(&p, rows * 8);
     g.delta = static_cast<float*>(p);
+    g.level = g.delta + rows;
     if (e == hipSuccess && dtype == FMS_F16) {
       e = w.get(&p, seqs * kv_heads * kAttnPeakParts * 8);
       g.peaks = static_cast<float*>(p);
     }
     if (e == hipSuccess) e = attn_packed(&a, &w);
-    g.lse = lse;
+    g.top = top;
     const int64_t width = a.units * (16 / esz), dense[3] = {0, heads * dim, dim};
     const void* from[3] = {dout, o, dtype == FMS_F32 ? nullptr : rest};
     const void** to[3] = {&g.dout, &g.o, &g.rest};

@@ -49,9 +49,6 @@ struct Parts {
 template <class Op>
 constexpr float kShift = std::is_same<Op, OpF16>::value ? 10.0f : 0.0f;
 
-// A score's factor, to base 2.  (Not zero, so that a masked score's -inf stays that.)
-__device__ __forceinline__ float factor(const AttnArgs& A) { return fmaxf(fabsf(A.scale) * kLog2e, 1e-30f); }
-
 template <class Op, int kD, int kWaves, bool kSplit>
 __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
     attn_forward_kernel(AttnArgs A, AttnOut out, Parts P, uint32_t tiles, uint32_t work) {
@@ -242,8 +239,7 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
       asm volatile("" : "+v"(acc[i]));
     }
     store_row<Op, T::kBlocks>(wave_rows<Op>(out.o, start, wt, width), at, acc, 1.0f, A.units, h);
-    if (out.lse && h == 0 && row < nrows)
-      out.lse[rows_at(A, b, hk, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
+    if (out.top && h == 0 && row < nrows) out.top[rows_at(A, b, hk, S.q0) + row] = m;
     if (Op::kEsz == 2 && out.rest) {
 #pragma unroll
       for (int i = 0; i < T::kBlocks; ++i)
@@ -302,8 +298,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs A, AttnOut out,
     static_cast<E*>(out.o)[at + d] = (E)o;
     if (Op::kEsz == 2 && out.rest) static_cast<E*>(out.rest)[at + d] = (E)((o - (float)(E)o) * kRestScale<Op>);
   }
-  if (out.lse && threadIdx.x == 0)
-    out.lse[rows_at(A, b, hk, S.q0) + row] = any ? m * c + __builtin_amdgcn_logf(l) - kShift<Op> : -INFINITY;
+  if (out.top && threadIdx.x == 0) out.top[rows_at(A, b, hk, S.q0) + row] = m;
 }
 
 template <class E>

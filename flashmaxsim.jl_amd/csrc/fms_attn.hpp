@@ -40,25 +40,26 @@ struct AttnArgs {
 
 constexpr int64_t kAttnMaxDim = 128;
 
-// o (token rows, heads, whole units of dim, 16-byte aligned); lse (seqs, kv_heads, tq * group) or ragged (kv_heads, nq * group),
-// base-2 logarithms of the rows' sums, and rest, what o's rounding left (16-bit types): both null
-// where no pullback follows.
+// o (token rows, heads, whole units of dim, 16-byte aligned); top (seqs, kv_heads, tq * group) or ragged (kv_heads, nq * group),
+// the rows' largest products q_i k_j (of the other sign under a negative scale; -inf where no key counts), and rest,
+// what o's rounding left (16-bit types): both null where no pullback follows.
 struct AttnOut {
   void* o;
-  float* lse;
+  float* top;
   void* rest;
 };
 hipError_t attn_forward(const AttnArgs& a, const AttnOut& out, hipStream_t stream);
 
 struct AttnGrads {
   const void *dout, *o, *rest;  // as o: token rows of heads * dim
-  const float* lse;
+  const float* top;
   void *dq, *dk, *dv;  // dense
-  float* delta;        // as lse: sum_j p_ij dp_ij, from the first kernel to the second
+  float* delta;        // as top: sum_j p_ij dp_ij, from the first kernel to the second
+  float* level;        // as top: what the rows' sums are brought to one by, likewise
   float* peaks;        // (units, kPeakParts, 2): largest squared norms of v and dout rows (fp16)
 };
 constexpr int kAttnPeakParts = 16;
-// g.delta and g.peaks are the caller's; rows of o, rest and dout are whole units apart.
+// g.delta, g.level and g.peaks are the caller's; rows of o, rest and dout are whole units apart.
 hipError_t attn_pullback(const AttnArgs& a, const AttnGrads& g, hipStream_t stream);
 
 // ---- host helpers of both ----------------------------------------------------------------
@@ -87,6 +88,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+// A score's factor, to base 2.  (Not zero, so that a masked score's -inf stays that.)
+__device__ __forceinline__ float factor(const AttnArgs& A) { return fmaxf(fabsf(A.scale) * kLog2e, 1e-30f); }
 constexpr int kFar = (int)0x80000000u;  // a byte offset past every resource: reads as zero
 constexpr int kRows = 64;               // rows of a tile in LDS
 constexpr int kMaskSpan = 16384;        // rows whose mask bits are held at a time
@@ -121,7 +124,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& A, int64_t b) {
 __device__ __forceinline__ int64_t seq_at(const int64_t (&st)[3], bool ragged, int64_t b, int64_t first) {
   return ragged ? first * st[1] : b * st[0];
 }
-// Where a unit's rows start in lse and the like.
+// Where a unit's rows start in top and the like.
 __device__ __forceinline__ int64_t rows_at(const AttnArgs& A, int64_t b, int hk, int64_t q0) {
   return A.cu_q ? ((int64_t)hk * A.nq + q0) * A.group : (b * A.kv_heads + hk) * ((int64_t)A.tq * A.group);
 }

@@ -1,6 +1,6 @@
 // fms_attn_back.hip -- the pullback of attention over heads.
 //
-// With p_ij as in the forward, computed again from q, k and the kept logarithms of its sums:
+// With p_ij as in the forward, computed again from q, k and the kept maxima of its rows:
 //   dv_j = sum_i p_ij do_i                     dp_ij = do_i v_j
 //   ds_ij = p_ij (dp_ij - delta_i)             delta_i = sum_j p_ij dp_ij = do_i o_i
 //   dq_i = scale sum_j ds_ij k_j               dk_j = scale sum_i ds_ij q_i
@@ -9,6 +9,10 @@
 // there and the rows passing by (dk, dv): seven products where one kernel would need five, but
 // each sum stays in registers, in fp32, in a fixed order, with no atomics and no partial sums in
 // memory; the heads that share a key head are rows of one run, so their sums are one too.
+//
+// The maximum goes before the scale, as in the forward, so that p is as exact for large scores as for small ones (a
+// kept logarithm of the sum would be off by its own last bit: p by 8e-5 at scores of 1000).  The sums are made again by
+// the first kernel, which divides by them at its end and leaves them to the second.
 //
 // delta takes o with what its rounding left (the forward keeps that): where one key has nearly all
 // the weight, dp - delta is a small difference of nearly equal terms.  In 16-bit types p and ds go into their
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   const int t = token_of(row, A), head = row - t * A.group;  // (of the key head's)
   const int wt = token_of(row0 + wave * 32, A);              // the wave's first token
   const int64_t at = rows_at(A, b, hk, S.q0) + row;
-  const float lse = row < nrows ? G.lse[at] : 0.0f;
+  const float top = row < nrows ? G.top[at] : 0.0f, base = top == -INFINITY ? 0.0f : top;
   const bool there = row < nrows && (!A.qmask || A.qmask[b * A.tq + t]);
   u32x4 q[T::kK], d[T::kK], o[T::kK], rest[T::kK];
   own_row<T>(q, wave_rows<Op>(A.q, seq_at(A.qs, A.cu_q, b, S.q0) + (int64_t)hk * A.group * A.qs[2], wt, A.qs[1]),
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
   if (!__syncthreads_or(there)) {  // padding: zeros, and no keys are read
     store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), place, acc, 0.0f, A.units, h);
-    if (h == 0 && row < nrows) G.delta[at] = 0.0f;
+    if (h == 0 && row < nrows) G.delta[at] = G.level[at] = 0.0f;
     return;
   }
   const Reaches wide = reaches(reach(row0 + wave * 32), reach(row0 + wave * 32 + 31), __any(there));
@@ -207,8 +211,8 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   if (h == 0 && row < nrows) G.delta[at] = delta;
   float by = 1.0f;
   if constexpr (kShift<Op> != 0.0f) by = scale_below_one(norm, peak(G.peaks, unit, 0));
-  const float c = fabsf(A.scale) * kLog2e;
-  const float off = lse > -INFINITY ? kShift<Op> - lse : 0.0f;  // (no key counts: nothing to make infinite)
+  const float c = factor(A);
+  float l = 0.0f;  // of this half's keys
   if (A.scale < 0) negate<T>(q);
 
   const char* kbase = static_cast<const char*>(A.k) + (seq_at(A.ks, A.cu_k, b, S.k0) + (int64_t)hk * A.ks[2]) * Op::kEsz;
@@ -254,16 +258,22 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
           x = mma<Op>(T::rows(K, 32 * half, kb, lane), q[kb], x);
           y = mma<Op>(T::rows(V, 32 * half, kb, lane), d[kb], y);
         }
-        float s[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, off)) * ((y[r] - delta) * by);
         if (!whole_tile) {
           const int j = now + 32 * half;
           const uint32_t keep = (w[half] & bits_between(mine.lo - j, mine.hi - j)) >> (4 * h);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = masked(s[r], keep, r, 0.0f);
+          for (int r = 0; r < 16; ++r) x[r] = masked(x[r], keep, r, -INFINITY);
         }
+        float s[16], sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - base, c, kShift<Op>));
+          sum += s[r];
+          s[r] *= (y[r] - delta) * by;
+          // (four at a time: all sixteen at once take as many registers more, and a wave of each SIMD with them)
+          if (r % 4 == 3) asm volatile("" : "+v"(sum), "+v"(s[r]));
+        }
+        l += sum;
         constexpr int kPer = 32 / kGroups<Op>;
 #pragma unroll
         for (int g = 0; g < kGroups<Op>; ++g) {
@@ -275,11 +285,17 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
       }
     }
   }
-  if (A.qmask && !there)
+  l += __builtin_bit_cast(float, lane_xor32(__builtin_bit_cast(uint32_t, l), h));
+  if (A.qmask && !there) {
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) acc[i] = f32x16{};
-  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), place, acc, A.scale * kUnshift<Op> / by, A.units,
-                            h);
+    l = 0.0f;
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (no key counts: the sums are zeros)
+  store_row<Op, T::kBlocks>(wave_rows<Op>(G.dq, start, wt, width), place, acc, A.scale / by * inv, A.units, h);
+  // (what the second kernel's exponents take, or in fp32, where that would cost bits, its exponentials are multiplied by)
+  if (h == 0 && row < nrows)
+    G.level[at] = Op::kEsz == 4 ? inv : inv > 0.0f ? 2.0f * kShift<Op> - __builtin_amdgcn_logf(l) : inv;
 }
 
 // `splits` workgroups share the rows of a tile of keys; with more than one their sums go to `parts`:
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
     attn_dkv_kernel(AttnArgs A, AttnGrads G, float* parts, uint32_t splits, uint32_t tiles, uint32_t work) {
   typedef Tile<Op, kD> T;
   constexpr int kThreads = kWaves * 64;
-  constexpr int kBuffer = 2 * T::kBytes + 2 * kRows * 4;  // q, do, lse, delta
+  constexpr int kBuffer = 2 * T::kBytes + 3 * kRows * 4;  // q, do, top, delta, level
   __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer + kMaskSpan / 8];
   uint64_t* const words = reinterpret_cast<uint64_t*>(lds + 2 * kBuffer);
   const uint32_t piece = piece_of(work);
@@ -342,7 +358,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
   for (int i = 0; i < T::kBlocks; ++i) dk[i] = dv[i] = f32x16{};
   if (!__syncthreads_or(there)) last = first;  // (padding: zeros, and no rows are read)
   const Reaches wide = reaches(reach(key0 + wave * 32), reach(key0 + wave * 32 + 31), __any(there));
-  const float c = fabsf(A.scale) * kLog2e;
+  const float c = factor(A);
   if (A.scale < 0) negate<T>(k);
   float by = 1.0f;
   if constexpr (kShift<Op> != 0.0f) by = scale_below_one(peak(G.peaks, unit, 1), peak(G.peaks, unit, 0));
@@ -365,14 +381,12 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
       char* const base = lds + buffer * kBuffer;
       T::template request_rows<kThreads>(base, qbase, A.qs[1], A.qs[2], A.units, r0, A, bits);
       T::template request_rows<kThreads>(base + T::kBytes, dbase, A.heads * width, width, A.units, r0, A, bits);
-      if (wave < 2 || kWaves == 1) {
-#pragma unroll
-        for (int i = 0; i < (kWaves == 1 ? 2 : 1); ++i) {
-          const int which = kWaves == 1 ? i : wave;
-          const rsrc_t from_stat = make_rsrc_u((which ? G.delta : G.lse) + stat + r0, 0x7fffffffu);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(from_stat, (lds_ptr)(base + 2 * T::kBytes + which * kRows * 4), 4,
-                                                   r0 + lane < to ? lane * 4 : kFar, 0, 0, 0);
-        }
+      static_assert(kWaves >= 3, "a wave for each of a row's numbers");
+      if (wave < 3) {
+        const float* const of = wave == 0 ? G.top : wave == 1 ? G.delta : G.level;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc_u(of + stat + r0, 0x7fffffffu),
+                                                 (lds_ptr)(base + 2 * T::kBytes + wave * kRows * 4), 4,
+                                                 r0 + lane < to ? lane * 4 : kFar, 0, 0, 0);
       }
     };
     uint64_t bits, bits1;  // of this tile, and of the next
@@ -385,7 +399,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
       if (r1 < to) request(r1, bits1, buffer ^ 1);
       const char* const Q = lds + buffer * kBuffer;
       const char* const D = Q + T::kBytes;
-      const float* const lse = reinterpret_cast<const float*>(D + T::kBytes);
+      const float* const top = reinterpret_cast<const float*>(D + T::kBytes);
       const bool none = r0 >= wide.any.hi || r0 + kRows <= wide.any.lo;
       const int now = r0;
       const uint32_t w[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
@@ -429,12 +443,17 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
         float p[16], ds[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + 32 * half + 8 * g + 4 * h);
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(lse + kRows + 32 * half + 8 * g + 4 * h);
+          const float* const of = top + 32 * half + 8 * g + 4 * h;
+          const f32x4 t4 = *reinterpret_cast<const f32x4*>(of);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(of + kRows);
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(of + 2 * kRows);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, kShift<Op> - l4[e]));
+            if constexpr (Op::kEsz == 4)
+              p[r] = __builtin_amdgcn_exp2f((x[r] - t4[e]) * c) * l4[e];
+            else
+              p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - t4[e], c, l4[e]));
             ds[r] = p[r] * ((y[r] - d4[e]) * by);
           }
         }

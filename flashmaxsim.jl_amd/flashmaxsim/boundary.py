@@ -818,29 +818,29 @@ def _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k):
             ptr(cu_q), ptr(cu_k), seqs, max_q, max_k, nq, nk, heads, kv_heads, dim)
 
 
-def launch_attention(o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, scale, causal,
+def launch_attention(o, top, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, scale, causal,
                      window):
-    """o <- attention of q over k and v; lse and rest (both or neither) keep what the pullback needs."""
+    """o <- attention of q over k and v; top and rest (both or neither) keep what the pullback needs."""
     dev = _heads(q, k, v)
     _check_block(o, (q.shape, "o rest", (o, rest)))
     args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
-    if lse is not None:
-        _buf(_beside(lse, dev), "lse", torch.float32, q.shape[:-1].numel())
-    st = _call_with_workspace(_lib.lib().fms_attention, dev, dtype_code(q), o.data_ptr(), ptr(lse),
+    if top is not None:
+        _buf(_beside(top, dev), "top", torch.float32, q.shape[:-1].numel())
+    st = _call_with_workspace(_lib.lib().fms_attention, dev, dtype_code(q), o.data_ptr(), ptr(top),
                               ptr(rest), *args, scale, causal, window, stream_handle(dev))
     if st:
         _lib.check(st, "launch_attention")
 
 
-def attention_apply_pullback(dq, dk, dv, do, o, lse, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q,
+def attention_apply_pullback(dq, dk, dv, do, o, top, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q,
                              max_k, scale, causal, window):
-    """dq, dk, dv <- pullback of do; o, lse and rest are the forward's."""
+    """dq, dk, dv <- pullback of do; o, top and rest are the forward's."""
     dev = _heads(q, k, v)
     _check_block(dq, (q.shape, "dq do o rest", (dq, do, o, rest)), (k.shape, "dk dv", (dk, dv)))
     args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
-    _buf(_beside(lse, dev), "lse", torch.float32, q.shape[:-1].numel())
+    _buf(_beside(top, dev), "top", torch.float32, q.shape[:-1].numel())
     st = _call_with_workspace(_lib.lib().fms_attention_pullback, dev, dtype_code(q), dq.data_ptr(),
-                              dk.data_ptr(), dv.data_ptr(), do.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                              dk.data_ptr(), dv.data_ptr(), do.data_ptr(), o.data_ptr(), top.data_ptr(),
                               ptr(rest), *args, scale, causal, window, stream_handle(dev))
     if st:
         _lib.check(st, "attention_apply_pullback")

@@ -159,9 +159,10 @@ def head_rotary(q, k, table, positions=None, *, q_weight=None, k_weight=None, ki
 # ---- attention -----------------------------------------------------------------------------
 
 class AttentionKept(NamedTuple):
-    """What ``attention_pullback`` needs of the forward beside its output: base-2 logarithms of the
-    rows' sums, and what the output's rounding left (None in float32)."""
-    lse: torch.Tensor
+    """What ``attention_pullback`` needs of the forward beside its output: the rows' largest q k (of the
+    other sign under a negative scale; -inf where a query sees no key), and what the output's rounding
+    left (None in float32)."""
+    top: torch.Tensor
     rest: torch.Tensor | None
 
 
@@ -208,15 +209,15 @@ def attention_forward(q, k, v, qmask=None, kmask=None, *, cu_q=None, cu_k=None, 
     """o (q's shape), dense; with ``keep`` (o, kept) for ``attention_pullback``.  See ``attention``."""
     options = _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, window, scale)
     o = q.new_empty(q.shape)
-    lse = rest = None
+    top = rest = None
     if keep:
         *lead, tokens, heads, _ = q.shape
         shared = k.shape[-2]
-        lse = torch.empty((*lead, shared, tokens * (heads // max(shared, 1))), dtype=torch.float32,
+        top = torch.empty((*lead, shared, tokens * (heads // max(shared, 1))), dtype=torch.float32,
                           device=q.device)
         rest = None if q.dtype is torch.float32 else q.new_empty(q.shape)
-    boundary.launch_attention(o, lse, rest, q, k, v, *options)
-    return (o, AttentionKept(lse, rest)) if keep else o
+    boundary.launch_attention(o, top, rest, q, k, v, *options)
+    return (o, AttentionKept(top, rest)) if keep else o
 
 
 def attention_pullback(do, q, k, v, o, kept, qmask=None, kmask=None, *, cu_q=None, cu_k=None, max_q=None,
@@ -228,7 +229,7 @@ def attention_pullback(do, q, k, v, o, kept, qmask=None, kmask=None, *, cu_q=Non
     if do is None:
         raise DimensionMismatch("do: missing")
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    boundary.attention_apply_pullback(dq, dk, dv, do, o, kept.lse, kept.rest, q, k, v, *options)
+    boundary.attention_apply_pullback(dq, dk, dv, do, o, kept.top, kept.rest, q, k, v, *options)
     return dq, dk, dv
 
 
@@ -243,8 +244,8 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, rest, qmask, kmask, cu_q, cu_k = ctx.saved_tensors
-        grads = attention_pullback(do, q, k, v, o, AttentionKept(lse, rest), qmask, kmask, cu_q=cu_q,
+        q, k, v, o, top, rest, qmask, kmask, cu_q, cu_k = ctx.saved_tensors
+        grads = attention_pullback(do, q, k, v, o, AttentionKept(top, rest), qmask, kmask, cu_q=cu_q,
                                    cu_k=cu_k, **ctx.args)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 5
 

@@ -955,7 +955,7 @@ end
 
 """
     attention(q, k, v, qmask = nothing, kmask = nothing; cu_q, cu_k, max_q, max_k, causal = false,
-              window = -1, scale = dim^-0.5, keep = false) -> o, or (o, (lse, rest)) with `keep`
+              window = -1, scale = dim^-0.5, keep = false) -> o, or (o, (top, rest)) with `keep`
 
 `softmax(scale q'k) v` over heads; q (dim, heads, T, B), k and v with as many or fewer heads, masks (T, B).
 Ragged sequences: token rows (dim, heads, N) with `PackedSeq`'s 1-based `cu`.  A query sees keys that
@@ -970,17 +970,17 @@ function attention(q::ROCArray{T}, k::ROCArray{T}, v::ROCArray{T},
     seqs, tq, tk, nq, nk, heads, kv_heads, dim =
         attention_sizes(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
     o = similar(q)
-    lse = keep ? similar(q, Float32, size(q)[2:end]) : nothing
+    top = keep ? similar(q, Float32, size(q)[2:end]) : nothing
     rest = keep && T !== Float32 ? similar(q) : nothing
     check(ccall((:fms_attention, libfms), Int32,
                 (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
                  Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64,
                  Int64, Int64, Int64, Int64, Float32, Int32, Int64, Ptr{Cvoid}),
-                dtype_code(T), dptr(o), dptr(lse), dptr(rest), dptr(q), dptr(k), dptr(v), C_NULL,
+                dtype_code(T), dptr(o), dptr(top), dptr(rest), dptr(q), dptr(k), dptr(v), C_NULL,
                 dptr(qmask), dptr(kmask), dptr(cu_q), dptr(cu_k), seqs, tq, tk, nq, nk, heads, kv_heads,
                 dim, Float32(something(scale, max(dim, 1)^-0.5)), Int32(causal), window, stream_ptr()),
           "attention")
-    keep ? (o, (lse, rest)) : o
+    keep ? (o, (top, rest)) : o
 end
 
 """
@@ -1000,8 +1000,8 @@ function attention_pullback(dout::ROCArray{T}, q::ROCArray{T}, k::ROCArray{T}, v
         attention_sizes(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
     same_size(dout, q, "dout")
     same_size(o, q, "o")
-    lse, rest = kept
-    length(lse) == length(q) ÷ max(dim, 1) || throw(DimensionMismatch("lse"))
+    top, rest = kept
+    length(top) == length(q) ÷ max(dim, 1) || throw(DimensionMismatch("top"))
     T === Float32 || same_size(rest, q, "rest")
     dq, dk, dv = similar(q), similar(k), similar(v)
     check(ccall((:fms_attention_pullback, libfms), Int32,
@@ -1009,7 +1009,7 @@ function attention_pullback(dout::ROCArray{T}, q::ROCArray{T}, k::ROCArray{T}, v
                  Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
                  Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Int64, Float32,
                  Int32, Int64, Ptr{Cvoid}),
-                dtype_code(T), dptr(dq), dptr(dk), dptr(dv), dptr(dout), dptr(o), dptr(lse), dptr(rest),
+                dtype_code(T), dptr(dq), dptr(dk), dptr(dv), dptr(dout), dptr(o), dptr(top), dptr(rest),
                 dptr(q), dptr(k), dptr(v), C_NULL, dptr(qmask), dptr(kmask), dptr(cu_q), dptr(cu_k),
                 seqs, tq, tk, nq, nk, heads, kv_heads, dim,
                 Float32(something(scale, max(dim, 1)^-0.5)), Int32(causal), window, stream_ptr()),

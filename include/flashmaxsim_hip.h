@@ -520,13 +520,13 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
  * strides and masks are not used (masks NULL).  A longer sequence is cut to tq and tk; rows
  * of no sequence give zeros.  nq and nk are not read for padded sequences.
  *
- * lse and rest, both or neither, keep what the pullback needs: lse seqs * tq * heads (ragged:
- * nq * heads) floats, rest like o (what o's rounding left; not
- * written, and may be NULL, for FMS_F32).  Values that count
+ * top and rest, both or neither, keep what the pullback needs: top seqs * tq * heads (ragged:
+ * nq * heads) floats (the rows' largest q k, of the other sign under a negative scale; -inf where
+ * no key counts), rest like o (what o's rounding left; not written, and may be NULL, for FMS_F32).  Values that count
  * for some query of a sequence should be finite: under causal and window an infinite value also
  * makes rows NaN that share a tile with it.  dim is at most 128, tq and tk are below 2^29.
  */
-fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const void* q, const void* k,
+fms_status fms_attention(int32_t dtype, void* o, float* top, void* rest, const void* q, const void* k,
                          const void* v, const int64_t* strides, const uint8_t* qmask,
                          const uint8_t* kmask, const int32_t* cu_q, const int32_t* cu_k, int64_t seqs,
                          int64_t tq, int64_t tk, int64_t nq, int64_t nk, int64_t heads,
@@ -535,11 +535,11 @@ fms_status fms_attention(int32_t dtype, void* o, float* lse, void* rest, const v
 
 /*
  * Its pullback for the cotangent dout (dense, like o): dq, dk and dv, dense, overwritten in full.
- * o, lse and rest are what fms_attention gave for the same arguments; the probabilities are
+ * o, top and rest are what fms_attention gave for the same arguments; the probabilities are
  * computed again.  Cotangents of masked queries are not read.  Deterministic.
  */
 fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, const void* dout,
-                                  const void* o, const float* lse, const void* rest, const void* q,
+                                  const void* o, const float* top, const void* rest, const void* q,
                                   const void* k, const void* v, const int64_t* strides,
                                   const uint8_t* qmask, const uint8_t* kmask, const int32_t* cu_q,
                                   const int32_t* cu_k, int64_t seqs, int64_t tq, int64_t tk,

@@ -85,3 +85,15 @@ def test_first_of_a_causal_sequence(dtype, scale, device):
     o, dq, _, _ = both(q, k, v, do, causal=True, scale=scale)
     assert torch.equal(o[:, 0], v[:, 0])
     assert not dq[:, 0].any() and dq[:, 1:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1.0, 30.0, 100.0])
+@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("scale", [None, 2.0, -0.7])
+def test_value_gradients(dtype, size, d, scale, device):
+    """Each key seen by one query alone: dv is that query's cotangent, however large the score."""
+    q, k, v, do = inputs((2, 200, 2, d), (2, 200, 2, d), dtype, device, size)
+    assert torch.equal(both(q, k, v, do, window=0, scale=scale)[3], do)
+    q, k, v, do = inputs((30, 1, 3, d), (30, 1, 3, d), dtype, device, size)
+    assert torch.equal(both(q, k, v, do, scale=scale)[3], do)

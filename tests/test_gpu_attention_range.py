@@ -79,3 +79,38 @@ def test_forward(dtype, name, shape, device):
     o = fm.attention_forward(q, k, v, scale=scale)
     close(o, p @ V, ((off + rough) * p) @ V.abs() + grid * V.abs().sum(1, keepdim=True), "o")
     assert torch.equal(o, fm.attention_forward(-q, k, v, scale=-scale))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", SCORES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_pullback(dtype, name, shape, device):
+    """ds = p (dp - delta): dp and delta are sums over a head's values, delta of the output, which in 16 bits
+    comes with what its rounding left."""
+    q, k, v, do, scale = inputs(name, *shape, dtype, device)
+    Tq, Tk, H, Hk, d = shape
+    group = H // Hk
+    p, off = weights(wide(q), wide(k, group), scale, dtype)
+    Q, K, V, D = wide(q), wide(k, group), wide(v, group), wide(do)
+    rough, grid = rounding(dtype)
+    half = torch.finfo(dtype).eps / 2
+    dp = D @ V.transpose(1, 2).contiguous()
+    dp_size = D.abs() @ V.abs().transpose(1, 2).contiguous()
+    delta, delta_size = (p * dp).sum(-1, keepdim=True), (p * dp_size).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    left = half if dtype == torch.float32 else 4 * half * half
+    delta_off = (UNIT * (d + 8) + left + rough) * delta_size + (off * p * dp_size).sum(-1, keepdim=True) \
+        + grid * dp_size.sum(-1, keepdim=True)
+    ds_off = p * (UNIT * (d + 8) * dp_size + delta_off) + (off + rough) * ds.abs()
+    if dtype == torch.float16:  # ds on its grid: 2^15 p times a factor that brings 2 |do| |v| to 1/2 at least
+        ds_off = ds_off + 4 * D.norm(dim=-1).amax() * V.norm(dim=-1).amax() * 2.0 ** -40
+    sums = UNIT * (Tq * group + Tk)
+    turned = lambda t: t.transpose(1, 2).contiguous()  # noqa: E731
+    share = lambda t: t.view(Hk, group, *t.shape[1:]).sum(1)  # noqa: E731
+    o, kept = fm.attention_forward(q, k, v, scale=scale, keep=True)
+    dq, dk, dv = fm.attention_pullback(do, q, k, v, o, kept, scale=scale)
+    close(dq, scale * ds @ K, scale * ((ds_off + sums * ds.abs()) @ K.abs()), "dq")
+    close(dk, share(scale * turned(ds) @ Q), share(scale * turned(ds_off + sums * ds.abs()) @ Q.abs()), "dk")
+    close(dv, share(turned(p) @ D), share(turned((off + rough + sums) * p + grid) @ D.abs()), "dv")
+    assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), (lambda x: (-x[0], x[1], x[2]))(
+        fm.attention_pullback(do, -q, k, v, o, kept, scale=-scale))))
