@@ -62,9 +62,9 @@ __global__ void __launch_bounds__(kWaves * 64, (kSimdWaves<Op, kD, kWaves>))
   if (piece >= work) return;
   const uint32_t whole = kSplit ? piece / (uint32_t)P.splits : piece;
   const int split = (int)(piece - whole * (kSplit ? (uint32_t)P.splits : 1u));
-  const uint32_t unit = whole / tiles;
+  const uint32_t nth = whole / tiles, unit = A.unit0 + nth;
   // (under a causal mask the last tiles have the most keys: they start first)
-  const int tile = (int)(A.causal ? tiles - 1 - (whole - unit * tiles) : whole - unit * tiles);
+  const int tile = (int)(A.causal ? tiles - 1 - (whole - nth * tiles) : whole - nth * tiles);
   const int64_t b = unit / (uint32_t)A.kv_heads;
   const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
@@ -370,9 +370,10 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
     const hipError_t ef = workspace_free(mem, stream);
     return e != hipSuccess ? e : ef;
   }
-  hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(pieces)), dim3(kWaves * 64), 0,
-                     stream, a, out, Parts{}, (uint32_t)tiles, (uint32_t)pieces);
-  return hipGetLastError();
+  return by_units(a, tiles, [&](const AttnArgs& part, int64_t n) {
+    hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(n * tiles)), dim3(kWaves * 64), 0,
+                       stream, part, out, Parts{}, (uint32_t)tiles, (uint32_t)(n * tiles));
+  });
 }
 
 template <class Op, int kD>

@@ -30,6 +30,7 @@ struct AttnArgs {
   int32_t window;  // < 0: none
   float scale;
   int64_t seqs;
+  uint32_t unit0;      // first (sequence, key head) of a launch
   int32_t tq, tk;      // tokens of a sequence, or of the longest one
   int64_t nq, nk;      // token rows in all
   const void *q, *k, *v;
@@ -140,6 +141,20 @@ __device__ __forceinline__ uint32_t piece_of(uint32_t work) {
   return (blockIdx.x & 7) * ((work + 7) / 8) + (blockIdx.x >> 3);
 }
 inline unsigned piece_blocks(int64_t work) { return (unsigned)((work + 7) / 8 * 8); }
+// launch(args, units) for all units, so many at a time that a launch's threads, up to 256 for each of a unit's `pieces`,
+// can be counted in 32 bits.  (A unit has at most 2^30 rows, 2^23 pieces.)
+constexpr int64_t kMostPieces = (int64_t)1 << 23;
+template <class F>
+hipError_t by_units(AttnArgs a, int64_t pieces, F&& launch) {
+  const int64_t units = a.seqs * a.kv_heads, most = pieces < kMostPieces ? kMostPieces / (pieces > 0 ? pieces : 1) : 1;
+  for (int64_t u = 0; u < units; u += most) {
+    a.unit0 = (uint32_t)u;
+    launch(a, units - u < most ? units - u : most);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
 
 // The keys that count by position for a query token, or the tokens that count for a key: [lo, hi).
 struct Reach {

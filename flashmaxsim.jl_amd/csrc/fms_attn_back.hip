@@ -83,7 +83,7 @@ __device__ __forceinline__ float diagonal(const f32x16& x, int lane) {
 // Largest squared norms of a unit's v and do rows, in kAttnPeakParts parts.
 __global__ void __launch_bounds__(256) attn_peaks_kernel(AttnArgs A, AttnGrads G) {
   __shared__ float lds[4][2];
-  const int64_t unit = blockIdx.x / kAttnPeakParts;
+  const int64_t unit = A.unit0 + blockIdx.x / kAttnPeakParts;
   const int part = blockIdx.x % kAttnPeakParts;
   const int64_t b = unit / A.kv_heads;
   const int hk = (int)(unit % A.kv_heads);
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256) attn_peaks_kernel(AttnArgs A, AttnGrads G
   __syncthreads();
   if (threadIdx.x < 2) {
     const int i = threadIdx.x;
-    G.peaks[(int64_t)blockIdx.x * 2 + i] = fmaxf(fmaxf(lds[0][i], lds[1][i]), fmaxf(lds[2][i], lds[3][i]));
+    G.peaks[(unit * kAttnPeakParts + part) * 2 + i] = fmaxf(fmaxf(lds[0][i], lds[1][i]), fmaxf(lds[2][i], lds[3][i]));
   }
 }
 __device__ __forceinline__ float peak(const float* peaks, int64_t unit, int which) {
@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
   uint64_t* const words = reinterpret_cast<uint64_t*>(lds + 4 * T::kBytes);
   const uint32_t piece = piece_of(work);
   if (piece >= work) return;
-  const uint32_t unit = piece / tiles;
-  const int tile = (int)(A.causal ? tiles - 1 - (piece - unit * tiles) : piece - unit * tiles);
+  const uint32_t nth = piece / tiles, unit = A.unit0 + nth;
+  const int tile = (int)(A.causal ? tiles - 1 - (piece - nth * tiles) : piece - nth * tiles);
   const int64_t b = unit / (uint32_t)A.kv_heads;
   const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
@@ -311,8 +311,8 @@ __global__ void __launch_bounds__(kWaves * 64, 1)
   const uint32_t piece = piece_of(work);
   if (piece >= work) return;
   const uint32_t shared = piece / splits, split = piece - shared * splits;
-  const uint32_t unit = shared / tiles;
-  const int tile = (int)(shared - unit * tiles);  // (under a causal mask the first tiles have the most rows)
+  const uint32_t nth = shared / tiles, unit = A.unit0 + nth;
+  const int tile = (int)(shared - nth * tiles);  // (under a causal mask the first tiles have the most rows)
   const int64_t b = unit / (uint32_t)A.kv_heads;
   const int hk = (int)(unit % (uint32_t)A.kv_heads);
   const Span S = span_of(A, b);
@@ -536,11 +536,12 @@ constexpr int kWaves = 4;
 
 template <class Op, int kD>
 hipError_t launch_dq(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
-  const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), work = a.seqs * a.kv_heads * tiles;
-  if (work)
-    hipLaunchKernelGGL((attn_dq_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
-                       (uint32_t)tiles, (uint32_t)work);
-  return hipGetLastError();
+  const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves);
+  if (!tiles) return hipSuccess;
+  return by_units(a, tiles, [&](const AttnArgs& part, int64_t n) {
+    hipLaunchKernelGGL((attn_dq_kernel<Op, kD, kWaves>), dim3(piece_blocks(n * tiles)), dim3(kWaves * 64), 0, stream,
+                       part, g, (uint32_t)tiles, (uint32_t)(n * tiles));
+  });
 }
 
 // Few workgroups of many rows each: the rows of a tile of keys are shared out, eight tiles of them to a
@@ -556,10 +557,14 @@ int64_t dkv_splits(const AttnArgs& a) {
 
 template <class Op, int kD>
 hipError_t launch_dkv(const AttnArgs& a, const AttnGrads& g, float* parts, int64_t splits, hipStream_t stream) {
-  const int64_t units = a.seqs * a.kv_heads, tiles = cdiv(a.tk, 32 * kWaves), work = units * tiles * splits;
-  if (!work) return hipSuccess;
-  hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, a, g,
-                     parts, (uint32_t)splits, (uint32_t)tiles, (uint32_t)work);
+  const int64_t units = a.seqs * a.kv_heads, tiles = cdiv(a.tk, 32 * kWaves);
+  if (!tiles) return hipSuccess;
+  const hipError_t e = by_units(a, tiles * splits, [&](const AttnArgs& part, int64_t n) {
+    const int64_t work = n * tiles * splits;
+    hipLaunchKernelGGL((attn_dkv_kernel<Op, kD, kWaves>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0, stream, part,
+                       g, parts, (uint32_t)splits, (uint32_t)tiles, (uint32_t)work);
+  });
+  if (e != hipSuccess) return e;
   if (splits > 1)
     hipLaunchKernelGGL((attn_dkv_join_kernel<Op, kD>), dim3((unsigned)cdiv(units * a.tk * (kD / 4), 256), 2), dim3(256),
                        0, stream, a, g, static_cast<const float*>(parts), (int)splits);
@@ -574,8 +579,10 @@ hipError_t pullback_dim(const AttnArgs& a, const AttnGrads& g, hipStream_t strea
   if (splits > 1) e = workspace_alloc(&parts, (size_t)(splits * 2 * units * a.tk * kD * 4), stream, true);
   if (e != hipSuccess) return e;
   if (std::is_same<Op, OpF16>::value)
-    hipLaunchKernelGGL(attn_peaks_kernel, dim3((unsigned)(units * kAttnPeakParts)), dim3(256), 0, stream, a, g);
-  e = launch_dq<Op, kD>(a, g, stream);
+    e = by_units(a, kAttnPeakParts, [&](const AttnArgs& part, int64_t n) {
+      hipLaunchKernelGGL(attn_peaks_kernel, dim3((unsigned)(n * kAttnPeakParts)), dim3(256), 0, stream, part, g);
+    });
+  if (e == hipSuccess) e = launch_dq<Op, kD>(a, g, stream);
   if (e == hipSuccess) e = launch_dkv<Op, kD>(a, g, static_cast<float*>(parts), splits, stream);
   const hipError_t ef = parts ? workspace_free(parts, stream) : hipSuccess;
   return e != hipSuccess ? e : ef;

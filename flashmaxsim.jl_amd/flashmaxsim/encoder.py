@@ -266,7 +266,8 @@ def attention(q, k, v, qmask=None, kmask=None, *, cu_q=None, cu_k=None, max_q=No
     A query that sees none gives zeros.  Ragged sequences come as token rows q (Nq, heads, dim), k and
     v (Nk, kv_heads, dim) with the 1-based Int32 ``cu`` of a ``PackedSeq`` (cu_q and cu_k, one array
     twice for self-attention) and the longest lengths, max_q and max_k (the token counts if not given:
-    as right, and slower); masks are for padded sequences.
+    as right, but the work is laid out for sequences of that length, so many of them take long, and very
+    many are refused); masks are for padded sequences.
 
     The pullback computes the probabilities again; kept for it are the inputs, the output, and 4
     bytes a query and head and (16-bit types) what the output's rounding left.  dim is at most 128."""

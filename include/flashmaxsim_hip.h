@@ -524,7 +524,8 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
  * nq * heads) floats (the rows' largest q k, of the other sign under a negative scale; -inf where
  * no key counts), rest like o (what o's rounding left; not written, and may be NULL, for FMS_F32).  Values that count
  * for some query of a sequence should be finite: under causal and window an infinite value also
- * makes rows NaN that share a tile with it.  dim is at most 128, tq and tk are below 2^29.
+ * makes rows NaN that share a tile with it.  dim is at most 128, tq and tk are below 2^29, and
+ * seqs * kv_heads * (max(tq * heads / kv_heads, tk) / 32 + 1) is below 2^27.
  */
 fms_status fms_attention(int32_t dtype, void* o, float* top, void* rest, const void* q, const void* k,
                          const void* v, const int64_t* strides, const uint8_t* qmask,
