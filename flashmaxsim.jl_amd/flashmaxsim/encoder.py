@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import boundary
@@ -272,6 +273,8 @@ def attention(q, k, v, qmask=None, kmask=None, *, cu_q=None, cu_k=None, max_q=No
     The pullback computes the probabilities again; kept for it are the inputs, the output, and 4
     bytes a query and head and (16-bit types) what the output's rounding left.  dim is at most 128."""
     args = dict(max_q=max_q, max_k=max_k, causal=causal, window=window, scale=scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    # (forward mode's dual tensors need no gradient; the recorded call refuses them, as the other verbs do)
+    if (forward_ad._current_level >= 0
+            or torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         return _Attention.apply(q, k, v, qmask, kmask, cu_q, cu_k, args)
     return attention_forward(q, k, v, qmask, kmask, cu_q=cu_q, cu_k=cu_k, **args)
