@@ -669,24 +669,24 @@ def varlen_apply_pullback(dQ, dD, Qp, Dp, cu_q, cu_d, args, Delta, inv_n):
 
 # ---- token block (no reference method) --------------------------------------------------
 
-def _check_block(x, *groups):
+def _check_block(x, *groups, dense=True):
     """Device, density, eltype and shapes of a call's arrays: groups of (shape, names, arrays), an
-    array None where it is not given.  The device."""
+    array None where it is not given.  The device.  (Not dense: x lies as it likes.)"""
     dtype, at = x.dtype, x.get_device()
-    good = at >= 0 and x.is_contiguous()
+    good = at >= 0 and (not dense or x.is_contiguous())
     for shape, _, arrays in groups:
         for t in arrays:
             if t is not None:
                 good = (good and t.dtype is dtype and t.shape == shape and t.get_device() == at
                         and t.is_contiguous())
     if not good:
-        _refuse_block(x, groups)
+        _refuse_block(x, groups, dense)
     return x.device
 
 
-def _refuse_block(x, groups):
+def _refuse_block(x, groups, dense):
     """Says what _check_block found."""
-    require_device(x, *(t for _, _, arrays in groups for t in arrays))
+    require_device(x if dense else x.new_empty(0), *(t for _, _, arrays in groups for t in arrays))
     for shape, names, arrays in groups:
         for what, t in zip(names.split(), arrays):
             if t is None:
@@ -802,7 +802,10 @@ def _beside(t, dev):
 def _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k):
     """The sizes and pointers that both attention calls take, after the checks of masks and cu."""
     *lead, nq, heads, dim = q.shape
-    nk, kv_heads = k.shape[-3:-1]
+    *lead_k, nk, kv_heads, dim_k = k.shape
+    if v.shape != k.shape or dim_k != dim or lead_k != lead:
+        raise DimensionMismatch(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be alike, and have q's batch and dim: "
+                                f"q is {tuple(q.shape)}")
     if cu_q is not None:
         seqs = cu_q.numel() - 1
         _cu(_beside(cu_q, dev), "cu_q", seqs + 1)
@@ -822,7 +825,7 @@ def launch_attention(o, top, rest, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max
                      window):
     """o <- attention of q over k and v; top and rest (both or neither) keep what the pullback needs."""
     dev = _heads(q, k, v)
-    _check_block(o, (q.shape, "o rest", (o, rest)))
+    _check_block(q, (q.shape, "o rest", (o, rest)), dense=False)
     args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
     if top is not None:
         _buf(_beside(top, dev), "top", torch.float32, q.shape[:-1].numel())
@@ -836,7 +839,7 @@ def attention_apply_pullback(dq, dk, dv, do, o, top, rest, q, k, v, qmask, kmask
                              max_k, scale, causal, window):
     """dq, dk, dv <- pullback of do; o, top and rest are the forward's."""
     dev = _heads(q, k, v)
-    _check_block(dq, (q.shape, "dq do o rest", (dq, do, o, rest)), (k.shape, "dk dv", (dk, dv)))
+    _check_block(q, (q.shape, "dq do o rest", (dq, do, o, rest)), (k.shape, "dk dv", (dk, dv)), dense=False)
     args = _attention_call(dev, q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
     _buf(_beside(top, dev), "top", torch.float32, q.shape[:-1].numel())
     st = _call_with_workspace(_lib.lib().fms_attention_pullback, dev, dtype_code(q), dq.data_ptr(),
@@ -850,6 +853,8 @@ def _rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps):
     """The arguments that both calls take from the heads on, after the checks of the others."""
     *lead, heads, dim = shape = q.shape
     tokens, seqs = lead[-1], lead[0] if len(lead) == 2 else 1
+    if k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != dim):
+        raise DimensionMismatch(f"k {tuple(k.shape)} must have q's tokens and dim: q is {tuple(shape)}")
     rows, turned = table.shape if table.dim() == 2 else (-1, 0)
     _beside(table, dev)
     if table.dtype is not torch.float32:
@@ -885,7 +890,7 @@ def _rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps):
 def launch_head_rotary(q_out, k_out, q, k, table, positions, wq, wk, kind, pairing, eps):
     """q_out, k_out <- norm and rotation of the heads of q and k (k, k_out may be None)."""
     dev = _heads(q) if k is None else _heads(q, k)
-    _check_block(q_out, (q.shape, "q_out", (q_out,)), (None if k is None else k.shape, "k_out", (k_out,)))
+    _check_block(q, (q.shape, "q_out", (q_out,)), (None if k is None else k.shape, "k_out", (k_out,)), dense=False)
     st = _lib.lib().fms_head_rotary(dtype_code(q), q_out.data_ptr(), ptr(k_out),
                                     *_rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps),
                                     stream_handle(dev))
@@ -896,9 +901,9 @@ def launch_head_rotary(q_out, k_out, q, k, table, positions, wq, wk, kind, pairi
 def head_rotary_apply_pullback(dq, dk, dwq, dwk, dq_out, dk_out, q, k, table, positions, wq, wk, kind,
                                pairing, eps):
     dev = _heads(q) if k is None else _heads(q, k)
-    _check_block(dq, (q.shape, "dq dq_out", (dq, dq_out)),
+    _check_block(q, (q.shape, "dq dq_out", (dq, dq_out)),
                  (None if k is None else k.shape, "dk dk_out", (dk, dk_out)),
-                 (q.shape[-1:], "dq_weight dk_weight", (dwq, dwk)))
+                 (q.shape[-1:], "dq_weight dk_weight", (dwq, dwk)), dense=False)
     st = _call_with_workspace(
         _lib.lib().fms_head_rotary_pullback, dev, dtype_code(q), dq.data_ptr(), ptr(dk), ptr(dwq), ptr(dwk),
         dq_out.data_ptr(), ptr(dk_out), *_rotary_call(dev, q, k, table, positions, wq, wk, kind, pairing, eps),

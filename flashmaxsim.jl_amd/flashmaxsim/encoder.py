@@ -87,8 +87,6 @@ def _rotary_codes(q, k, kind, pairing):
     qs = q.shape
     if len(qs) not in (3, 4):
         raise DimensionMismatch("head_rotary takes q (B, T, heads, dim) or (T, heads, dim)")
-    if k is not None and (k.dim() != len(qs) or k.shape[:-2] != qs[:-2] or k.shape[-1] != qs[-1]):
-        raise DimensionMismatch(f"k {tuple(k.shape)} must have q's tokens and dim: q is {tuple(qs)}")
     if qs[-1] % 2:
         raise DimensionMismatch(f"head_rotary takes heads of an even number of values, got {qs[-1]}")
     return _code(kind, NORMS, "kind"), _code(pairing, PAIRINGS, "pairing")
@@ -174,11 +172,9 @@ def _attention_options(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k, causal, 
     """Shapes of the heads and the options as the boundary takes them (it checks the rest)."""
     qs, ks = q.shape, k.shape
     n = len(qs)
-    if n not in (3, 4) or len(ks) != n or v.shape != ks:
+    if n not in (3, 4) or len(ks) != n:
         raise DimensionMismatch("attention takes q (B, Tq, heads, dim) and k, v (B, Tk, kv_heads, dim), "
                                 "or all of them without B")
-    if qs[-1] != ks[-1] or n == 4 and qs[0] != ks[0]:
-        raise DimensionMismatch(f"q {tuple(qs)} and k {tuple(ks)} differ in batch or dim")
     if qs[-2] != ks[-2] and (not ks[-2] or not qs[-2] or qs[-2] % ks[-2]):
         raise DimensionMismatch(f"{qs[-2]} query heads cannot share {ks[-2]} key heads evenly")
     if cu_q is None and cu_k is None:
