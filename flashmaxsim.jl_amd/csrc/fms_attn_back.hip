@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(256) attn_peaks_kernel(AttnArgs A, AttnGrads G
     s += __shfl_xor(s, 1);
     s += __shfl_xor(s, 2);
     s += __shfl_xor(s, 4);
-    return s;
+    return s < INFINITY ? s : 0.0f;  // (a row that is not finite has no say in the scale of the others)
   };
   const int step = kAttnPeakParts * 32, at = part * 32 + wave * 8 + sub;
   const _Float16* v = static_cast<const _Float16*>(A.v) + seq_at(A.vs, A.cu_k, b, S.k0) + hk * A.vs[2];

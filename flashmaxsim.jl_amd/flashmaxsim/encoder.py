@@ -260,7 +260,9 @@ def attention(q, k, v, qmask=None, kmask=None, *, cu_q=None, cu_k=None, max_q=No
     * are not behind it (``causal``) and at most ``window`` tokens away, the last query beside the
       last key.
 
-    A query that sees none gives zeros.  Ragged sequences come as token rows q (Nq, heads, dim), k and
+    A query that sees none gives zeros.  What counts for some query should be finite: with ``causal`` or a
+    window, a value that is not also makes results and gradients NaN of tokens close by that do not
+    see it (those in reach of the same 64 keys or query rows).  Ragged sequences come as token rows q (Nq, heads, dim), k and
     v (Nk, kv_heads, dim) with the 1-based Int32 ``cu`` of a ``PackedSeq`` (cu_q and cu_k, one array
     twice for self-attention) and the longest lengths, max_q and max_k (the token counts if not given:
     as right, but the work is laid out for sequences of that length, so many of them take long, and very

@@ -523,8 +523,8 @@ fms_status fms_block_norm_pullback(int32_t dtype, void* dx, void* df, void* dgat
  * top and rest, both or neither, keep what the pullback needs: top seqs * tq * heads (ragged:
  * nq * heads) floats (the rows' largest q k, of the other sign under a negative scale; -inf where
  * no key counts), rest like o (what o's rounding left; not written, and may be NULL, for FMS_F32).  Values that count
- * for some query of a sequence should be finite: under causal and window an infinite value also
- * makes rows NaN that share a tile with it.  dim is at most 128, tq and tk are below 2^29, and
+ * for some query of a sequence should be finite: under causal and window v that is not also makes o
+ * NaN of queries that only see keys of the same 64 (counted from the sequence's first).  dim is at most 128, tq and tk are below 2^29, and
  * seqs * kv_heads * (max(tq * heads / kv_heads, tk) / 32 + 1) is below 2^27.
  */
 fms_status fms_attention(int32_t dtype, void* o, float* top, void* rest, const void* q, const void* k,
@@ -537,7 +537,11 @@ fms_status fms_attention(int32_t dtype, void* o, float* top, void* rest, const v
 /*
  * Its pullback for the cotangent dout (dense, like o): dq, dk and dv, dense, overwritten in full.
  * o, top and rest are what fms_attention gave for the same arguments; the probabilities are
- * computed again.  Cotangents of masked queries are not read.  Deterministic.
+ * computed again.  Cotangents of masked queries are not read.  Deterministic.  Beside the gradients that it
+ * belongs to, a value that is not finite reaches, under causal and window, dq of queries that only see
+ * keys of the same 64 (k, v), and dk and dv of keys that only queries of the same 64 rows see (q, dout,
+ * and o that is NaN itself; a row is a token and one of the heads that share a key head).  It reaches
+ * no other sequence and no other key head.
  */
 fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, const void* dout,
                                   const void* o, const float* top, const void* rest, const void* q,
