@@ -89,8 +89,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-// A score's factor, to base 2.  (Not zero, so that a masked score's -inf stays that.)
-__device__ __forceinline__ float factor(const AttnArgs& A) { return fmaxf(fabsf(A.scale) * kLog2e, 1e-30f); }
+// A score's factor, to base 2.  (Not zero, so that a masked score's -inf stays that: the smallest normal number, which
+// makes at most 4 of a score; a NaN stays one.)
+__device__ __forceinline__ float factor(const AttnArgs& A) {
+  const float c = fabsf(A.scale) * kLog2e;
+  return c < 1.17549435e-38f ? 1.17549435e-38f : c;
+}
 constexpr int kFar = (int)0x80000000u;  // a byte offset past every resource: reads as zero
 constexpr int kRows = 64;               // rows of a tile in LDS
 constexpr int kMaskSpan = 16384;        // rows whose mask bits are held at a time

@@ -18,11 +18,12 @@ UNIT = 2.0 ** -24
 # base-2 logarithms of q's and k's common factors, how many bits below the score its steps lie, the scale
 SCORES = {"10": (2, 4, 2.0 ** -5), "1e3": (4, 11, 2.0 ** -3), "3e4": (4, 16, 2.0 ** 2), "4e6": (4, 22, 2.0 ** 8),
           "1e8": (12, 20, 2.0 ** -2), "3e10": (15, 23, 1.0)}
+SMALL = {"2^-108": (60, 20, 2.0 ** -108)}  # a small scale of scores near the end of the range (not in fp16)
 SHAPES = [(70, 100, 2, 2, 64), (130, 90, 4, 2, 128), (1, 3000, 2, 1, 64), (33, 70, 2, 2, 40)]
 
 
 def inputs(name, Tq, Tk, H, Hk, d, dtype, device):
-    factor, bits, scale = SCORES[name]
+    factor, bits, scale = (SCORES | SMALL)[name]
     top = 5 + 2 * factor  # 32 products of 2^factor 2^factor
     g = torch.Generator(device=device).manual_seed(bits)
     q, k = torch.zeros(1, Tq, H, d, device=device), torch.zeros(1, Tk, Hk, d, device=device)
@@ -114,3 +115,19 @@ def test_pullback(dtype, name, shape, device):
     close(dv, share(turned(p) @ D), share(turned((off + rough + sums) * p + grid) @ D.abs()), "dv")
     assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), (lambda x: (-x[0], x[1], x[2]))(
         fm.attention_pullback(do, -q, k, v, o, kept, scale=-scale))))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_small_scale(dtype, shape, device):
+    test_forward(dtype, "2^-108", shape, device)
+    test_pullback(dtype, "2^-108", shape, device)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_number_for_a_scale(dtype, device):
+    q, k, v, do, _ = inputs("10", 33, 70, 2, 2, 40, dtype, device)
+    o, kept = fm.attention_forward(q, k, v, scale=float("nan"), keep=True)
+    assert all(torch.isnan(t).all() for t in (o, *fm.attention_pullback(do, q, k, v, o, kept, scale=float("nan"))))
+    mask = torch.zeros(1, 70, dtype=torch.bool, device=device)
+    assert not fm.attention_forward(q, k, v, kmask=mask, scale=float("nan")).any()
