@@ -941,7 +941,7 @@ function attention_sizes(q, k, v, qmask, kmask, cu_q, cu_k, max_q, max_k)
     ndims(q) == ndims(k) && ndims(q) in (3, 4) && size(q, 1) == size(k, 1) && size(q, 4) == size(k, 4) ||
         throw(DimensionMismatch("q must be (dim, heads, T) or (dim, heads, T, B), k and v alike"))
     heads, kv_heads, nq, nk = size(q, 2), size(k, 2), size(q, 3), size(k, 3)
-    heads == kv_heads || (kv_heads > 0 && heads % kv_heads == 0) || throw(DimensionMismatch("heads"))
+    heads == kv_heads || (heads > 0 && kv_heads > 0 && heads % kv_heads == 0) || throw(DimensionMismatch("heads"))
     (cu_q === nothing) == (cu_k === nothing) || throw(ArgumentError("cu_q and cu_k go together"))
     if cu_q === nothing
         qmask === nothing || length(qmask) == nq * size(q, 4) || throw(DimensionMismatch("qmask"))
