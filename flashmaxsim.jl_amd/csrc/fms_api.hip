@@ -1223,8 +1223,27 @@ struct Pieces {
   }
 };
 
+// Copies into rows of whole units, run once a call has all its workspace.
+struct Packs {
+  struct One {
+    void* to;
+    const void* from;
+    int64_t st[3], seqs, tokens, heads;
+  } of[6];
+  int n = 0;
+  hipError_t run(const AttnArgs& a, hipStream_t stream) const {
+    const int32_t width = a.units * (16 / (int32_t)elem_bytes(a.dtype));
+    for (int i = 0; i < n; ++i) {
+      const One& x = of[i];
+      const hipError_t e = attn_pack(a.dtype, x.to, x.from, x.st, x.seqs, x.tokens, x.heads, a.dim, width, stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
+};
+
 // Dense copies, zeros behind dim, of the arrays that the kernels cannot read as they lie.
-hipError_t attn_packed(AttnArgs* a, Pieces* w) {
+hipError_t attn_packed(AttnArgs* a, Pieces* w, Packs* packs) {
   const int64_t esz = elem_bytes(a->dtype), unit = 16 / esz;
   const int64_t width = (a->dim + unit - 1) / unit * unit;
   a->units = (int32_t)(width / unit);
@@ -1238,12 +1257,11 @@ hipError_t attn_packed(AttnArgs* a, Pieces* w) {
     if (attn_reads(*a, *x.p, *x.st, x.heads)) continue;
     const int64_t rows = i == 0 ? a->nq : a->nk;
     void* to;
-    hipError_t e = w->get(&to, rows * x.heads * width * esz);
+    const hipError_t e = w->get(&to, rows * x.heads * width * esz);
     if (e != hipSuccess) return e;
     const bool ragged = a->cu_q != nullptr;
-    e = attn_pack(a->dtype, to, *x.p, *x.st, ragged ? 1 : a->seqs, ragged ? rows : x.tokens, x.heads, a->dim,
-                  (int32_t)width, w->stream);
-    if (e != hipSuccess) return e;
+    packs->of[packs->n++] = {to, *x.p, {(*x.st)[0], (*x.st)[1], (*x.st)[2]}, ragged ? 1 : a->seqs,
+                             ragged ? rows : x.tokens, x.heads};
     *x.p = to;
     (*x.st)[0] = x.tokens * x.heads * width;
     (*x.st)[1] = x.heads * width;
@@ -1286,9 +1304,13 @@ fms_status fms_attention(int32_t dtype, void* o, float* top, void* rest, const v
   out.top = top;
   hipError_t e = hipSuccess;
   if (seqs > 0 && tq > 0) {
-    if (e == hipSuccess) e = attn_packed(&a, &w);
+    Packs packs;
+    e = attn_packed(&a, &w, &packs);
     if (e == hipSuccess) e = attn_place(a, &w, o, a.nq, heads, &out.o);
     if (e == hipSuccess && dtype != FMS_F32 && rest) e = attn_place(a, &w, rest, a.nq, heads, &out.rest);
+    const int64_t bytes = attn_forward_bytes(a);
+    if (e == hipSuccess && bytes) e = w.get(&out.parts, bytes);
+    if (e == hipSuccess) e = packs.run(a, st);
     if (e == hipSuccess) e = attn_forward(a, out, st);
     if (e == hipSuccess) e = attn_unpack(a, o, out.o, a.nq, heads, st);
     if (e == hipSuccess && out.rest) e = attn_unpack(a, rest, out.rest, a.nq, heads, st);
@@ -1321,6 +1343,7 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
   if (seqs > 0) {
     const int64_t rows = a.nq * heads, esz = elem_bytes(dtype);
     void* p;
+    Packs packs;
     e = w.get(&p, rows * 8);
     g.delta = static_cast<float*>(p);
     g.level = g.delta + rows;
@@ -1328,21 +1351,24 @@ fms_status fms_attention_pullback(int32_t dtype, void* dq, void* dk, void* dv, c
       e = w.get(&p, seqs * kv_heads * kAttnPeakParts * 8);
       g.peaks = static_cast<float*>(p);
     }
-    if (e == hipSuccess) e = attn_packed(&a, &w);
+    if (e == hipSuccess) e = attn_packed(&a, &w, &packs);
     g.top = top;
-    const int64_t width = a.units * (16 / esz), dense[3] = {0, heads * dim, dim};
+    const int64_t width = a.units * (16 / esz);
     const void* from[3] = {dout, o, dtype == FMS_F32 ? nullptr : rest};
     const void** to[3] = {&g.dout, &g.o, &g.rest};
     for (int i = 0; i < 3 && e == hipSuccess; ++i) {
       *to[i] = from[i];
       if (!from[i] || (width == dim && aligned16(from[i]))) continue;
       e = w.get(&p, rows * width * esz);
-      if (e == hipSuccess) e = attn_pack(dtype, p, from[i], dense, 1, a.nq, heads, (int32_t)dim, (int32_t)width, st);
+      packs.of[packs.n++] = {p, from[i], {0, heads * dim, dim}, 1, a.nq, heads};
       *to[i] = p;
     }
     if (e == hipSuccess) e = attn_place(a, &w, dq, a.nq, heads, &g.dq);
     if (e == hipSuccess) e = attn_place(a, &w, dk, a.nk, kv_heads, &g.dk);
     if (e == hipSuccess) e = attn_place(a, &w, dv, a.nk, kv_heads, &g.dv);
+    const int64_t bytes = attn_pullback_bytes(a);
+    if (e == hipSuccess && bytes) e = w.get(&g.parts, bytes);
+    if (e == hipSuccess) e = packs.run(a, st);
     if (e == hipSuccess) e = attn_pullback(a, g, st);
     if (e == hipSuccess) e = attn_unpack(a, dq, g.dq, a.nq, heads, st);
     if (e == hipSuccess) e = attn_unpack(a, dk, g.dk, a.nk, kv_heads, st);

@@ -29,7 +29,6 @@
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
-#include "fms_group.hpp"
 
 namespace fms {
 namespace attn {
@@ -44,6 +43,25 @@ struct Parts {
   int splits;
   int keys;  // of a split, a multiple of kRows
 };
+
+// Few workgroups of many keys each leave most of the card idle: their keys are split, 256 to a
+// workgroup at least, until there are two to a CU (16 heads on 4 of 128 values in bf16, one token, 32768
+// keys: 1414 us in 4 workgroups, 20 and 5 for the join in 512).
+struct SplitPlan {
+  int64_t tiles, pieces, keys, splits, slots;
+};
+int waves_of(const AttnArgs& a) { return (int64_t)a.tq * a.group <= 32 ? 1 : 4; }
+SplitPlan split_plan(const AttnArgs& a) {
+  SplitPlan p;
+  const int rows = 32 * waves_of(a);
+  p.tiles = cdiv((int64_t)a.tq * a.group, rows);
+  p.pieces = a.seqs * a.kv_heads * p.tiles;
+  const int64_t wanted = p.pieces <= 128 ? 512 / p.pieces : 1;
+  p.keys = (cdiv(a.tk, wanted) + 255) / 256 * 256;
+  p.splits = a.tk > p.keys ? cdiv(a.tk, p.keys) : 1;
+  p.slots = p.splits > 1 ? p.pieces * p.splits * rows : 0;
+  return p;
+}
 
 // p in fp16 is held 2^10 times as large, so that small ones keep their bits.
 template <class Op>
@@ -345,30 +363,21 @@ hipError_t by_type(int32_t dtype, F&& f) {
 
 template <class Op, int kD, int kWaves>
 hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {
-  const int64_t tiles = cdiv((int64_t)a.tq * a.group, 32 * kWaves), units = a.seqs * a.kv_heads;
-  // Few workgroups of many keys each leave most of the card idle: their keys are split, 256 to a
-  // workgroup at least, until there are two to a CU (16 heads on 4 of 128 values in bf16, one token, 32768
-  // keys: 1414 us in 4 workgroups, 20 and 5 for the join in 512).
-  const int64_t pieces = units * tiles, wanted = pieces <= 128 ? 512 / pieces : 1;
-  const int64_t keys = (cdiv(a.tk, wanted) + 255) / 256 * 256;
-  if (a.tk > keys) {
+  const SplitPlan plan = split_plan(a);
+  const int64_t tiles = plan.tiles, units = a.seqs * a.kv_heads;
+  if (plan.splits > 1) {
     Parts p;
-    p.splits = (int)cdiv(a.tk, keys);
-    p.keys = (int)keys;
-    const int64_t slots = pieces * p.splits * (32 * kWaves);
-    void* mem;
-    hipError_t e = workspace_alloc(&mem, (size_t)(slots * (kD + 2) * 4), stream, true);
-    if (e != hipSuccess) return e;
-    p.acc = static_cast<float*>(mem);
-    p.stat = p.acc + slots * kD;
-    hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, true>), dim3(piece_blocks(pieces * p.splits)),
-                       dim3(kWaves * 64), 0, stream, a, out, p, (uint32_t)tiles, (uint32_t)(pieces * p.splits));
+    p.splits = (int)plan.splits;
+    p.keys = (int)plan.keys;
+    p.acc = static_cast<float*>(out.parts);
+    p.stat = p.acc + plan.slots * kD;
+    const int64_t work = plan.pieces * plan.splits;
+    hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, true>), dim3(piece_blocks(work)), dim3(kWaves * 64), 0,
+                       stream, a, out, p, (uint32_t)tiles, (uint32_t)work);
     const int most = a.tq * a.group;
     hipLaunchKernelGGL((attn_join_kernel<Op, kD, kWaves>), dim3((unsigned)(units * most)), dim3(256), 0, stream, a,
                        out, p, (int)tiles, most);
-    e = hipGetLastError();
-    const hipError_t ef = workspace_free(mem, stream);
-    return e != hipSuccess ? e : ef;
+    return hipGetLastError();
   }
   return by_units(a, tiles, [&](const AttnArgs& part, int64_t n) {
     hipLaunchKernelGGL((attn_forward_kernel<Op, kD, kWaves, false>), dim3(piece_blocks(n * tiles)), dim3(kWaves * 64), 0,
@@ -378,16 +387,16 @@ hipError_t forward_waves(const AttnArgs& a, const AttnOut& out, hipStream_t stre
 
 template <class Op, int kD>
 hipError_t forward_dim(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.tq * a.group;
-  if (rows <= 32) return forward_waves<Op, kD, 1>(a, out, stream);
-  return forward_waves<Op, kD, 4>(a, out, stream);
+  return waves_of(a) == 1 ? forward_waves<Op, kD, 1>(a, out, stream) : forward_waves<Op, kD, 4>(a, out, stream);
 }
 
 template <class Op>
 hipError_t forward_op(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {
-  if (a.dim <= 32) return forward_dim<Op, 32>(a, out, stream);
-  if (a.dim <= 64) return forward_dim<Op, 64>(a, out, stream);
-  return forward_dim<Op, 128>(a, out, stream);
+  switch (instance_dim(a)) {
+    case 32: return forward_dim<Op, 32>(a, out, stream);
+    case 64: return forward_dim<Op, 64>(a, out, stream);
+    default: return forward_dim<Op, 128>(a, out, stream);
+  }
 }
 
 }  // namespace
@@ -420,6 +429,8 @@ hipError_t attn_zero_gaps(int32_t dtype, const AttnGaps& gaps, hipStream_t strea
     hipLaunchKernelGGL((attn::attn_gap_kernel<uint16_t>), blocks, dim3(256), 0, stream, gaps);
   return hipGetLastError();
 }
+
+int64_t attn_forward_bytes(const AttnArgs& a) { return attn::split_plan(a).slots * (attn::instance_dim(a) + 2) * 4; }
 
 hipError_t attn_forward(const AttnArgs& a, const AttnOut& out, hipStream_t stream) {
   return attn::by_type(a.dtype, [&](auto op) { return attn::forward_op<decltype(op)>(a, out, stream); });

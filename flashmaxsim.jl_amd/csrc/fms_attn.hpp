@@ -48,7 +48,9 @@ struct AttnOut {
   void* o;
   float* top;
   void* rest;
+  void* parts;  // attn_forward_bytes of workspace
 };
+int64_t attn_forward_bytes(const AttnArgs& a);
 hipError_t attn_forward(const AttnArgs& a, const AttnOut& out, hipStream_t stream);
 
 struct AttnGrads {
@@ -58,9 +60,12 @@ struct AttnGrads {
   float* delta;        // as top: sum_j p_ij dp_ij, from the first kernel to the second
   float* level;        // as top: what the rows' sums are brought to one by, likewise
   float* peaks;        // (units, kPeakParts, 2): largest squared norms of v and dout rows (fp16)
+  void* parts;         // attn_pullback_bytes of workspace
 };
+int64_t attn_pullback_bytes(const AttnArgs& a);
 constexpr int kAttnPeakParts = 16;
-// g.delta, g.level and g.peaks are the caller's; rows of o, rest and dout are whole units apart.
+// All workspace is the caller's, who has it before anything is launched: a captured call that is lent too little
+// adds nothing.  Rows of o, rest and dout are whole units apart.
 hipError_t attn_pullback(const AttnArgs& a, const AttnGrads& g, hipStream_t stream);
 
 // ---- host helpers of both ----------------------------------------------------------------
@@ -97,6 +102,7 @@ __device__ __forceinline__ float factor(const AttnArgs& A) {
 }
 constexpr int kFar = (int)0x80000000u;  // a byte offset past every resource: reads as zero
 constexpr int kRows = 64;               // rows of a tile in LDS
+inline int instance_dim(const AttnArgs& a) { return a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128; }
 constexpr int kMaskSpan = 16384;        // rows whose mask bits are held at a time
 
 // A sequence's place: first token rows and lengths.

@@ -35,7 +35,6 @@
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
-#include "fms_group.hpp"
 
 namespace fms {
 namespace attn {
@@ -573,29 +572,31 @@ hipError_t launch_dkv(const AttnArgs& a, const AttnGrads& g, float* parts, int64
 
 template <class Op, int kD>
 hipError_t pullback_dim(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
-  const int64_t units = a.seqs * a.kv_heads, splits = dkv_splits(a);
-  void* parts = nullptr;  // (before anything is launched: a captured call without workspace adds nothing)
   hipError_t e = hipSuccess;
-  if (splits > 1) e = workspace_alloc(&parts, (size_t)(splits * 2 * units * a.tk * kD * 4), stream, true);
-  if (e != hipSuccess) return e;
   if (std::is_same<Op, OpF16>::value)
     e = by_units(a, kAttnPeakParts, [&](const AttnArgs& part, int64_t n) {
       hipLaunchKernelGGL(attn_peaks_kernel, dim3((unsigned)(n * kAttnPeakParts)), dim3(256), 0, stream, part, g);
     });
   if (e == hipSuccess) e = launch_dq<Op, kD>(a, g, stream);
-  if (e == hipSuccess) e = launch_dkv<Op, kD>(a, g, static_cast<float*>(parts), splits, stream);
-  const hipError_t ef = parts ? workspace_free(parts, stream) : hipSuccess;
-  return e != hipSuccess ? e : ef;
+  if (e == hipSuccess) e = launch_dkv<Op, kD>(a, g, static_cast<float*>(g.parts), dkv_splits(a), stream);
+  return e;
 }
 template <class Op>
 hipError_t pullback_op(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
-  if (a.dim <= 32) return pullback_dim<Op, 32>(a, g, stream);
-  if (a.dim <= 64) return pullback_dim<Op, 64>(a, g, stream);
-  return pullback_dim<Op, 128>(a, g, stream);
+  switch (instance_dim(a)) {
+    case 32: return pullback_dim<Op, 32>(a, g, stream);
+    case 64: return pullback_dim<Op, 64>(a, g, stream);
+    default: return pullback_dim<Op, 128>(a, g, stream);
+  }
 }
 
 }  // namespace
 }  // namespace attn
+
+int64_t attn_pullback_bytes(const AttnArgs& a) {
+  const int64_t splits = attn::dkv_splits(a);
+  return splits > 1 ? splits * 2 * a.seqs * a.kv_heads * a.tk * attn::instance_dim(a) * 4 : 0;
+}
 
 hipError_t attn_pullback(const AttnArgs& a, const AttnGrads& g, hipStream_t stream) {
   switch (a.dtype) {
