@@ -14,13 +14,14 @@
 // worked on the next is on its way into LDS.  Masked rows and keys are not loaded, tiles in which no
 // key counts are skipped.
 //
-// What bounds it, as measured:
-//   256 documents of up to 180 tokens, masked, 12 heads of 64, bf16: 62 us.  Vector
-//     instructions (about 8 a score, one of them at a quarter of the rate) are issued in 52 % of the cycles, the
+// What bounds it, as measured (a card that has run for a while; the first passes take a tenth more):
+//   256 documents of up to 180 tokens, masked, 12 heads of 64, bf16: 66 us.  Vector
+//     instructions (about 9 a score, one of them at a quarter of the rate) are issued in 53 % of the cycles, the
 //     matrix cores busy in 11 %: a workgroup has one to three tiles, whose first loads and last stores
 //     other workgroups of the CU hide in part.
-//   8192 causal tokens, 16 heads on 4 of 128, bf16: 560 us, three products' work (p in two values), 0.73
-//     PFLOP/s of it, matrix cores busy in 54 % of the cycles, vector units in 57; one rounding of p took 440, and results 1.4 times as far off.
+//   8192 causal tokens, 16 heads on 4 of 128, bf16: 507 us, three products' work (p in two values), 0.81
+//     PFLOP/s of it, matrix cores busy in 53 % of the cycles, vector units in 60; one rounding of p took a fifth
+//     less, and results were 1.4 times as far off.
 //   one token on 32768 keys, 16 heads on 4 of 128, bf16: 20 us and 5 for the join, 67 MB at 3.4 TB/s:
 //     512 workgroups of a wave have four tiles each, and wait for the first.
 #include <algorithm>
@@ -46,7 +47,9 @@ struct Parts {
 
 // Few workgroups of many keys each leave most of the card idle: their keys are split, 256 to a
 // workgroup at least, until there are two to a CU (16 heads on 4 of 128 values in bf16, one token, 32768
-// keys: 1414 us in 4 workgroups, 20 and 5 for the join in 512).
+// keys: 1414 us in 4 workgroups, 20 and 5 for the join in 512).  Above 128 workgroups none are: single tokens of 16
+// sequences on 8192 keys each, 32 heads on 8 of 128 in bf16, take 111 us in 128 times four, those of 17 sequences 337
+// in 136.
 struct SplitPlan {
   int64_t tiles, pieces, keys, splits, slots;
 };
@@ -319,6 +322,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs A, AttnOut out,
   if (out.top && threadIdx.x == 0) out.top[rows_at(A, b, hk, S.q0) + row] = m;
 }
 
+// A thread a value.  What heads of no whole 16 bytes cost: with 16 heads of 60 in bf16 instead of 64, 128 x 180 tokens
+// forward and back take 1099 us instead of 202, 14 copies of 65 us each (forward alone 301 instead of 46).
 template <class E>
 __global__ void __launch_bounds__(256) attn_pack_kernel(E* to, const E* from, int64_t s0, int64_t s1, int64_t s2,
                                                         int64_t tokens, int64_t heads, int dim, int packed,

@@ -290,7 +290,7 @@ struct Tile {
 };
 
 // Waves of a SIMD that the forward's registers should leave room for: as many as the LDS does.  (256 documents of up
-// to 180 tokens, 12 heads of 64 in bf16: 61 us with four, 71 with three, though four spill a few registers.)
+// to 180 tokens, 12 heads of 64 in bf16: 66 us with four, 72 with three, though four spill a few registers.)
 template <class Op, int kD, int kWaves>
 constexpr int kSimdWaves = kWaves < 4 ? 1 : kD * Op::kEsz <= 128 ? 4 : kD * Op::kEsz <= 256 ? 2 : 1;
 

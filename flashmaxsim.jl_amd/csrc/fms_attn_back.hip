@@ -20,18 +20,19 @@
 // two: p by 2^15, dp - delta by a bound of its size from the norms of do and v, so that neither small
 // probabilities nor small cotangents lose their bits.
 //
-// What bounds it, as measured (matrix cores busy, vector instructions issued, of the cycles):
-//   128 documents of up to 180 tokens, masked, 16 heads of 64, bf16: dq 62 us (13 %, 35 %), dk and dv 84 (12 %,
+// What bounds it, as measured (matrix cores busy, vector instructions issued, of the cycles; a card that has run for a
+// while, the first passes take a tenth more):
+//   128 documents of up to 180 tokens, masked, 16 heads of 64, bf16: dq 62 us (13 %, 39 %), dk and dv 82 (12 %,
 //     37 %).  One to three tiles a workgroup: its loads at the start and its stores at the end, which three
-//     and two waves a SIMD (accumulators and operands) hide in part.  (dq with four: 84, twenty registers spill.)
-//   48 ragged documents of up to 1999 tokens, window 64, 12 heads of 64, fp16: norms 28, dq 142 (20 %, 46 %), dk and dv
-//     188 (20 %, 47 %); tiles on the window's edge are half empty.
-//   8192 causal tokens, 16 heads on 4 of 128, bf16: dq 645 (63 %, 46 %; four products' work, 0.85 PFLOP/s), dk and
-//     dv 1310 and 23 for the join (42 %, 41 %; six, 0.63 PFLOP/s), with one wave a SIMD, whose exponentials nothing else
-//     hides.  With p and ds rounded once 530 and 1077; gradients were then 1.4 to 1.5 times as far off as
+//     and two waves a SIMD (accumulators and operands) hide in part.  (dq with four: 83, twenty registers spill.)
+//   48 ragged documents of up to 1999 tokens, window 64, 12 heads of 64, fp16: norms 28, dq 137 (19 %, 50 %), dk and dv
+//     179 (20 %, 45 %); tiles on the window's edge are half empty.
+//   8192 causal tokens, 16 heads on 4 of 128, bf16: dq 587 (61 %, 53 %; four products' work, 0.94 PFLOP/s), dk and
+//     dv 1220 and 23 for the join (40 %, 39 %; six, 0.68 PFLOP/s), with one wave a SIMD, whose exponentials nothing else
+//     hides.  With p and ds rounded once both took a sixth less; gradients were then 1.4 to 1.5 times as far off as
 //     their own rounding takes them.
-//   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 40 (47 %) and 43 (43 %): the path of the
-//     longest sequence's workgroups, one wave a SIMD; fp32 products run at about an eighth of the rate.
+//   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 40 (45 %) and 43 (43 %): the path of the
+//     longest sequence's workgroups, two waves and one a SIMD; fp32 products run at about an eighth of the rate.
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
@@ -269,7 +270,8 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
           s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - base, c, kShift<Op>));
           sum += s[r];
           s[r] *= (y[r] - delta) * by;
-          // (four at a time: all sixteen at once take as many registers more, and a wave of each SIMD with them)
+          // (four at a time: all sixteen at once take as many registers more, and a wave of each SIMD with them: 8192
+          // causal tokens, 16 heads on 4 of 128 in bf16, 917 us for 654, on a card that has just begun)
           if (r % 4 == 3) asm volatile("" : "+v"(sum), "+v"(s[r]));
         }
         l += sum;

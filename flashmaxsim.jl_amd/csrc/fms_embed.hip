@@ -4,14 +4,14 @@
 //
 // Bound by memory: the lookup writes every e once (its reads repeat), the gradient reads every de once
 // and writes all of dW (128 x 180 tokens, 70 % of them real, 32768 rows
-// of 1024 in bf16: lookup 11 us; gradient 31 for the sort, whose short kernels are latency, 25 for the
-// rows, 14 for the longer runs).  For the gradient the tokens are grouped by id (the candidate scans'
+// of 1024 in bf16: lookup 11 us; gradient 31 for the sort, 16 of it for the order inside its buckets and the
+// rest short kernels that are latency, 25 for the rows, 14 for the longer runs).  For the gradient the tokens are grouped by id (the candidate scans'
 // counting sort, whose atomics stay in LDS); a wave takes a row of dW and adds its tokens' rows in
 // fp32 and in the order of the tokens, which it restores first (the sort leaves a group's order
 // open), so the sums are the same every time.  Ids of more than 64 tokens (a text's most frequent
 // words: one token in fifteen can be of one id) are left to a second kernel, in which a workgroup
-// spreads such a row's tokens, as bits of a map that is in order by itself, over 64 sixteenths of
-// waves, and joins their sums in order.
+// spreads such a row's tokens, as bits of a map that is in order by itself, over 64 quarters of
+// waves (16 lanes), and joins their sums in a fixed order.
 #include "fms_embed.hpp"
 
 #include "../../include/flashmaxsim_hip.h"

@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(1024) rotary_join_kernel(T* dwq, T* dwk, const
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Units of 16 bytes: every part of a head, and every head, is whole ones.
+// Units of 16 bytes: every part of a head, and every head, is whole ones.  (Other widths take a value at a time: 128 x
+// 180 tokens of 16 and 16 heads in bf16, forward and back, 558 us with heads of 72 and 169 with heads of 80.)
 bool whole_units(const RotaryArgs& a, std::initializer_list<const void*> ptrs) {
   const int64_t esz = a.dtype == FMS_F32 ? 4 : 2;
   if (a.dim * esz % 32 != 0 || a.turned * esz % 32 != 0) return false;

@@ -66,7 +66,7 @@ def embed_tokens(ids, weight, scale=1.0):
     """scale * weight[ids - 1], recorded by autograd: ids (Int32 or Int64, any shape) are 1-based rows of
     weight (vocabulary, dim), as every index of the package.  An id outside 1 .. vocabulary gives
     zeros and takes no part in the gradient; 0 pads.  The gradient is the whole table's, its sums in
-    fp32 and in the order of the tokens."""
+    fp32 and in an order that the tokens' own fixes (partial sums, joined, for frequent ids)."""
     return _EmbedTokens.apply(ids, weight, scale)
 
 

@@ -596,7 +596,8 @@ fms_status fms_embed_tokens(int32_t dtype, void* e, const void* ids, int32_t id_
 
 /*
  * Its pullback: dweight (vocabulary, dim), overwritten in full, = scale * the sums of the cotangent
- * de's rows by id, in fp32 and in the order of the tokens.  Deterministic.
+ * de's rows by id, in fp32: in the order of the tokens, for ids of more than 64 tokens by parts of that
+ * order, joined in a fixed one.  Deterministic.
  */
 fms_status fms_embed_tokens_pullback(int32_t dtype, void* dweight, const void* de, const void* ids,
                                      int32_t id_bytes, float scale, int64_t tokens,
