@@ -32,7 +32,7 @@
 //     hides.  With p and ds rounded once both took a sixth less; gradients were then 1.4 to 1.5 times as far off as
 //     their own rounding takes them.
 //   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 40 (45 %) and 43 (43 %): the path of the
-//     longest sequence's workgroups, two waves and one a SIMD; fp32 products run at about an eighth of the rate.
+//     longest sequence's workgroups, one wave a SIMD; fp32 products run at about an eighth of the rate.
 #include "fms_attn.hpp"
 
 #include "../../include/flashmaxsim_hip.h"
@@ -271,8 +271,10 @@ __global__ void __launch_bounds__(kWaves * 64) attn_dq_kernel(AttnArgs A, AttnGr
           sum += s[r];
           s[r] *= (y[r] - delta) * by;
           // (four at a time: all sixteen at once take as many registers more, and a wave of each SIMD with them: 8192
-          // causal tokens, 16 heads on 4 of 128 in bf16, 917 us for 654, on a card that has just begun)
-          if (r % 4 == 3) asm volatile("" : "+v"(sum), "+v"(s[r]));
+          // causal tokens, 16 heads on 4 of 128 in bf16, 917 us for 654, on a card that has just begun.  Not in fp32: a
+          // second wave only shares the matrix cores, 8 sequences of 700 causal tokens, 8 heads on 4 of 64, 139 us for
+          // 101)
+          if (Op::kEsz == 2 && r % 4 == 3) asm volatile("" : "+v"(sum), "+v"(s[r]));
         }
         l += sum;
         constexpr int kPer = 32 / kGroups<Op>;
