@@ -31,7 +31,7 @@
 //     dv 1220 and 23 for the join (40 %, 39 %; six, 0.68 PFLOP/s), with one wave a SIMD, whose exponentials nothing else
 //     hides.  With p and ds rounded once both took a sixth less; gradients were then 1.4 to 1.5 times as far off as
 //     their own rounding takes them.
-//   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 40 (45 %) and 43 (43 %): the path of the
+//   16 sequences of up to 237 queries and 301 keys, 6 heads of 48, fp32: 41 (45 %) and 44 (43 %): the path of the
 //     longest sequence's workgroups, one wave a SIMD; fp32 products run at about an eighth of the rate.
 #include "fms_attn.hpp"
 
